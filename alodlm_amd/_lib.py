@@ -108,6 +108,13 @@ SIGNATURES = {
     "alodlm_scale_add_f32": [P, P, I64, P, I32, P],
     "alodlm_transpose": [P, P, I64, I64, I32, P],
     "alodlm_check_finite": [P, I64, I32, P, P],
+    "alodlm_paged_append": [P, P, P, I64, P, I64, P, I64, P, I64, P, P, P],
+    "alodlm_paged_retire": [P, P, P, P],
+    "alodlm_paged_attention_workspace": [P, P, I64],
+    "alodlm_paged_attention": [P, P, P, I64, P, I64, F32, I32, P, P],
+    "alodlm_token_log_probs_workspace": [I64, I64, I64],
+    "alodlm_token_log_probs": [P, I64, P, I64, I64, I64, F32, I64, P, P, P, P, P, P, I32, P],
+    "alodlm_token_log_probs_bwd": [P, I64, P, P, P, P, P, P, P, I64, I64, I64, F32, I64, P, I32, P],
 }
 _RESTYPE = {
     "alodlm_last_error": ctypes.c_char_p,
@@ -125,6 +132,8 @@ _RESTYPE = {
     "alodlm_attention_ds_blocks": I64,
     "alodlm_objective_workspace": I64,
     "alodlm_gate_bwd_workspace": I64,
+    "alodlm_paged_attention_workspace": I64,
+    "alodlm_token_log_probs_workspace": I64,
 }
 
 _lib = None

@@ -7,12 +7,18 @@ Q_s the per-sequence sums of the detached credit and of log q.  Arguments are
 validated with the reference's ValueError messages (alodlm/credit.py:8-35);
 the sums run in one workgroup with a fixed order (float32), so results are
 deterministic.
+
+``token_log_probs(logits, targets)`` gives the per-token log probabilities that the
+score function takes, with the entropy and the top alternatives, from logits over
+the vocabulary.
 """
+
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import call, ptr
+from ._lib import call, ptr, query
 
 
 def _require_gpu(t, what):
@@ -92,3 +98,80 @@ def sequence_score_function(credit, log_prob, sequence_ids, sequence_count):
         raise ValueError('Sequence IDs must be within the declared sequence count')
     _require_gpu(credit, "sequence_score_function")
     return _SequenceScore.apply(credit, log_prob, sequence_ids, int(sequence_count))
+
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_log_probs`` returns."""
+    log_prob: torch.Tensor  # float32 [rows]
+    entropy: torch.Tensor  # float32 [rows]
+    top_log_prob: torch.Tensor  # float32 [rows, top]
+    top_ids: torch.Tensor  # int64 [rows, top]
+
+
+MAX_TOP = 64
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top, inv_temperature, ignore_index):
+        R, V = logits.shape
+        dev, code = logits.device, _lib.dtype_code(logits.dtype)
+        x = logits.detach()
+        x = x if x.stride(1) == 1 and x.stride(0) >= V else x.contiguous()
+        log_prob, entropy, lse = torch.empty(3, R, dtype=torch.float32, device=dev).unbind()
+        top_log_prob = torch.empty(R, top, dtype=torch.float32, device=dev)
+        top_ids = torch.empty(R, top, dtype=torch.int64, device=dev)
+        need = query("alodlm_token_log_probs_workspace", R, V, top)
+        ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
+        with torch.cuda.device(dev):
+            call("alodlm_token_log_probs", ptr(x), x.stride(0), ptr(targets), R, V, top,
+                 inv_temperature, ignore_index, ptr(log_prob), ptr(entropy), ptr(lse),
+                 ptr(top_log_prob), ptr(top_ids), ptr(ws), code, _lib.stream_handle(dev))
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, targets, top_ids, lse, entropy)
+            ctx.args = top, inv_temperature, ignore_index
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return log_prob, entropy, top_log_prob, top_ids
+
+    @staticmethod
+    def backward(ctx, d_log_prob, d_entropy, d_top, _d_ids):
+        logits, targets, top_ids, lse, entropy = ctx.saved_tensors
+        top, inv_temperature, ignore_index = ctx.args
+        R, V = logits.shape
+        x = logits if logits.stride(1) == 1 and logits.stride(0) >= V else logits.contiguous()
+        out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+        grads = [None if g is None else g.to(torch.float32).contiguous()
+                 for g in (d_log_prob, d_entropy, d_top)]
+        with torch.cuda.device(x.device):
+            call("alodlm_token_log_probs_bwd", ptr(x), x.stride(0), ptr(targets), ptr(top_ids),
+                 ptr(lse), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
+                 ptr(out), _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
+        return out, None, None, None, None
+
+
+def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
+    """Log probabilities of the tokens ``targets`` (int64 [rows]) under logits [rows,
+    vocab] over ``temperature``, with each row's entropy and its ``top`` most likely
+    tokens (up to 64, in order, the lower id first among equal logits) and their log
+    probabilities: a ``TokenLogProbs``, all float32 but the ids.  Differentiable in
+    ``logits``, through the entropies and the alternatives' log probabilities too.
+
+    A target of ``ignore_index`` has log probability 0 and no gradient; any other
+    target outside the vocabulary gives NaN.  A logit of -inf is a token that cannot
+    be; in a row of nothing else log_prob is -inf, the entropy 0 and the gradient 0.
+    A NaN in a row makes its results NaN."""
+    if logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError('Logits must be [rows, vocabulary]')
+    _lib.dtype_code(logits.dtype)
+    if targets.dtype != torch.int64 or targets.shape != logits.shape[:1]:
+        raise ValueError('Targets must be int64, one per row of logits')
+    if targets.device != logits.device:
+        raise ValueError('Targets and logits must share a device')
+    if not 0 <= top <= min(MAX_TOP, logits.shape[1]):
+        raise ValueError(f'top must be between 0 and {MAX_TOP} and at most the vocabulary')
+    if not 0 < temperature < float("inf"):
+        raise ValueError('temperature must be positive and finite')
+    _require_gpu(logits, "token_log_probs")
+    return TokenLogProbs(*_TokenLogProbs.apply(logits, targets.contiguous(), int(top),
+                                               1.0 / temperature, int(ignore_index)))

@@ -1,0 +1,337 @@
+// Attention of each sequence's new rows over its paged cache.
+//
+// Mathematics: o = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m) with s = scale * q.k,
+// one pass over the keys with the running maximum m and sum (base 2: the scale
+// carries log2 e).  The keys of a sequence are cut into chunks that run apart; their
+// (m, sum, unnormalised o) in float32 are joined by a second launch, in chunk order.
+//
+// paged_rows_kernel (float32, and head sizes that the matrix-core kernels do not
+// take): one wavefront per query row, head and chunk; 64 keys at a time, one per
+// lane for the scores, then one output column per lane for the values, which lie
+// token by token.
+#include "paged.h"
+
+#define ROWS_WAVES 4
+#define LOG2E 1.44269504088896341f
+
+struct AttendArgs {
+  const void* q;
+  void* out;
+  int64_t ldq;
+  float* part;  // partial outputs [chunks][rows * heads][head_dim]
+  float2* stat;  // (m, sum) [chunks][rows * heads]
+  int heads, group, chunk_keys, chunks;
+  float scale2;  // softmax scale * log2 e
+  int zero_rest;
+};
+
+// Where the 8-bit pages of a sequence end (keys before it are sealed).
+__device__ __forceinline__ int sealed_keys(const PagedBatch& bt, int held, int end, int page,
+                                           bool eight) {
+  if (!eight) return end;
+  return (bt.final_rows ? end : held) / page * page;
+}
+
+// The first key whose place in the open pages another one has taken (windows longer
+// than the open pages are refused by the host; this bounds what is read).
+__device__ __forceinline__ int open_end(const PagedCache& c, int sealed, int end) {
+  return (int)min((int64_t)end, (int64_t)sealed + (int64_t)c.open_pages * c.page);
+}
+
+// Four e4m3 codes as floats.
+__device__ __forceinline__ void unpack_e4m3(uint32_t w, float* v) {
+  v[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+  v[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+  v[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+  v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else if constexpr (sizeof(T) == 2) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+    v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+  } else {
+    unpack_e4m3(*reinterpret_cast<const uint32_t*>(p), v);
+  }
+}
+
+// q . (the key at p) over dh dimensions, q in LDS.
+template <typename T>
+__device__ __forceinline__ float dot_key(const float* q, const T* p, int dh) {
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < dh; d += 4) {
+    float v[4];
+    load4(p + d, v);
+    const float4 x = *reinterpret_cast<const float4*>(q + d);
+    acc[0] = fmaf(x.x, v[0], acc[0]);
+    acc[1] = fmaf(x.y, v[1], acc[1]);
+    acc[2] = fmaf(x.z, v[2], acc[2]);
+    acc[3] = fmaf(x.w, v[3], acc[3]);
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+
+// acc + sum over the first n (<= 16) of 16 keys of p * v.
+template <typename T>
+__device__ __forceinline__ float add_values(float acc, const float* p, const T* v, int n,
+                                            float scale) {
+  float a = 0.f;
+  if (n == 16) {
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      float x[4];
+      load4(v + k, x);
+      const float4 w = *reinterpret_cast<const float4*>(p + k);
+      a = fmaf(w.x, x[0], a);
+      a = fmaf(w.y, x[1], a);
+      a = fmaf(w.z, x[2], a);
+      a = fmaf(w.w, x[3], a);
+    }
+  } else {  // keys that the row does not see are not touched, whatever they hold
+    for (int k = 0; k < n; ++k) {
+      float x;
+      if constexpr (sizeof(T) == 1) x = __builtin_amdgcn_cvt_f32_fp8((int)v[k], 0);
+      else x = Elem<T>::load(v, k);
+      a = fmaf(p[k], x, a);
+    }
+  }
+  return fmaf(a, scale, acc);
+}
+
+template <typename T, bool EIGHT>
+__global__ void __launch_bounds__(64 * ROWS_WAVES)
+paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) float qs[ROWS_WAVES][256];
+  __shared__ __attribute__((aligned(16))) float ps[ROWS_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int dh = c.head_dim, page = c.page;
+  const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  // unit: (chunk, sequence row, query head), heads of a row side by side
+  const int64_t unit = (int64_t)blockIdx.x * ROWS_WAVES + wave;
+  const int64_t per_chunk = (int64_t)bt.sequences * bt.max_rows * a.heads;
+  const int chunk = (int)(unit / per_chunk);
+  const int64_t rest = unit % per_chunk;
+  const int head = (int)(rest % a.heads);
+  const int i = (int)(rest / a.heads % bt.max_rows);
+  const int b = (int)(rest / a.heads / bt.max_rows);
+  bool live = chunk < a.chunks;
+  int held = 0, limit = 0, sealed = 0, last = 0, slot = -1;
+  int64_t row = 0;
+  if (live) {
+    held = bt.held(b, page);
+    const int n = held < 0 ? 0 : bt.row_count(b, held, page);
+    row = (int64_t)bt.first_row(b) + i;
+    const int64_t given = (int64_t)min(max(bt.offsets[b + 1], 0), bt.rows) - bt.first_row(b);
+    live = i < min(given, (int64_t)bt.max_rows);
+    if (i < n) {
+      const int end = held + n;
+      sealed = sealed_keys(bt, held, end, page, EIGHT);
+      last = EIGHT ? open_end(c, sealed, end) : end;
+      limit = min(held + i + 1, last);
+      if (EIGHT) slot = bt.slot(b, c.slots);
+    }
+  }
+  const int k0 = chunk * a.chunk_keys;
+  const int k1 = min(limit, k0 + a.chunk_keys);
+  float* q = qs[wave];
+  if (live && k1 > k0)
+    for (int d = lane; d < dh; d += 64)
+      q[d] = Elem<T>::load((const T*)a.q + row * a.ldq + (int64_t)head * dh, d) * a.scale2;
+  __builtin_amdgcn_wave_barrier();
+  const int kvh = head / a.group;
+  const int64_t block = (int64_t)page * dh;
+  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  // the place of the 16 keys from `key` on: codes (and their exponents' place), or rows
+  auto locate = [&](int key, int64_t* at, int64_t* id) {
+    const int p = key / page;
+    if (EIGHT && key >= sealed) {
+      *id = -1;
+      *at = slot < 0 ? -1 : (open_page(c, slot, p) * c.kv_heads + kvh) * block;
+    } else {
+      *id = bt.page_of(b, p, c.pages);
+      *at = *id < 0 ? -1 : (*id * c.kv_heads + kvh) * block;
+    }
+  };
+  for (int t = k0; live && t < k1; t += 64) {
+    const int key = t + lane;
+    float s = -INFINITY;
+    if (key < k1) {
+      int64_t at, id;
+      locate(key, &at, &id);
+      if (at >= 0) {
+        const int64_t k_at = at + (int64_t)(key % page) * dh;
+        if (!EIGHT) s = dot_key(q, (const T*)c.keys + k_at, dh);
+        else if (id < 0) s = dot_key(q, (const T*)c.open_keys + k_at, dh);
+        else s = dot_key(q, (const e4m3_t*)c.keys + k_at, dh) *
+                 exp2_int(c.exponents[id * 2 * c.kv_heads + kvh]);
+      }
+    }
+    const float m_new = fmaxf(m, wave_max(s));
+    // a NaN score makes the row's sum, and with it the row, NaN
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float p = exp2f(s - base);
+    const float alpha = exp2f(m - base);
+    m = m_new;
+    sum = fmaf(sum, alpha, wave_sum(p));
+    ps[wave][lane] = p;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] *= alpha;
+    for (int g = 0; g < 64 && t + g < k1; g += 16) {
+      int64_t at, id;
+      locate(t + g, &at, &id);
+      if (at < 0) continue;
+      const int n = min(k1 - t - g, 16);
+      const float scale = EIGHT && id >= 0 ? exp2_int(c.exponents[(id * 2 + 1) * c.kv_heads + kvh]) : 1.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = lane + 64 * j;
+        if (d >= dh) break;
+        const int64_t v_at = at + (int64_t)d * page + (t + g) % page;
+        if (!EIGHT) o[j] = add_values(o[j], ps[wave] + g, (const T*)c.values + v_at, n, 1.f);
+        else if (id < 0) o[j] = add_values(o[j], ps[wave] + g, (const T*)c.open_values + v_at, n, 1.f);
+        else o[j] = add_values(o[j], ps[wave] + g, (const e4m3_t*)c.values + v_at, n, scale);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (!live) return;
+  const int64_t at = row * a.heads + head;
+  if (a.chunks == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key is zero
+    for (int j = 0, d = lane; d < dh; ++j, d += 64)
+      Elem<T>::store((T*)a.out + at * dh, d, o[j] * inv);
+    return;
+  }
+  if (k1 <= k0 && chunk > 0) return;  // the join knows which chunks a row has
+  if (lane == 0) a.stat[chunk * T_heads + at] = make_float2(m, sum);
+  for (int j = 0, d = lane; d < dh; ++j, d += 64) a.part[(chunk * T_heads + at) * dh + d] = o[j];
+}
+
+// Joins the chunks of every row and head, one wavefront each, in chunk order.
+template <typename T, bool EIGHT>
+__global__ void __launch_bounds__(256)
+paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
+  const int lane = threadIdx.x & 63, dh = c.head_dim, page = c.page;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  if (unit >= (int64_t)bt.sequences * bt.max_rows * a.heads) return;
+  const int head = (int)(unit % a.heads);
+  const int i = (int)(unit / a.heads % bt.max_rows);
+  const int b = (int)(unit / a.heads / bt.max_rows);
+  const int64_t r0 = bt.first_row(b);
+  if (i >= min((int64_t)min(max(bt.offsets[b + 1], 0), bt.rows) - r0, (int64_t)bt.max_rows)) return;
+  const int held = bt.held(b, page);
+  const int n = held < 0 ? 0 : bt.row_count(b, held, page);
+  int limit = 0;
+  if (i < n) {
+    const int end = held + n, sealed = sealed_keys(bt, held, end, page, EIGHT);
+    limit = min(held + i + 1, EIGHT ? open_end(c, sealed, end) : end);
+  }
+  const int count = max((limit + a.chunk_keys - 1) / a.chunk_keys, 1);
+  const int64_t at = (r0 + i) * a.heads + head;
+  float M = -INFINITY;
+  for (int k = lane; k < count; k += 64) M = fmaxf(M, a.stat[k * T_heads + at].x);
+  M = wave_max(M);
+  const float base = M == -INFINITY ? 0.f : M;
+  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < count; ++k) {
+    const float2 st = a.stat[k * T_heads + at];
+    const float f = exp2f(st.x - base);
+    sum = fmaf(st.y, f, sum);
+    for (int j = 0, d = lane; d < dh; ++j, d += 64)
+      o[j] = fmaf(a.part[(k * T_heads + at) * dh + d], f, o[j]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int j = 0, d = lane; d < dh; ++j, d += 64)
+    Elem<T>::store((T*)a.out + at * dh, d, o[j] * inv);
+}
+
+// Zeros in the rows behind the last sequence.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_zero_rest_kernel(PagedBatch bt, T* out, int64_t width) {
+  const int64_t from = (int64_t)min(max(bt.offsets[bt.sequences], 0), bt.rows) * width;
+  const int64_t to = (int64_t)bt.rows * width;
+  for (int64_t i = from + (int64_t)blockIdx.x * 256 + threadIdx.x; i < to; i += (int64_t)gridDim.x * 256)
+    Elem<T>::store(out, i, 0.f);
+}
+
+// ----------------------------------------------------------------------------
+// Host
+// ----------------------------------------------------------------------------
+struct AttendPlan {
+  int64_t chunk_keys, chunks;
+};
+
+// Keys per chunk: as many chunks as give every compute unit several workgroups, of
+// 256 keys at least.
+static AttendPlan attend_plan(const alodlm_paged_batch* b, int64_t heads) {
+  const int64_t units = b->sequences * b->max_rows * heads;  // wavefronts per chunk
+  const int64_t want = units > 0 ? (8192 + units - 1) / units : 1;
+  const int64_t most = max((b->max_keys + 255) / 256, (int64_t)1);
+  const int64_t chunks = min(max(want, (int64_t)1), most);
+  int64_t keys = (b->max_keys + chunks - 1) / chunks;
+  keys = max((keys + 63) / 64 * 64, (int64_t)64);
+  return {keys, max((b->max_keys + keys - 1) / keys, (int64_t)1)};
+}
+
+static int64_t attend_floats(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
+  const AttendPlan p = attend_plan(b, heads);
+  return p.chunks == 1 ? 0 : p.chunks * b->rows * heads * (c->head_dim + 2);
+}
+
+extern "C" int64_t alodlm_paged_attention_workspace(const alodlm_paged_cache* cache,
+                                                    const alodlm_paged_batch* batch, int64_t heads) {
+  if (paged_check(cache, batch) || heads < 1) return 0;
+  return attend_floats(cache, batch, heads);
+}
+
+template <typename T, bool EIGHT>
+static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, AttendArgs a,
+                         hipStream_t st) {
+  const PagedCache dc = paged_cache(c);
+  const PagedBatch db = paged_batch(b);
+  const int64_t units = b->sequences * b->max_rows * a.heads;
+  if (units > 0) {
+    const int64_t blocks = (units * a.chunks + ROWS_WAVES - 1) / ROWS_WAVES;
+    ALODLM_CHECK_ARG(blocks < (1ll << 31), "paged_attention: too many rows in one call");
+    paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
+    if (a.chunks > 1)
+      paged_join_kernel<T, EIGHT><<<ceil_div_u(units, 4), 256, 0, st>>>(dc, db, a);
+  }
+  if (a.zero_rest && b->rows > 0)
+    paged_zero_rest_kernel<T><<<256, 256, 0, st>>>(db, (T*)a.out, a.heads * c->head_dim);
+  ALODLM_CHECK_LAUNCH("paged_attention");
+  return ALODLM_OK;
+}
+
+extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_batch* batch,
+                                      const void* q, int64_t ldq, void* out, int64_t heads,
+                                      float scale, int zero_rest, float* workspace, void* stream) {
+  const int rc = paged_check(cache, batch);
+  if (rc) return rc;
+  const int64_t es = cache->dtype == ALODLM_BF16 ? 2 : 4;
+  ALODLM_CHECK_ARG(heads >= 1 && heads <= 65536 && heads % cache->kv_heads == 0,
+                   "paged_attention: heads must be a multiple of the cache's kv_heads");
+  ALODLM_CHECK_ARG(ldq >= heads * cache->head_dim, "paged_attention: row stride below the row width");
+  ALODLM_CHECK_ARG(scale > 0.f && scale < INFINITY, "paged_attention: scale must be positive");
+  ALODLM_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
+                       ldq * es % 16 == 0,
+                   "paged_attention: rows must be 16-byte aligned");
+  if (batch->rows == 0) return ALODLM_OK;
+  ALODLM_CHECK_ARG(q && out, "paged_attention: no rows");
+  const AttendPlan plan = attend_plan(batch, heads);
+  ALODLM_CHECK_ARG(plan.chunks == 1 || workspace, "paged_attention: no workspace");
+  AttendArgs a = {q, out, ldq, workspace, nullptr, (int)heads, (int)(heads / cache->kv_heads),
+                  (int)plan.chunk_keys, (int)plan.chunks, scale * LOG2E, zero_rest};
+  a.stat = reinterpret_cast<float2*>(workspace + plan.chunks * batch->rows * heads * cache->head_dim);
+  ALODLM_DISPATCH(cache->dtype, T, {
+    if (cache->eight_bit) return attend_launch<T, true>(cache, batch, a, as_stream(stream));
+    return attend_launch<T, false>(cache, batch, a, as_stream(stream));
+  });
+}

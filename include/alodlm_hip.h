@@ -664,6 +664,106 @@ int alodlm_transpose(const void* src, void* dst, int64_t rows, int64_t cols, int
  * loss. */
 int alodlm_check_finite(const void* x, int64_t n, int dtype, int32_t* flag, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A key/value cache of many sequences in pages (the many-request counterpart of
+ * the prefix cache of alodlm/inference.py:34-63), one per layer.
+ *
+ * Page p of sequence b holds its tokens [p * page_size, (p + 1) * page_size) and
+ * is page table[b * width + p] of the pool:
+ *   keys   [pages, kv_heads, page_size, head_dim]
+ *   values [pages, kv_heads, head_dim, page_size] (a page's tokens contiguous:
+ *          the operand order of the product with the probabilities).
+ * With eight_bit the pool holds e4m3 codes and exponents [pages, 2, kv_heads]
+ * (keys, values): a code stands for code * 2^exponent, the exponent the smallest
+ * e >= -100 with max|x| <= 448 * 2^e over the page and head (-100 for zeros; inf
+ * and NaN become NaN and do not count).  The scale is exact both ways, so a
+ * value is rounded once, and every value is exact in bf16.  A page is sealed
+ * (written in 8 bits) when its last token is kept; until then its tokens are
+ * rows of `dtype` in an open page: open_keys [slots, open_pages, kv_heads,
+ * page_size, head_dim], open_values the same with the last two exchanged; page p
+ * is open page p % open_pages of slot slots[b].  Without eight_bit the pool holds
+ * `dtype` and tokens are written straight into it.
+ *
+ * A batch is one step's rows: sequence b holds lengths[b] tokens and has the
+ * rows [offsets[b], offsets[b + 1]) (at most max_rows), whose positions follow
+ * them; with `final` the rows are kept, else only alodlm_paged_retire keeps the
+ * first of them (a decoding window).  max_keys bounds lengths[b] plus its rows.
+ * Arrays are on the device: entries out of range (a page outside the pool, a
+ * slot outside the slots, a length below zero or past the table) are never
+ * followed - such tokens are not written and not attended to.
+ * ------------------------------------------------------------------------ */
+typedef struct alodlm_paged_cache {
+  void* keys;
+  void* values;
+  int8_t* exponents;
+  void* open_keys;
+  void* open_values;
+  int64_t pages, page_size, kv_heads, head_dim, slots, open_pages;
+  int32_t dtype, eight_bit;
+} alodlm_paged_cache;
+
+typedef struct alodlm_paged_batch {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* offsets;
+  const int32_t* slots; /* NULL: sequence b uses slot b */
+  int64_t sequences, width, rows, max_rows, max_keys;
+  int32_t final_rows, reserved;
+} alodlm_paged_batch;
+
+/* Writes the batch's keys k and values v (rows of kv_heads * head_dim, row
+ * strides ldk, ldv) behind their sequences.  With cos/sin [rows, head_dim] the
+ * keys are rotated on the way (x * cos + rotate_half(x) * sin in float32, rounded
+ * once to dtype), and the queries q (rows of heads * head_dim, stride ldq; may be
+ * NULL) into q_out [rows, heads, head_dim].  A sequence's cached tokens do not
+ * depend on how its rows were split into calls.  Rows and strides 16-byte
+ * aligned. */
+int alodlm_paged_append(const alodlm_paged_cache* cache, const alodlm_paged_batch* batch,
+                        const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
+                        int64_t ldq, void* q_out, int64_t heads, const void* cos_tab,
+                        const void* sin_tab, void* stream);
+/* Keeps the first counts[b] (0 to its rows) rows of a batch that is not final:
+ * seals the pages they fill. */
+int alodlm_paged_retire(const alodlm_paged_cache* cache, const alodlm_paged_batch* batch,
+                        const int32_t* counts, void* stream);
+/* out [rows, heads, head_dim] = softmax(scale * q . k) . v of each row over its
+ * sequence's tokens up to its own position (row i of sequence b: the first
+ * lengths[b] + i + 1; the batch's tokens are in the cache).  Grouped-query heads:
+ * query head h reads key/value head h / (heads / kv_heads).  A row that sees no
+ * key is zero.  Rows behind the last sequence are left as they were, or set to
+ * zero with zero_rest.  The workspace query (floats) depends on the shapes and
+ * bounds of the two structs, not on device data. */
+int64_t alodlm_paged_attention_workspace(const alodlm_paged_cache* cache,
+                                         const alodlm_paged_batch* batch, int64_t heads);
+int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_batch* batch,
+                           const void* q, int64_t ldq, void* out, int64_t heads, float scale,
+                           int zero_rest, float* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens: what sequence_score (alodlm/credit.py:23-40)
+ * takes, from logits [rows, vocab] (dtype, row stride ld).
+ * With x = logits * inv_temperature, lse = logsumexp(x), p = exp(x - lse):
+ *   log_prob[r] = x[target] - lse  (0 for target == ignore, NaN for another
+ *                 target outside the vocabulary)
+ *   entropy[r]  = -sum p log p
+ *   top_ids / top_log_prob [rows, top]: the `top` largest logits in order, the
+ *                 lower index first among equal ones
+ * and lse[r], which the backward takes.  A logit of -inf has probability zero; a
+ * row of nothing else has log_prob -inf, entropy 0 and zero gradient.
+ * The backward writes dlogits [rows, vocab] for the upstream gradients d_log_prob,
+ * d_entropy [rows] and d_top [rows, top] (each may be NULL).
+ * ------------------------------------------------------------------------ */
+int64_t alodlm_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top);
+int alodlm_token_log_probs(const void* logits, int64_t ld, const int64_t* targets, int64_t rows,
+                           int64_t vocab, int64_t top, float inv_temperature, int64_t ignore,
+                           float* log_prob, float* entropy, float* lse, float* top_log_prob,
+                           int64_t* top_ids, float* workspace, int dtype, void* stream);
+int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targets,
+                               const int64_t* top_ids, const float* lse, const float* entropy,
+                               const float* d_log_prob, const float* d_entropy, const float* d_top,
+                               int64_t rows, int64_t vocab, int64_t top, float inv_temperature,
+                               int64_t ignore, void* dlogits, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,572 @@
+"""The paged cache and its attention on the GPU against plain token lists and 64-bit
+attention: every type and page size, steps, windows and prompts, strided and
+misaligned rows, padding, empty sequences, entries out of range, rows that hold inf or
+NaN, more than 2^32 values in a pool, several streams, captured graphs, and a run of a
+small decoder's steps."""
+
+import math
+
+import pytest
+import torch
+
+from alodlm_amd.credit import sequence_score_function, token_log_probs
+from alodlm_amd.inference import rope_tables
+from alodlm_amd.paged import PagedBatch, PagedCache, paged_attention
+from tests.helpers import log
+from tests.paged_oracle import (OracleCache, attend, attention_tolerance, quantise, rotate)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+class Run:
+    """A paged cache on the GPU beside its plain form on the CPU."""
+
+    def __init__(self, sequences, heads, kv_heads, dh, dtype, page, eight_bit, tokens=600, window=1,
+                 seed=0):
+        self.B, self.heads, self.kv_heads, self.dh, self.dtype = sequences, heads, kv_heads, dh, dtype
+        self.page, self.eight_bit = page, eight_bit
+        self.g = torch.Generator().manual_seed(seed)
+        width = -(-tokens // page)
+        pages = sequences * width + 2
+        self.cache = PagedCache.allocate(pages, kv_heads, dh, dtype, DEV, page_size=page,
+                                         eight_bit=eight_bit, slots=sequences + 2, window=window)
+        self.table = torch.randperm(pages, generator=self.g)[:sequences * width].view(sequences, width)
+        self.table = self.table.to(torch.int32).to(DEV)
+        self.slots = torch.randperm(sequences + 2, generator=self.g)[:sequences].to(torch.int32).to(DEV)
+        self.lengths = [0] * sequences
+        self.plain = OracleCache(sequences, page, eight_bit)
+
+    def randn(self, *shape, scale=1.0):
+        return (scale * torch.randn(*shape, generator=self.g)).to(self.dtype)
+
+    def batch(self, counts, rows=None, **more):
+        offsets = [0]
+        for n in counts:
+            offsets.append(offsets[-1] + n)
+        if "max_rows" not in more:
+            more["max_rows"] = max(counts)
+        return PagedBatch(self.table, torch.tensor(self.lengths, dtype=torch.int32, device=DEV),
+                          torch.tensor(offsets, dtype=torch.int32, device=DEV),
+                          rows=offsets[-1] if rows is None else rows, slots=self.slots, **more)
+
+    def step(self, counts, final=True, rotated=True, pad=0, keep=None, k=None, v=None, check=True):
+        """Appends counts[b] rows to every sequence, attends, and compares; a window
+        (not final) keeps the first keep[b] rows afterwards."""
+        T = sum(counts) + pad
+        q = self.randn(T, self.heads, self.dh, scale=2.0)
+        k = self.randn(T, self.kv_heads, self.dh) if k is None else k
+        v = self.randn(T, self.kv_heads, self.dh) if v is None else v
+        batch = self.batch(counts, rows=T, final=final)
+        cos = sin = None
+        if rotated:
+            where = torch.tensor([self.lengths[b] + i for b, n in enumerate(counts) for i in range(n)]
+                                 + [0] * pad)
+            inv = 1.0 / 10000.0 ** (torch.arange(0, self.dh, 2).float() / self.dh)
+            cos, sin = rope_tables(where, inv, self.dtype)
+        out = self.cache.append(k.to(DEV), v.to(DEV), batch, q=q.to(DEV) if rotated else None,
+                                cos=cos.to(DEV) if rotated else None,
+                                sin=sin.to(DEV) if rotated else None)
+        q, k = rotate(q, cos, sin), rotate(k, cos, sin)
+        if rotated:
+            assert torch.equal(out.cpu(), q)
+        got = paged_attention(q.to(DEV), self.cache, batch).cpu()
+        r = 0
+        for b, n in enumerate(counts):
+            new = [k[r + i] for i in range(n)], [v[r + i] for i in range(n)]
+            if final:
+                self.plain.k[b] += new[0]
+                self.plain.v[b] += new[1]
+                K, V = self.plain.tokens(b)
+            else:
+                K, V = self.plain.tokens(b, *new)
+            if check and n:
+                limits = [self.lengths[b] + i + 1 for i in range(n)]
+                self.compare(got[r:r + n], q[r:r + n], K, V, limits)
+            r += n
+        assert not bool(got[sum(counts):].any())
+        if final:
+            self.lengths = [a + n for a, n in zip(self.lengths, counts)]
+        elif keep is not None:
+            self.cache.retire(batch, torch.tensor(keep, dtype=torch.int32, device=DEV))
+            r = 0
+            for b, n in enumerate(counts):
+                self.plain.k[b] += [k[r + i] for i in range(keep[b])]
+                self.plain.v[b] += [v[r + i] for i in range(keep[b])]
+                r += n
+            self.lengths = [a + n for a, n in zip(self.lengths, keep)]
+        return got
+
+    def compare(self, got, q, K, V, limits, scale=None):
+        scale = self.dh ** -0.5 if scale is None else scale
+        ref, mag, size = attend(q, K, V, limits, scale)
+        tol = attention_tolerance(ref, mag, size, max(limits), self.dtype, self.dh)
+        off = ((got.double() - ref).abs() / tol).max()
+        assert float(off) <= 1.0, f"{float(off)} times the tolerance"
+
+    def check_cache(self):
+        """Every kept token's bits in the GPU's pages and open pages."""
+        c = self.cache
+        for b, length in enumerate(self.lengths):
+            for p in range(-(-length // self.page)):
+                n = min(length - p * self.page, self.page)
+                rows = slice(p * self.page, p * self.page + n)
+                K, V = torch.stack(self.plain.k[b][rows]), torch.stack(self.plain.v[b][rows])
+                at = int(self.table[b, p])
+                if not self.eight_bit or n < self.page:
+                    if self.eight_bit:
+                        slot, ring = int(self.slots[b]), p % c.open_keys.shape[1]
+                        gk, gv = c.open_keys[slot, ring], c.open_values[slot, ring]
+                    else:
+                        gk, gv = c.keys[at], c.values[at]
+                    assert torch.equal(gk[:, :n].cpu(), K.transpose(0, 1))
+                    assert torch.equal(gv[:, :, :n].cpu(), V.permute(1, 2, 0))
+                    continue
+                for h in range(self.kv_heads):
+                    for side, got, x in ((0, c.keys[at, h].float(), K[:, h]),
+                                         (1, c.values[at, h].float().T, V[:, h])):
+                        codes, e = quantise(x)
+                        assert int(c.exponents[at, side, h]) == e
+                        torch.testing.assert_close(got.cpu().double(), codes, rtol=0, atol=0,
+                                                   equal_nan=True)
+
+
+SHAPES = [  # heads, kv_heads, head_dim, dtype, page, eight_bit
+    (4, 2, 128, BF16, 64, True), (4, 2, 128, BF16, 16, True), (14, 2, 64, BF16, 32, True),
+    (3, 3, 64, BF16, 128, True), (8, 1, 128, BF16, 128, True), (4, 2, 128, BF16, 64, False),
+    (6, 2, 64, BF16, 16, False), (4, 2, 128, F32, 64, True), (4, 2, 128, F32, 64, False),
+    (2, 1, 8, F32, 16, True), (2, 2, 40, F32, 32, False), (3, 1, 256, BF16, 64, True),
+    (2, 1, 24, BF16, 64, True), (2, 1, 256, F32, 64, True),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_steps_and_prompts(shape):
+    """Prompts of different lengths (none, one token, whole pages, odd ones), then
+    chunks and single tokens over page borders: bits of the cache, attention."""
+    log(f"paged steps {shape}")
+    page = shape[4]
+    run = Run(5, *shape, tokens=4 * page + 200)
+    run.step([0, 1, page, 2 * page + 5, 37])
+    run.check_cache()
+    run.step([page - 1, 1, 0, 3, 2 * page], pad=3)
+    run.check_cache()
+    for _ in range(3):
+        run.step([1] * 5)
+    run.check_cache()
+    run.step([1, 0, 1, 0, 0], rotated=False, pad=1)
+    run.check_cache()
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[2] in (128, 64, 8)])
+def test_windows(shape):
+    """Windows whose rows are rewritten, then kept in part: over page borders, none of
+    them, all of them."""
+    log(f"paged windows {shape}")
+    page = shape[4]
+    run = Run(4, *shape, tokens=6 * page + 200, window=page + 9)
+    run.step([page - 3, 2 * page, 5, 1])
+    for keep in ([4, 0, 9, 1], [3, page, 1, page + 9]):
+        counts = [9, page + 9, 9, page + 9]
+        run.step(counts, final=False)  # a pass whose rows the next one rewrites
+        run.step(counts, final=False, keep=keep)
+        run.check_cache()
+    run.step([1, 2, 3, 4])
+    run.check_cache()
+
+
+@pytest.mark.parametrize("eight_bit", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_split_into_calls(dtype, eight_bit):
+    """The cache holds the same bits however its tokens came."""
+    log(f"paged split {dtype} {eight_bit}")
+    bits = []
+    for parts in ([203], [1] * 203, [63, 1, 64, 75], [150, 53]):
+        run = Run(1, 2, 2, 64, dtype, 64, eight_bit, seed=3)
+        k, v = run.randn(203, 2, 64), run.randn(203, 2, 64)
+        at = 0
+        for n in parts:
+            run.cache.append(k[at:at + n].to(DEV), v[at:at + n].to(DEV), run.batch([n]))
+            run.lengths[0] += n
+            at += n
+        c = run.cache
+        held = [c.keys[run.table[0].long()[:3]].view(torch.uint8), c.values[run.table[0].long()[:3]].view(torch.uint8)]
+        if eight_bit:
+            held += [c.exponents[run.table[0].long()[:3]], c.open_keys[run.slots[0], 0, :, :11],
+                     c.open_values[run.slots[0], 0, :, :, :11]]
+        bits.append([t.cpu() for t in held])
+    for other in bits[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(bits[0], other))
+
+
+def test_values_of_every_size():
+    """Pages whose scales run over the type's whole range, zeros, inf and NaN."""
+    log("paged value sizes")
+    run = Run(1, 2, 2, 64, BF16, 16, True, tokens=400)
+    x = run.randn(320, 2, 64)
+    sizes = [2.0 ** e for e in (127, 100, 30, 8, 0, -8, -40, -90, -100, -110, -126)] + [0.0]
+    for i, size in enumerate(sizes):
+        x[16 * i:16 * i + 16] *= size / 4
+    x[200, 0, 3], x[201, 1, 5], x[230, 0, 0] = math.inf, -math.inf, math.nan
+    x[240:256, 1] = math.nan
+    run.step([320], rotated=False, k=x, v=x.flip(0), check=False)
+    run.check_cache()
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, BF16, 64, True), (4, 2, 128, BF16, 64, False),
+                                   (6, 2, 64, BF16, 16, True), (4, 2, 128, F32, 64, True),
+                                   (4, 2, 128, F32, 32, False)])
+@pytest.mark.parametrize("counts", [[40, 40], [150, 7], [1, 1]])
+@pytest.mark.parametrize("final", [True, False])
+def test_hidden_rows_take_no_part(shape, counts, final):
+    """Rows whose later neighbours hold inf or NaN are those of clean neighbours; the
+    neighbours' own rows are NaN or inf in the columns concerned."""
+    log(f"paged hidden rows {shape} {counts} {final}")
+    clean, dirty = (Run(2, *shape, tokens=600, window=150, seed=5) for _ in range(2))
+    before = [70, 3]
+    for run in (clean, dirty):
+        run.step(before)
+    T = sum(counts)
+    k, v, q = (clean.randn(T, n, shape[2]) for n in (shape[1], shape[1], shape[0]))
+    bad_k, bad_v = k.clone(), v.clone()
+    last = [counts[0] - 1, T - 1]
+    for r, x in zip(last, (math.nan, math.inf)):
+        bad_v[r, :, 5] = x
+    bad_k[last[0], 0, 1] = math.nan
+    outs = []
+    for run, a, b in ((clean, k, v), (dirty, bad_k, bad_v)):
+        batch = run.batch(counts, final=final)
+        run.cache.append(a.to(DEV), b.to(DEV), batch)
+        outs.append(paged_attention(q.to(DEV), run.cache, batch).cpu())
+    sealed = shape[5] and final  # a page that is sealed takes another scale, not these rows
+    mine = torch.ones(T, dtype=torch.bool)
+    mine[last] = False
+    if not sealed:
+        assert torch.equal(outs[0][mine], outs[1][mine])
+    assert bool(outs[1][mine].isfinite().all())
+    assert not bool(outs[1][last][:, :, 5].isfinite().any())
+    assert bool(outs[1][last[0], :shape[0] // shape[1]].isnan().all())  # its own key is NaN
+    other = [d for d in range(shape[2]) if d != 5]
+    assert bool(outs[1][last[1]][:, other].isfinite().all())
+
+
+def test_rows_behind_open_pages_hold_anything():
+    """What open pages and unsealed places hold beyond a sequence's tokens takes no
+    part."""
+    log("paged garbage")
+    for shape in ((4, 2, 128, BF16, 64, True), (4, 2, 64, BF16, 16, False), (4, 2, 128, F32, 64, True)):
+        run = Run(3, *shape, tokens=400)
+        for t in (run.cache.keys, run.cache.values):
+            t.copy_(torch.full(t.shape, math.nan).to(t.dtype))
+        if run.eight_bit:
+            run.cache.open_keys.fill_(math.nan)
+            run.cache.open_values.fill_(math.inf)
+        run.step([70, 1, 128])
+        run.step([1, 1, 1])
+
+
+def test_strided_and_misaligned_rows():
+    """Rows that are slices of one projection, heads in another order, odd offsets."""
+    log("paged strides")
+    for shape in ((4, 2, 128, BF16, 64, True), (4, 2, 40, F32, 16, False), (4, 2, 24, BF16, 16, True)):
+        heads, kv, dh, dtype = shape[:4]
+        a, b = (Run(2, *shape, tokens=200, seed=9) for _ in range(2))
+        T = 90
+        qkv = a.randn(T, heads + 2 * kv, dh).to(DEV)
+        q, k, v = (t.contiguous() for t in qkv.split([heads, kv, kv], 1))
+        cos, sin = (t.to(DEV) for t in rope_tables(torch.arange(T), 10000.0 ** -(torch.arange(0, dh, 2) / dh), dtype))
+        batch = a.batch([80, 10])
+        ref = a.cache.append(k, v, batch, cos=cos, sin=sin, q=q)
+        want = paged_attention(ref, a.cache, batch)
+        views = qkv.split([heads, kv, kv], 1)  # row stride of the whole projection
+        odd = [torch.empty(t.numel() + 1, dtype=dtype, device=DEV)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+        turned = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+        for form in (views, odd, turned):
+            batch = b.batch([80, 10])
+            got = b.cache.append(form[1], form[2], batch, cos=cos[None], sin=sin, q=form[0])
+            assert torch.equal(got, ref)
+            assert torch.equal(paged_attention(got, b.cache, batch), want)
+            assert torch.equal(b.cache.keys.view(torch.uint8), a.cache.keys.view(torch.uint8))
+            assert torch.equal(b.cache.values.view(torch.uint8), a.cache.values.view(torch.uint8))
+
+
+def test_refusals():
+    log("paged refusals")
+    run = Run(2, 4, 2, 64, BF16, 16, True, tokens=64)
+    batch = run.batch([2, 1])
+    k, q = torch.zeros(3, 2, 64, dtype=BF16, device=DEV), torch.zeros(3, 4, 64, dtype=BF16, device=DEV)
+    cos = torch.zeros(3, 64, dtype=BF16, device=DEV)
+    for call, match in (
+            (lambda: run.cache.append(k.float(), k, batch), "bfloat16"),
+            (lambda: run.cache.append(k[:2], k, batch), "k must be"),
+            (lambda: run.cache.append(k, q, batch), "v must be"),
+            (lambda: run.cache.append(k, k.cpu(), batch), "must be on"),
+            (lambda: run.cache.append(k, k, batch, cos=cos), "belong together"),
+            (lambda: run.cache.append(k, k, batch, q=q), "rotated"),
+            (lambda: run.cache.append(k, k, batch, cos=cos[:, :32], sin=cos), "cos/sin"),
+            (lambda: run.cache.retire(batch, run.slots), "kept already"),
+            (lambda: run.cache.retire(run.batch([1, 1], final=False), run.slots[:1]), "counts"),
+            (lambda: run.cache.append(k[:2], k[:2], run.batch([2, 0], final=False)), "window"),
+            (lambda: paged_attention(q[:, :3], run.cache, batch), "heads"),
+            (lambda: paged_attention(q, run.cache, batch, scale=-1.0), "scale"),
+            (lambda: paged_attention(q, run.cache, batch, out=q[:, :, :32]), "out must be"),
+            (lambda: paged_attention(q, run.cache, batch, out=q.float()), "out must be")):
+        with pytest.raises(ValueError, match=match):
+            call()
+
+
+def test_out_rows_behind_the_last_sequence():
+    log("paged out")
+    run = Run(2, 4, 2, 128, BF16, 64, True, tokens=128)
+    q = run.randn(9, 4, 128).to(DEV)
+    k = run.randn(9, 2, 128).to(DEV)
+    batch = run.batch([5, 2], rows=9)
+    run.cache.append(k, k, batch)
+    fresh = paged_attention(q, run.cache, batch)
+    assert not bool(fresh[7:].any())
+    out = torch.full((9, 4, 128), 7.0, dtype=BF16, device=DEV)
+    assert paged_attention(q, run.cache, batch, out=out) is out
+    assert torch.equal(out[:7], fresh[:7]) and bool((out[7:] == 7.0).all())
+
+
+def test_no_rows():
+    log("paged no rows")
+    for shape in ((4, 2, 128, BF16, 64, True), (4, 2, 40, F32, 16, False)):
+        run = Run(2, *shape, tokens=128)
+        run.step([0, 0])
+        run.step([3, 0])
+        run.step([0, 0], pad=2)
+        run.step([0, 0], final=False, keep=[0, 0])
+        empty = PagedBatch(run.table[:0], run.slots[:0], torch.zeros(1, dtype=torch.int32, device=DEV), rows=2)
+        q = run.randn(2, 4, shape[2]).to(DEV)
+        run.cache.append(q[:, :2], q[:, :2], empty)
+        assert not bool(paged_attention(q, run.cache, empty).any())
+        run.check_cache()
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, BF16, 64, True), (4, 2, 64, BF16, 16, False),
+                                   (4, 2, 128, F32, 64, True), (2, 1, 16, F32, 16, False)])
+def test_entries_out_of_range_are_not_followed(shape):
+    """A table entry, slot, length or row range outside its array: the sequences
+    concerned are not written and see nothing of it, the others are as they were."""
+    log(f"paged out of range {shape}")
+    page = shape[4]
+    good = Run(3, *shape, tokens=5 * page, seed=2)
+    for bad in ("page", "length", "negative", "slot", "offsets", "keys"):
+        run = Run(3, *shape, tokens=5 * page, seed=2)
+        counts = [page + 3, page + 3, 5]
+        T = sum(counts)
+        k, v, q = (run.randn(T, n, shape[2]).to(DEV) for n in (2 if shape[1] == 2 else 1,) * 2 + (shape[0],))
+        batch = run.batch(counts)
+        good.lengths = [0] * 3
+        reference = good.batch(counts)
+        good.cache.append(k, v, reference)
+        want = paged_attention(q, good.cache, reference)
+        before = run.cache.keys.clone().view(torch.uint8)
+        if bad == "page":
+            batch.table[1, 0] = 10 ** 6
+            batch.table[1, 1:] = -7
+        elif bad == "length":
+            batch.lengths[1] = 5 * page + 1
+        elif bad == "negative":
+            batch.lengths[1] = -2 ** 31
+        elif bad == "slot" and run.eight_bit:
+            batch.slots[1] = 10 ** 6
+        elif bad == "offsets":
+            batch.offsets[2] = 10 ** 6
+        elif bad == "keys":
+            batch.lengths[1] = 5 * page - 1  # one place, page + 3 rows
+        run.cache.append(k, v, batch)
+        got = paged_attention(q, run.cache, batch)
+        a = page + 3
+        assert torch.equal(got[:a], want[:a]), bad
+        if bad == "offsets":  # the second sequence takes max_rows rows, the third has none
+            assert torch.equal(got[a:2 * a], want[a:2 * a])
+        else:
+            assert torch.equal(got[2 * a:], want[2 * a:]), bad
+        assert bool(got[:2 * a if bad == "offsets" else None].isfinite().all()), bad
+        mine = torch.cat([run.table[0], run.table[2]] + ([run.table[1]] if bad in ("offsets", "keys", "slot") else []))
+        others = [p for p in range(before.shape[0]) if p not in set(mine.tolist())]
+        after = run.cache.keys.view(torch.uint8)
+        assert torch.equal(after[others], before[others]), bad
+        if bad in ("length", "negative"):
+            assert not bool(got[a:2 * a].any())
+
+
+@pytest.mark.parametrize("dtype,eight_bit", [(BF16, True), (BF16, False), (F32, False)])
+def test_offsets_past_32_bits(dtype, eight_bit):
+    """A pool of more than 2^32 values: pages on both sides of the border."""
+    log(f"paged large pool {dtype} {eight_bit}")
+    heads, dh, page = 8, 128, 64
+    pages = 2 ** 32 // (heads * dh * page) + 40
+    cache = PagedCache.allocate(pages, heads, dh, dtype, DEV, page_size=page, eight_bit=eight_bit)
+    table = torch.tensor([[pages - 1, 3, pages - 2, pages - 39, 0]], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(1)
+    k, v, q = ((s * torch.randn(300, n, dh, generator=g)).to(dtype) for n, s in ((heads, 1), (heads, 1), (heads, 2)))
+    batch = PagedBatch(table, torch.zeros(1, dtype=torch.int32, device=DEV),
+                       torch.tensor([0, 300], dtype=torch.int32, device=DEV))
+    cache.append(k.to(DEV), v.to(DEV), batch)
+    out = paged_attention(q.to(DEV), cache, batch).cpu()
+    plain = OracleCache(1, page, eight_bit)
+    plain.k[0], plain.v[0] = list(k), list(v)
+    K, V = plain.tokens(0)
+    rows = [0, 63, 64, 130, 299]
+    ref, mag, size = attend(q[rows], K, V, [r + 1 for r in rows], dh ** -0.5)
+    tol = attention_tolerance(ref, mag, size, 300, dtype, dh)
+    assert bool(((out[rows].double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, BF16, 64, True), (4, 2, 128, F32, 64, False)])
+def test_long_contexts(shape):
+    """A row over many chunks of keys, and beside it short ones."""
+    log(f"paged long {shape}")
+    heads, kv, dh, dtype, page, eight_bit = shape
+    run = Run(3, *shape, tokens=20480)
+    counts = [20011, 70, 1]
+    T = sum(counts)
+    k, v = (run.randn(T, kv, dh) for _ in range(2))
+    run.cache.append(k.to(DEV), v.to(DEV), run.batch(counts))
+    run.lengths = counts
+    r = 0
+    for b, n in enumerate(counts):
+        run.plain.k[b], run.plain.v[b] = list(k[r:r + n]), list(v[r:r + n])
+        r += n
+    run.step([1, 1, 1])
+    run.step([2, 5, 3])
+
+
+def test_scale_and_max_keys():
+    log("paged scale")
+    run = Run(2, 4, 2, 128, BF16, 64, True, tokens=640)
+    run.step([100, 300])
+    batch = run.batch([1, 1], max_keys=301)
+    q, k, v = run.randn(2, 4, 128), run.randn(2, 2, 128), run.randn(2, 2, 128)
+    run.cache.append(k.to(DEV), v.to(DEV), batch)
+    got = paged_attention(q.to(DEV), run.cache, batch, scale=0.5).cpu()
+    for b, n in enumerate((100, 300)):
+        run.plain.k[b].append(k[b])
+        run.plain.v[b].append(v[b])
+        run.compare(got[b:b + 1], q[b:b + 1], *run.plain.tokens(b), [n + 1], scale=0.5)
+
+
+def test_streams():
+    """Two caches stepped on two streams at once: the results of one after the other."""
+    log("paged streams")
+    results = []
+    for concurrent in (False, True):
+        outs, runs = [], [Run(4, 8, 2, 128, BF16, 64, True, tokens=640, seed=s) for s in (1, 2)]
+        streams = [torch.cuda.Stream() for _ in runs] if concurrent else [torch.cuda.current_stream()] * 2
+        data = [[r.randn(4 * 120, n, 128).to(DEV) for n in (8, 2, 2)] for r in runs]
+        batches = [r.batch([120] * 4) for r in runs]
+        torch.cuda.synchronize()
+        for r, d, b, s in zip(runs, data, batches, streams):
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    r.cache.append(d[1], d[2], b)
+                    outs.append(paged_attention(d[0], r.cache, b))
+        torch.cuda.synchronize()
+        results.append([o.cpu() for o in outs])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128, BF16, 64, True), (4, 2, 64, F32, 16, False)])
+def test_captured_step(shape):
+    """A decoding step captured once and replayed while its lengths and rows change:
+    the bits of eager steps, over page borders."""
+    log(f"paged graph {shape}")
+    heads, kv, dh = shape[:3]
+    a, b = (Run(3, *shape, tokens=2000, seed=4) for _ in range(2))
+    for run in (a, b):
+        run.step([100, 1, 62], check=False)
+    lengths = torch.tensor(b.lengths, dtype=torch.int32, device=DEV)
+    one = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV)
+    batch = PagedBatch(b.table, lengths, one, rows=3, max_rows=1, slots=b.slots)
+    q, k, v = (torch.zeros(3, n, dh, dtype=shape[3], device=DEV) for n in (heads, kv, kv))
+    cos, sin = torch.ones(3, dh, dtype=shape[3], device=DEV), torch.zeros(3, dh, dtype=shape[3], device=DEV)
+
+    def step():
+        turned = b.cache.append(k, v, batch, cos=cos, sin=sin, q=q)
+        out = paged_attention(turned, b.cache, batch)
+        lengths.add_(1)
+        return out
+    saved = [t.clone() for t in (b.cache.keys.view(torch.uint8), b.cache.values.view(torch.uint8))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    lengths.copy_(torch.tensor(b.lengths, dtype=torch.int32))  # as before the warm-up step
+    b.cache.keys.view(torch.uint8).copy_(saved[0])
+    b.cache.values.view(torch.uint8).copy_(saved[1])
+    for i in range(5):
+        new = [a.randn(3, n, dh).to(DEV) for n in (heads, kv, kv)]
+        for t, x in zip((q, k, v), new):
+            t.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = a.batch([1, 1, 1])
+        turned = a.cache.append(new[1], new[2], eager, cos=cos, sin=sin, q=new[0])
+        want = paged_attention(turned, a.cache, eager)
+        a.lengths = [n + 1 for n in a.lengths]
+        assert torch.equal(out, want), i
+        torch.randn(1000, device=DEV).sum().item()  # eager work between the replays
+
+
+@pytest.mark.parametrize("dtype,eight_bit", [(BF16, True), (F32, False)])
+def test_many_requests_decoded_together(dtype, eight_bit):
+    """A small attention layer with a readout serving three requests: prompts, then
+    tokens chosen from the readout, the log probabilities of the answers and their
+    sequences' scores, against the same run in 64 bits over plain token lists."""
+    log(f"paged decoding {dtype} {eight_bit}")
+    heads, kv, dh, vocab, B = 4, 2, 64, 300, 3
+    run = Run(B, heads, kv, dh, dtype, 16, eight_bit, tokens=160, seed=8)
+    H = heads * dh
+    embed = run.randn(vocab, H)
+    wqkv = run.randn((heads + 2 * kv) * dh, H, scale=H ** -0.5)
+    head = run.randn(vocab, H, scale=3 * H ** -0.5)
+    inv = 1.0 / 10000.0 ** (torch.arange(0, dh, 2).float() / dh)
+    tokens = [torch.randint(0, vocab, (n,), generator=run.g).tolist() for n in (37, 1, 16)]
+    pending = [list(t) for t in tokens]
+    for step in range(6):
+        counts = [len(p) for p in pending]
+        ids = torch.tensor([t for p in pending for t in p])
+        where = torch.tensor([run.lengths[b] + i for b in range(B) for i in range(counts[b])])
+        x = embed[ids].to(DEV)
+        qkv = (x @ wqkv.to(DEV).T).view(-1, heads + 2 * kv, dh)
+        q, k, v = qkv.split([heads, kv, kv], 1)
+        cos, sin = (t.to(DEV) for t in rope_tables(where, inv, dtype))
+        batch = run.batch(counts)
+        turned = run.cache.append(k, v, batch, cos=cos, sin=sin, q=q)
+        o = paged_attention(turned, run.cache, batch)
+        # the plain run takes the GPU's projections (a product's own rounding is not at stake)
+        qr, kr, vr = rotate(q.cpu(), cos.cpu(), sin.cpu()), rotate(k.cpu(), cos.cpu(), sin.cpu()), v.cpu()
+        r = 0
+        for b, n in enumerate(counts):
+            run.plain.k[b] += list(kr[r:r + n])
+            run.plain.v[b] += list(vr[r:r + n])
+            run.compare(o[r:r + n].cpu(), qr[r:r + n], *run.plain.tokens(b),
+                        [run.lengths[b] + i + 1 for i in range(n)])
+            r += n
+        run.lengths = [a + n for a, n in zip(run.lengths, counts)]
+        last = (torch.tensor(counts).cumsum(0) - 1).to(DEV)
+        logits = (o[last].reshape(B, H) + x[last]) @ head.to(DEV).T
+        best = token_log_probs(logits, torch.full((B,), -100, device=DEV), top=3)
+        chosen = best.top_ids[:, step % 3].contiguous()
+        given = token_log_probs(logits.requires_grad_(), chosen)
+        want = logits.detach().double().log_softmax(-1)
+        assert torch.equal(best.top_ids[:, 0].cpu(), logits.detach().cpu().argmax(-1))
+        torch.testing.assert_close(given.log_prob.detach(), want.gather(1, chosen[:, None])[:, 0].float(),
+                                   rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(given.log_prob.detach(), best.top_log_prob[:, step % 3], rtol=0, atol=0)
+        score = sequence_score_function(torch.ones(B, device=DEV), given.log_prob,
+                                        torch.arange(B, device=DEV), B)
+        grad = torch.autograd.grad(score, logits)[0].double()
+        ref = torch.nn.functional.one_hot(chosen, vocab).double() - want.exp()
+        eps = 2.0 ** -8 if dtype == BF16 else 1e-5
+        torch.testing.assert_close(grad, ref / B, rtol=eps, atol=1e-6)
+        pending = [[int(t)] for t in chosen]
+    run.check_cache()
