@@ -118,17 +118,18 @@ class _TokenLogProbs(torch.autograd.Function):
         dev, code = logits.device, _lib.dtype_code(logits.dtype)
         x = logits.detach()
         x = x if x.stride(1) == 1 and x.stride(0) >= V else x.contiguous()
-        log_prob, entropy, lse = torch.empty(3, R, dtype=torch.float32, device=dev).unbind()
+        log_prob, entropy = (torch.empty(R, dtype=torch.float32, device=dev) for _ in range(2))
+        stats = torch.empty(R, 2, dtype=torch.float32, device=dev)
         top_log_prob = torch.empty(R, top, dtype=torch.float32, device=dev)
         top_ids = torch.empty(R, top, dtype=torch.int64, device=dev)
         need = query("alodlm_token_log_probs_workspace", R, V, top)
         ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
         with torch.cuda.device(dev):
             call("alodlm_token_log_probs", ptr(x), x.stride(0), ptr(targets), R, V, top,
-                 inv_temperature, ignore_index, ptr(log_prob), ptr(entropy), ptr(lse),
+                 inv_temperature, ignore_index, ptr(log_prob), ptr(entropy), ptr(stats),
                  ptr(top_log_prob), ptr(top_ids), ptr(ws), code, _lib.stream_handle(dev))
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, targets, top_ids, lse, entropy)
+            ctx.save_for_backward(logits, targets, top_ids, stats, entropy)
             ctx.args = top, inv_temperature, ignore_index
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
@@ -136,7 +137,7 @@ class _TokenLogProbs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_log_prob, d_entropy, d_top, _d_ids):
-        logits, targets, top_ids, lse, entropy = ctx.saved_tensors
+        logits, targets, top_ids, stats, entropy = ctx.saved_tensors
         top, inv_temperature, ignore_index = ctx.args
         R, V = logits.shape
         x = logits if logits.stride(1) == 1 and logits.stride(0) >= V else logits.contiguous()
@@ -145,7 +146,7 @@ class _TokenLogProbs(torch.autograd.Function):
                  for g in (d_log_prob, d_entropy, d_top)]
         with torch.cuda.device(x.device):
             call("alodlm_token_log_probs_bwd", ptr(x), x.stride(0), ptr(targets), ptr(top_ids),
-                 ptr(lse), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
+                 ptr(stats), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
                  ptr(out), _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
         return out, None, None, None, None
 

@@ -3,182 +3,546 @@
 //
 // Mathematics: with x = logits / T and m = max x, one pass keeps s = sum exp(x - m)
 // and t = sum exp(x - m) (x - m) in float32 (rescaled when m moves), from which
-// lse = m + log s and the entropy is log s - t / s: t is summed relative to the
-// maximum, so nothing large cancels.
+// log p = (x - m) - log s and the entropy is log s - t / s: everything is summed
+// relative to the maximum, so nothing large cancels.
+//
+// Alternatives in the same pass: every thread also knows its own largest logit.  The
+// top-th largest of those, tau, is a lower bound of the top-th largest logit, and only
+// the threads whose largest reaches it hold candidates: their logits are read again
+// (about top / 256 of the row), those >= tau are listed in LDS and ranked by
+// comparison.  Where too many reach tau (rows of equal logits, masked vocabularies),
+// a radix select over the row finds the threshold and the first of its equals.
+//
+// Split: one workgroup per row where there are rows enough, else a row is cut into
+// chunks whose sums and ordered candidates a second launch joins.
 #include "common.h"
 
 #define LP_THREADS 256
+#define LP_WAVES (LP_THREADS / 64)
+#define LP_MAX_TOP 64
+#define LP_LIST 512  // candidates ranked by comparison
+#define LP_LOG2E 1.44269504088896341f
+#define LP_LN2 0.69314718055994531f
 
-// Running (m, s, t) of the logits seen so far.
+// Running maximum of the raw logits and sums in base 2: with y = (logit - m) * c, c =
+// log2 e / T, s = sum 2^y and t = sum 2^y y.
 struct Softmax {
   float m, s, t;
   static __device__ __forceinline__ Softmax none() { return {-INFINITY, 0.f, 0.f}; }
-  // x with a finite or -inf maximum so far; NaN and +inf end up in s.
-  __device__ __forceinline__ void add(float x) {
-    if (x > m) {
-      rescale(x);
-    }
-    const float d = x - (m == -INFINITY ? 0.f : m);
-    const float e = expf(d);
-    s += e;
-    t = fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf does not count
-  }
-  __device__ __forceinline__ void rescale(float to) {
+  __device__ __forceinline__ void rescale(float to, float c) {
     if (m > -INFINITY) {
-      const float d = fmaxf(m - to, -1e30f), f = expf(d);  // 0 * overflow does not count
+      const float d = fmaxf((m - to) * c, -1e30f), f = __builtin_amdgcn_exp2f(d);
       t = f * fmaf(s, d, t);
       s *= f;
     }
     m = to;
   }
-  __device__ __forceinline__ void join(const Softmax& o) {
+  __device__ __forceinline__ void join(const Softmax& o, float c) {
     const float to = fmaxf(m, o.m);
     Softmax b = o;
-    if (to > m) rescale(to);
-    if (to > b.m) b.rescale(to);
+    if (to > m) rescale(to, c);
+    if (to > b.m) b.rescale(to, c);
     s += b.s;
     t += b.t;
   }
+  template <int N>
+  __device__ __forceinline__ void add(const float* x, float c) {
+    float g = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) g = fmaxf(g, x[i]);
+    if (g > m) rescale(g, c);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = (x[i] - base) * c;
+      const float e = __builtin_amdgcn_exp2f(y);
+      s += e;
+      t = fmaf(e, fmaxf(y, -1e30f), t);  // 0 * -inf does not count
+    }
+  }
 };
 
-__device__ __forceinline__ Softmax shfl_xor(const Softmax& x, int off) {
-  Softmax o;
-  o.m = __shfl_xor(x.m, off, 64);
-  o.s = __shfl_xor(x.s, off, 64);
-  o.t = __shfl_xor(x.t, off, 64);
-  return o;
+__device__ __forceinline__ Softmax wave_join(Softmax a, float c) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    Softmax o;
+    o.m = __shfl_xor(a.m, off, 64);
+    o.s = __shfl_xor(a.s, off, 64);
+    o.t = __shfl_xor(a.t, off, 64);
+    a.join(o, c);
+  }
+  return a;
 }
 
+// Unsigned keys in the order of the floats; NaN lowest, both zeros alike.  0 is
+// below every key.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (!(x == x)) return 1u;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k <= 1u) return NAN;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// One whole number per logit: larger ones first, the lower index among equals.
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) {
+  return (uint64_t)key << 32 | (0xffffffffu - index);
+}
+
+// 16 bytes of a row.
+template <typename T> struct Granule;
+template <> struct Granule<bf16_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const bf16_t* p, float* v) { Vec8<bf16_t>::load(p, v); }
+};
+template <> struct Granule<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  }
+};
+
+// A row's elements: up to N - 1 before the first 16-byte boundary, whole granules, and
+// up to N - 1 behind them.
+struct RowParts {
+  int head, granules, tail;  // tail: its first element
+  template <typename T> static __device__ __forceinline__ RowParts of(const T* x, int V) {
+    constexpr int N = Granule<T>::N;
+    const int head = min((int)(-(intptr_t)x & 15) / (int)sizeof(T), V);
+    const int g = (V - head) / N;
+    return {head, g, head + g * N};
+  }
+};
+
+struct TopShared {
+  uint64_t list[LP_LIST];
+  uint64_t sorted[LP_MAX_TOP];
+  uint32_t keys[LP_THREADS];
+  uint32_t hist[256];
+  int members[LP_THREADS];
+  int scan[LP_WAVES];
+  uint32_t threshold, digit;
+  int count, listed, above;
+};
+
+// Rank of every thread's key (larger first, the lower thread among equals) among the
+// workgroup's; the thread of rank top - 1 publishes its key.
+__device__ __forceinline__ void publish_threshold(TopShared& sh, uint32_t key, int top) {
+  sh.keys[threadIdx.x] = key;
+  if (threadIdx.x == 0) sh.count = sh.listed = 0;
+  __syncthreads();
+  int rank = 0;
+  const uint4* k4 = reinterpret_cast<const uint4*>(sh.keys);
+  const int me = threadIdx.x;
+#pragma unroll 4
+  for (int i = 0; i < LP_THREADS / 4; ++i) {
+    const uint4 k = k4[i];
+    rank += (k.x > key || (k.x == key && 4 * i < me)) + (k.y > key || (k.y == key && 4 * i + 1 < me)) +
+            (k.z > key || (k.z == key && 4 * i + 2 < me)) + (k.w > key || (k.w == key && 4 * i + 3 < me));
+  }
+  if (rank == top - 1) sh.threshold = key;
+  __syncthreads();
+}
+
+// The `top` largest of the listed entries, in order, into sh.sorted; 0 where there are
+// fewer.
+__device__ __forceinline__ void rank_list(TopShared& sh, int n, int top) {
+  for (int i = threadIdx.x; i < top; i += LP_THREADS) sh.sorted[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+    const uint64_t e = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.list[j] > e;
+    if (rank < top) sh.sorted[rank] = e;
+  }
+  __syncthreads();
+}
+
+// Radix select of the elements [first, last) of a row: those above the top-th largest
+// key, and the first of its equals, are listed (top of them, fewer if the range has
+// fewer).  Any data, whole passes over the range.
+template <typename T>
+__device__ void select_any(TopShared& sh, const T* x, int first, int last, int top) {
+  const int n = last - first, want = min(top, n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t prefix = 0;
+  int need = want;  // rank of the threshold among the keys with the prefix found so far
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    sh.hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int c = first + threadIdx.x; c < last; c += LP_THREADS) {
+      const uint32_t k = order_key(Elem<T>::load(x, c));
+      if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
+      // the first lane's digit is counted once for all lanes that have it: rows of
+      // equal logits would queue up at one counter
+      const uint32_t digit = (k >> shift) & 255u, first_digit = __builtin_amdgcn_readfirstlane(digit);
+      const uint64_t alike = __ballot(digit == first_digit);
+      if (digit != first_digit) atomicAdd(&sh.hist[digit], 1u);
+      else if ((alike & ((1ull << lane) - 1)) == 0) atomicAdd(&sh.hist[digit], (uint32_t)__popcll(alike));
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int left = need, d = 255;
+      while (d > 0 && (int)sh.hist[d] < left) left -= sh.hist[d--];
+      sh.digit = d;
+      sh.above = left;
+    }
+    __syncthreads();
+    prefix |= sh.digit << shift;
+    need = sh.above;
+    __syncthreads();
+  }
+  // listed: everything above the threshold (fewer than want), then the first `need` equals
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  int equals = 0;
+  for (int base = first; base < last; base += LP_THREADS) {
+    const int c = base + threadIdx.x;
+    const uint32_t k = c < last ? order_key(Elem<T>::load(x, c)) : 0u;
+    if (k > prefix) sh.list[atomicAdd(&sh.listed, 1)] = entry_of(k, c);
+    const uint64_t same = __ballot(k == prefix);
+    if (lane == 0) sh.scan[wave] = __popcll(same);
+    __syncthreads();
+    int before = equals, all = equals;
+    for (int w = 0; w < LP_WAVES; ++w) {
+      if (w < wave) before += sh.scan[w];
+      all += sh.scan[w];
+    }
+    before += __popcll(same & ((1ull << lane) - 1));
+    // places from the end of the list: the ones above the threshold fill its start
+    if (k == prefix && before < need) sh.list[want - 1 - before] = entry_of(k, c);
+    equals = all;
+    __syncthreads();
+  }
+}
+
+// The `top` first of the elements that this workgroup's threads went through, sorted
+// into sh.sorted: granules [g0, g1) (thread j those at g0 + j + 256 i), the row's head
+// and tail where they belong to it (thread j element j, value in `edge`).
+template <typename T>
+__device__ void select_top(TopShared& sh, const T* x, const RowParts& parts, int g0, int g1,
+                           bool has_head, bool has_tail, int V, float largest, int top) {
+  constexpr int N = Granule<T>::N;
+  publish_threshold(sh, order_key(largest), top);
+  const uint32_t tau = sh.threshold;
+  if (order_key(largest) >= tau) sh.members[atomicAdd(&sh.count, 1)] = threadIdx.x;
+  __syncthreads();
+  const int members = sh.count, rounds = (g1 - g0 + LP_THREADS - 1) / LP_THREADS;
+  auto list = [&](float v, int index) {
+    const uint32_t k = order_key(v);
+    if (k < tau) return;
+    const int at = atomicAdd(&sh.listed, 1);
+    if (at < LP_LIST) sh.list[at] = entry_of(k, index);
+  };
+  const int lo = has_head ? 0 : parts.head + g0 * N, hi = has_tail ? V : parts.head + g1 * N;
+  // distinct logits have `top` members; with far more of them tau is a value that the
+  // row is full of, which the list cannot hold
+  const bool few = members <= 2 * top + 64;
+  if (few) {
+    for (int u = threadIdx.x; u < members * rounds; u += LP_THREADS) {
+      const int g = g0 + sh.members[u % members] + u / members * LP_THREADS;
+      if (g >= g1) continue;
+      float v[N];
+      const int c = parts.head + g * N;
+      Granule<T>::load(x + c, v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) list(v[i], c + i);
+    }
+    if (has_head && (int)threadIdx.x < parts.head) list(Elem<T>::load(x, threadIdx.x), threadIdx.x);
+    if (has_tail && parts.tail + (int)threadIdx.x < V)
+      list(Elem<T>::load(x, parts.tail + threadIdx.x), parts.tail + threadIdx.x);
+  }
+  __syncthreads();
+  int n = sh.listed;
+  const int want = min(top, hi - lo);
+  __syncthreads();
+  if (!few || n > LP_LIST || n < want) {  // fewer: NaN, which no thread's largest shows
+    select_any(sh, x, lo, hi, top);
+    n = want;
+  }
+  rank_list(sh, n, top);
+}
+
+struct LogProbArgs {
+  const int64_t* targets;
+  float *log_prob, *entropy, *stats, *top_log_prob;
+  int64_t* top_ids;
+  Softmax* part;      // [rows, chunks]
+  uint64_t* entries;  // [rows, chunks, top]
+  int64_t ld, ignore;
+  int V, top, chunks, chunk_granules;
+  float inv_t;
+};
+
+// A row's results from its sums (every thread) and its ordered entries (LDS).
+template <typename T>
+__device__ void finish_row(const LogProbArgs& a, const T* x, int64_t row, const Softmax& r,
+                           const uint64_t* sorted) {
+  const bool empty = r.m == -INFINITY && r.s == 0.f;
+  const float log_s = logf(r.s);
+  if (threadIdx.x == 0) {
+    const int64_t tg = a.targets[row];
+    float lp = 0.f;
+    if (tg != a.ignore) {
+      const bool known = tg >= 0 && tg < a.V;
+      lp = !known ? NAN : empty ? -INFINITY : (Elem<T>::load(x, tg) - r.m) * a.inv_t - log_s;
+    }
+    a.log_prob[row] = lp;
+    a.entropy[row] = empty ? 0.f : log_s - r.t / r.s * LP_LN2;
+    a.stats[2 * row] = r.m;
+    a.stats[2 * row + 1] = log_s;
+  }
+  for (int k = threadIdx.x; k < a.top; k += LP_THREADS) {
+    const uint64_t e = sorted[k];
+    a.top_ids[row * a.top + k] = 0xffffffffu - (uint32_t)e;
+    a.top_log_prob[row * a.top + k] =
+        empty ? -INFINITY : (key_value((uint32_t)(e >> 32)) - r.m) * a.inv_t - log_s;
+  }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_THREADS)
+token_log_probs_kernel(const T* __restrict__ logits, LogProbArgs a) {
+  constexpr int N = Granule<T>::N, UNROLL = 4;
+  __shared__ __attribute__((aligned(16))) TopShared sh;
+  __shared__ float red[3][LP_WAVES];
+  const int64_t row = blockIdx.x / a.chunks;
+  const int chunk = (int)(blockIdx.x % a.chunks);
+  const T* x = logits + row * a.ld;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const RowParts parts = RowParts::of(x, a.V);
+  const int g0 = min(chunk * a.chunk_granules, parts.granules);
+  const int g1 = chunk == a.chunks - 1 ? parts.granules : min(g0 + a.chunk_granules, parts.granules);
+  const bool has_head = chunk == 0, has_tail = chunk == a.chunks - 1;
+  const float c = a.inv_t * LP_LOG2E;
+  Softmax r = Softmax::none();
+  int g = g0 + threadIdx.x;
+  for (; g + (UNROLL - 1) * LP_THREADS < g1; g += UNROLL * LP_THREADS) {
+    float v[UNROLL][N];
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) Granule<T>::load(x + parts.head + (g + j * LP_THREADS) * N, v[j]);
+    r.add<UNROLL * N>(v[0], c);
+  }
+  for (; g < g1; g += LP_THREADS) {
+    float v[N];
+    Granule<T>::load(x + parts.head + g * N, v);
+    r.add<N>(v, c);
+  }
+  if (has_head && (int)threadIdx.x < parts.head) {
+    const float v = Elem<T>::load(x, threadIdx.x);
+    r.add<1>(&v, c);
+  }
+  if (has_tail && parts.tail + (int)threadIdx.x < a.V) {
+    const float v = Elem<T>::load(x, parts.tail + threadIdx.x);
+    r.add<1>(&v, c);
+  }
+  const float mine = r.m;  // this thread's largest logit
+  r = wave_join(r, c);
+  if (lane == 0) { red[0][wave] = r.m; red[1][wave] = r.s; red[2][wave] = r.t; }
+  __syncthreads();
+  r = {red[0][0], red[1][0], red[2][0]};
+#pragma unroll
+  for (int w = 1; w < LP_WAVES; ++w) r.join({red[0][w], red[1][w], red[2][w]}, c);
+  if constexpr (TOP) select_top(sh, x, parts, g0, g1, has_head, has_tail, a.V, mine, a.top);
+  if (a.chunks == 1) {
+    finish_row(a, x, row, r, sh.sorted);
+    return;
+  }
+  const int64_t at = row * a.chunks + chunk;
+  if (threadIdx.x == 0) a.part[at] = r;
+  if constexpr (TOP)
+    for (int k = threadIdx.x; k < a.top; k += LP_THREADS) a.entries[at * a.top + k] = sh.sorted[k];
+}
+
+// Joins a row's chunks, one workgroup each: sums in chunk order, then the largest of
+// the chunks' entries.
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
-token_log_probs_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ targets,
-                       int64_t V, int top, float inv_t, int64_t ignore, float* __restrict__ log_prob,
-                       float* __restrict__ entropy, float* __restrict__ lse_out,
-                       float* __restrict__ top_log_prob, int64_t* __restrict__ top_ids) {
-  __shared__ Softmax part[LP_THREADS / 64];
-  __shared__ float best_v[LP_THREADS / 64];
-  __shared__ int64_t best_i[LP_THREADS / 64];
+token_log_probs_join_kernel(const T* __restrict__ logits, LogProbArgs a) {
+  __shared__ __attribute__((aligned(16))) TopShared sh;
   const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Softmax a = Softmax::none();
-  for (int64_t c = threadIdx.x; c < V; c += LP_THREADS) a.add(Elem<T>::load(x, c) * inv_t);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) a.join(shfl_xor(a, off));
-  if (lane == 0) part[wave] = a;
-  __syncthreads();
-  a = part[0];
-  for (int w = 1; w < LP_THREADS / 64; ++w) a.join(part[w]);
-  const bool empty = a.m == -INFINITY && a.s == 0.f;
-  const float lse = empty ? -INFINITY : a.m + logf(a.s);
-  if (threadIdx.x == 0) {
-    const int64_t tg = targets[row];
-    float lp = 0.f;
-    if (tg != ignore) {
-      lp = tg >= 0 && tg < V ? Elem<T>::load(x, tg) * inv_t : NAN;
-      lp = empty && tg >= 0 && tg < V ? -INFINITY : lp - lse;
-    }
-    log_prob[row] = lp;
-    entropy[row] = empty ? 0.f : logf(a.s) - a.t / a.s;
-    lse_out[row] = lse;
-  }
-  // alternatives: the largest behind the one found last, in (value, index) order
-  float last_v = INFINITY;
-  int64_t last_i = -1;
-  for (int k = 0; k < top; ++k) {
-    float bv = -INFINITY;
-    int64_t bi = V;
-    for (int64_t c = threadIdx.x; c < V; c += LP_THREADS) {
-      float v = Elem<T>::load(x, c);
-      if (!(v == v)) v = -INFINITY;  // NaN ranks lowest
-      if (v > last_v || (v == last_v && c <= last_i)) continue;
-      if (v > bv || (v == bv && c < bi)) { bv = v; bi = c; }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const float ov = __shfl_xor(bv, off, 64);
-      const int64_t oi = __shfl_xor((long long)bi, off, 64);
-      if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+  const float c = a.inv_t * LP_LOG2E;
+  const int lane = threadIdx.x & 63;
+  // every wave sums the same way
+  Softmax r = Softmax::none();
+  for (int k = lane; k < a.chunks; k += 64) r.join(a.part[row * a.chunks + k], c);
+  r = wave_join(r, c);
+  if (a.top) {
+    // a chunk's entries are in order: its first bounds the rest
+    const uint64_t* e = a.entries + row * a.chunks * a.top;
+    const int n = a.chunks * a.top;
+    uint64_t best = 0;
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) best = max(best, e[i]);
+    publish_threshold(sh, (uint32_t)(best >> 32), a.top);
+    const uint32_t tau = sh.threshold;
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+      const uint64_t v = e[i];
+      if (v == 0 || (uint32_t)(v >> 32) < tau) continue;
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < LP_LIST) sh.list[at] = v;
     }
     __syncthreads();
-    if (lane == 0) { best_v[wave] = bv; best_i[wave] = bi; }
+    const int listed = sh.listed;
     __syncthreads();
-    for (int w = 0; w < LP_THREADS / 64; ++w)
-      if (w == 0 || best_v[w] > bv || (best_v[w] == bv && best_i[w] < bi)) { bv = best_v[w]; bi = best_i[w]; }
-    last_v = bv;
-    last_i = bi;
-    if (threadIdx.x == 0) {
-      top_ids[row * top + k] = bi;
-      top_log_prob[row * top + k] = empty ? -INFINITY : Elem<T>::load(x, bi) * inv_t - lse;
+    if (listed <= LP_LIST) {
+      rank_list(sh, listed, a.top);
+    } else {  // many equals: each next one is the largest below the one before
+      uint64_t last = ~0ull;
+      for (int k = 0; k < a.top; ++k) {
+        uint64_t m = 0;
+        for (int i = threadIdx.x; i < n; i += LP_THREADS)
+          if (e[i] < last) m = max(m, e[i]);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) m = max(m, (uint64_t)__shfl_xor((unsigned long long)m, off, 64));
+        __syncthreads();
+        if (lane == 0) sh.list[threadIdx.x >> 6] = m;
+        __syncthreads();
+        for (int w = 0; w < LP_WAVES; ++w) m = max(m, sh.list[w]);
+        if (threadIdx.x == 0) sh.sorted[k] = m;
+        last = m;
+      }
+      __syncthreads();
     }
   }
+  finish_row(a, logits + row * a.ld, row, r, sh.sorted);
 }
 
 // dlogits = (g_target [c = target] + sum_k g_k [c = top_k] - p (g_target + sum_k g_k)
-//            - g_entropy p (log p + entropy)) / T
+//            - g_entropy p (log p + entropy)) / T,  log p = (x - m) - log s.
+// A stream: each logit read once and each gradient written once, 16 bytes a thread.  The
+// few elements with a term of their own are written again behind a barrier.
+struct LogProbGrad {
+  const int64_t *targets, *top_ids;
+  const float *stats, *entropy, *d_log_prob, *d_entropy, *d_top;
+  int64_t ld, ignore;
+  int V, top, chunks;
+  float inv_t;
+};
+
+#define LP_BWD_GRANULES (LP_THREADS * 4)
+
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
-token_log_probs_bwd_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ targets,
-                           const int64_t* __restrict__ top_ids, const float* __restrict__ lse_in,
-                           const float* __restrict__ entropy, const float* __restrict__ d_log_prob,
-                           const float* __restrict__ d_entropy, const float* __restrict__ d_top,
-                           int64_t V, int top, float inv_t, int64_t ignore, T* __restrict__ dlogits) {
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  const float lse = lse_in[row];
-  const int64_t tg = targets[row];
-  const float gt = d_log_prob && tg != ignore ? d_log_prob[row] : 0.f;
-  const float gh = d_entropy ? d_entropy[row] : 0.f, H = entropy[row];
+token_log_probs_bwd_kernel(const T* __restrict__ logits, LogProbGrad a, T* __restrict__ dlogits) {
+  constexpr int N = Granule<T>::N;
+  const int64_t row = blockIdx.x / a.chunks;
+  const int chunk = (int)(blockIdx.x % a.chunks);
+  const T* x = logits + row * a.ld;
+  T* out = dlogits + row * (int64_t)a.V;
+  const float m = a.stats[2 * row], log_s = a.stats[2 * row + 1];
+  const bool empty = m == -INFINITY && log_s == -INFINITY;
+  const int64_t tg = a.targets[row];
+  const float gt = a.d_log_prob && tg != a.ignore ? a.d_log_prob[row] : 0.f;
+  const float gh = a.d_entropy ? a.d_entropy[row] : 0.f;
   float all = gt;
-  if (d_top)
-    for (int k = 0; k < top; ++k) all += d_top[row * top + k];
-  for (int64_t c = threadIdx.x; c < V; c += LP_THREADS) {
-    const float lp = Elem<T>::load(x, c) * inv_t - lse;
-    float g = 0.f;
-    if (lse != -INFINITY) {
-      const float p = expf(lp);
-      g = -p * fmaf(gh, fmaxf(lp, -1e30f) + H, all);
-      if (c == tg) g += gt;
-      if (d_top)
-        for (int k = 0; k < top; ++k)
-          if (top_ids[row * top + k] == c) g += d_top[row * top + k];
-    }
-    Elem<T>::store(dlogits + row * V, c, g * inv_t);
+  if (a.d_top)
+    for (int k = 0; k < a.top; ++k) all += a.d_top[row * a.top + k];
+  const float flat = fmaf(gh, a.entropy[row], all);
+  const float base = empty ? 0.f : m;
+  auto gradient = [&](float v) {  // without the elements' own terms
+    const float lp = (v - base) * a.inv_t - log_s;
+    const float p = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
+    return -p * fmaf(gh, fmaxf(lp, -1e4f), flat) * a.inv_t;  // p is 0 long before -1e4
+  };
+  // parts by the gradient's alignment; logits that lie otherwise are read one by one
+  const RowParts parts = RowParts::of(out, a.V);
+  const bool together = ((uintptr_t)(x + parts.head) & 15) == 0;
+  const int g0 = chunk * LP_BWD_GRANULES, g1 = min(g0 + LP_BWD_GRANULES, parts.granules);
+#pragma unroll 2
+  for (int g = g0 + threadIdx.x; g < g1; g += LP_THREADS) {
+    const int at = parts.head + g * N;
+    float v[N];
+    if (together) Granule<T>::load(x + at, v);
+    else
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = Elem<T>::load(x, at + i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = empty ? 0.f : gradient(v[i]);
+    if constexpr (N == 8) Vec8<T>::store_nt(out + at, v);
+    else __builtin_nontemporal_store(nt_f32x4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<nt_f32x4_t*>(out + at));
+  }
+  const bool last = chunk == a.chunks - 1;
+  auto single = [&](int at) { Elem<T>::store(out, at, empty ? 0.f : gradient(Elem<T>::load(x, at))); };
+  if (chunk == 0 && (int)threadIdx.x < parts.head) single(threadIdx.x);
+  if (last && parts.tail + (int)threadIdx.x < a.V) single(parts.tail + threadIdx.x);
+  if (empty) return;
+  __syncthreads();
+  const int lo = chunk == 0 ? 0 : parts.head + g0 * N, hi = last ? a.V : parts.head + g1 * N;
+  const int n = a.d_top ? a.top : 0;
+  for (int k = threadIdx.x; k <= n; k += LP_THREADS) {
+    const int64_t at = k < n ? a.top_ids[row * a.top + k] : tg;
+    if (at < lo || at >= hi || (k == n && gt == 0.f)) continue;
+    float own = at == tg ? gt : 0.f;
+    bool listed = false;
+    for (int j = 0; j < n; ++j)
+      if (a.top_ids[row * a.top + j] == at) {
+        own += a.d_top[row * a.top + j];
+        listed = true;
+      }
+    if (k == n && listed) continue;  // the alternative's thread writes it
+    Elem<T>::store(out, at, fmaf(own, a.inv_t, gradient(Elem<T>::load(x, at))));
   }
 }
 
+// ----------------------------------------------------------------------------
+// Host
+// ----------------------------------------------------------------------------
 static int check_shape(int64_t rows, int64_t vocab, int64_t top, int64_t ld, float inv_t) {
-  ALODLM_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "token_log_probs: rows out of range");
-  ALODLM_CHECK_ARG(vocab >= 1 && vocab < (1ll << 31) && ld >= vocab,
+  ALODLM_CHECK_ARG(rows >= 0 && rows < (1ll << 24), "token_log_probs: rows out of range");
+  ALODLM_CHECK_ARG(vocab >= 1 && vocab < (1ll << 30) && ld >= vocab,
                    "token_log_probs: vocabulary or row stride out of range");
-  ALODLM_CHECK_ARG(top >= 0 && top <= 64 && top <= vocab,
+  ALODLM_CHECK_ARG(top >= 0 && top <= LP_MAX_TOP && top <= vocab,
                    "token_log_probs: top must be 0 to 64 and at most the vocabulary");
   ALODLM_CHECK_ARG(inv_t > 0.f && inv_t < INFINITY, "token_log_probs: the temperature must be positive");
   return ALODLM_OK;
 }
 
-extern "C" int64_t alodlm_token_log_probs_workspace(int64_t, int64_t, int64_t) { return 0; }
+// Chunks of a row: one where the rows alone give every compute unit two workgroups,
+// else as many as do, of 2048 elements at least.
+static int64_t row_chunks(int64_t rows, int64_t vocab) {
+  if (rows >= 512 || rows == 0) return 1;
+  const int64_t want = (512 + rows - 1) / rows, most = max(vocab / 2048, (int64_t)1);
+  return min(min(want, most), (int64_t)128);
+}
+
+extern "C" int64_t alodlm_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top) {
+  const int64_t chunks = row_chunks(rows, vocab);
+  // 8-byte entries first, then three floats a chunk
+  return chunks == 1 ? 0 : rows * chunks * (2 * top + 3);
+}
 
 extern "C" int alodlm_token_log_probs(const void* logits, int64_t ld, const int64_t* targets,
                                       int64_t rows, int64_t vocab, int64_t top,
                                       float inv_temperature, int64_t ignore, float* log_prob,
-                                      float* entropy, float* lse, float* top_log_prob,
+                                      float* entropy, float* stats, float* top_log_prob,
                                       int64_t* top_ids, float* workspace, int dtype, void* stream) {
   const int rc = check_shape(rows, vocab, top, ld, inv_temperature);
   if (rc) return rc;
   if (rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(top == 0 || (top_log_prob && top_ids), "token_log_probs: no room for the alternatives");
+  const int64_t chunks = row_chunks(rows, vocab);
+  ALODLM_CHECK_ARG(chunks == 1 || workspace, "token_log_probs: no workspace");
+  ALODLM_CHECK_ARG(chunks == 1 || (uintptr_t)workspace % 8 == 0, "token_log_probs: workspace not 8-byte aligned");
+  const hipStream_t st = as_stream(stream);
   ALODLM_DISPATCH(dtype, T, {
-    token_log_probs_kernel<T><<<(unsigned)rows, LP_THREADS, 0, as_stream(stream)>>>(
-        (const T*)logits, ld, targets, vocab, (int)top, inv_temperature, ignore, log_prob, entropy,
-        lse, top_log_prob, top_ids);
+    const int64_t granules = (vocab * (int64_t)sizeof(T) + 15) / 16;
+    LogProbArgs a = {targets, log_prob, entropy, stats, top_log_prob, top_ids, nullptr,
+                     reinterpret_cast<uint64_t*>(workspace), ld, ignore, (int)vocab, (int)top,
+                     (int)chunks, (int)((granules + chunks - 1) / chunks), inv_temperature};
+    if (chunks > 1) a.part = reinterpret_cast<Softmax*>(workspace + 2 * rows * chunks * top);
+    const unsigned grid = (unsigned)(rows * chunks);
+    if (top) token_log_probs_kernel<T, true><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
+    else token_log_probs_kernel<T, false><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
+    if (chunks > 1) token_log_probs_join_kernel<T><<<(unsigned)rows, LP_THREADS, 0, st>>>((const T*)logits, a);
   });
   ALODLM_CHECK_LAUNCH("token_log_probs");
   return ALODLM_OK;
 }
 
 extern "C" int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targets,
-                                          const int64_t* top_ids, const float* lse,
+                                          const int64_t* top_ids, const float* stats,
                                           const float* entropy, const float* d_log_prob,
                                           const float* d_entropy, const float* d_top, int64_t rows,
                                           int64_t vocab, int64_t top, float inv_temperature,
@@ -188,9 +552,13 @@ extern "C" int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const 
   if (rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(!d_top || top == 0 || top_ids, "token_log_probs_bwd: no alternatives");
   ALODLM_DISPATCH(dtype, T, {
-    token_log_probs_bwd_kernel<T><<<(unsigned)rows, LP_THREADS, 0, as_stream(stream)>>>(
-        (const T*)logits, ld, targets, top_ids, lse, entropy, d_log_prob, d_entropy, d_top, vocab,
-        (int)top, inv_temperature, ignore, (T*)dlogits);
+    const int64_t granules = (vocab * (int64_t)sizeof(T) + 15) / 16;
+    const int64_t chunks = (granules + LP_BWD_GRANULES - 1) / LP_BWD_GRANULES;
+    ALODLM_CHECK_ARG(rows * chunks < (1ll << 31), "token_log_probs_bwd: too many rows in one call");
+    const LogProbGrad a = {targets, top_ids, stats, entropy, d_log_prob, d_entropy, d_top, ld, ignore,
+                           (int)vocab, (int)top, (int)chunks, inv_temperature};
+    token_log_probs_bwd_kernel<T><<<(unsigned)(rows * chunks), LP_THREADS, 0, as_stream(stream)>>>(
+        (const T*)logits, a, (T*)dlogits);
   });
   ALODLM_CHECK_LAUNCH("token_log_probs_bwd");
   return ALODLM_OK;

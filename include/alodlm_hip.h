@@ -748,18 +748,20 @@ int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_b
  *   entropy[r]  = -sum p log p
  *   top_ids / top_log_prob [rows, top]: the `top` largest logits in order, the
  *                 lower index first among equal ones
- * and lse[r], which the backward takes.  A logit of -inf has probability zero; a
- * row of nothing else has log_prob -inf, entropy 0 and zero gradient.
+ * and stats [rows, 2], the largest logit and log sum exp(x - max x), which the
+ * backward takes.  A logit of -inf has probability zero; a row of nothing else has
+ * log_prob -inf, entropy 0 and zero gradient.  The workspace (floats; none for many
+ * rows) is 8-byte aligned.
  * The backward writes dlogits [rows, vocab] for the upstream gradients d_log_prob,
  * d_entropy [rows] and d_top [rows, top] (each may be NULL).
  * ------------------------------------------------------------------------ */
 int64_t alodlm_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top);
 int alodlm_token_log_probs(const void* logits, int64_t ld, const int64_t* targets, int64_t rows,
                            int64_t vocab, int64_t top, float inv_temperature, int64_t ignore,
-                           float* log_prob, float* entropy, float* lse, float* top_log_prob,
+                           float* log_prob, float* entropy, float* stats, float* top_log_prob,
                            int64_t* top_ids, float* workspace, int dtype, void* stream);
 int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* targets,
-                               const int64_t* top_ids, const float* lse, const float* entropy,
+                               const int64_t* top_ids, const float* stats, const float* entropy,
                                const float* d_log_prob, const float* d_entropy, const float* d_top,
                                int64_t rows, int64_t vocab, int64_t top, float inv_temperature,
                                int64_t ignore, void* dlogits, int dtype, void* stream);

@@ -163,6 +163,11 @@ def test_nan_inf_and_bad_targets(dtype):
     for r in (0, 3, 7):
         assert all(torch.equal(a[r], b[r]) for a, b in zip(out, clean))
     assert bool(((out.top_ids >= 0) & (out.top_ids < 5000)).all())
+    logits[1, :] = math.nan  # ids still name tokens, each once
+    logits[2, 5:] = math.nan
+    ids = token_log_probs(logits, targets, top=9).top_ids
+    assert bool(((ids >= 0) & (ids < 5000)).all())
+    assert all(len(set(row)) == 9 for row in ids.tolist())
     x = logits.clone().requires_grad_()
     out = token_log_probs(x, targets)
     grad = torch.autograd.grad(out.log_prob.nan_to_num().sum() + out.entropy.nan_to_num().sum(), x)[0]
