@@ -61,6 +61,52 @@ __device__ __forceinline__ int64_t open_page(const PagedCache& c, int slot, int 
 // 2^e as a float, e in [-126, 127].
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// ----------------------------------------------------------------------------
+// Attention (csrc/paged_attention.hip and its matrix-core kernels)
+// ----------------------------------------------------------------------------
+struct AttendArgs {
+  const void* q;
+  void* out;
+  int64_t ldq;
+  float* part;   // unnormalised outputs [chunks][rows * heads][head_dim]
+  float2* stat;  // (maximum in base 2, sum) [chunks][rows * heads]
+  int heads, group, chunk_keys, chunks;
+  float scale2;  // softmax scale * log2 e
+  int zero_rest;
+};
+
+// Where the 8-bit pages of a sequence end (keys before it are sealed).
+__device__ __forceinline__ int sealed_keys(const PagedBatch& bt, int held, int end, int page,
+                                           bool eight) {
+  if (!eight) return end;
+  return (bt.final_rows ? end : held) / page * page;
+}
+
+// The first key whose place in the open pages another one has taken (windows longer
+// than the open pages are refused by the host; this bounds what is read).
+__device__ __forceinline__ int open_end(const PagedCache& c, int sealed, int end) {
+  return (int)min((int64_t)end, (int64_t)sealed + (int64_t)c.open_pages * c.page);
+}
+
+// Rows of sequence b that results are written for: those of the batch, up to max_rows,
+// whether or not the sequence takes part.
+__device__ __forceinline__ int given_rows(const PagedBatch& bt, int b) {
+  const int r0 = bt.first_row(b);
+  return min(min(max(bt.offsets[b + 1], r0), bt.rows) - r0, bt.max_rows);
+}
+
+// How a call is cut up.
+struct AttendPlan {
+  int64_t chunk_keys, chunks;
+  int column_tiles, query_tiles;  // matrix-core kernels: 16-column tiles a wave, tiles a sequence
+};
+
+// bf16 with head_dim 64 or 128 (csrc/paged_split.hip): the keys of a chunk over the
+// waves of a workgroup.
+bool paged_split_takes(const alodlm_paged_cache* c);
+void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
+                        const AttendPlan& p, hipStream_t st);
+
 // Host: checks of the two structs shared by the entry points (abi errors), and
 // their device forms.
 int paged_check(const alodlm_paged_cache* c, const alodlm_paged_batch* b);

@@ -14,30 +14,6 @@
 #define ROWS_WAVES 4
 #define LOG2E 1.44269504088896341f
 
-struct AttendArgs {
-  const void* q;
-  void* out;
-  int64_t ldq;
-  float* part;  // partial outputs [chunks][rows * heads][head_dim]
-  float2* stat;  // (m, sum) [chunks][rows * heads]
-  int heads, group, chunk_keys, chunks;
-  float scale2;  // softmax scale * log2 e
-  int zero_rest;
-};
-
-// Where the 8-bit pages of a sequence end (keys before it are sealed).
-__device__ __forceinline__ int sealed_keys(const PagedBatch& bt, int held, int end, int page,
-                                           bool eight) {
-  if (!eight) return end;
-  return (bt.final_rows ? end : held) / page * page;
-}
-
-// The first key whose place in the open pages another one has taken (windows longer
-// than the open pages are refused by the host; this bounds what is read).
-__device__ __forceinline__ int open_end(const PagedCache& c, int sealed, int end) {
-  return (int)min((int64_t)end, (int64_t)sealed + (int64_t)c.open_pages * c.page);
-}
-
 // Four e4m3 codes as floats.
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, float* v) {
   v[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
@@ -126,8 +102,7 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     held = bt.held(b, page);
     const int n = held < 0 ? 0 : bt.row_count(b, held, page);
     row = (int64_t)bt.first_row(b) + i;
-    const int64_t given = (int64_t)min(max(bt.offsets[b + 1], 0), bt.rows) - bt.first_row(b);
-    live = i < min(given, (int64_t)bt.max_rows);
+    live = i < given_rows(bt, b);
     if (i < n) {
       const int end = held + n;
       sealed = sealed_keys(bt, held, end, page, EIGHT);
@@ -213,19 +188,18 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   for (int j = 0, d = lane; d < dh; ++j, d += 64) a.part[(chunk * T_heads + at) * dh + d] = o[j];
 }
 
-// Joins the chunks of every row and head, one wavefront each, in chunk order.
+// Joins the chunks of a row and head, one workgroup each: its waves take the chunks in
+// turn, and their sums are added in wave order.
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
-  const int lane = threadIdx.x & 63, dh = c.head_dim, page = c.page;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t T_heads = (int64_t)bt.rows * a.heads;
-  if (unit >= (int64_t)bt.sequences * bt.max_rows * a.heads) return;
+  __shared__ float sum_of[4], o_of[4][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dh = c.head_dim, page = c.page;
+  const int64_t unit = blockIdx.x, T_heads = (int64_t)bt.rows * a.heads;
   const int head = (int)(unit % a.heads);
   const int i = (int)(unit / a.heads % bt.max_rows);
   const int b = (int)(unit / a.heads / bt.max_rows);
-  const int64_t r0 = bt.first_row(b);
-  if (i >= min((int64_t)min(max(bt.offsets[b + 1], 0), bt.rows) - r0, (int64_t)bt.max_rows)) return;
+  if (i >= given_rows(bt, b)) return;
   const int held = bt.held(b, page);
   const int n = held < 0 ? 0 : bt.row_count(b, held, page);
   int limit = 0;
@@ -234,22 +208,30 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     limit = min(held + i + 1, EIGHT ? open_end(c, sealed, end) : end);
   }
   const int count = max((limit + a.chunk_keys - 1) / a.chunk_keys, 1);
-  const int64_t at = (r0 + i) * a.heads + head;
+  const int64_t at = ((int64_t)bt.first_row(b) + i) * a.heads + head;
   float M = -INFINITY;
   for (int k = lane; k < count; k += 64) M = fmaxf(M, a.stat[k * T_heads + at].x);
   M = wave_max(M);
   const float base = M == -INFINITY ? 0.f : M;
   float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < count; ++k) {
+#pragma unroll 4
+  for (int k = wave; k < count; k += 4) {
     const float2 st = a.stat[k * T_heads + at];
     const float f = exp2f(st.x - base);
     sum = fmaf(st.y, f, sum);
-    for (int j = 0, d = lane; d < dh; ++j, d += 64)
-      o[j] = fmaf(a.part[(k * T_heads + at) * dh + d], f, o[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 64 * j < dh) o[j] = fmaf(a.part[(k * T_heads + at) * dh + lane + 64 * j], f, o[j]);
   }
+  if (lane == 0) sum_of[wave] = sum;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o_of[wave][lane + 64 * j] = o[j];
+  __syncthreads();
+  sum = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int j = 0, d = lane; d < dh; ++j, d += 64)
-    Elem<T>::store((T*)a.out + at * dh, d, o[j] * inv);
+  const int d = threadIdx.x;
+  if (d < dh)
+    Elem<T>::store((T*)a.out + at * dh, d, ((o_of[0][d] + o_of[1][d]) + (o_of[2][d] + o_of[3][d])) * inv);
 }
 
 // Zeros in the rows behind the last sequence.
@@ -264,45 +246,54 @@ __global__ void __launch_bounds__(256) paged_zero_rest_kernel(PagedBatch bt, T* 
 // ----------------------------------------------------------------------------
 // Host
 // ----------------------------------------------------------------------------
-struct AttendPlan {
-  int64_t chunk_keys, chunks;
-};
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Keys per chunk: as many chunks as give every compute unit several workgroups, of
-// 256 keys at least.
-static AttendPlan attend_plan(const alodlm_paged_batch* b, int64_t heads) {
-  const int64_t units = b->sequences * b->max_rows * heads;  // wavefronts per chunk
-  const int64_t want = units > 0 ? (8192 + units - 1) / units : 1;
-  const int64_t most = max((b->max_keys + 255) / 256, (int64_t)1);
-  const int64_t chunks = min(max(want, (int64_t)1), most);
-  int64_t keys = (b->max_keys + chunks - 1) / chunks;
-  keys = max((keys + 63) / 64 * 64, (int64_t)64);
-  return {keys, max((b->max_keys + keys - 1) / keys, (int64_t)1)};
+// Keys per chunk, in whole 64-key tiles: `want` workgroups or wavefronts in all where
+// `units` take a chunk each, but no chunk below `least` keys.
+static void cut_keys(AttendPlan& p, int64_t max_keys, int64_t units, int64_t want, int64_t least) {
+  const int64_t most = max(ceil_div(max_keys, least), (int64_t)1);
+  const int64_t chunks = min(units > 0 ? ceil_div(want, units) : 1, most);
+  p.chunk_keys = max(ceil_div(ceil_div(max_keys, chunks), 64) * 64, (int64_t)64);
+  p.chunks = max(ceil_div(max_keys, p.chunk_keys), (int64_t)1);
+}
+
+static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
+  AttendPlan p = {};
+  if (paged_split_takes(c)) {
+    const int64_t columns = b->max_rows * (heads / c->kv_heads);
+    p.column_tiles = columns <= 16 ? 1 : 2;
+    p.query_tiles = (int)ceil_div(max(columns, (int64_t)1), 16 * p.column_tiles);
+    cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, 4096, 512);
+  } else {
+    cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, 256);
+  }
+  return p;
 }
 
 static int64_t attend_floats(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
-  const AttendPlan p = attend_plan(b, heads);
+  const AttendPlan p = attend_plan(c, b, heads);
   return p.chunks == 1 ? 0 : p.chunks * b->rows * heads * (c->head_dim + 2);
 }
 
 extern "C" int64_t alodlm_paged_attention_workspace(const alodlm_paged_cache* cache,
                                                     const alodlm_paged_batch* batch, int64_t heads) {
-  if (paged_check(cache, batch) || heads < 1) return 0;
+  if (paged_check(cache, batch) || heads < 1 || heads % cache->kv_heads) return 0;
   return attend_floats(cache, batch, heads);
 }
 
 template <typename T, bool EIGHT>
 static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, AttendArgs a,
-                         hipStream_t st) {
+                         const AttendPlan& plan, hipStream_t st) {
   const PagedCache dc = paged_cache(c);
   const PagedBatch db = paged_batch(b);
   const int64_t units = b->sequences * b->max_rows * a.heads;
   if (units > 0) {
-    const int64_t blocks = (units * a.chunks + ROWS_WAVES - 1) / ROWS_WAVES;
-    ALODLM_CHECK_ARG(blocks < (1ll << 31), "paged_attention: too many rows in one call");
-    paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
-    if (a.chunks > 1)
-      paged_join_kernel<T, EIGHT><<<ceil_div_u(units, 4), 256, 0, st>>>(dc, db, a);
+    const int64_t blocks = plan.query_tiles ? b->sequences * c->kv_heads * plan.query_tiles * a.chunks
+                                            : ceil_div(units * a.chunks, ROWS_WAVES);
+    ALODLM_CHECK_ARG(blocks < (1ll << 31) && units < (1ll << 31), "paged_attention: too many rows in one call");
+    if (plan.query_tiles) paged_split_launch(c, b, a, plan, st);
+    else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
+    if (a.chunks > 1) paged_join_kernel<T, EIGHT><<<(unsigned)units, 256, 0, st>>>(dc, db, a);
   }
   if (a.zero_rest && b->rows > 0)
     paged_zero_rest_kernel<T><<<256, 256, 0, st>>>(db, (T*)a.out, a.heads * c->head_dim);
@@ -325,13 +316,13 @@ extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alo
                    "paged_attention: rows must be 16-byte aligned");
   if (batch->rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(q && out, "paged_attention: no rows");
-  const AttendPlan plan = attend_plan(batch, heads);
+  const AttendPlan plan = attend_plan(cache, batch, heads);
   ALODLM_CHECK_ARG(plan.chunks == 1 || workspace, "paged_attention: no workspace");
   AttendArgs a = {q, out, ldq, workspace, nullptr, (int)heads, (int)(heads / cache->kv_heads),
                   (int)plan.chunk_keys, (int)plan.chunks, scale * LOG2E, zero_rest};
   a.stat = reinterpret_cast<float2*>(workspace + plan.chunks * batch->rows * heads * cache->head_dim);
   ALODLM_DISPATCH(cache->dtype, T, {
-    if (cache->eight_bit) return attend_launch<T, true>(cache, batch, a, as_stream(stream));
-    return attend_launch<T, false>(cache, batch, a, as_stream(stream));
+    if (cache->eight_bit) return attend_launch<T, true>(cache, batch, a, plan, as_stream(stream));
+    return attend_launch<T, false>(cache, batch, a, plan, as_stream(stream));
   });
 }
