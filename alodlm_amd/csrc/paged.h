@@ -72,8 +72,17 @@ struct AttendArgs {
   float2* stat;  // (maximum in base 2, sum) [chunks][rows * heads]
   int heads, group, chunk_keys, chunks;
   float scale2;  // softmax scale * log2 e
-  int zero_rest;
+  int zero_blocks;  // workgroups behind the launch's others that clear the rows behind the last sequence
 };
+
+// Zeros in the rows behind the last sequence, by `blocks` workgroups of 256 threads.
+template <typename T>
+__device__ __forceinline__ void zero_rest(const PagedBatch& bt, T* out, int64_t width, int block, int blocks) {
+  const int64_t from = (int64_t)min(max(bt.offsets[bt.sequences], 0), bt.rows) * width;
+  const int64_t to = (int64_t)bt.rows * width;
+  for (int64_t i = from + (int64_t)block * 256 + threadIdx.x; i < to; i += (int64_t)blocks * 256)
+    Elem<T>::store(out, i, 0.f);
+}
 
 // Where the 8-bit pages of a sequence end (keys before it are sealed).
 __device__ __forceinline__ int sealed_keys(const PagedBatch& bt, int held, int end, int page,
@@ -105,7 +114,7 @@ struct AttendPlan {
 // waves of a workgroup.
 bool paged_split_takes(const alodlm_paged_cache* c);
 void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
-                        const AttendPlan& p, hipStream_t st);
+                        const AttendPlan& p, unsigned blocks, hipStream_t st);
 
 // Host: checks of the two structs shared by the entry points (abi errors), and
 // their device forms.

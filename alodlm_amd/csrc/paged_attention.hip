@@ -87,6 +87,10 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int dh = c.head_dim, page = c.page;
   const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  if (blockIdx.x >= gridDim.x - a.zero_blocks) {
+    zero_rest(bt, (T*)a.out, (int64_t)a.heads * dh, gridDim.x - 1 - blockIdx.x, a.zero_blocks);
+    return;
+  }
   // unit: (chunk, sequence row, query head), heads of a row side by side
   const int64_t unit = (int64_t)blockIdx.x * ROWS_WAVES + wave;
   const int64_t per_chunk = (int64_t)bt.sequences * bt.max_rows * a.heads;
@@ -188,13 +192,14 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   for (int j = 0, d = lane; d < dh; ++j, d += 64) a.part[(chunk * T_heads + at) * dh + d] = o[j];
 }
 
-// Joins the chunks of a row and head, one workgroup each: its waves take the chunks in
-// turn, and their sums are added in wave order.
+// Joins the chunks of a row and head, one workgroup each.  Four dimensions a thread;
+// as many chunks at once as that leaves threads for, added in a fixed order.
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
-  __shared__ float sum_of[4], o_of[4][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dh = c.head_dim, page = c.page;
+  __shared__ __attribute__((aligned(16))) float4 o_of[256];
+  __shared__ float sum_of[256];
+  const int lane = threadIdx.x & 63, dh = c.head_dim, page = c.page;
   const int64_t unit = blockIdx.x, T_heads = (int64_t)bt.rows * a.heads;
   const int head = (int)(unit % a.heads);
   const int i = (int)(unit / a.heads % bt.max_rows);
@@ -213,39 +218,49 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   for (int k = lane; k < count; k += 64) M = fmaxf(M, a.stat[k * T_heads + at].x);
   M = wave_max(M);
   const float base = M == -INFINITY ? 0.f : M;
-  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int quads = dh / 4, ways = min(256 / quads, 16);
+  const int way = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (way < ways) {
 #pragma unroll 4
-  for (int k = wave; k < count; k += 4) {
-    const float2 st = a.stat[k * T_heads + at];
-    const float f = exp2f(st.x - base);
-    sum = fmaf(st.y, f, sum);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (lane + 64 * j < dh) o[j] = fmaf(a.part[(k * T_heads + at) * dh + lane + 64 * j], f, o[j]);
+    for (int k = way; k < count; k += ways) {
+      const float2 st = a.stat[k * T_heads + at];
+      const float f = exp2f(st.x - base);
+      const float4 x = *reinterpret_cast<const float4*>(a.part + (k * T_heads + at) * dh + d);
+      sum = fmaf(st.y, f, sum);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    }
   }
-  if (lane == 0) sum_of[wave] = sum;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o_of[wave][lane + 64 * j] = o[j];
+  o_of[threadIdx.x] = o;
+  sum_of[threadIdx.x] = sum;
   __syncthreads();
-  sum = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+  if (way != 0) return;
+  for (int w = 1; w < ways; ++w) {
+    const float4 x = o_of[w * quads + threadIdx.x];
+    sum += sum_of[w * quads + threadIdx.x];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int d = threadIdx.x;
-  if (d < dh)
-    Elem<T>::store((T*)a.out + at * dh, d, ((o_of[0][d] + o_of[1][d]) + (o_of[2][d] + o_of[3][d])) * inv);
-}
-
-// Zeros in the rows behind the last sequence.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_zero_rest_kernel(PagedBatch bt, T* out, int64_t width) {
-  const int64_t from = (int64_t)min(max(bt.offsets[bt.sequences], 0), bt.rows) * width;
-  const int64_t to = (int64_t)bt.rows * width;
-  for (int64_t i = from + (int64_t)blockIdx.x * 256 + threadIdx.x; i < to; i += (int64_t)gridDim.x * 256)
-    Elem<T>::store(out, i, 0.f);
+  T* out = (T*)a.out + at * dh + d;
+  Elem<T>::store(out, 0, o.x * inv);
+  Elem<T>::store(out, 1, o.y * inv);
+  Elem<T>::store(out, 2, o.z * inv);
+  Elem<T>::store(out, 3, o.w * inv);
 }
 
 // ----------------------------------------------------------------------------
 // Host
 // ----------------------------------------------------------------------------
+#ifndef SPLIT_WANT
+#define SPLIT_WANT 2048
+#endif
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Keys per chunk, in whole 64-key tiles: `want` workgroups or wavefronts in all where
@@ -263,7 +278,7 @@ static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_ba
     const int64_t columns = b->max_rows * (heads / c->kv_heads);
     p.column_tiles = columns <= 16 ? 1 : 2;
     p.query_tiles = (int)ceil_div(max(columns, (int64_t)1), 16 * p.column_tiles);
-    cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, 4096, 512);
+    cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, SPLIT_WANT, 512 * p.column_tiles);
   } else {
     cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, 256);
   }
@@ -287,16 +302,14 @@ static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* 
   const PagedCache dc = paged_cache(c);
   const PagedBatch db = paged_batch(b);
   const int64_t units = b->sequences * b->max_rows * a.heads;
-  if (units > 0) {
-    const int64_t blocks = plan.query_tiles ? b->sequences * c->kv_heads * plan.query_tiles * a.chunks
-                                            : ceil_div(units * a.chunks, ROWS_WAVES);
-    ALODLM_CHECK_ARG(blocks < (1ll << 31) && units < (1ll << 31), "paged_attention: too many rows in one call");
-    if (plan.query_tiles) paged_split_launch(c, b, a, plan, st);
-    else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
-    if (a.chunks > 1) paged_join_kernel<T, EIGHT><<<(unsigned)units, 256, 0, st>>>(dc, db, a);
-  }
-  if (a.zero_rest && b->rows > 0)
-    paged_zero_rest_kernel<T><<<256, 256, 0, st>>>(db, (T*)a.out, a.heads * c->head_dim);
+  const int64_t main = plan.query_tiles ? b->sequences * c->kv_heads * plan.query_tiles * a.chunks
+                                        : ceil_div(units * a.chunks, ROWS_WAVES);
+  const int64_t blocks = (units ? main : 0) + a.zero_blocks;
+  ALODLM_CHECK_ARG(blocks < (1ll << 31) && units < (1ll << 31), "paged_attention: too many rows in one call");
+  if (blocks == 0) return ALODLM_OK;
+  if (plan.query_tiles) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
+  else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
+  if (a.chunks > 1 && units) paged_join_kernel<T, EIGHT><<<(unsigned)units, 256, 0, st>>>(dc, db, a);
   ALODLM_CHECK_LAUNCH("paged_attention");
   return ALODLM_OK;
 }
@@ -319,7 +332,8 @@ extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alo
   const AttendPlan plan = attend_plan(cache, batch, heads);
   ALODLM_CHECK_ARG(plan.chunks == 1 || workspace, "paged_attention: no workspace");
   AttendArgs a = {q, out, ldq, workspace, nullptr, (int)heads, (int)(heads / cache->kv_heads),
-                  (int)plan.chunk_keys, (int)plan.chunks, scale * LOG2E, zero_rest};
+                  (int)plan.chunk_keys, (int)plan.chunks, scale * LOG2E, 0};
+  if (zero_rest) a.zero_blocks = (int)min(ceil_div(batch->rows * heads * cache->head_dim, 8192), (int64_t)64);
   a.stat = reinterpret_cast<float2*>(workspace + plan.chunks * batch->rows * heads * cache->head_dim);
   ALODLM_DISPATCH(cache->dtype, T, {
     if (cache->eight_bit) return attend_launch<T, true>(cache, batch, a, plan, as_stream(stream));

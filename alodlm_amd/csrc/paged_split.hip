@@ -3,8 +3,9 @@
 //
 // A decoding step reads every key and value once and does a few operations with each:
 // it is bound by the bytes.  So nothing is staged: every wave takes 64-key tiles of its
-// own straight from memory into the registers that the matrix instructions read, one
-// tile ahead, and no wave waits for another until the end.
+// own straight from memory into the registers that the matrix instructions read, the
+// next keys on their way during the products with the values and the next values during
+// those with the keys, and no wave waits for another until the end.
 //
 // Transposed products keep the probabilities in registers: S^T = K Q^T and O^T = V^T
 // P^T on 16x16x32 tiles.  The lane that holds query column c = lane % 16 of S^T holds the
@@ -45,20 +46,20 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {
   return r;
 }
 
-// A lane's places in the pages of one tile: for the keys (16-key group (lane % 16) / 4)
-// and for the values (group lane / 16); -1 where a page is missing.
-struct Places {
-  int64_t k, v;
-};
-
-// One 64-key tile in registers.  8 bits: k[t][c] 16 dims of a key, v[d] 16 keys of a
+// A lane's part of one 64-key tile.  8 bits: k[t][c] 16 dims of a key, v[d] 16 keys of a
 // dimension; 16 bits: the same in twice the registers.
-template <int DH, bool EIGHT> struct Tile {
-  static constexpr int KC = DH / (EIGHT ? 64 : 32), VC = EIGHT ? 1 : 2;
-  uint4 k[4][KC];
-  uint4 v[DH / 16][VC];
-  float k_scale, v_scale;
-  bool k_ok, v_ok;
+template <int DH, bool EIGHT> struct KeyTile {
+  static constexpr bool E = EIGHT;
+  static constexpr int N = DH / (EIGHT ? 64 : 32);
+  uint4 w[4][N];
+  float scale;
+};
+template <int DH, bool EIGHT> struct ValueTile {
+  static constexpr bool E = EIGHT;
+  static constexpr int N = EIGHT ? 1 : 2;
+  uint4 w[DH / 16][N];
+  float scale;
+  bool ok;
 };
 
 template <int DH, int CT, bool EIGHT>
@@ -69,13 +70,19 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   __shared__ float m_of[SPLIT_WAVES][16], l_of[SPLIT_WAVES][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
+  if (blockIdx.x >= gridDim.x - a.zero_blocks) {
+    zero_rest(bt, (bf16_t*)a.out, (int64_t)a.heads * DH, gridDim.x - 1 - blockIdx.x, a.zero_blocks);
+    return;
+  }
   const int page = c.page, shift = 31 - __builtin_clz(page);
-  // query tiles of one (sequence, head, chunk) lie a multiple of the others apart, so
-  // that they tend to meet on one die's cache
-  const int per_tile = bt.sequences * c.kv_heads * a.chunks;
+  // Neighbouring workgroups go to different dies.  Heads side by side, then sequences,
+  // turned on by one per chunk, then chunks: every die gets long and short sequences, and
+  // the chunks that few sequences reach come last.  Query tiles lie a multiple of all
+  // that apart, so that they tend to meet on one die's cache.
+  const int per_chunk = bt.sequences * c.kv_heads, per_tile = per_chunk * a.chunks;
   const int qt = blockIdx.x / per_tile, rest = blockIdx.x % per_tile;
-  const int chunk = rest % a.chunks, h = rest / a.chunks % c.kv_heads;
-  const int b = rest / a.chunks / c.kv_heads;
+  const int chunk = rest / per_chunk, h = rest % c.kv_heads;
+  const int b = (rest % per_chunk / c.kv_heads + chunk) % bt.sequences;
   const int given = given_rows(bt, b), first_col = qt * 16 * CT;
   if (first_col >= given * a.group) return;
   const int held = bt.held(b, page);
@@ -130,48 +137,41 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     const int64_t id = bt.page_of(b, p, c.pages);
     return id < 0 ? -1 : id * c.kv_heads + h;
   };
-  auto places = [&](int base, int lo, int hi, auto eight) {
-    return Places{find(base + (col >> 2) * 16, lo, hi, eight), find(base + grp * 16, lo, hi, eight)};
-  };
-  auto load = [&](int base, const Places& pl, auto eight) {
-    constexpr bool E = decltype(eight)::value;
+  // The keys: group (lane % 16) / 4 of the tile; a block of -1 gives zeros.
+  auto load_keys = [&](auto& t, int base, int64_t block) {
+    constexpr bool E = std::decay_t<decltype(t)>::E;
     typedef typename std::conditional<E, e4m3_t, bf16_t>::type S;
-    Tile<DH, E> t;
+    t.scale = 1.f;
     const S* keys = (const S*)(EIGHT && !E ? c.open_keys : c.keys);
-    const S* values = (const S*)(EIGHT && !E ? c.open_values : c.values);
-    t.k_ok = pl.k >= 0;
-    t.v_ok = pl.v >= 0;
-    t.k_scale = t.v_scale = 1.f;
+    const int in_page = (base + (col >> 2) * 16) & (page - 1);
+    const S* p = keys + block * head_block + (int64_t)(in_page + (col & 3)) * DH + grp * 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < Tile<DH, E>::KC; ++j) t.k[i][j] = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < KeyTile<DH, E>::N; ++j) {
+        t.w[i][j] = make_uint4(0, 0, 0, 0);
+        if (block >= 0)
+          t.w[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + (E ? j * 64 : (j / 2) * 64 + (j % 2) * 8));
+      }
+    if (E && block >= 0) t.scale = exp2_int(c.exponents[block / c.kv_heads * 2 * c.kv_heads + h]);
+  };
+  // The values: group lane / 16.
+  auto load_values = [&](auto& t, int base, int64_t block) {
+    constexpr bool E = std::decay_t<decltype(t)>::E;
+    typedef typename std::conditional<E, e4m3_t, bf16_t>::type S;
+    t.scale = 1.f;
+    t.ok = block >= 0;
+    const S* values = (const S*)(EIGHT && !E ? c.open_values : c.values);
+    const int in_page = (base + grp * 16) & (page - 1);
+    const S* p = values + block * head_block + (int64_t)col * page + in_page;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int j = 0; j < Tile<DH, E>::VC; ++j) t.v[d][j] = make_uint4(0, 0, 0, 0);
-    if (t.k_ok) {
-      const int in_page = (base + (col >> 2) * 16) & (page - 1);
-      const S* p = keys + pl.k * head_block + (int64_t)(in_page + (col & 3)) * DH + grp * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < Tile<DH, E>::KC; ++j)
-          t.k[i][j] = *reinterpret_cast<const uint4*>(
-              p + 4 * i * DH + (E ? j * 64 : (j / 2) * 64 + (j % 2) * 8));
-      if (E) t.k_scale = exp2_int(c.exponents[pl.k / c.kv_heads * 2 * c.kv_heads + h]);
-    }
-    if (t.v_ok) {
-      const int in_page = (base + grp * 16) & (page - 1);
-      const S* p = values + pl.v * head_block + (int64_t)col * page + in_page;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int j = 0; j < Tile<DH, E>::VC; ++j)
-          t.v[d][j] = *reinterpret_cast<const uint4*>(p + d * 16 * page + j * 8);
-      if (E) t.v_scale = exp2_int(c.exponents[(pl.v / c.kv_heads * 2 + 1) * c.kv_heads + h]);
-    }
-    return t;
+      for (int j = 0; j < ValueTile<DH, E>::N; ++j) {
+        t.w[d][j] = make_uint4(0, 0, 0, 0);
+        if (block >= 0) t.w[d][j] = *reinterpret_cast<const uint4*>(p + d * 16 * page + j * 8);
+      }
+    if (E && block >= 0) t.scale = exp2_int(c.exponents[(block / c.kv_heads * 2 + 1) * c.kv_heads + h]);
   };
   // p * v of the values that are inf or NaN, one by one, for the rows that see them: in
   // the products they are zeros, since 0 times one of them would not be 0 for the rows
@@ -213,9 +213,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       }
     }
   };
-  auto compute = [&](Tile<DH, true>* t8, Tile<DH, false>* t16, int base, int lo, int hi, auto eight) {
-    constexpr bool E = decltype(eight)::value;
-    f32x4 s[CT][4];
+  auto scores = [&](const auto& keys, f32x4 (&s)[CT][4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -223,29 +221,19 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
       for (int f = 0; f < FR; ++f) {
         bf16x8 k;
-        if constexpr (E) {
-          const uint4 w = t8->k[i][f / 2];
-          k = f % 2 ? widen(w.z, w.w, t8->k_scale) : widen(w.x, w.y, t8->k_scale);
+        if constexpr (std::decay_t<decltype(keys)>::E) {
+          const uint4 w = keys.w[i][f / 2];
+          k = f % 2 ? widen(w.z, w.w, keys.scale) : widen(w.x, w.y, keys.scale);
         } else {
-          k = __builtin_bit_cast(bf16x8, t16->k[i][f]);
+          k = __builtin_bit_cast(bf16x8, keys.w[i][f]);
         }
 #pragma unroll
         for (int t = 0; t < CT; ++t) s[t][i] = mfma16(k, q[t][f], s[t][i]);
       }
     }
-    const bool v_ok = E ? t8->v_ok : t16->v_ok;
-    // tiles that every row sees whole need no mask
-    const bool masked = base < lo || base + SPLIT_TILE > min(hi, least) || !__all(v_ok);
-    if (masked) {
-#pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = base + grp * 16 + i;
-          if (!(key >= lo && key < min(hi, limit[t]) && v_ok)) s[t][i / 4][i % 4] = -INFINITY;
-        }
-    }
-    bf16x8 p[CT][2];
+  };
+  // Scores -> probabilities in bf16; the maximum and what goes with it move along.
+  auto softmax = [&](const f32x4 (&s)[CT][4], bf16x8 (&p)[CT][2]) {
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       float top = s[t][0][0];
@@ -263,41 +251,11 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       }
       const float base_m = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], a.scale2, -base_m));
-        p[t][i / 8][i % 8] = (__bf16)e;
-      }
+      for (int i = 0; i < 16; ++i)
+        p[t][i / 8][i % 8] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], a.scale2, -base_m));
     }
-    bool special = false;  // a value that is inf or NaN, in a tile that not all rows see whole
-    if (masked) {
-      uint32_t odd = 0;
-      auto clean = [&](uint32_t& w, bool write) {  // bytes (halves) of all ones in the exponent -> 0
-        if constexpr (E) {
-          const uint32_t z = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-          odd |= z;
-          if (write) w &= ~((z >> 7) * 0xffu);
-        } else {
-          const uint32_t z = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-          odd |= z;
-          if (write) w &= ~((z >> 15) * 0xffffu);
-        }
-      };
-      auto sweep = [&](bool write) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int j = 0; j < (E ? 1 : 2); ++j) {
-            uint4& w = E ? t8->v[d][0] : t16->v[d][j];
-            clean(w.x, write);
-            clean(w.y, write);
-            clean(w.z, write);
-            clean(w.w, write);
-          }
-      };
-      sweep(false);
-      special = __any(odd);
-      if (special) sweep(true);
-    }
+  };
+  auto add_values = [&](const auto& values, const bf16x8 (&p)[CT][2]) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -305,50 +263,111 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         bf16x8 v;
-        if constexpr (E) {
-          const uint4 w = t8->v[d][0];
-          v = j ? widen(w.z, w.w, t8->v_scale) : widen(w.x, w.y, t8->v_scale);
+        if constexpr (std::decay_t<decltype(values)>::E) {
+          const uint4 w = values.w[d][0];
+          v = j ? widen(w.z, w.w, values.scale) : widen(w.x, w.y, values.scale);
         } else {
-          v = __builtin_bit_cast(bf16x8, t16->v[d][j]);
+          v = __builtin_bit_cast(bf16x8, values.w[d][j]);
         }
 #pragma unroll
         for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v, p[t][j], o[t][d]);
       }
     }
-    if (special) add_special(base, p, lo, hi, eight);
+  };
+  // Keys outside [lo, hi), beyond a row's own, or in a page that is missing are hidden.
+  auto hide = [&](f32x4 (&s)[CT][4], int base, int lo, int hi, bool there) {
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = base + grp * 16 + i;
+        if (!(key >= lo && key < min(hi, limit[t]) && there)) s[t][i / 4][i % 4] = -INFINITY;
+      }
+  };
+  // inf and NaN among a tile's values -> zero; whether there was any.
+  auto clean = [&](auto& tile) -> bool {
+    constexpr bool E = std::decay_t<decltype(tile)>::E;
+    uint32_t odd = 0;
+    auto word = [&](uint32_t& w, bool write) {  // bytes (halves) with all ones for an exponent
+      const uint32_t z = E ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
+                           : ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      odd |= z;
+      if (write) w &= E ? ~((z >> 7) * 0xffu) : ~((z >> 15) * 0xffffu);
+    };
+    auto sweep = [&](bool write) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < ValueTile<DH, E>::N; ++j) {
+          word(tile.w[d][j].x, write);
+          word(tile.w[d][j].y, write);
+          word(tile.w[d][j].z, write);
+          word(tile.w[d][j].w, write);
+        }
+    };
+    sweep(false);
+    if (!__any(odd)) return false;
+    sweep(true);
+    return true;
   };
 
   constexpr int STEP = SPLIT_WAVES * SPLIT_TILE;
-  if constexpr (EIGHT) {  // sealed pages, one tile ahead
-    const int hi = min(k1, sealed);
-    int base = k0 + wave * SPLIT_TILE;
-    if (base < hi) {
-      Places pl = places(base, 0, hi, std::true_type());
-      Tile<DH, true> tile = load(base, pl, std::true_type());
-      pl = places(base + STEP, 0, hi, std::true_type());
-      while (true) {
-        Tile<DH, true> now = tile;
-        const bool more = base + STEP < hi;
-        if (more) {
-          tile = load(base + STEP, pl, std::true_type());
-          pl = places(base + 2 * STEP, 0, hi, std::true_type());
-        }
-        compute(&now, nullptr, base, 0, hi, std::true_type());
-        if (!more) break;
-        base += STEP;
-      }
-    }
-  }
-  {  // 16-bit pages: the pool's, or the open ones behind the sealed
-    const int lo = EIGHT ? max(k0, sealed) : k0;
-    const int start = lo / SPLIT_TILE * SPLIT_TILE;
-    // tiles keep the waves' turns
-    for (int base = start + ((wave - start / SPLIT_TILE) & (SPLIT_WAVES - 1)) * SPLIT_TILE; base < k1;
+  // Tiles [from, to) of keys [lo, hi) that some row does not see whole.
+  auto edge_tiles = [&](int from, int to, int lo, int hi, auto eight) {
+    constexpr bool E = decltype(eight)::value;
+    for (int base = from + ((wave - from / SPLIT_TILE) & (SPLIT_WAVES - 1)) * SPLIT_TILE; base < to;
          base += STEP) {
-      const Places pl = places(base, lo, k1, std::false_type());
-      Tile<DH, false> tile = load(base, pl, std::false_type());
-      compute(nullptr, &tile, base, lo, k1, std::false_type());
+      KeyTile<DH, E> keys;
+      ValueTile<DH, E> values;
+      load_keys(keys, base, find(base + (col >> 2) * 16, lo, hi, eight));
+      load_values(values, base, find(base + grp * 16, lo, hi, eight));
+      f32x4 s[CT][4];
+      bf16x8 p[CT][2];
+      scores(keys, s);
+      hide(s, base, lo, hi, values.ok);
+      softmax(s, p);
+      const bool special = clean(values);
+      add_values(values, p);
+      if (special) add_special(base, p, lo, hi, eight);
     }
+  };
+  // Whole tiles of keys [k0, to) that every row sees: the next tile's keys are on their
+  // way while this one's values are used, and its values while those keys are.
+  auto whole_tiles = [&](int to, auto eight) {
+    constexpr bool E = decltype(eight)::value;
+    int base = k0 + ((wave - k0 / SPLIT_TILE) & (SPLIT_WAVES - 1)) * SPLIT_TILE;
+    if (base >= to) return;
+    KeyTile<DH, E> keys;
+    ValueTile<DH, E> values;
+    load_keys(keys, base, find(base + (col >> 2) * 16, 0, to, eight));
+    load_values(values, base, find(base + grp * 16, 0, to, eight));
+    int64_t k_next = find(base + STEP + (col >> 2) * 16, 0, to, eight);
+    int64_t v_next = find(base + STEP + grp * 16, 0, to, eight);
+    while (true) {
+      const bool more = base + STEP < to;
+      f32x4 s[CT][4];
+      bf16x8 p[CT][2];
+      scores(keys, s);
+      if (more) load_keys(keys, base + STEP, k_next);
+      if (!__all(values.ok)) hide(s, base, 0, to, values.ok);
+      softmax(s, p);
+      add_values(values, p);
+      if (!more) break;
+      base += STEP;
+      load_values(values, base, v_next);
+      k_next = find(base + STEP + (col >> 2) * 16, 0, to, eight);
+      v_next = find(base + STEP + grp * 16, 0, to, eight);
+    }
+  };
+  // 8 bits: the sealed pages, then the open ones; 16 bits: the pool's
+  const int hi = EIGHT ? min(k1, sealed) : k1;
+  const int whole = max(min(hi, least) / SPLIT_TILE * SPLIT_TILE, k0);
+  typedef std::integral_constant<bool, EIGHT> Pool;
+  whole_tiles(whole, Pool());
+  edge_tiles(whole, hi, k0, hi, Pool());
+  if constexpr (EIGHT) {
+    const int lo = max(k0, sealed);
+    if (lo < k1) edge_tiles(lo / SPLIT_TILE * SPLIT_TILE, k1, lo, k1, std::false_type());
   }
 
   // join the waves, 16 columns at a time
@@ -410,8 +429,7 @@ static void launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, con
 }
 
 void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
-                        const AttendPlan& p, hipStream_t st) {
-  const unsigned grid = (unsigned)(b->sequences * c->kv_heads * p.query_tiles * a.chunks);
+                        const AttendPlan& p, unsigned grid, hipStream_t st) {
   if (c->head_dim == 64) {
     if (p.column_tiles == 1) launch<64, 1>(c, b, a, grid, st);
     else launch<64, 2>(c, b, a, grid, st);
