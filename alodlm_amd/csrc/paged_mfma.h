@@ -1,0 +1,239 @@
+// What the matrix-core kernels of the paged attention share: 64-key tiles against query
+// columns of 16, in transposed products S^T = K Q^T and O^T = V^T P^T on 16x16x32.
+//
+// The lane that holds query column c = lane % 16 of S^T holds the same column of P^T, so
+// the probabilities never leave their registers.  The order in which keys are given to
+// the rows of S^T makes a lane's 16 scores 16 keys in a row, lane / 16 saying which 16
+// of the 64: row r of subtile i is key (r / 4) * 16 + 4 i + r % 4.  The second product
+// then takes a value row's tokens in their order, 8 a fragment; and since page sizes are
+// multiples of 16, each lane's 16 keys lie in one page.
+//
+// 8-bit codes become bf16 times the page's power of two in one instruction a pair
+// (v_cvt_scalef32_pk_bf16_fp8), exactly.  Scores, maxima, sums and outputs are float32;
+// the probabilities are rounded to bf16 for the second product, and the sum is that of
+// the rounded ones (one more product with ones), so that the weights add up to one.
+#pragma once
+
+#include "paged.h"
+
+#include <type_traits>
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+#define PAGED_TILE 64   // keys of a tile
+#define PAGED_WAVES 4   // waves of a workgroup
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Eight e4m3 codes times a power of two as bf16.
+__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {
+  bf16x8 r;
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
+  r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  return r;
+}
+
+// inf and NaN in a word of codes (bf16 pairs) -> zero; nonzero where there was any.
+template <bool EIGHT>
+__device__ __forceinline__ uint32_t special_bits(uint32_t w) {
+  return EIGHT ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
+               : ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+template <bool EIGHT>
+__device__ __forceinline__ uint32_t without_special(uint32_t w) {
+  const uint32_t z = special_bits<EIGHT>(w);
+  return w & (EIGHT ? ~((z >> 7) * 0xffu) : ~((z >> 15) * 0xffffu));
+}
+
+// The sequence, head and keys that a workgroup (or a wave) works on.
+struct Span {
+  int b, h, slot;
+  int held, n, given;    // tokens before the step; rows that take part; rows of the batch
+  int sealed, reach;     // ends of the 8-bit pages and of the keys that are there
+  int64_t row0;
+
+  template <bool EIGHT>
+  static __device__ __forceinline__ Span of(const PagedCache& c, const PagedBatch& bt, int b, int h) {
+    Span s;
+    s.b = b;
+    s.h = h;
+    s.given = given_rows(bt, b);
+    const int held = bt.held(b, c.page);
+    s.n = held < 0 ? 0 : bt.row_count(b, held, c.page);
+    s.held = max(held, 0);
+    const int end = s.held + s.n;
+    s.sealed = EIGHT ? sealed_keys(bt, s.held, end, c.page, true) : end;
+    s.reach = EIGHT ? open_end(c, s.sealed, end) : end;
+    s.slot = EIGHT ? bt.slot(b, c.slots) : 0;
+    s.row0 = bt.first_row(b);
+    return s;
+  }
+  // Keys that row i sees.
+  __device__ __forceinline__ int limit(int i) const { return i < n ? min(held + i + 1, reach) : 0; }
+  // The block (page and head, of the pool or among the open pages) of the 16 keys from
+  // `key` on, as far as [lo, hi) reaches into them; -1 for none.
+  template <bool POOL>
+  __device__ __forceinline__ int64_t block(const PagedCache& c, const PagedBatch& bt, int key, int lo,
+                                           int hi) const {
+    if (key + 15 < lo || key >= hi) return -1;
+    const int p = key / c.page;
+    if (!POOL) return slot < 0 ? -1 : open_page(c, slot, p) * c.kv_heads + h;
+    const int64_t id = bt.page_of(b, p, c.pages);
+    return id < 0 ? -1 : id * c.kv_heads + h;
+  }
+};
+
+// 2^exponent of a pool block's keys (side 0) or values (side 1).
+__device__ __forceinline__ float block_scale(const PagedCache& c, int64_t block, int side) {
+  const int64_t id = block / c.kv_heads;
+  return exp2_int(c.exponents[(id * 2 + side) * c.kv_heads + (block - id * c.kv_heads)]);
+}
+
+// CT times 16 query columns of one wave and what becomes of them.  Column x is row x /
+// group and query head h * group + x % group.
+template <int DH, int CT> struct Columns {
+  static constexpr int FR = DH / 32, DT = DH / 16;  // query fragments, 16-row tiles of the output
+  bf16x8 q[CT][FR];
+  f32x4 o[CT][DT], l[CT];
+  float m[CT];
+  int limit[CT];
+
+  // Lane group g holds dims dim(f, g) .. + 8 of fragment f.
+  template <typename Dim>
+  __device__ __forceinline__ void start(const AttendArgs& a, const Span& s, int first, Dim dim) {
+    const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int x = first + t * 16 + col, i = x / a.group, head = s.h * a.group + x % a.group;
+      limit[t] = s.limit(i);
+      const bf16_t* p = (const bf16_t*)a.q + (s.row0 + i) * a.ldq + (int64_t)head * DH;
+#pragma unroll
+      for (int f = 0; f < FR; ++f) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (i < s.n) w = *reinterpret_cast<const uint4*>(p + dim(f, grp));
+        q[t][f] = __builtin_bit_cast(bf16x8, w);
+      }
+      m[t] = -INFINITY;
+      l[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // key(i, f): the lane's part of subtile i's rows, dims of fragment f.
+  template <typename Key>
+  __device__ __forceinline__ void scores(f32x4 (&s)[CT][4], Key key) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t) s[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < FR; ++f) {
+        const bf16x8 k = key(i, f);
+#pragma unroll
+        for (int t = 0; t < CT; ++t) s[t][i] = mfma16(k, q[t][f], s[t][i]);
+      }
+    }
+  }
+  // Keys outside [lo, hi), beyond a row's own, or in a page that is missing are hidden.
+  __device__ __forceinline__ void hide(f32x4 (&s)[CT][4], int base, int lo, int hi, bool there) const {
+    const int grp = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int end = there ? min(hi, limit[t]) : 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = base + grp * 16 + i;
+        if (!(key >= lo && key < end)) s[t][i / 4][i % 4] = -INFINITY;
+      }
+    }
+  }
+  // Scores -> probabilities in bf16; the maximum and what goes with it move along.
+  __device__ __forceinline__ void softmax(const f32x4 (&s)[CT][4], bf16x8 (&p)[CT][2], float scale2) {
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      float top = s[t][0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[t][i / 4][i % 4]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
+      if (__any(top > m[t])) {
+        const float to = fmaxf(m[t], top);
+        const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - to);
+        m[t] = to;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] *= f;
+      }
+      const float base = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        p[t][i / 8][i % 8] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale2, -base));
+    }
+  }
+  // value(d, j): dimension d * 16 + lane % 16, keys (lane / 16) * 16 + 8 j .. + 8.
+  template <typename Value>
+  __device__ __forceinline__ void add_values(const bf16x8 (&p)[CT][2], Value value) {
+    bf16x8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t) l[t] = mfma16(ones, p[t][j], l[t]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const bf16x8 v = value(d, j);
+#pragma unroll
+        for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v, p[t][j], o[t][d]);
+      }
+    }
+  }
+  // p * v of the values that are inf or NaN, one by one, for the rows that see them: in
+  // the products they are zeros, since 0 times one of them would not be 0 for the rows
+  // that do not.  `mine`: 64 * 16 floats (or bf16) of LDS for this wave alone.
+  template <bool POOL, bool EIGHT, typename S>
+  __device__ __forceinline__ void add_special(const PagedCache& c, const PagedBatch& bt, const Span& sp,
+                                           const bf16x8 (&p)[CT][2], int base, int lo, int hi, S* mine) {
+    constexpr bool E = POOL && EIGHT;
+    const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
+    const void* values = EIGHT && !POOL ? c.open_values : c.values;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (sizeof(S) == 4) mine[(grp * 16 + i) * 16 + col] = (float)p[t][i / 8][i % 8];
+        else mine[(grp * 16 + i) * 16 + col] = p[t][i / 8][i % 8];
+      }
+      __builtin_amdgcn_wave_barrier();
+      for (int k = 0; k < PAGED_TILE; ++k) {
+        const int key = base + k;
+        if (key < lo || key >= hi) continue;
+        const int64_t at = sp.block<POOL>(c, bt, key & ~15, lo, hi);
+        if (at < 0) continue;
+        const float w = (float)mine[k * 16 + col];
+        const int64_t v_at = at * c.page * DH + (key & (c.page - 1));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          __builtin_amdgcn_sched_barrier(0);  // a rare path: no registers for loads ahead
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t x = v_at + (int64_t)(d * 16 + grp * 4 + i) * c.page;
+            float v;
+            if constexpr (E) v = __builtin_amdgcn_cvt_f32_fp8(((const e4m3_t*)values)[x], 0);
+            else v = bf16_to_float(((const bf16_t*)values)[x]);
+            if (key < limit[t] && !(fabsf(v) < INFINITY)) o[t][d][i] = fmaf(w, v, o[t][d][i]);
+          }
+        }
+      }
+    }
+  }
+};
