@@ -70,7 +70,7 @@ struct AttendArgs {
   int64_t ldq;
   float* part;   // unnormalised outputs [chunks][rows * heads][head_dim]
   float2* stat;  // (maximum in base 2, sum) [chunks][rows * heads]
-  int heads, group, chunk_keys, chunks;
+  int heads, group, chunk_keys, chunks, query_tiles;
   float scale2;  // softmax scale * log2 e
   int zero_blocks;  // workgroups behind the launch's others that clear the rows behind the last sequence
 };
@@ -107,13 +107,17 @@ __device__ __forceinline__ int given_rows(const PagedBatch& bt, int b) {
 // How a call is cut up.
 struct AttendPlan {
   int64_t chunk_keys, chunks;
-  int column_tiles, query_tiles;  // matrix-core kernels: 16-column tiles a wave, tiles a sequence
+  // matrix-core kernels: whether the waves split the query columns (else the keys),
+  // 16-column tiles a wave, workgroups along a sequence's columns
+  bool split_columns;
+  int column_tiles, query_tiles;
 };
 
-// bf16 with head_dim 64 or 128 (csrc/paged_split.hip): the keys of a chunk over the
-// waves of a workgroup.
-bool paged_split_takes(const alodlm_paged_cache* c);
+// Matrix-core kernels, bf16 with head_dim 64 or 128: the keys (csrc/paged_split.hip) or
+// the query columns (csrc/paged_tiles.hip) over the waves of a workgroup.
 void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
+                        const AttendPlan& p, unsigned blocks, hipStream_t st);
+void paged_tiles_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
                         const AttendPlan& p, unsigned blocks, hipStream_t st);
 
 // Host: checks of the two structs shared by the entry points (abi errors), and

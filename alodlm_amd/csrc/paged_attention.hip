@@ -274,14 +274,17 @@ static void cut_keys(AttendPlan& p, int64_t max_keys, int64_t units, int64_t wan
 
 static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
   AttendPlan p = {};
-  if (paged_split_takes(c)) {
-    const int64_t columns = b->max_rows * (heads / c->kv_heads);
-    p.column_tiles = columns <= 16 ? 1 : 2;
-    p.query_tiles = (int)ceil_div(max(columns, (int64_t)1), 16 * p.column_tiles);
-    cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, SPLIT_WANT, 512 * p.column_tiles);
-  } else {
+  if (c->dtype != ALODLM_BF16 || (c->head_dim != 64 && c->head_dim != 128)) {
     cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, 256);
+    return p;
   }
+  const int64_t columns = max(b->max_rows * (heads / c->kv_heads), (int64_t)1);
+  p.split_columns = columns > 32;
+  const int waves = p.split_columns ? 4 : 1;
+  p.column_tiles = columns <= 16 * waves ? 1 : 2;
+  p.query_tiles = (int)ceil_div(columns, 16 * p.column_tiles * waves);
+  cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, p.split_columns ? 1024 : SPLIT_WANT,
+           512 * p.column_tiles);
   return p;
 }
 
@@ -307,7 +310,8 @@ static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* 
   const int64_t blocks = (units ? main : 0) + a.zero_blocks;
   ALODLM_CHECK_ARG(blocks < (1ll << 31) && units < (1ll << 31), "paged_attention: too many rows in one call");
   if (blocks == 0) return ALODLM_OK;
-  if (plan.query_tiles) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
+  if (plan.split_columns) paged_tiles_launch(c, b, a, plan, (unsigned)blocks, st);
+  else if (plan.query_tiles) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
   else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
   if (a.chunks > 1 && units) paged_join_kernel<T, EIGHT><<<(unsigned)units, 256, 0, st>>>(dc, db, a);
   ALODLM_CHECK_LAUNCH("paged_attention");
@@ -332,7 +336,7 @@ extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alo
   const AttendPlan plan = attend_plan(cache, batch, heads);
   ALODLM_CHECK_ARG(plan.chunks == 1 || workspace, "paged_attention: no workspace");
   AttendArgs a = {q, out, ldq, workspace, nullptr, (int)heads, (int)(heads / cache->kv_heads),
-                  (int)plan.chunk_keys, (int)plan.chunks, scale * LOG2E, 0};
+                  (int)plan.chunk_keys, (int)plan.chunks, plan.query_tiles, scale * LOG2E, 0};
   if (zero_rest) a.zero_blocks = (int)min(ceil_div(batch->rows * heads * cache->head_dim, 8192), (int64_t)64);
   a.stat = reinterpret_cast<float2*>(workspace + plan.chunks * batch->rows * heads * cache->head_dim);
   ALODLM_DISPATCH(cache->dtype, T, {

@@ -41,7 +41,7 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {
   return r;
 }
 
-// inf and NaN in a word of codes (bf16 pairs) -> zero; nonzero where there was any.
+// inf and NaN in a word of codes (bf16 pairs): nonzero where there is any; without them.
 template <bool EIGHT>
 __device__ __forceinline__ uint32_t special_bits(uint32_t w) {
   return EIGHT ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u
@@ -97,6 +97,26 @@ __device__ __forceinline__ float block_scale(const PagedCache& c, int64_t block,
   return exp2_int(c.exponents[(id * 2 + side) * c.kv_heads + (block - id * c.kv_heads)]);
 }
 
+// Tiles in which some row sees a key that another does not are multiplied with zeros in
+// the place of values that are inf or NaN: 0 times one of them would not be 0 for the
+// rows that do not see it.  Those that do get them afterwards: the sum of dimension d's
+// inf and NaN over keys [from, to) (a probability is positive, and inf times it is inf).
+template <int DH, bool EIGHT>
+__device__ __forceinline__ float special_sum(const PagedCache& c, const PagedBatch& bt, const Span& sp,
+                                             int d, int from, int to) {
+  float sum = 0.f;
+  for (int key = from; key < to; ++key) {
+    const bool pool = !EIGHT || key < sp.sealed;
+    const int64_t block = pool ? sp.block<true>(c, bt, key, key, key + 1) : sp.block<false>(c, bt, key, key, key + 1);
+    if (block < 0) continue;
+    const int64_t at = (block * DH + d) * c.page + (key & (c.page - 1));
+    const float v = EIGHT && pool ? __builtin_amdgcn_cvt_f32_fp8(((const e4m3_t*)c.values)[at], 0)
+                                  : bf16_to_float(((const bf16_t*)(EIGHT ? c.open_values : c.values))[at]);
+    if (!(fabsf(v) < INFINITY)) sum += v;
+  }
+  return sum;
+}
+
 // CT times 16 query columns of one wave and what becomes of them.  Column x is row x /
 // group and query head h * group + x % group.
 template <int DH, int CT> struct Columns {
@@ -141,6 +161,30 @@ template <int DH, int CT> struct Columns {
         for (int t = 0; t < CT; ++t) s[t][i] = mfma16(k, q[t][f], s[t][i]);
       }
     }
+  }
+  // The same with the next subtile's fragments read while this one's are multiplied (and
+  // no further ahead: the registers are taken).
+  template <typename Key>
+  __device__ __forceinline__ void scores_ahead(f32x4 (&s)[CT][4], Key key) const {
+    bf16x8 now[FR], next[FR];
+#pragma unroll
+    for (int f = 0; f < FR; ++f) now[f] = key(0, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i < 3)
+#pragma unroll
+        for (int f = 0; f < FR; ++f) next[f] = key(i + 1, f);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) s[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < FR; ++f)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) s[t][i] = mfma16(now[f], q[t][f], s[t][i]);
+#pragma unroll
+      for (int f = 0; f < FR; ++f) now[f] = next[f];
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
   // Keys outside [lo, hi), beyond a row's own, or in a page that is missing are hidden.
   __device__ __forceinline__ void hide(f32x4 (&s)[CT][4], int base, int lo, int hi, bool there) const {
@@ -196,44 +240,33 @@ template <int DH, int CT> struct Columns {
       }
     }
   }
-  // p * v of the values that are inf or NaN, one by one, for the rows that see them: in
-  // the products they are zeros, since 0 times one of them would not be 0 for the rows
-  // that do not.  `mine`: 64 * 16 floats (or bf16) of LDS for this wave alone.
-  template <bool POOL, bool EIGHT, typename S>
-  __device__ __forceinline__ void add_special(const PagedCache& c, const PagedBatch& bt, const Span& sp,
-                                           const bf16x8 (&p)[CT][2], int base, int lo, int hi, S* mine) {
-    constexpr bool E = POOL && EIGHT;
-    const int col = threadIdx.x & 15, grp = (threadIdx.x & 63) >> 4;
-    const void* values = EIGHT && !POOL ? c.open_values : c.values;
+  // The same four fragments at a time, the next four read meanwhile.
+  template <typename Value>
+  __device__ __forceinline__ void add_values_ahead(const bf16x8 (&p)[CT][2], Value value) {
+    bf16x8 ones;
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      __builtin_amdgcn_wave_barrier();
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
+    constexpr int STEPS = 2 * DT / 4;
+    bf16x8 now[4], next[4];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (sizeof(S) == 4) mine[(grp * 16 + i) * 16 + col] = (float)p[t][i / 8][i % 8];
-        else mine[(grp * 16 + i) * 16 + col] = p[t][i / 8][i % 8];
-      }
-      __builtin_amdgcn_wave_barrier();
-      for (int k = 0; k < PAGED_TILE; ++k) {
-        const int key = base + k;
-        if (key < lo || key >= hi) continue;
-        const int64_t at = sp.block<POOL>(c, bt, key & ~15, lo, hi);
-        if (at < 0) continue;
-        const float w = (float)mine[k * 16 + col];
-        const int64_t v_at = at * c.page * DH + (key & (c.page - 1));
+    for (int k = 0; k < 4; ++k) now[k] = value(k, 0);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          __builtin_amdgcn_sched_barrier(0);  // a rare path: no registers for loads ahead
+    for (int t = 0; t < CT; ++t) l[t] = mfma16(ones, p[t][1], mfma16(ones, p[t][0], l[t]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t x = v_at + (int64_t)(d * 16 + grp * 4 + i) * c.page;
-            float v;
-            if constexpr (E) v = __builtin_amdgcn_cvt_f32_fp8(((const e4m3_t*)values)[x], 0);
-            else v = bf16_to_float(((const bf16_t*)values)[x]);
-            if (key < limit[t] && !(fabsf(v) < INFINITY)) o[t][d][i] = fmaf(w, v, o[t][d][i]);
-          }
-        }
-      }
+    for (int g = 0; g < STEPS; ++g) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (g + 1 < STEPS)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) next[k] = value((g + 1) * 4 % DT + k, (g + 1) * 4 / DT);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+          o[t][g * 4 % DT + k] = mfma16(now[k], p[t][g * 4 / DT], o[t][g * 4 % DT + k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) now[k] = next[k];
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 };

@@ -21,6 +21,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   constexpr int DT = DH / 16;
   __shared__ __attribute__((aligned(16))) float buf[PAGED_WAVES][16 * (DH + 4)];
   __shared__ float m_of[PAGED_WAVES][16], l_of[PAGED_WAVES][16];
+  __shared__ int special_of[PAGED_WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   if (blockIdx.x >= gridDim.x - a.zero_blocks) {
@@ -90,6 +91,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
 
   constexpr int STEP = PAGED_WAVES * PAGED_TILE;
+  uint32_t odd = 0;  // inf or NaN among the values of a tile that not every row sees whole
   // tiles keep the waves' turns
   auto first_tile = [&](int from) {
     return from + ((wave - from / PAGED_TILE) & (PAGED_WAVES - 1)) * PAGED_TILE;
@@ -131,7 +133,6 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       cols.scores(s, [&](int i, int f) { return key_of(tile, i, f); });
       cols.hide(s, base, k0, to, tile.there);
       cols.softmax(s, p, a.scale2);
-      uint32_t odd = 0;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         uint32_t* w = &tile.v[d].x;
@@ -142,7 +143,6 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         }
       }
       cols.add_values(p, [&](int d, int j) { return value_of(tile, d, j); });
-      if (__any(odd)) cols.template add_special<true, EIGHT>(c, bt, sp, p, base, k0, to, buf[wave]);
     }
   };
   // Tiles [from, to) of keys [lo, to) in 16 bits, loaded as the products take them
@@ -165,7 +165,6 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       });
       if (!whole || !__all(v_block >= 0)) cols.hide(s, base, lo, to, v_block >= 0);
       cols.softmax(s, p, a.scale2);
-      uint32_t odd = 0;
       cols.add_values(p, [&](int d, int j) {
         uint4 w = make_uint4(0, 0, 0, 0);
         if (v_block >= 0) w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
@@ -177,7 +176,6 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         }
         return __builtin_bit_cast(bf16x8, w);
       });
-      if (!whole && __any(odd)) cols.template add_special<POOL, EIGHT>(c, bt, sp, p, base, lo, to, buf[wave]);
     }
   };
   const int hi = EIGHT ? min(k1, sp.sealed) : k1;
@@ -194,6 +192,8 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 
   // join the waves, 16 columns at a time
   const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  const bool any = __any(odd);
+  if (lane == 0) special_of[wave] = any;
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
     __syncthreads();
@@ -218,8 +218,17 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     const int y = first_col + t * 16 + x, i = y / a.group;
     if (i >= sp.given) continue;
     const int64_t to = (sp.row0 + i) * a.heads + sp.h * a.group + y % a.group;
+    if (special_of[0] | special_of[1] | special_of[2] | special_of[3])
+      for (int k = 0; k < DH / 16; ++k)
+        r[k] += special_sum<DH, EIGHT>(c, bt, sp, d0 + k, whole, min(sp.limit(i), k1));
+    if (sp.limit(i) == 0) {  // a row that sees no key is zero
+      M = -INFINITY;
+      sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < DH / 16; ++k) r[k] = 0.f;
+    }
     if (a.chunks == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key is zero
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       bf16_t* out = (bf16_t*)a.out + to * DH + d0;
 #pragma unroll
       for (int k = 0; k < DH / 16; k += 4)
@@ -234,10 +243,6 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       *reinterpret_cast<f32x4*>(part + k) = f32x4{r[k], r[k + 1], r[k + 2], r[k + 3]};
     if ((threadIdx.x & 15) == 0) a.stat[chunk * T_heads + to] = make_float2(M, sum);
   }
-}
-
-bool paged_split_takes(const alodlm_paged_cache* c) {
-  return c->dtype == ALODLM_BF16 && (c->head_dim == 64 || c->head_dim == 128);
 }
 
 template <int DH, int CT>

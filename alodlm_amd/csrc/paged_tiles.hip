@@ -1,0 +1,267 @@
+// Attention over paged keys on the matrix cores, the query rows split over the waves:
+// bf16, head_dim 64 and 128, windows and prompts.
+//
+// A workgroup's four waves hold 64 CT query columns (rows times the heads that share a
+// key/value head) against the same keys.  Each 64-key tile is fetched once, widened to
+// bf16 once and laid into LDS, from where every wave takes its fragments; the next
+// tile's bytes come in behind the products of the one before, into the other half of
+// the buffer: one barrier a tile.  The limits are then the matrix instructions, the
+// LDS reads (32 KB a wave and tile against 32 columns) and the exponentials, which
+// two workgroups a compute unit overlap.
+//
+// LDS layout: a key's row of DH values, a dimension's row of 64 keys, in 16-byte pieces
+// whose place is XORed with the row such that 16 lanes on 16 rows meet all banks.
+#include "paged_mfma.h"
+
+template <int DH> struct TileBuffer {
+  bf16_t k[PAGED_TILE * DH];
+  bf16_t v[DH * PAGED_TILE];
+};
+
+// Place (in values) of 16-byte piece `piece` of a key's, a dimension's row.  A fragment's
+// 16 rows are keys with different (key >> 4, key & 3), or 16 dimensions in a row.
+template <int DH>
+__device__ __forceinline__ int key_piece(int key, int piece) {
+  constexpr int MASK = DH / 8 - 1;
+  return key * DH + ((piece ^ (((key >> 4) << 2 | (key & 3)) & MASK)) << 3);
+}
+__device__ __forceinline__ int value_piece(int d, int piece) {
+  return d * PAGED_TILE + ((piece ^ ((d >> 1) & 7)) << 3);
+}
+
+template <int DH, int CT, bool EIGHT>
+__global__ void __launch_bounds__(64 * PAGED_WAVES, 2)
+paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
+  constexpr int DT = DH / 16, COLS = 16 * CT * PAGED_WAVES;
+  __shared__ __attribute__((aligned(16))) TileBuffer<DH> tiles[2];
+  __shared__ int there[2][4], special_of[PAGED_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  if (blockIdx.x >= gridDim.x - a.zero_blocks) {
+    zero_rest(bt, (bf16_t*)a.out, (int64_t)a.heads * DH, gridDim.x - 1 - blockIdx.x, a.zero_blocks);
+    return;
+  }
+  const int page = c.page;
+  // heads, sequences (turned on by one per chunk and query tile), chunks, query tiles,
+  // the last of which see the most keys and go first
+  const int per_chunk = bt.sequences * c.kv_heads, per_tile = per_chunk * a.chunks;
+  const int qt = a.query_tiles - 1 - blockIdx.x / per_tile, rest = blockIdx.x % per_tile;
+  const int chunk = rest / per_chunk;
+  const Span sp = Span::of<EIGHT>(c, bt, (rest % per_chunk / c.kv_heads + chunk + qt) % bt.sequences,
+                                  rest % c.kv_heads);
+  const int first_col = qt * COLS;
+  if (first_col >= sp.given * a.group) return;
+  const int row_lo = first_col / a.group, row_hi = min((first_col + COLS - 1) / a.group, sp.n - 1);
+  const int least = sp.limit(row_lo), most = row_hi < row_lo ? 0 : sp.limit(row_hi);
+  const int k0 = chunk * a.chunk_keys, k1 = min(most, k0 + a.chunk_keys);
+  if (k1 <= k0 && chunk > 0) return;
+  // this wave's columns
+  const int my_col = first_col + wave * 16 * CT;
+  const int my_lo = my_col / a.group, my_hi = min((my_col + 16 * CT - 1) / a.group, sp.n - 1);
+  const int my_least = sp.limit(my_lo), my_most = my_hi < my_lo ? 0 : sp.limit(my_hi);
+  Columns<DH, CT> cols;
+  cols.start(a, sp, my_col, [](int f, int g) { return f * 32 + g * 8; });
+
+  // Tiles in order: the sealed pages' (or all of a 16-bit pool's), then the open pages'.
+  const int hi = EIGHT ? min(k1, sp.sealed) : k1;
+  const int lo_open = EIGHT ? max(k0, sp.sealed) : k1, start_open = lo_open / PAGED_TILE * PAGED_TILE;
+  const int pool_tiles = hi > k0 ? (hi - k0 + PAGED_TILE - 1) / PAGED_TILE : 0;
+  const int count = pool_tiles + (k1 > lo_open ? (k1 - start_open + PAGED_TILE - 1) / PAGED_TILE : 0);
+  auto base_of = [&](int i) {
+    return i < pool_tiles ? k0 + i * PAGED_TILE : start_open + (i - pool_tiles) * PAGED_TILE;
+  };
+
+  // A thread's part of a tile.  Keys: key tid / 4, a quarter of its row.  Values:
+  // dimensions tid / 4 + 64 r, 16 keys (group tid % 4).
+  constexpr int KW = DH / 64, KW16 = DH / 32, VR = DH / 64;  // 16-byte words of codes, of bf16
+  const int head_block = page * DH, t_key = tid >> 2, t_part = tid & 3, t_dim = tid >> 2;
+  struct Place {
+    int64_t k_block, v_block, k, v;
+  };
+  auto place = [&](int i) {
+    const int base = base_of(i);
+    const bool pool = i < pool_tiles;
+    const int lo = pool ? k0 : lo_open, end = pool ? hi : k1;
+    const int k_at = base + (t_key & ~15), v_at = base + t_part * 16;
+    Place p;
+    p.k_block = pool ? sp.block<true>(c, bt, k_at, lo, end) : sp.block<false>(c, bt, k_at, lo, end);
+    p.v_block = pool ? sp.block<true>(c, bt, v_at, lo, end) : sp.block<false>(c, bt, v_at, lo, end);
+    p.k = p.k_block * head_block + ((k_at & (page - 1)) + (t_key & 15)) * DH + t_part * (DH / 4);
+    p.v = p.v_block * head_block + t_dim * page + (v_at & (page - 1));
+    return p;
+  };
+  // What comes in behind the products: codes, or the keys of a 16-bit pool (its values
+  // as well would not fit the registers of two waves a SIMD).
+  uint4 raw_k[EIGHT ? KW : KW16], raw_v[VR];
+  Place ahead;
+  auto fetch = [&](int i) {
+    if (EIGHT && i >= pool_tiles) return;
+    ahead = place(i);
+#pragma unroll
+    for (int j = 0; j < (EIGHT ? KW : KW16); ++j) {
+      raw_k[j] = make_uint4(0, 0, 0, 0);
+      if (ahead.k_block >= 0)
+        raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + ahead.k + j * 16)
+                         : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + ahead.k + j * 8);
+    }
+    if constexpr (EIGHT) {
+#pragma unroll
+      for (int r = 0; r < VR; ++r) {
+        raw_v[r] = make_uint4(0, 0, 0, 0);
+        if (ahead.v_block >= 0)
+          raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + ahead.v + r * 64 * page);
+      }
+    }
+  };
+  // Tile i -> bf16 in LDS.  In tiles that some row does not see whole, values that are
+  // inf or NaN become zeros.
+  uint32_t odd = 0;
+  auto stage_codes = [&](int i) {
+    TileBuffer<DH>& t = tiles[i & 1];
+    const bool edge = base_of(i) + PAGED_TILE > min(hi, least);
+    const float ks = ahead.k_block >= 0 ? block_scale(c, ahead.k_block, 0) : 1.f;
+    const float vs = ahead.v_block >= 0 ? block_scale(c, ahead.v_block, 1) : 1.f;
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      const uint4 w = raw_k[j];
+      const int piece = t_part * (DH / 32) + 2 * j;
+      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece)) = widen(w.x, w.y, ks);
+      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece + 1)) = widen(w.z, w.w, ks);
+    }
+#pragma unroll
+    for (int r = 0; r < VR; ++r) {
+      uint4 w = raw_v[r];
+      if (edge) {
+        odd |= special_bits<true>(w.x) | special_bits<true>(w.y) | special_bits<true>(w.z) | special_bits<true>(w.w);
+        w = make_uint4(without_special<true>(w.x), without_special<true>(w.y), without_special<true>(w.z),
+                       without_special<true>(w.w));
+      }
+      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part)) = widen(w.x, w.y, vs);
+      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + 1)) = widen(w.z, w.w, vs);
+    }
+    if (tid < 4) there[i & 1][tid] = ahead.v_block >= 0;  // thread t holds group t
+  };
+  auto stage_plain = [&](int i) {
+    TileBuffer<DH>& t = tiles[i & 1];
+    const bool pool = i < pool_tiles, edge = !pool || base_of(i) + PAGED_TILE > min(hi, least);
+    const Place p = EIGHT ? place(i) : ahead;
+    const bf16_t* values = (const bf16_t*)(EIGHT ? c.open_values : c.values);
+#pragma unroll
+    for (int j = 0; j < KW16; ++j) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if constexpr (!EIGHT) w = raw_k[j];
+      else if (p.k_block >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + p.k + j * 8);
+      *reinterpret_cast<uint4*>(t.k + key_piece<DH>(t_key, t_part * (DH / 32) + j)) = w;
+    }
+#pragma unroll
+    for (int r = 0; r < VR; ++r)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (p.v_block >= 0) w = *reinterpret_cast<const uint4*>(values + p.v + r * 64 * page + j * 8);
+        if (edge) {
+          odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
+          w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
+                         without_special<false>(w.w));
+        }
+        *reinterpret_cast<uint4*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + j)) = w;
+      }
+    if (tid < 4) there[i & 1][tid] = p.v_block >= 0;
+  };
+  auto stage = [&](int i) {
+    if (EIGHT && i < pool_tiles) stage_codes(i);
+    else stage_plain(i);
+  };
+
+  if (count > 0) {
+    fetch(0);
+    stage(0);
+  }
+  __syncthreads();
+  for (int i = 0; i < count; ++i) {
+    const bool more = i + 1 < count;
+    if (more) fetch(i + 1);
+    const int base = base_of(i);
+    const bool pool = i < pool_tiles;
+    const int lo = pool ? k0 : lo_open, end = pool ? hi : k1;
+    if (base < my_most) {
+      const TileBuffer<DH>& t = tiles[i & 1];
+      f32x4 s[CT][4];
+      bf16x8 p[CT][2];
+      cols.scores_ahead(s, [&](int sub, int f) {
+        const int key = (col >> 2) * 16 + 4 * sub + (col & 3);
+        return *reinterpret_cast<const bf16x8*>(t.k + key_piece<DH>(key, f * 4 + grp));
+      });
+      const bool mine = there[i & 1][grp];
+      if (base < lo || base + PAGED_TILE > min(end, my_least) || !__all(mine)) cols.hide(s, base, lo, end, mine);
+      cols.softmax(s, p, a.scale2);
+      cols.add_values_ahead(p, [&](int d, int j) {
+        return *reinterpret_cast<const bf16x8*>(t.v + value_piece(d * 16 + col, 2 * grp + j));
+      });
+    }
+    if (more) stage(i + 1);
+    __syncthreads();
+  }
+
+  // every wave writes its own columns
+  const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  const bool any = __any(odd);
+  if (lane == 0) special_of[wave] = any;
+  __syncthreads();
+  const int whole = max(min(hi, least) / PAGED_TILE * PAGED_TILE, k0);
+  const bool special = special_of[0] | special_of[1] | special_of[2] | special_of[3];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const int x = my_col + t * 16 + col, i = x / a.group;
+    if (i >= sp.given) continue;
+    const int64_t to = (sp.row0 + i) * a.heads + sp.h * a.group + x % a.group;
+    if (special) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          cols.o[t][d][k] += special_sum<DH, EIGHT>(c, bt, sp, d * 16 + grp * 4 + k, whole, min(sp.limit(i), k1));
+    }
+    if (sp.limit(i) == 0) {  // a row that sees no key is zero
+      cols.m[t] = -INFINITY;
+      cols.l[t][0] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) cols.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (a.chunks == 1) {
+      const float sum = cols.l[t][0], inv = sum == 0.f ? 0.f : 1.f / sum;
+      bf16_t* out = (bf16_t*)a.out + to * DH + grp * 4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<uint2*>(out + d * 16) =
+            make_uint2(pack_bf16x2(cols.o[t][d][0] * inv, cols.o[t][d][1] * inv),
+                       pack_bf16x2(cols.o[t][d][2] * inv, cols.o[t][d][3] * inv));
+      continue;
+    }
+    if (sp.limit(i) <= k0 && chunk > 0) continue;  // the join knows which chunks a row has
+    float* part = a.part + (chunk * T_heads + to) * DH + grp * 4;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(part + d * 16) = cols.o[t][d];
+    if (grp == 0) a.stat[chunk * T_heads + to] = make_float2(cols.m[t], cols.l[t][0]);
+  }
+}
+
+template <int DH, int CT>
+static void launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
+                   unsigned grid, hipStream_t st) {
+  if (c->eight_bit)
+    paged_tiles_kernel<DH, CT, true><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
+  else
+    paged_tiles_kernel<DH, CT, false><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
+}
+
+void paged_tiles_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
+                        const AttendPlan& p, unsigned grid, hipStream_t st) {
+  if (c->head_dim == 64) {
+    if (p.column_tiles == 1) launch<64, 1>(c, b, a, grid, st);
+    else launch<64, 2>(c, b, a, grid, st);
+  } else {
+    if (p.column_tiles == 1) launch<128, 1>(c, b, a, grid, st);
+    else launch<128, 2>(c, b, a, grid, st);
+  }
+}
