@@ -13,8 +13,7 @@ struct PagedCache {
   int8_t* exponents;
   void* open_keys;
   void* open_values;
-  int64_t pages;
-  int page, kv_heads, head_dim, slots, open_pages;
+  int pages, page, shift, kv_heads, head_dim, slots, open_pages;  // page = 1 << shift
 };
 
 struct PagedBatch {
@@ -41,9 +40,9 @@ struct PagedBatch {
     return (int)min((int64_t)n, (int64_t)width * page - held);
   }
   // Page of the pool, -1 where the table names none.
-  __device__ __forceinline__ int64_t page_of(int b, int p, int64_t pages) const {
+  __device__ __forceinline__ int page_of(int b, int p, int pages) const {
     if (p < 0 || p >= width) return -1;
-    const int64_t id = table[(int64_t)b * width + p];
+    const int id = table[(int64_t)b * width + p];
     return id >= 0 && id < pages ? id : -1;
   }
   // Slot of the open pages, -1 where there is none.
@@ -54,8 +53,8 @@ struct PagedBatch {
 };
 
 // Open page `p` of a slot: its index among all open pages.
-__device__ __forceinline__ int64_t open_page(const PagedCache& c, int slot, int p) {
-  return (int64_t)slot * c.open_pages + p % c.open_pages;
+__device__ __forceinline__ int open_page(const PagedCache& c, int slot, int p) {
+  return slot * c.open_pages + p % c.open_pages;
 }
 
 // 2^e as a float, e in [-126, 127].
@@ -70,7 +69,7 @@ struct AttendArgs {
   int64_t ldq;
   float* part;   // unnormalised outputs [chunks][rows * heads][head_dim]
   float2* stat;  // (maximum in base 2, sum) [chunks][rows * heads]
-  int heads, group, chunk_keys, chunks, query_tiles;
+  int heads, group, chunk_keys, chunks, query_tiles, join_ways;
   float scale2;  // softmax scale * log2 e
   int zero_blocks;  // workgroups behind the launch's others that clear the rows behind the last sequence
 };
@@ -85,10 +84,10 @@ __device__ __forceinline__ void zero_rest(const PagedBatch& bt, T* out, int64_t 
 }
 
 // Where the 8-bit pages of a sequence end (keys before it are sealed).
-__device__ __forceinline__ int sealed_keys(const PagedBatch& bt, int held, int end, int page,
+__device__ __forceinline__ int sealed_keys(const PagedCache& c, const PagedBatch& bt, int held, int end,
                                            bool eight) {
   if (!eight) return end;
-  return (bt.final_rows ? end : held) / page * page;
+  return (bt.final_rows ? end : held) >> c.shift << c.shift;
 }
 
 // The first key whose place in the open pages another one has taken (windows longer

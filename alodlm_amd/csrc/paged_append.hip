@@ -229,7 +229,7 @@ paged_append_kernel(PagedCache c, PagedBatch bt, AppendInputs<T> in) {
   int held = bt.held(b, ps);
   if (held < 0) return;
   int n = bt.row_count(b, held, ps);
-  const int first = held / ps;
+  const int first = held >> c.shift;
   if (in.counts) {  // retire: everything kept is in open pages already
     n = min(max(in.counts[b], 0), n);
     held += n;
@@ -239,9 +239,9 @@ paged_append_kernel(PagedCache c, PagedBatch bt, AppendInputs<T> in) {
   const int64_t head_block = (int64_t)ps * dh;
   if constexpr (!EIGHT) {
     const int p = first + i, start = p * ps;
-    const int64_t page = bt.page_of(b, p, c.pages);
+    const int page = bt.page_of(b, p, c.pages);
     if (page < 0 || start >= end) return;
-    const int64_t at = (page * c.kv_heads + h) * head_block;
+    const int64_t at = ((int64_t)page * c.kv_heads + h) * head_block;
     write_rows<VEC, T>(c, in, (T*)c.keys + at, (T*)c.values + at, h, start, max(held - start, 0),
                        min(end - start, ps), row0, held);
     return;
@@ -249,10 +249,10 @@ paged_append_kernel(PagedCache c, PagedBatch bt, AppendInputs<T> in) {
   const int slot = bt.slot(b, c.slots);
   if (slot < 0) return;
   // pages [first, sealed) fill up; `sealed` is the first one that stays open
-  const int sealed = bt.final_rows || in.counts ? end / ps : first;
+  const int sealed = bt.final_rows || in.counts ? end >> c.shift : first;
   if (first + i < sealed) {
     const int p = first + i;
-    const int64_t page = bt.page_of(b, p, c.pages);
+    const int page = bt.page_of(b, p, c.pages);
     if (page >= 0)
       seal_page<VEC, T>(c, in, page, open_page(c, slot, p), h, p * ps, row0, held, (T*)lds_raw, red);
   }
@@ -263,7 +263,7 @@ paged_append_kernel(PagedCache c, PagedBatch bt, AppendInputs<T> in) {
   const int start = p * ps;
   // rows further on than the open pages reach would take each other's place
   if (start >= end || p - sealed >= c.open_pages) return;
-  const int64_t at = (open_page(c, slot, p) * c.kv_heads + h) * head_block;
+  const int64_t at = ((int64_t)open_page(c, slot, p) * c.kv_heads + h) * head_block;
   write_rows<VEC, T>(c, in, (T*)c.open_keys + at, (T*)c.open_values + at, h, start,
                      max(held - start, 0), min(end - start, ps), row0, held);
 }
@@ -289,8 +289,9 @@ int paged_check(const alodlm_paged_cache* c, const alodlm_paged_batch* b) {
   ALODLM_CHECK_ARG(c->kv_heads >= 1 && c->kv_heads <= 1024, "paged: kv_heads out of range");
   ALODLM_CHECK_ARG(c->pages >= 1 && c->pages < (1ll << 31), "paged: pages out of range");
   ALODLM_CHECK_ARG(!c->eight_bit || (c->slots >= 1 && c->slots < (1ll << 31) &&
-                                     c->open_pages >= 1 && c->open_pages < (1ll << 20)),
-                   "paged: an 8-bit cache needs slots and open pages");
+                                     c->open_pages >= 1 && c->open_pages < (1ll << 20) &&
+                                     c->slots * c->open_pages < (1ll << 31)),
+                   "paged: an 8-bit cache needs slots and open pages (fewer than 2^31)");
   ALODLM_CHECK_ARG(b->sequences >= 0 && b->sequences < (1ll << 24) && b->rows >= 0 &&
                        b->rows < (1ll << 30) && b->max_rows >= 0 && b->max_rows <= b->rows,
                    "paged: sequences, rows or max_rows out of range");
@@ -305,8 +306,8 @@ int paged_check(const alodlm_paged_cache* c, const alodlm_paged_batch* b) {
 }
 
 PagedCache paged_cache(const alodlm_paged_cache* c) {
-  return {c->keys, c->values, c->exponents, c->open_keys, c->open_values, c->pages,
-          (int)c->page_size, (int)c->kv_heads, (int)c->head_dim, (int)c->slots,
+  return {c->keys, c->values, c->exponents, c->open_keys, c->open_values, (int)c->pages,
+          (int)c->page_size, __builtin_ctz((unsigned)c->page_size), (int)c->kv_heads, (int)c->head_dim, (int)c->slots,
           (int)c->open_pages};
 }
 

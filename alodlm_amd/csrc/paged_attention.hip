@@ -36,6 +36,12 @@ __device__ __forceinline__ void load4(const T* p, float* v) {
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float x, float y, float z, float w) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(x, y, z, w);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x, y), pack_bf16x2(z, w));
+}
+
 // q . (the key at p) over dh dimensions, q in LDS.
 template <typename T>
 __device__ __forceinline__ float dot_key(const float* q, const T* p, int dh) {
@@ -109,7 +115,7 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     live = i < given_rows(bt, b);
     if (i < n) {
       const int end = held + n;
-      sealed = sealed_keys(bt, held, end, page, EIGHT);
+      sealed = sealed_keys(c, bt, held, end, EIGHT);
       last = EIGHT ? open_end(c, sealed, end) : end;
       limit = min(held + i + 1, last);
       if (EIGHT) slot = bt.slot(b, c.slots);
@@ -127,10 +133,10 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   // the place of the 16 keys from `key` on: codes (and their exponents' place), or rows
   auto locate = [&](int key, int64_t* at, int64_t* id) {
-    const int p = key / page;
+    const int p = key >> c.shift;
     if (EIGHT && key >= sealed) {
       *id = -1;
-      *at = slot < 0 ? -1 : (open_page(c, slot, p) * c.kv_heads + kvh) * block;
+      *at = slot < 0 ? -1 : ((int64_t)open_page(c, slot, p) * c.kv_heads + kvh) * block;
     } else {
       *id = bt.page_of(b, p, c.pages);
       *at = *id < 0 ? -1 : (*id * c.kv_heads + kvh) * block;
@@ -143,7 +149,7 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       int64_t at, id;
       locate(key, &at, &id);
       if (at >= 0) {
-        const int64_t k_at = at + (int64_t)(key % page) * dh;
+        const int64_t k_at = at + (int64_t)(key & (page - 1)) * dh;
         if (!EIGHT) s = dot_key(q, (const T*)c.keys + k_at, dh);
         else if (id < 0) s = dot_key(q, (const T*)c.open_keys + k_at, dh);
         else s = dot_key(q, (const e4m3_t*)c.keys + k_at, dh) *
@@ -171,7 +177,7 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       for (int j = 0; j < 4; ++j) {
         const int d = lane + 64 * j;
         if (d >= dh) break;
-        const int64_t v_at = at + (int64_t)d * page + (t + g) % page;
+        const int64_t v_at = at + (int64_t)d * page + ((t + g) & (page - 1));
         if (!EIGHT) o[j] = add_values(o[j], ps[wave] + g, (const T*)c.values + v_at, n, 1.f);
         else if (id < 0) o[j] = add_values(o[j], ps[wave] + g, (const T*)c.open_values + v_at, n, 1.f);
         else o[j] = add_values(o[j], ps[wave] + g, (const e4m3_t*)c.values + v_at, n, scale);
@@ -192,37 +198,39 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   for (int j = 0, d = lane; d < dh; ++j, d += 64) a.part[(chunk * T_heads + at) * dh + d] = o[j];
 }
 
-// Joins the chunks of a row and head, one workgroup each.  Four dimensions a thread;
-// as many chunks at once as that leaves threads for, added in a fixed order.
+// Joins the chunks of every row and head.  Four dimensions a thread, a.join_ways
+// threads' worth of chunks at once, as many rows and heads a workgroup as that leaves
+// room for; a way takes every join_ways-th chunk, and the ways are added in order.
 template <typename T, bool EIGHT>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   __shared__ __attribute__((aligned(16))) float4 o_of[256];
-  __shared__ float sum_of[256];
-  const int lane = threadIdx.x & 63, dh = c.head_dim, page = c.page;
-  const int64_t unit = blockIdx.x, T_heads = (int64_t)bt.rows * a.heads;
+  __shared__ float m_of[256], sum_of[256];
+  const int dh = c.head_dim, page = c.page, quads = dh / 4, ways = a.join_ways;
+  const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  const int per_unit = quads * ways, inside = threadIdx.x % per_unit;
+  const int64_t unit = (int64_t)blockIdx.x * (256 / per_unit) + threadIdx.x / per_unit;
+  const int way = inside / quads, d = inside % quads * 4;
   const int head = (int)(unit % a.heads);
   const int i = (int)(unit / a.heads % bt.max_rows);
   const int b = (int)(unit / a.heads / bt.max_rows);
-  if (i >= given_rows(bt, b)) return;
-  const int held = bt.held(b, page);
-  const int n = held < 0 ? 0 : bt.row_count(b, held, page);
-  int limit = 0;
-  if (i < n) {
-    const int end = held + n, sealed = sealed_keys(bt, held, end, page, EIGHT);
-    limit = min(held + i + 1, EIGHT ? open_end(c, sealed, end) : end);
-  }
-  const int count = max((limit + a.chunk_keys - 1) / a.chunk_keys, 1);
-  const int64_t at = ((int64_t)bt.first_row(b) + i) * a.heads + head;
-  float M = -INFINITY;
-  for (int k = lane; k < count; k += 64) M = fmaxf(M, a.stat[k * T_heads + at].x);
-  M = wave_max(M);
-  const float base = M == -INFINITY ? 0.f : M;
-  const int quads = dh / 4, ways = min(256 / quads, 16);
-  const int way = threadIdx.x / quads, d = threadIdx.x % quads * 4;
-  float sum = 0.f;
+  const bool live = (int)threadIdx.x < 256 / per_unit * per_unit && b < bt.sequences && i < given_rows(bt, b);
+  float m = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (way < ways) {
+  int64_t at = 0;
+  if (live) {
+    const int held = bt.held(b, page);
+    const int n = held < 0 ? 0 : bt.row_count(b, held, page);
+    int limit = 0;
+    if (i < n) {
+      const int end = held + n, sealed = sealed_keys(c, bt, held, end, EIGHT);
+      limit = min(held + i + 1, EIGHT ? open_end(c, sealed, end) : end);
+    }
+    const int count = max((limit + a.chunk_keys - 1) / a.chunk_keys, 1);
+    at = ((int64_t)bt.first_row(b) + i) * a.heads + head;
+#pragma unroll 8
+    for (int k = way; k < count; k += ways) m = fmaxf(m, a.stat[k * T_heads + at].x);
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
     for (int k = way; k < count; k += ways) {
       const float2 st = a.stat[k * T_heads + at];
@@ -235,32 +243,36 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       o.w = fmaf(x.w, f, o.w);
     }
   }
-  o_of[threadIdx.x] = o;
-  sum_of[threadIdx.x] = sum;
-  __syncthreads();
-  if (way != 0) return;
-  for (int w = 1; w < ways; ++w) {
-    const float4 x = o_of[w * quads + threadIdx.x];
-    sum += sum_of[w * quads + threadIdx.x];
-    o.x += x.x;
-    o.y += x.y;
-    o.z += x.z;
-    o.w += x.w;
+  if (ways > 1) {
+    o_of[threadIdx.x] = o;
+    m_of[threadIdx.x] = m;
+    sum_of[threadIdx.x] = sum;
+    __syncthreads();
+    if (way != 0) return;
+    float M = m;
+    for (int w = 1; w < ways; ++w) M = fmaxf(M, m_of[threadIdx.x + w * quads]);
+    const float base = M == -INFINITY ? 0.f : M;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < ways; ++w) {
+      const int t = threadIdx.x + w * quads;
+      const float f = exp2f(m_of[t] - base);
+      const float4 x = o_of[t];
+      sum = fmaf(sum_of[t], f, sum);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
+    }
   }
+  if (!live) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* out = (T*)a.out + at * dh + d;
-  Elem<T>::store(out, 0, o.x * inv);
-  Elem<T>::store(out, 1, o.y * inv);
-  Elem<T>::store(out, 2, o.z * inv);
-  Elem<T>::store(out, 3, o.w * inv);
+  store4((T*)a.out + at * dh + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // ----------------------------------------------------------------------------
 // Host
 // ----------------------------------------------------------------------------
-#ifndef SPLIT_WANT
-#define SPLIT_WANT 2048
-#endif
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Keys per chunk, in whole 64-key tiles: `want` workgroups or wavefronts in all where
@@ -283,7 +295,7 @@ static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_ba
   const int waves = p.split_columns ? 4 : 1;
   p.column_tiles = columns <= 16 * waves ? 1 : 2;
   p.query_tiles = (int)ceil_div(columns, 16 * p.column_tiles * waves);
-  cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, p.split_columns ? 1024 : SPLIT_WANT,
+  cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, p.split_columns || b->sequences == 1 ? 1024 : 2048,
            512 * p.column_tiles);
   return p;
 }
@@ -313,7 +325,13 @@ static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* 
   if (plan.split_columns) paged_tiles_launch(c, b, a, plan, (unsigned)blocks, st);
   else if (plan.query_tiles) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
   else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
-  if (a.chunks > 1 && units) paged_join_kernel<T, EIGHT><<<(unsigned)units, 256, 0, st>>>(dc, db, a);
+  if (a.chunks > 1 && units) {
+    const int quads = (int)c->head_dim / 4;
+    a.join_ways = 1;
+    while (a.join_ways < min(a.chunks, 16) && quads * a.join_ways * 2 <= 256) a.join_ways *= 2;
+    const int64_t per_block = 256 / (quads * a.join_ways);
+    paged_join_kernel<T, EIGHT><<<(unsigned)ceil_div(units, per_block), 256, 0, st>>>(dc, db, a);
+  }
   ALODLM_CHECK_LAUNCH("paged_attention");
   return ALODLM_OK;
 }
@@ -336,7 +354,7 @@ extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alo
   const AttendPlan plan = attend_plan(cache, batch, heads);
   ALODLM_CHECK_ARG(plan.chunks == 1 || workspace, "paged_attention: no workspace");
   AttendArgs a = {q, out, ldq, workspace, nullptr, (int)heads, (int)(heads / cache->kv_heads),
-                  (int)plan.chunk_keys, (int)plan.chunks, plan.query_tiles, scale * LOG2E, 0};
+                  (int)plan.chunk_keys, (int)plan.chunks, plan.query_tiles, 1, scale * LOG2E, 0};
   if (zero_rest) a.zero_blocks = (int)min(ceil_div(batch->rows * heads * cache->head_dim, 8192), (int64_t)64);
   a.stat = reinterpret_cast<float2*>(workspace + plan.chunks * batch->rows * heads * cache->head_dim);
   ALODLM_DISPATCH(cache->dtype, T, {

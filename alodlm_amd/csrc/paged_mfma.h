@@ -70,7 +70,7 @@ struct Span {
     s.n = held < 0 ? 0 : bt.row_count(b, held, c.page);
     s.held = max(held, 0);
     const int end = s.held + s.n;
-    s.sealed = EIGHT ? sealed_keys(bt, s.held, end, c.page, true) : end;
+    s.sealed = EIGHT ? sealed_keys(c, bt, s.held, end, true) : end;
     s.reach = EIGHT ? open_end(c, s.sealed, end) : end;
     s.slot = EIGHT ? bt.slot(b, c.slots) : 0;
     s.row0 = bt.first_row(b);
@@ -78,24 +78,25 @@ struct Span {
   }
   // Keys that row i sees.
   __device__ __forceinline__ int limit(int i) const { return i < n ? min(held + i + 1, reach) : 0; }
-  // The block (page and head, of the pool or among the open pages) of the 16 keys from
-  // `key` on, as far as [lo, hi) reaches into them; -1 for none.
+  // The page (of the pool, or among all open ones) of the 16 keys from `key` on, as far as
+  // [lo, hi) reaches into them; -1 for none.
   template <bool POOL>
-  __device__ __forceinline__ int64_t block(const PagedCache& c, const PagedBatch& bt, int key, int lo,
-                                           int hi) const {
+  __device__ __forceinline__ int page(const PagedCache& c, const PagedBatch& bt, int key, int lo,
+                                      int hi) const {
     if (key + 15 < lo || key >= hi) return -1;
-    const int p = key / c.page;
-    if (!POOL) return slot < 0 ? -1 : open_page(c, slot, p) * c.kv_heads + h;
-    const int64_t id = bt.page_of(b, p, c.pages);
-    return id < 0 ? -1 : id * c.kv_heads + h;
+    const int p = key >> c.shift;
+    if (!POOL) return slot < 0 ? -1 : open_page(c, slot, p);
+    return bt.page_of(b, p, c.pages);
+  }
+  // First value of a page's block for this head.
+  __device__ __forceinline__ int64_t block(const PagedCache& c, int page, int head_block) const {
+    return ((int64_t)page * c.kv_heads + h) * head_block;
+  }
+  // 2^exponent of a pool page's keys (side 0) or values (side 1).
+  __device__ __forceinline__ float scale(const PagedCache& c, int page, int side) const {
+    return exp2_int(c.exponents[((int64_t)page * 2 + side) * c.kv_heads + h]);
   }
 };
-
-// 2^exponent of a pool block's keys (side 0) or values (side 1).
-__device__ __forceinline__ float block_scale(const PagedCache& c, int64_t block, int side) {
-  const int64_t id = block / c.kv_heads;
-  return exp2_int(c.exponents[(id * 2 + side) * c.kv_heads + (block - id * c.kv_heads)]);
-}
 
 // Tiles in which some row sees a key that another does not are multiplied with zeros in
 // the place of values that are inf or NaN: 0 times one of them would not be 0 for the
@@ -107,9 +108,9 @@ __device__ __forceinline__ float special_sum(const PagedCache& c, const PagedBat
   float sum = 0.f;
   for (int key = from; key < to; ++key) {
     const bool pool = !EIGHT || key < sp.sealed;
-    const int64_t block = pool ? sp.block<true>(c, bt, key, key, key + 1) : sp.block<false>(c, bt, key, key, key + 1);
-    if (block < 0) continue;
-    const int64_t at = (block * DH + d) * c.page + (key & (c.page - 1));
+    const int page = pool ? sp.page<true>(c, bt, key, key, key + 1) : sp.page<false>(c, bt, key, key, key + 1);
+    if (page < 0) continue;
+    const int64_t at = sp.block(c, page, c.page * DH) + (int64_t)d * c.page + (key & (c.page - 1));
     const float v = EIGHT && pool ? __builtin_amdgcn_cvt_f32_fp8(((const e4m3_t*)c.values)[at], 0)
                                   : bf16_to_float(((const bf16_t*)(EIGHT ? c.open_values : c.values))[at]);
     if (!(fabsf(v) < INFINITY)) sum += v;

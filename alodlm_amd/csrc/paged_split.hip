@@ -16,7 +16,7 @@ template <int DH> struct CodeTile {
 };
 
 template <int DH, int CT, bool EIGHT>
-__global__ void __launch_bounds__(64 * PAGED_WAVES, CT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(64 * PAGED_WAVES, CT == 1 ? 3 : 1)
 paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   constexpr int DT = DH / 16;
   __shared__ __attribute__((aligned(16))) float buf[PAGED_WAVES][16 * (DH + 4)];
@@ -49,37 +49,38 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   Columns<DH, CT> cols;
   cols.start(a, sp, first_col, [](int f, int g) { return (f / 2) * 64 + g * 16 + (f % 2) * 8; });
 
-  const int64_t head_block = (int64_t)page * DH;
-  // Places of a tile in a block: keys of group (lane % 16) / 4, values of group lane / 16.
-  auto key_place = [&](int base, int64_t block) {
+  const int head_block = page * DH;
+  // Places of a tile: keys of group (lane % 16) / 4, values of group lane / 16
+  // (of page `id`; not followed where that is -1).
+  auto key_place = [&](int base, int id) {
     const int in_page = (base + (col >> 2) * 16) & (page - 1);
-    return block * head_block + (int64_t)(in_page + (col & 3)) * DH + grp * 16;
+    return sp.block(c, id, head_block) + ((in_page + (col & 3)) * DH + grp * 16);
   };
-  auto value_place = [&](int base, int64_t block) {
-    return block * head_block + (int64_t)col * page + ((base + grp * 16) & (page - 1));
+  auto value_place = [&](int base, int id) {
+    return sp.block(c, id, head_block) + (col * page + ((base + grp * 16) & (page - 1)));
   };
-  auto load_key_codes = [&](CodeTile<DH>& t, int base, int64_t block) {
-    const e4m3_t* p = (const e4m3_t*)c.keys + key_place(base, block);
+  auto load_key_codes = [&](CodeTile<DH>& t, int base, int id) {
+    const e4m3_t* p = (const e4m3_t*)c.keys + key_place(base, id);
     t.k_scale = 1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < DH / 64; ++j) {
         t.k[i][j] = make_uint4(0, 0, 0, 0);
-        if (block >= 0) t.k[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + j * 64);
+        if (id >= 0) t.k[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + j * 64);
       }
-    if (block >= 0) t.k_scale = block_scale(c, block, 0);
+    if (id >= 0) t.k_scale = sp.scale(c, id, 0);
   };
-  auto load_value_codes = [&](CodeTile<DH>& t, int base, int64_t block) {
-    const e4m3_t* p = (const e4m3_t*)c.values + value_place(base, block);
+  auto load_value_codes = [&](CodeTile<DH>& t, int base, int id) {
+    const e4m3_t* p = (const e4m3_t*)c.values + value_place(base, id);
     t.v_scale = 1.f;
-    t.there = block >= 0;
+    t.there = id >= 0;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       t.v[d] = make_uint4(0, 0, 0, 0);
-      if (block >= 0) t.v[d] = *reinterpret_cast<const uint4*>(p + d * 16 * page);
+      if (id >= 0) t.v[d] = *reinterpret_cast<const uint4*>(p + d * 16 * page);
     }
-    if (block >= 0) t.v_scale = block_scale(c, block, 1);
+    if (id >= 0) t.v_scale = sp.scale(c, id, 1);
   };
   auto key_of = [&](const CodeTile<DH>& t, int i, int f) {
     const uint4 w = t.k[i][f / 2];
@@ -102,10 +103,10 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     int base = first_tile(k0);
     if (base >= to) return;
     CodeTile<DH> tile;
-    load_key_codes(tile, base, sp.block<true>(c, bt, base + (col >> 2) * 16, 0, to));
-    load_value_codes(tile, base, sp.block<true>(c, bt, base + grp * 16, 0, to));
-    int64_t k_next = sp.block<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
-    int64_t v_next = sp.block<true>(c, bt, base + STEP + grp * 16, 0, to);
+    load_key_codes(tile, base, sp.page<true>(c, bt, base + (col >> 2) * 16, 0, to));
+    load_value_codes(tile, base, sp.page<true>(c, bt, base + grp * 16, 0, to));
+    int k_next = sp.page<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
+    int v_next = sp.page<true>(c, bt, base + STEP + grp * 16, 0, to);
     while (true) {
       const bool more = base + STEP < to;
       f32x4 s[CT][4];
@@ -118,16 +119,16 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       if (!more) break;
       base += STEP;
       load_value_codes(tile, base, v_next);
-      k_next = sp.block<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
-      v_next = sp.block<true>(c, bt, base + STEP + grp * 16, 0, to);
+      k_next = sp.page<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
+      v_next = sp.page<true>(c, bt, base + STEP + grp * 16, 0, to);
     }
   };
   // Tiles [from, to) of codes that some row does not see whole.
   auto edge_code_tiles = [&](int from, int to) {
     for (int base = first_tile(from); base < to; base += STEP) {
       CodeTile<DH> tile;
-      load_key_codes(tile, base, sp.block<true>(c, bt, base + (col >> 2) * 16, k0, to));
-      load_value_codes(tile, base, sp.block<true>(c, bt, base + grp * 16, k0, to));
+      load_key_codes(tile, base, sp.page<true>(c, bt, base + (col >> 2) * 16, k0, to));
+      load_value_codes(tile, base, sp.page<true>(c, bt, base + grp * 16, k0, to));
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
       cols.scores(s, [&](int i, int f) { return key_of(tile, i, f); });
@@ -152,22 +153,22 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     const bf16_t* keys = (const bf16_t*)(POOL ? c.keys : c.open_keys);
     const bf16_t* values = (const bf16_t*)(POOL ? c.values : c.open_values);
     for (int base = first_tile(from); base < to; base += STEP) {
-      const int64_t k_block = sp.block<POOL>(c, bt, base + (col >> 2) * 16, lo, to);
-      const int64_t v_block = sp.block<POOL>(c, bt, base + grp * 16, lo, to);
-      const bf16_t* kp = keys + key_place(base, k_block);
-      const bf16_t* vp = values + value_place(base, v_block);
+      const int k_page = sp.page<POOL>(c, bt, base + (col >> 2) * 16, lo, to);
+      const int v_page = sp.page<POOL>(c, bt, base + grp * 16, lo, to);
+      const bf16_t* kp = keys + key_place(base, k_page);
+      const bf16_t* vp = values + value_place(base, v_page);
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
       cols.scores(s, [&](int i, int f) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (k_block >= 0) w = *reinterpret_cast<const uint4*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
+        if (k_page >= 0) w = *reinterpret_cast<const uint4*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
         return __builtin_bit_cast(bf16x8, w);
       });
-      if (!whole || !__all(v_block >= 0)) cols.hide(s, base, lo, to, v_block >= 0);
+      if (!whole || !__all(v_page >= 0)) cols.hide(s, base, lo, to, v_page >= 0);
       cols.softmax(s, p, a.scale2);
       cols.add_values(p, [&](int d, int j) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (v_block >= 0) w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
+        if (v_page >= 0) w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
         if (!whole) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) |
                  special_bits<false>(w.w);

@@ -76,7 +76,8 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   constexpr int KW = DH / 64, KW16 = DH / 32, VR = DH / 64;  // 16-byte words of codes, of bf16
   const int head_block = page * DH, t_key = tid >> 2, t_part = tid & 3, t_dim = tid >> 2;
   struct Place {
-    int64_t k_block, v_block, k, v;
+    int k_page, v_page;
+    int64_t k, v;
   };
   auto place = [&](int i) {
     const int base = base_of(i);
@@ -84,10 +85,10 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     const int lo = pool ? k0 : lo_open, end = pool ? hi : k1;
     const int k_at = base + (t_key & ~15), v_at = base + t_part * 16;
     Place p;
-    p.k_block = pool ? sp.block<true>(c, bt, k_at, lo, end) : sp.block<false>(c, bt, k_at, lo, end);
-    p.v_block = pool ? sp.block<true>(c, bt, v_at, lo, end) : sp.block<false>(c, bt, v_at, lo, end);
-    p.k = p.k_block * head_block + ((k_at & (page - 1)) + (t_key & 15)) * DH + t_part * (DH / 4);
-    p.v = p.v_block * head_block + t_dim * page + (v_at & (page - 1));
+    p.k_page = pool ? sp.page<true>(c, bt, k_at, lo, end) : sp.page<false>(c, bt, k_at, lo, end);
+    p.v_page = pool ? sp.page<true>(c, bt, v_at, lo, end) : sp.page<false>(c, bt, v_at, lo, end);
+    p.k = sp.block(c, p.k_page, head_block) + (((k_at & (page - 1)) + (t_key & 15)) * DH + t_part * (DH / 4));
+    p.v = sp.block(c, p.v_page, head_block) + (t_dim * page + (v_at & (page - 1)));
     return p;
   };
   // What comes in behind the products: codes, or the keys of a 16-bit pool (its values
@@ -100,7 +101,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
     for (int j = 0; j < (EIGHT ? KW : KW16); ++j) {
       raw_k[j] = make_uint4(0, 0, 0, 0);
-      if (ahead.k_block >= 0)
+      if (ahead.k_page >= 0)
         raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + ahead.k + j * 16)
                          : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + ahead.k + j * 8);
     }
@@ -108,7 +109,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
       for (int r = 0; r < VR; ++r) {
         raw_v[r] = make_uint4(0, 0, 0, 0);
-        if (ahead.v_block >= 0)
+        if (ahead.v_page >= 0)
           raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + ahead.v + r * 64 * page);
       }
     }
@@ -119,8 +120,8 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   auto stage_codes = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
     const bool edge = base_of(i) + PAGED_TILE > min(hi, least);
-    const float ks = ahead.k_block >= 0 ? block_scale(c, ahead.k_block, 0) : 1.f;
-    const float vs = ahead.v_block >= 0 ? block_scale(c, ahead.v_block, 1) : 1.f;
+    const float ks = ahead.k_page >= 0 ? sp.scale(c, ahead.k_page, 0) : 1.f;
+    const float vs = ahead.v_page >= 0 ? sp.scale(c, ahead.v_page, 1) : 1.f;
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
       const uint4 w = raw_k[j];
@@ -139,7 +140,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part)) = widen(w.x, w.y, vs);
       *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + 1)) = widen(w.z, w.w, vs);
     }
-    if (tid < 4) there[i & 1][tid] = ahead.v_block >= 0;  // thread t holds group t
+    if (tid < 4) there[i & 1][tid] = ahead.v_page >= 0;  // thread t holds group t
   };
   auto stage_plain = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
@@ -150,7 +151,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     for (int j = 0; j < KW16; ++j) {
       uint4 w = make_uint4(0, 0, 0, 0);
       if constexpr (!EIGHT) w = raw_k[j];
-      else if (p.k_block >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + p.k + j * 8);
+      else if (p.k_page >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + p.k + j * 8);
       *reinterpret_cast<uint4*>(t.k + key_piece<DH>(t_key, t_part * (DH / 32) + j)) = w;
     }
 #pragma unroll
@@ -158,7 +159,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (p.v_block >= 0) w = *reinterpret_cast<const uint4*>(values + p.v + r * 64 * page + j * 8);
+        if (p.v_page >= 0) w = *reinterpret_cast<const uint4*>(values + p.v + r * 64 * page + j * 8);
         if (edge) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
@@ -166,7 +167,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         }
         *reinterpret_cast<uint4*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + j)) = w;
       }
-    if (tid < 4) there[i & 1][tid] = p.v_block >= 0;
+    if (tid < 4) there[i & 1][tid] = p.v_page >= 0;
   };
   auto stage = [&](int i) {
     if (EIGHT && i < pool_tiles) stage_codes(i);

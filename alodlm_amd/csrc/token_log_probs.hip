@@ -63,14 +63,10 @@ struct Softmax {
 };
 
 __device__ __forceinline__ Softmax wave_join(Softmax a, float c) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    Softmax o;
-    o.m = __shfl_xor(a.m, off, 64);
-    o.s = __shfl_xor(a.s, off, 64);
-    o.t = __shfl_xor(a.t, off, 64);
-    a.join(o, c);
-  }
+  const float to = wave_max(a.m);  // one rescaling, then sums
+  if (to > a.m) a.rescale(to, c);
+  a.s = wave_sum(a.s);
+  a.t = wave_sum(a.t);
   return a;
 }
 
@@ -127,22 +123,23 @@ struct TopShared {
   int count, listed, above;
 };
 
-// Rank of every thread's key (larger first, the lower thread among equals) among the
-// workgroup's; the thread of rank top - 1 publishes its key.
+// The top-th largest of the workgroup's keys into sh.threshold: the smallest of those
+// that fewer than `top` exceed.
 __device__ __forceinline__ void publish_threshold(TopShared& sh, uint32_t key, int top) {
   sh.keys[threadIdx.x] = key;
-  if (threadIdx.x == 0) sh.count = sh.listed = 0;
+  if (threadIdx.x == 0) {
+    sh.count = sh.listed = 0;
+    sh.threshold = 0xffffffffu;
+  }
   __syncthreads();
-  int rank = 0;
+  int above = 0;
   const uint4* k4 = reinterpret_cast<const uint4*>(sh.keys);
-  const int me = threadIdx.x;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < LP_THREADS / 4; ++i) {
     const uint4 k = k4[i];
-    rank += (k.x > key || (k.x == key && 4 * i < me)) + (k.y > key || (k.y == key && 4 * i + 1 < me)) +
-            (k.z > key || (k.z == key && 4 * i + 2 < me)) + (k.w > key || (k.w == key && 4 * i + 3 < me));
+    above += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
   }
-  if (rank == top - 1) sh.threshold = key;
+  if (above < top) atomicMin(&sh.threshold, key);
   __syncthreads();
 }
 
@@ -154,6 +151,7 @@ __device__ __forceinline__ void rank_list(TopShared& sh, int n, int top) {
   for (int i = threadIdx.x; i < n; i += LP_THREADS) {
     const uint64_t e = sh.list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += sh.list[j] > e;
     if (rank < top) sh.sorted[rank] = e;
   }
@@ -220,14 +218,19 @@ __device__ void select_any(TopShared& sh, const T* x, int first, int last, int t
 
 // The `top` first of the elements that this workgroup's threads went through, sorted
 // into sh.sorted: granules [g0, g1) (thread j those at g0 + j + 256 i), the row's head
-// and tail where they belong to it (thread j element j, value in `edge`).
-template <typename T>
+// and tail where they belong to it (thread j its element j).  `each` gives a thread's
+// granules again where it holds them, else (HELD false) the members' are read again.
+template <bool HELD, typename T, typename Each>
 __device__ void select_top(TopShared& sh, const T* x, const RowParts& parts, int g0, int g1,
-                           bool has_head, bool has_tail, int V, float largest, int top) {
+                           bool has_head, bool has_tail, int V, float largest, int top, Each each) {
   constexpr int N = Granule<T>::N;
   publish_threshold(sh, order_key(largest), top);
   const uint32_t tau = sh.threshold;
-  if (order_key(largest) >= tau) sh.members[atomicAdd(&sh.count, 1)] = threadIdx.x;
+  const bool member = order_key(largest) >= tau;
+  if (member) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (!HELD) sh.members[at] = threadIdx.x;
+  }
   __syncthreads();
   const int members = sh.count, rounds = (g1 - g0 + LP_THREADS - 1) / LP_THREADS;
   auto list = [&](float v, int index) {
@@ -241,14 +244,18 @@ __device__ void select_top(TopShared& sh, const T* x, const RowParts& parts, int
   // row is full of, which the list cannot hold
   const bool few = members <= 2 * top + 64;
   if (few) {
-    for (int u = threadIdx.x; u < members * rounds; u += LP_THREADS) {
-      const int g = g0 + sh.members[u % members] + u / members * LP_THREADS;
-      if (g >= g1) continue;
-      float v[N];
-      const int c = parts.head + g * N;
-      Granule<T>::load(x + c, v);
+    if constexpr (HELD) {
+      if (member) each(list);
+    } else {
+      for (int u = threadIdx.x; u < members * rounds; u += LP_THREADS) {
+        const int g = g0 + sh.members[u % members] + u / members * LP_THREADS;
+        if (g >= g1) continue;
+        float v[N];
+        const int c = parts.head + g * N;
+        Granule<T>::load(x + c, v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) list(v[i], c + i);
+        for (int i = 0; i < N; ++i) list(v[i], c + i);
+      }
     }
     if (has_head && (int)threadIdx.x < parts.head) list(Elem<T>::load(x, threadIdx.x), threadIdx.x);
     if (has_tail && parts.tail + (int)threadIdx.x < V)
@@ -302,10 +309,12 @@ __device__ void finish_row(const LogProbArgs& a, const T* x, int64_t row, const 
   }
 }
 
-template <typename T, bool TOP>
+#define LP_HELD 4  // granules a thread holds where a chunk has no more than that
+
+template <typename T, bool TOP, bool HELD>
 __global__ void __launch_bounds__(LP_THREADS)
 token_log_probs_kernel(const T* __restrict__ logits, LogProbArgs a) {
-  constexpr int N = Granule<T>::N, UNROLL = 4;
+  constexpr int N = Granule<T>::N;
   __shared__ __attribute__((aligned(16))) TopShared sh;
   __shared__ float red[3][LP_WAVES];
   const int64_t row = blockIdx.x / a.chunks;
@@ -318,17 +327,25 @@ token_log_probs_kernel(const T* __restrict__ logits, LogProbArgs a) {
   const bool has_head = chunk == 0, has_tail = chunk == a.chunks - 1;
   const float c = a.inv_t * LP_LOG2E;
   Softmax r = Softmax::none();
+  float v[LP_HELD][N];
   int g = g0 + threadIdx.x;
-  for (; g + (UNROLL - 1) * LP_THREADS < g1; g += UNROLL * LP_THREADS) {
-    float v[UNROLL][N];
+  if constexpr (HELD) {
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) Granule<T>::load(x + parts.head + (g + j * LP_THREADS) * N, v[j]);
-    r.add<UNROLL * N>(v[0], c);
-  }
-  for (; g < g1; g += LP_THREADS) {
-    float v[N];
-    Granule<T>::load(x + parts.head + g * N, v);
-    r.add<N>(v, c);
+    for (int j = 0; j < LP_HELD; ++j)
+      if (g + j * LP_THREADS < g1) Granule<T>::load(x + parts.head + (g + j * LP_THREADS) * N, v[j]);
+#pragma unroll
+    for (int j = 0; j < LP_HELD; ++j)
+      if (g + j * LP_THREADS < g1) r.add<N>(v[j], c);
+  } else {
+    for (; g + (LP_HELD - 1) * LP_THREADS < g1; g += LP_HELD * LP_THREADS) {
+#pragma unroll
+      for (int j = 0; j < LP_HELD; ++j) Granule<T>::load(x + parts.head + (g + j * LP_THREADS) * N, v[j]);
+      r.add<LP_HELD * N>(v[0], c);
+    }
+    for (; g < g1; g += LP_THREADS) {
+      Granule<T>::load(x + parts.head + g * N, v[0]);
+      r.add<N>(v[0], c);
+    }
   }
   if (has_head && (int)threadIdx.x < parts.head) {
     const float v = Elem<T>::load(x, threadIdx.x);
@@ -345,7 +362,14 @@ token_log_probs_kernel(const T* __restrict__ logits, LogProbArgs a) {
   r = {red[0][0], red[1][0], red[2][0]};
 #pragma unroll
   for (int w = 1; w < LP_WAVES; ++w) r.join({red[0][w], red[1][w], red[2][w]}, c);
-  if constexpr (TOP) select_top(sh, x, parts, g0, g1, has_head, has_tail, a.V, mine, a.top);
+  if constexpr (TOP)
+    select_top<HELD>(sh, x, parts, g0, g1, has_head, has_tail, a.V, mine, a.top, [&](auto list) {
+#pragma unroll
+      for (int j = 0; j < LP_HELD; ++j)
+        if (g + j * LP_THREADS < g1)
+#pragma unroll
+          for (int i = 0; i < N; ++i) list(v[j][i], parts.head + (g + j * LP_THREADS) * N + i);
+    });
   if (a.chunks == 1) {
     finish_row(a, x, row, r, sh.sorted);
     return;
@@ -500,10 +524,12 @@ static int check_shape(int64_t rows, int64_t vocab, int64_t top, int64_t ld, flo
 }
 
 // Chunks of a row: one where the rows alone give every compute unit two workgroups,
-// else as many as do, of 2048 elements at least.
+// else as many as make 256 workgroups (few rows, where the join's latency counts) or
+// 1024, of 2048 elements at least.
 static int64_t row_chunks(int64_t rows, int64_t vocab) {
   if (rows >= 512 || rows == 0) return 1;
-  const int64_t want = (512 + rows - 1) / rows, most = max(vocab / 2048, (int64_t)1);
+  const int64_t total = rows < 32 ? 256 : 1024;
+  const int64_t want = (total + rows - 1) / rows, most = max(vocab / 2048, (int64_t)1);
   return min(min(want, most), (int64_t)128);
 }
 
@@ -533,8 +559,11 @@ extern "C" int alodlm_token_log_probs(const void* logits, int64_t ld, const int6
                      (int)chunks, (int)((granules + chunks - 1) / chunks), inv_temperature};
     if (chunks > 1) a.part = reinterpret_cast<Softmax*>(workspace + 2 * rows * chunks * top);
     const unsigned grid = (unsigned)(rows * chunks);
-    if (top) token_log_probs_kernel<T, true><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
-    else token_log_probs_kernel<T, false><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
+    // the last chunk has what the others leave, never more than they have
+    const bool held = a.chunk_granules <= LP_HELD * LP_THREADS;
+    if (!top) token_log_probs_kernel<T, false, false><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
+    else if (held) token_log_probs_kernel<T, true, true><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
+    else token_log_probs_kernel<T, true, false><<<grid, LP_THREADS, 0, st>>>((const T*)logits, a);
     if (chunks > 1) token_log_probs_join_kernel<T><<<(unsigned)rows, LP_THREADS, 0, st>>>((const T*)logits, a);
   });
   ALODLM_CHECK_LAUNCH("token_log_probs");
