@@ -200,16 +200,20 @@ template <int DH, int CT> struct Columns {
       }
     }
   }
-  // Scores -> probabilities in bf16; the maximum and what goes with it move along.
+  // Scores -> probabilities in bf16.  The reference m that they are taken against is the
+  // running maximum, but follows it only when that has grown by more than 2^8: until
+  // then the probabilities stay below 2^8 of what they would be, which costs float32
+  // sums and bf16 factors nothing, and no output is rescaled.
   __device__ __forceinline__ void softmax(const f32x4 (&s)[CT][4], bf16x8 (&p)[CT][2], float scale2) {
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       float top = s[t][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, s[t][i / 4][i % 4]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
-      if (__any(top > m[t])) {
+      top *= scale2;
+      if (__any(top > m[t] + 8.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));  // the four lanes of a column agree
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float to = fmaxf(m[t], top);
         const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] - to);
         m[t] = to;

@@ -75,43 +75,48 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   // dimensions tid / 4 + 64 r, 16 keys (group tid % 4).
   constexpr int KW = DH / 64, KW16 = DH / 32, VR = DH / 64;  // 16-byte words of codes, of bf16
   const int head_block = page * DH, t_key = tid >> 2, t_part = tid & 3, t_dim = tid >> 2;
-  struct Place {
-    int k_page, v_page;
-    int64_t k, v;
+  struct Pages {
+    int k, v;
   };
-  auto place = [&](int i) {
-    const int base = base_of(i);
-    const bool pool = i < pool_tiles;
-    const int lo = pool ? k0 : lo_open, end = pool ? hi : k1;
-    const int k_at = base + (t_key & ~15), v_at = base + t_part * 16;
-    Place p;
-    p.k_page = pool ? sp.page<true>(c, bt, k_at, lo, end) : sp.page<false>(c, bt, k_at, lo, end);
-    p.v_page = pool ? sp.page<true>(c, bt, v_at, lo, end) : sp.page<false>(c, bt, v_at, lo, end);
-    p.k = sp.block(c, p.k_page, head_block) + (((k_at & (page - 1)) + (t_key & 15)) * DH + t_part * (DH / 4));
-    p.v = sp.block(c, p.v_page, head_block) + (t_dim * page + (v_at & (page - 1)));
-    return p;
+  auto pages_of = [&](int i) {
+    const int base = base_of(i), k_at = base + (t_key & ~15), v_at = base + t_part * 16;
+    if (i >= count) return Pages{-1, -1};
+    if (i < pool_tiles) return Pages{sp.page<true>(c, bt, k_at, k0, hi), sp.page<true>(c, bt, v_at, k0, hi)};
+    return Pages{sp.page<false>(c, bt, k_at, lo_open, k1), sp.page<false>(c, bt, v_at, lo_open, k1)};
+  };
+  // the thread's first value in its pages
+  auto key_at = [&](int i, int id) {
+    return sp.block(c, id, head_block) + (((base_of(i) + t_key) & (page - 1)) * DH + t_part * (DH / 4));
+  };
+  auto value_at = [&](int i, int id) {
+    return sp.block(c, id, head_block) + (t_dim * page + ((base_of(i) + t_part * 16) & (page - 1)));
   };
   // What comes in behind the products: codes, or the keys of a 16-bit pool (its values
-  // as well would not fit the registers of two waves a SIMD).
+  // as well would not fit the registers of two waves a SIMD).  `next` runs a tile ahead
+  // of that, so that no load waits for the table.
   uint4 raw_k[EIGHT ? KW : KW16], raw_v[VR];
-  Place ahead;
+  float k_scale = 1.f, v_scale = 1.f;
+  Pages ahead, next;
   auto fetch = [&](int i) {
+    ahead = next;
+    next = pages_of(i + 1);
     if (EIGHT && i >= pool_tiles) return;
-    ahead = place(i);
+    const int64_t kp = key_at(i, ahead.k), vp = value_at(i, ahead.v);
 #pragma unroll
     for (int j = 0; j < (EIGHT ? KW : KW16); ++j) {
       raw_k[j] = make_uint4(0, 0, 0, 0);
-      if (ahead.k_page >= 0)
-        raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + ahead.k + j * 16)
-                         : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + ahead.k + j * 8);
+      if (ahead.k >= 0)
+        raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + kp + j * 16)
+                         : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + kp + j * 8);
     }
     if constexpr (EIGHT) {
 #pragma unroll
       for (int r = 0; r < VR; ++r) {
         raw_v[r] = make_uint4(0, 0, 0, 0);
-        if (ahead.v_page >= 0)
-          raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + ahead.v + r * 64 * page);
+        if (ahead.v >= 0) raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + vp + r * 64 * page);
       }
+      k_scale = ahead.k >= 0 ? sp.scale(c, ahead.k, 0) : 1.f;
+      v_scale = ahead.v >= 0 ? sp.scale(c, ahead.v, 1) : 1.f;
     }
   };
   // Tile i -> bf16 in LDS.  In tiles that some row does not see whole, values that are
@@ -120,14 +125,12 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   auto stage_codes = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
     const bool edge = base_of(i) + PAGED_TILE > min(hi, least);
-    const float ks = ahead.k_page >= 0 ? sp.scale(c, ahead.k_page, 0) : 1.f;
-    const float vs = ahead.v_page >= 0 ? sp.scale(c, ahead.v_page, 1) : 1.f;
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
       const uint4 w = raw_k[j];
       const int piece = t_part * (DH / 32) + 2 * j;
-      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece)) = widen(w.x, w.y, ks);
-      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece + 1)) = widen(w.z, w.w, ks);
+      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece)) = widen(w.x, w.y, k_scale);
+      *reinterpret_cast<bf16x8*>(t.k + key_piece<DH>(t_key, piece + 1)) = widen(w.z, w.w, k_scale);
     }
 #pragma unroll
     for (int r = 0; r < VR; ++r) {
@@ -137,21 +140,21 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         w = make_uint4(without_special<true>(w.x), without_special<true>(w.y), without_special<true>(w.z),
                        without_special<true>(w.w));
       }
-      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part)) = widen(w.x, w.y, vs);
-      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + 1)) = widen(w.z, w.w, vs);
+      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part)) = widen(w.x, w.y, v_scale);
+      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + 1)) = widen(w.z, w.w, v_scale);
     }
-    if (tid < 4) there[i & 1][tid] = ahead.v_page >= 0;  // thread t holds group t
+    if (tid < 4) there[i & 1][tid] = ahead.v >= 0;  // thread t holds group t
   };
   auto stage_plain = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
     const bool pool = i < pool_tiles, edge = !pool || base_of(i) + PAGED_TILE > min(hi, least);
-    const Place p = EIGHT ? place(i) : ahead;
+    const int64_t kp = key_at(i, ahead.k), vp = value_at(i, ahead.v);
     const bf16_t* values = (const bf16_t*)(EIGHT ? c.open_values : c.values);
 #pragma unroll
     for (int j = 0; j < KW16; ++j) {
       uint4 w = make_uint4(0, 0, 0, 0);
       if constexpr (!EIGHT) w = raw_k[j];
-      else if (p.k_page >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + p.k + j * 8);
+      else if (ahead.k >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + kp + j * 8);
       *reinterpret_cast<uint4*>(t.k + key_piece<DH>(t_key, t_part * (DH / 32) + j)) = w;
     }
 #pragma unroll
@@ -159,7 +162,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint4 w = make_uint4(0, 0, 0, 0);
-        if (p.v_page >= 0) w = *reinterpret_cast<const uint4*>(values + p.v + r * 64 * page + j * 8);
+        if (ahead.v >= 0) w = *reinterpret_cast<const uint4*>(values + vp + r * 64 * page + j * 8);
         if (edge) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
@@ -167,7 +170,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         }
         *reinterpret_cast<uint4*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + j)) = w;
       }
-    if (tid < 4) there[i & 1][tid] = p.v_page >= 0;
+    if (tid < 4) there[i & 1][tid] = ahead.v >= 0;
   };
   auto stage = [&](int i) {
     if (EIGHT && i < pool_tiles) stage_codes(i);
@@ -175,6 +178,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
 
   if (count > 0) {
+    next = pages_of(0);
     fetch(0);
     stage(0);
   }
