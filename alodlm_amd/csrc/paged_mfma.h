@@ -92,9 +92,10 @@ struct Span {
   __device__ __forceinline__ int64_t block(const PagedCache& c, int page, int head_block) const {
     return ((int64_t)page * c.kv_heads + h) * head_block;
   }
-  // 2^exponent of a pool page's keys (side 0) or values (side 1).
-  __device__ __forceinline__ float scale(const PagedCache& c, int page, int side) const {
-    return exp2_int(c.exponents[((int64_t)page * 2 + side) * c.kv_heads + h]);
+  // Exponent of a pool page's keys (side 0) or values (side 1).  Made a scale where that is
+  // used: the arithmetic would wait for this load and all that went before it.
+  __device__ __forceinline__ int exponent(const PagedCache& c, int page, int side) const {
+    return c.exponents[((int64_t)page * 2 + side) * c.kv_heads + h];
   }
 };
 

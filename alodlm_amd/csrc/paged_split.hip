@@ -11,7 +11,7 @@
 // A lane's part of one 64-key tile of codes: 16 dims of a key, 16 keys of a dimension.
 template <int DH> struct CodeTile {
   uint4 k[4][DH / 64], v[DH / 16];
-  float k_scale, v_scale;
+  int k_exponent, v_exponent;
   bool there;
 };
 
@@ -61,7 +61,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
   auto load_key_codes = [&](CodeTile<DH>& t, int base, int id) {
     const e4m3_t* p = (const e4m3_t*)c.keys + key_place(base, id);
-    t.k_scale = 1.f;
+    t.k_exponent = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -69,26 +69,32 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         t.k[i][j] = make_uint4(0, 0, 0, 0);
         if (id >= 0) t.k[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + j * 64);
       }
-    if (id >= 0) t.k_scale = sp.scale(c, id, 0);
+    if (id >= 0) t.k_exponent = sp.exponent(c, id, 0);
   };
   auto load_value_codes = [&](CodeTile<DH>& t, int base, int id) {
     const e4m3_t* p = (const e4m3_t*)c.values + value_place(base, id);
-    t.v_scale = 1.f;
+    t.v_exponent = 0;
     t.there = id >= 0;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       t.v[d] = make_uint4(0, 0, 0, 0);
       if (id >= 0) t.v[d] = *reinterpret_cast<const uint4*>(p + d * 16 * page);
     }
-    if (id >= 0) t.v_scale = sp.scale(c, id, 1);
+    if (id >= 0) t.v_exponent = sp.exponent(c, id, 1);
   };
-  auto key_of = [&](const CodeTile<DH>& t, int i, int f) {
-    const uint4 w = t.k[i][f / 2];
-    return f % 2 ? widen(w.z, w.w, t.k_scale) : widen(w.x, w.y, t.k_scale);
+  auto scores = [&](const CodeTile<DH>& t, f32x4 (&s)[CT][4]) {
+    const float scale = exp2_int(t.k_exponent);
+    cols.scores(s, [&](int i, int f) {
+      const uint4 w = t.k[i][f / 2];
+      return f % 2 ? widen(w.z, w.w, scale) : widen(w.x, w.y, scale);
+    });
   };
-  auto value_of = [&](const CodeTile<DH>& t, int d, int j) {
-    const uint4 w = t.v[d];
-    return j ? widen(w.z, w.w, t.v_scale) : widen(w.x, w.y, t.v_scale);
+  auto add_values = [&](const CodeTile<DH>& t, const bf16x8 (&p)[CT][2]) {
+    const float scale = exp2_int(t.v_exponent);
+    cols.add_values(p, [&](int d, int j) {
+      const uint4 w = t.v[d];
+      return j ? widen(w.z, w.w, scale) : widen(w.x, w.y, scale);
+    });
   };
 
   constexpr int STEP = PAGED_WAVES * PAGED_TILE;
@@ -111,11 +117,11 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       const bool more = base + STEP < to;
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
-      cols.scores(s, [&](int i, int f) { return key_of(tile, i, f); });
+      scores(tile, s);
       if (more) load_key_codes(tile, base + STEP, k_next);
       if (!__all(tile.there)) cols.hide(s, base, 0, to, tile.there);
       cols.softmax(s, p, a.scale2);
-      cols.add_values(p, [&](int d, int j) { return value_of(tile, d, j); });
+      add_values(tile, p);
       if (!more) break;
       base += STEP;
       load_value_codes(tile, base, v_next);
@@ -131,7 +137,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       load_value_codes(tile, base, sp.page<true>(c, bt, base + grp * 16, k0, to));
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
-      cols.scores(s, [&](int i, int f) { return key_of(tile, i, f); });
+      scores(tile, s);
       cols.hide(s, base, k0, to, tile.there);
       cols.softmax(s, p, a.scale2);
 #pragma unroll
@@ -143,7 +149,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
           w[i] = without_special<true>(w[i]);
         }
       }
-      cols.add_values(p, [&](int d, int j) { return value_of(tile, d, j); });
+      add_values(tile, p);
     }
   };
   // Tiles [from, to) of keys [lo, to) in 16 bits, loaded as the products take them

@@ -95,7 +95,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   // as well would not fit the registers of two waves a SIMD).  `next` runs a tile ahead
   // of that, so that no load waits for the table.
   uint4 raw_k[EIGHT ? KW : KW16], raw_v[VR];
-  float k_scale = 1.f, v_scale = 1.f;
+  int k_exponent = 0, v_exponent = 0;
   Pages ahead, next;
   auto fetch = [&](int i) {
     ahead = next;
@@ -115,8 +115,8 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         raw_v[r] = make_uint4(0, 0, 0, 0);
         if (ahead.v >= 0) raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + vp + r * 64 * page);
       }
-      k_scale = ahead.k >= 0 ? sp.scale(c, ahead.k, 0) : 1.f;
-      v_scale = ahead.v >= 0 ? sp.scale(c, ahead.v, 1) : 1.f;
+      if (ahead.k >= 0) k_exponent = sp.exponent(c, ahead.k, 0);
+      if (ahead.v >= 0) v_exponent = sp.exponent(c, ahead.v, 1);
     }
   };
   // Tile i -> bf16 in LDS.  In tiles that some row does not see whole, values that are
@@ -125,6 +125,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   auto stage_codes = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
     const bool edge = base_of(i) + PAGED_TILE > min(hi, least);
+    const float k_scale = exp2_int(k_exponent), v_scale = exp2_int(v_exponent);
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
       const uint4 w = raw_k[j];
