@@ -88,6 +88,14 @@ struct Span {
     if (!POOL) return slot < 0 ? -1 : open_page(c, slot, p);
     return bt.page_of(b, p, c.pages);
   }
+  // The same in two steps, so that no arithmetic waits for the table: its entry (any, for
+  // keys past the table), and what page that is.
+  __device__ __forceinline__ int entry(const PagedCache& c, const PagedBatch& bt, int key) const {
+    return bt.table[(int64_t)b * bt.width + min(key >> c.shift, bt.width - 1)];
+  }
+  __device__ __forceinline__ int page_in(const PagedCache& c, int entry, int key, int lo, int hi) const {
+    return key + 15 < lo || key >= hi || entry < 0 || entry >= c.pages ? -1 : entry;
+  }
   // First value of a page's block for this head.
   __device__ __forceinline__ int64_t block(const PagedCache& c, int page, int head_block) const {
     return ((int64_t)page * c.kv_heads + h) * head_block;

@@ -59,28 +59,30 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   auto value_place = [&](int base, int id) {
     return sp.block(c, id, head_block) + (col * page + ((base + grp * 16) & (page - 1)));
   };
+  // Codes are loaded whether or not there is a page (from page 0 where there is none):
+  // branches between loads would wait for the ones before.  The scores of keys that are
+  // not there are hidden, their values cleared.
   auto load_key_codes = [&](CodeTile<DH>& t, int base, int id) {
+    id = max(id, 0);
     const e4m3_t* p = (const e4m3_t*)c.keys + key_place(base, id);
-    t.k_exponent = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < DH / 64; ++j) {
-        t.k[i][j] = make_uint4(0, 0, 0, 0);
-        if (id >= 0) t.k[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + j * 64);
-      }
-    if (id >= 0) t.k_exponent = sp.exponent(c, id, 0);
+      for (int j = 0; j < DH / 64; ++j) t.k[i][j] = *reinterpret_cast<const uint4*>(p + 4 * i * DH + j * 64);
+    t.k_exponent = sp.exponent(c, id, 0);
   };
   auto load_value_codes = [&](CodeTile<DH>& t, int base, int id) {
-    const e4m3_t* p = (const e4m3_t*)c.values + value_place(base, id);
-    t.v_exponent = 0;
     t.there = id >= 0;
+    id = max(id, 0);
+    const e4m3_t* p = (const e4m3_t*)c.values + value_place(base, id);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      t.v[d] = make_uint4(0, 0, 0, 0);
-      if (id >= 0) t.v[d] = *reinterpret_cast<const uint4*>(p + d * 16 * page);
-    }
-    if (id >= 0) t.v_exponent = sp.exponent(c, id, 1);
+    for (int d = 0; d < DT; ++d) t.v[d] = *reinterpret_cast<const uint4*>(p + d * 16 * page);
+    t.v_exponent = sp.exponent(c, id, 1);
+  };
+  auto clear_values = [&](CodeTile<DH>& t) {
+    if (!t.there)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) t.v[d] = make_uint4(0, 0, 0, 0);
   };
   auto scores = [&](const CodeTile<DH>& t, f32x4 (&s)[CT][4]) {
     const float scale = exp2_int(t.k_exponent);
@@ -111,22 +113,25 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     CodeTile<DH> tile;
     load_key_codes(tile, base, sp.page<true>(c, bt, base + (col >> 2) * 16, 0, to));
     load_value_codes(tile, base, sp.page<true>(c, bt, base + grp * 16, 0, to));
-    int k_next = sp.page<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
-    int v_next = sp.page<true>(c, bt, base + STEP + grp * 16, 0, to);
+    int k_next = sp.entry(c, bt, base + STEP + (col >> 2) * 16);
+    int v_next = sp.entry(c, bt, base + STEP + grp * 16);
     while (true) {
       const bool more = base + STEP < to;
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
       scores(tile, s);
-      if (more) load_key_codes(tile, base + STEP, k_next);
-      if (!__all(tile.there)) cols.hide(s, base, 0, to, tile.there);
+      if (more) load_key_codes(tile, base + STEP, sp.page_in(c, k_next, base + STEP, 0, to));
+      if (!__all(tile.there)) {
+        cols.hide(s, base, 0, to, tile.there);
+        clear_values(tile);
+      }
       cols.softmax(s, p, a.scale2);
       add_values(tile, p);
       if (!more) break;
       base += STEP;
-      load_value_codes(tile, base, v_next);
-      k_next = sp.page<true>(c, bt, base + STEP + (col >> 2) * 16, 0, to);
-      v_next = sp.page<true>(c, bt, base + STEP + grp * 16, 0, to);
+      load_value_codes(tile, base, sp.page_in(c, v_next, base, 0, to));
+      k_next = sp.entry(c, bt, base + STEP + (col >> 2) * 16);
+      v_next = sp.entry(c, bt, base + STEP + grp * 16);
     }
   };
   // Tiles [from, to) of codes that some row does not see whole.
@@ -139,6 +144,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       bf16x8 p[CT][2];
       scores(tile, s);
       cols.hide(s, base, k0, to, tile.there);
+      clear_values(tile);
       cols.softmax(s, p, a.scale2);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -161,20 +167,18 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     for (int base = first_tile(from); base < to; base += STEP) {
       const int k_page = sp.page<POOL>(c, bt, base + (col >> 2) * 16, lo, to);
       const int v_page = sp.page<POOL>(c, bt, base + grp * 16, lo, to);
-      const bf16_t* kp = keys + key_place(base, k_page);
-      const bf16_t* vp = values + value_place(base, v_page);
+      const bf16_t* kp = keys + key_place(base, max(k_page, 0));
+      const bf16_t* vp = values + value_place(base, max(v_page, 0));
       f32x4 s[CT][4];
       bf16x8 p[CT][2];
       cols.scores(s, [&](int i, int f) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (k_page >= 0) w = *reinterpret_cast<const uint4*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
-        return __builtin_bit_cast(bf16x8, w);
+        return *reinterpret_cast<const bf16x8*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
       });
       if (!whole || !__all(v_page >= 0)) cols.hide(s, base, lo, to, v_page >= 0);
       cols.softmax(s, p, a.scale2);
       cols.add_values(p, [&](int d, int j) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (v_page >= 0) w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
+        uint4 w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
+        if (v_page < 0) w = make_uint4(0, 0, 0, 0);
         if (!whole) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) |
                  special_bits<false>(w.w);

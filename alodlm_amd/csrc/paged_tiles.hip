@@ -78,11 +78,9 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   struct Pages {
     int k, v;
   };
-  auto pages_of = [&](int i) {
-    const int base = base_of(i), k_at = base + (t_key & ~15), v_at = base + t_part * 16;
-    if (i >= count) return Pages{-1, -1};
-    if (i < pool_tiles) return Pages{sp.page<true>(c, bt, k_at, k0, hi), sp.page<true>(c, bt, v_at, k0, hi)};
-    return Pages{sp.page<false>(c, bt, k_at, lo_open, k1), sp.page<false>(c, bt, v_at, lo_open, k1)};
+  auto entries_of = [&](int i) {
+    const int base = base_of(min(i, max(pool_tiles - 1, 0)));
+    return Pages{sp.entry(c, bt, base + (t_key & ~15)), sp.entry(c, bt, base + t_part * 16)};
   };
   // the thread's first value in its pages
   auto key_at = [&](int i, int id) {
@@ -93,30 +91,31 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
   // What comes in behind the products: codes, or the keys of a 16-bit pool (its values
   // as well would not fit the registers of two waves a SIMD).  `next` runs a tile ahead
-  // of that, so that no load waits for the table.
+  // of that, so that nothing waits for the table.
   uint4 raw_k[EIGHT ? KW : KW16], raw_v[VR];
   int k_exponent = 0, v_exponent = 0;
   Pages ahead, next;
   auto fetch = [&](int i) {
-    ahead = next;
-    next = pages_of(i + 1);
-    if (EIGHT && i >= pool_tiles) return;
-    const int64_t kp = key_at(i, ahead.k), vp = value_at(i, ahead.v);
+    const int k_at = base_of(i) + (t_key & ~15), v_at = base_of(i) + t_part * 16;
+    if (EIGHT && i >= pool_tiles) {
+      ahead = Pages{sp.page<false>(c, bt, k_at, lo_open, k1), sp.page<false>(c, bt, v_at, lo_open, k1)};
+      return;
+    }
+    ahead = Pages{sp.page_in(c, next.k, k_at, k0, hi), sp.page_in(c, next.v, v_at, k0, hi)};
+    next = entries_of(i + 1);
+    // from page 0 where there is none: branches between loads would wait for the ones before
+    const int64_t kp = key_at(i, max(ahead.k, 0)), vp = value_at(i, max(ahead.v, 0));
 #pragma unroll
     for (int j = 0; j < (EIGHT ? KW : KW16); ++j) {
-      raw_k[j] = make_uint4(0, 0, 0, 0);
-      if (ahead.k >= 0)
-        raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + kp + j * 16)
-                         : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + kp + j * 8);
+      raw_k[j] = EIGHT ? *reinterpret_cast<const uint4*>((const e4m3_t*)c.keys + kp + j * 16)
+                       : *reinterpret_cast<const uint4*>((const bf16_t*)c.keys + kp + j * 8);
     }
     if constexpr (EIGHT) {
 #pragma unroll
-      for (int r = 0; r < VR; ++r) {
-        raw_v[r] = make_uint4(0, 0, 0, 0);
-        if (ahead.v >= 0) raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + vp + r * 64 * page);
-      }
-      if (ahead.k >= 0) k_exponent = sp.exponent(c, ahead.k, 0);
-      if (ahead.v >= 0) v_exponent = sp.exponent(c, ahead.v, 1);
+      for (int r = 0; r < VR; ++r)
+        raw_v[r] = *reinterpret_cast<const uint4*>((const e4m3_t*)c.values + vp + r * 64 * page);
+      k_exponent = sp.exponent(c, max(ahead.k, 0), 0);
+      v_exponent = sp.exponent(c, max(ahead.v, 0), 1);
     }
   };
   // Tile i -> bf16 in LDS.  In tiles that some row does not see whole, values that are
@@ -136,6 +135,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
     for (int r = 0; r < VR; ++r) {
       uint4 w = raw_v[r];
+      if (ahead.v < 0) w = make_uint4(0, 0, 0, 0);
       if (edge) {
         odd |= special_bits<true>(w.x) | special_bits<true>(w.y) | special_bits<true>(w.z) | special_bits<true>(w.w);
         w = make_uint4(without_special<true>(w.x), without_special<true>(w.y), without_special<true>(w.z),
@@ -149,21 +149,26 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   auto stage_plain = [&](int i) {
     TileBuffer<DH>& t = tiles[i & 1];
     const bool pool = i < pool_tiles, edge = !pool || base_of(i) + PAGED_TILE > min(hi, least);
-    const int64_t kp = key_at(i, ahead.k), vp = value_at(i, ahead.v);
+    const int64_t kp = key_at(i, max(ahead.k, 0)), vp = value_at(i, max(ahead.v, 0));
     const bf16_t* values = (const bf16_t*)(EIGHT ? c.open_values : c.values);
+    uint4 wv[VR][2];
+#pragma unroll
+    for (int r = 0; r < VR; ++r)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) wv[r][j] = *reinterpret_cast<const uint4*>(values + vp + r * 64 * page + j * 8);
 #pragma unroll
     for (int j = 0; j < KW16; ++j) {
-      uint4 w = make_uint4(0, 0, 0, 0);
+      uint4 w;
       if constexpr (!EIGHT) w = raw_k[j];
-      else if (ahead.k >= 0) w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + kp + j * 8);
+      else w = *reinterpret_cast<const uint4*>((const bf16_t*)c.open_keys + kp + j * 8);
       *reinterpret_cast<uint4*>(t.k + key_piece<DH>(t_key, t_part * (DH / 32) + j)) = w;
     }
 #pragma unroll
     for (int r = 0; r < VR; ++r)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (ahead.v >= 0) w = *reinterpret_cast<const uint4*>(values + vp + r * 64 * page + j * 8);
+        uint4 w = wv[r][j];
+        if (ahead.v < 0) w = make_uint4(0, 0, 0, 0);
         if (edge) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
@@ -179,7 +184,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
 
   if (count > 0) {
-    next = pages_of(0);
+    next = entries_of(0);
     fetch(0);
     stage(0);
   }
