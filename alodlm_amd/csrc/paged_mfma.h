@@ -193,6 +193,8 @@ template <int DH, int CT> struct Columns {
         for (int t = 0; t < CT; ++t) s[t][i] = mfma16(now[f], q[t][f], s[t][i]);
 #pragma unroll
       for (int f = 0; f < FR; ++f) now[f] = next[f];
+      if (i < 3) __builtin_amdgcn_sched_group_barrier(0x100, FR, 0);  // LDS reads first,
+      __builtin_amdgcn_sched_group_barrier(0x8, FR * CT, 0);          // then the products
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -280,6 +282,8 @@ template <int DH, int CT> struct Columns {
           o[t][g * 4 % DT + k] = mfma16(now[k], p[t][g * 4 / DT], o[t][g * 4 % DT + k]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) now[k] = next[k];
+      if (g + 1 < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 4 * CT, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
