@@ -8,9 +8,6 @@
 // the buffer: one barrier a tile.  The limits are then the matrix instructions, the
 // LDS reads (32 KB a wave and tile against 32 columns) and the exponentials, which
 // two workgroups a compute unit overlap.
-//
-// LDS layout: a key's row of DH values, a dimension's row of 64 keys, in 16-byte pieces
-// whose place is XORed with the row such that 16 lanes on 16 rows meet all banks.
 #include "paged_mfma.h"
 
 template <int DH> struct TileBuffer {
@@ -18,15 +15,18 @@ template <int DH> struct TileBuffer {
   bf16_t v[DH * PAGED_TILE];
 };
 
-// Place (in values) of 16-byte piece `piece` of a key's, a dimension's row.  A fragment's
-// 16 rows are keys with different (key >> 4, key & 3), or 16 dimensions in a row.
+// Places (in values) of 16-byte pieces.  A fragment's lanes read 16 rows of 4 pieces that
+// lie together: keys in the order of a subtile's rows, 32 dims a block; dimensions, 8 of
+// every group's 16 keys a block.  Within a row the pieces are XORed with the row (reads)
+// and the block (writes of one key's blocks) so that no 16 lanes meet in a bank.
 template <int DH>
 __device__ __forceinline__ int key_piece(int key, int piece) {
-  constexpr int MASK = DH / 8 - 1;
-  return key * DH + ((piece ^ (((key >> 4) << 2 | (key & 3)) & MASK)) << 3);
+  const int f = piece >> 2, r = ((key >> 2) & 3) * 16 + (key >> 4) * 4 + (key & 3);
+  return (f * PAGED_TILE + r) * 32 + (((piece ^ (r >> 1) ^ f) & 3) << 3);
 }
-__device__ __forceinline__ int value_piece(int d, int piece) {
-  return d * PAGED_TILE + ((piece ^ ((d >> 1) & 7)) << 3);
+template <int DH>
+__device__ __forceinline__ int value_piece(int d, int group, int j) {
+  return (j * DH + d) * 32 + (((group ^ (d >> 1)) & 3) << 3);
 }
 
 template <int DH, int CT, bool EIGHT>
@@ -141,8 +141,8 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         w = make_uint4(without_special<true>(w.x), without_special<true>(w.y), without_special<true>(w.z),
                        without_special<true>(w.w));
       }
-      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part)) = widen(w.x, w.y, v_scale);
-      *reinterpret_cast<bf16x8*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + 1)) = widen(w.z, w.w, v_scale);
+      *reinterpret_cast<bf16x8*>(t.v + value_piece<DH>(t_dim + 64 * r, t_part, 0)) = widen(w.x, w.y, v_scale);
+      *reinterpret_cast<bf16x8*>(t.v + value_piece<DH>(t_dim + 64 * r, t_part, 1)) = widen(w.z, w.w, v_scale);
     }
     if (tid < 4) there[i & 1][tid] = ahead.v >= 0;  // thread t holds group t
   };
@@ -174,7 +174,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
                          without_special<false>(w.w));
         }
-        *reinterpret_cast<uint4*>(t.v + value_piece(t_dim + 64 * r, 2 * t_part + j)) = w;
+        *reinterpret_cast<uint4*>(t.v + value_piece<DH>(t_dim + 64 * r, t_part, j)) = w;
       }
     if (tid < 4) there[i & 1][tid] = ahead.v >= 0;
   };
@@ -207,7 +207,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       if (base < lo || base + PAGED_TILE > min(end, my_least) || !__all(mine)) cols.hide(s, base, lo, end, mine);
       cols.softmax(s, p, a.scale2);
       cols.add_values_ahead(p, [&](int d, int j) {
-        return *reinterpret_cast<const bf16x8*>(t.v + value_piece(d * 16 + col, 2 * grp + j));
+        return *reinterpret_cast<const bf16x8*>(t.v + value_piece<DH>(d * 16 + col, grp, j));
       });
     }
     if (more) stage(i + 1);
