@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._lib import call, ptr, query
+from ._lib import call, call_on, ptr, query
 
 
 def _require_gpu(t, what):
@@ -111,43 +111,51 @@ class TokenLogProbs(NamedTuple):
 MAX_TOP = 64
 
 
+def _vocabulary_rows(logits):
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+
+
+def _log_probs(logits, targets, top, inv_temperature, ignore_index):
+    """The four results and the buffer that starts with the backward's statistics."""
+    R, V = logits.shape
+    dev = logits.device
+    x = _vocabulary_rows(logits)
+    log_prob = torch.empty(R, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(log_prob)
+    top_log_prob = torch.empty(R, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(R, top, dtype=torch.int64, device=dev)
+    # statistics [R, 2], then the workspace (8-byte aligned)
+    buf = torch.empty(2 * R + query("alodlm_token_log_probs_workspace", R, V, top),
+                      dtype=torch.float32, device=dev)
+    stats = buf.data_ptr()
+    call_on(dev, "alodlm_token_log_probs", x.data_ptr(), x.stride(0), targets.data_ptr(), R, V, top,
+            inv_temperature, ignore_index, log_prob.data_ptr(), entropy.data_ptr(), stats,
+            top_log_prob.data_ptr(), top_ids.data_ptr(), stats + 8 * R, _lib.dtype_code(x.dtype))
+    return log_prob, entropy, top_log_prob, top_ids, buf
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, inv_temperature, ignore_index):
-        R, V = logits.shape
-        dev, code = logits.device, _lib.dtype_code(logits.dtype)
-        x = logits.detach()
-        x = x if x.stride(1) == 1 and x.stride(0) >= V else x.contiguous()
-        log_prob, entropy = (torch.empty(R, dtype=torch.float32, device=dev) for _ in range(2))
-        stats = torch.empty(R, 2, dtype=torch.float32, device=dev)
-        top_log_prob = torch.empty(R, top, dtype=torch.float32, device=dev)
-        top_ids = torch.empty(R, top, dtype=torch.int64, device=dev)
-        need = query("alodlm_token_log_probs_workspace", R, V, top)
-        ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
-        with torch.cuda.device(dev):
-            call("alodlm_token_log_probs", ptr(x), x.stride(0), ptr(targets), R, V, top,
-                 inv_temperature, ignore_index, ptr(log_prob), ptr(entropy), ptr(stats),
-                 ptr(top_log_prob), ptr(top_ids), ptr(ws), code, _lib.stream_handle(dev))
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, targets, top_ids, stats, entropy)
-            ctx.args = top, inv_temperature, ignore_index
-        ctx.mark_non_differentiable(top_ids)
+        *outs, buf = _log_probs(logits, targets, top, inv_temperature, ignore_index)
+        ctx.save_for_backward(logits, targets, outs[3], outs[1], buf)
+        ctx.args = top, inv_temperature, ignore_index
+        ctx.mark_non_differentiable(outs[3])
         ctx.set_materialize_grads(False)
-        return log_prob, entropy, top_log_prob, top_ids
+        return tuple(outs)
 
     @staticmethod
     def backward(ctx, d_log_prob, d_entropy, d_top, _d_ids):
-        logits, targets, top_ids, stats, entropy = ctx.saved_tensors
+        logits, targets, top_ids, entropy, buf = ctx.saved_tensors
         top, inv_temperature, ignore_index = ctx.args
         R, V = logits.shape
-        x = logits if logits.stride(1) == 1 and logits.stride(0) >= V else logits.contiguous()
+        x = _vocabulary_rows(logits)
         out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
-        grads = [None if g is None else g.to(torch.float32).contiguous()
-                 for g in (d_log_prob, d_entropy, d_top)]
-        with torch.cuda.device(x.device):
-            call("alodlm_token_log_probs_bwd", ptr(x), x.stride(0), ptr(targets), ptr(top_ids),
-                 ptr(stats), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
-                 ptr(out), _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
+        grads = [g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
+                 else g.to(torch.float32).contiguous() for g in (d_log_prob, d_entropy, d_top)]
+        call_on(x.device, "alodlm_token_log_probs_bwd", ptr(x), x.stride(0), ptr(targets), ptr(top_ids),
+                ptr(buf), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
+                ptr(out), _lib.dtype_code(x.dtype))
         return out, None, None, None, None
 
 
@@ -174,5 +182,7 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
     if not 0 < temperature < float("inf"):
         raise ValueError('temperature must be positive and finite')
     _require_gpu(logits, "token_log_probs")
-    return TokenLogProbs(*_TokenLogProbs.apply(logits, targets.contiguous(), int(top),
-                                               1.0 / temperature, int(ignore_index)))
+    args = logits, targets.contiguous(), int(top), 1.0 / temperature, int(ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogProbs(*_TokenLogProbs.apply(*args))
+    return TokenLogProbs(*_log_probs(*args)[:4])

@@ -46,6 +46,7 @@ __device__ __forceinline__ void store4(T* p, float x, float y, float z, float w)
 template <typename T>
 __device__ __forceinline__ float dot_key(const float* q, const T* p, int dh) {
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int d = 0; d < dh; d += 4) {
     float v[4];
     load4(p + d, v);
@@ -273,6 +274,9 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 // ----------------------------------------------------------------------------
 // Host
 // ----------------------------------------------------------------------------
+#ifndef ROWS_LEAST
+#define ROWS_LEAST 128
+#endif
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Keys per chunk, in whole 64-key tiles: `want` workgroups or wavefronts in all where
@@ -287,7 +291,7 @@ static void cut_keys(AttendPlan& p, int64_t max_keys, int64_t units, int64_t wan
 static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
   AttendPlan p = {};
   if (c->dtype != ALODLM_BF16 || (c->head_dim != 64 && c->head_dim != 128)) {
-    cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, 256);
+    cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, ROWS_LEAST);
     return p;
   }
   const int64_t columns = max(b->max_rows * (heads / c->kv_heads), (int64_t)1);
@@ -328,7 +332,7 @@ static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* 
   if (a.chunks > 1 && units) {
     const int quads = (int)c->head_dim / 4;
     a.join_ways = 1;
-    while (a.join_ways < min(a.chunks, 16) && quads * a.join_ways * 2 <= 256) a.join_ways *= 2;
+    while (a.join_ways < 16 && a.join_ways * 4 < a.chunks && quads * a.join_ways * 2 <= 256) a.join_ways *= 2;
     const int64_t per_block = 256 / (quads * a.join_ways);
     paged_join_kernel<T, EIGHT><<<(unsigned)ceil_div(units, per_block), 256, 0, st>>>(dc, db, a);
   }

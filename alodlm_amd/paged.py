@@ -30,7 +30,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import call, ptr, query
+from ._lib import call_on, ptr, query
+from .layers import table
 
 PAGE_SIZES = (16, 32, 64, 128)
 E4M3 = torch.float8_e4m3fn
@@ -133,57 +134,65 @@ class PagedCache:
     def _rows(self, t, heads, batch, what):
         """``t`` as the kernels read it: rows [heads, head_dim] behind one another,
         the row stride free, 16-byte aligned (copied where it is not)."""
-        _need(t.dtype == self.dtype, f"{what} must be {self.dtype}, got {t.dtype}")
-        _need(t.device == self.device, f"{what} must be on {self.device}")
-        _need(t.ndim == 3 and t.shape[0] == batch.rows and t.shape[2] == self.head_dim
-              and (t.shape[1] == heads or heads is None),
-              f"{what} must be [{batch.rows}, {heads or 'heads'}, {self.head_dim}], got {list(t.shape)}")
-        size = t.element_size()
-        if (t.stride(2) != 1 or t.stride(1) != self.head_dim or t.stride(0) < t.shape[1] * self.head_dim
-                or t.stride(0) * size % 16 or t.data_ptr() % 16):
+        if t.dtype != self.dtype:
+            raise ValueError(f"{what} must be {self.dtype}, got {t.dtype}")
+        if t.device != self.device:
+            raise ValueError(f"{what} must be on {self.device}")
+        shape, dh = t.shape, self.head_dim
+        if (len(shape) != 3 or shape[0] != batch.rows or shape[2] != dh
+                or (shape[1] != heads and heads is not None)):
+            raise ValueError(f"{what} must be [{batch.rows}, {heads or 'heads'}, {dh}], "
+                             f"got {list(shape)}")
+        row, head, dim = t.stride()
+        if (dim != 1 or head != dh or row < shape[1] * dh or row * t.element_size() % 16
+                or t.data_ptr() % 16):
             t = t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()
         return t
 
-    def _stream(self, batch):
+    def _table(self, t, batch, like):
+        """A rotary table as the kernels read it (``layers.table``), 16-byte aligned."""
+        if (t.dtype != like.dtype or t.device != like.device or t.shape != (batch.rows, self.head_dim)
+                or not t.is_contiguous()):
+            t = table(t, batch.rows, self.head_dim, like)
+        return t.clone() if t.data_ptr() % 16 else t
+
+    def _check(self, batch):
         if self.device.type != "cuda":
             raise ValueError("the paged cache runs on the HIP kernels; allocate it on a CUDA (ROCm) "
                              "device")
-        _need(batch.device == self.device, f"the batch is on {batch.device}, the cache on {self.device}")
-        return _lib.stream_handle(self.device)
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
 
     def append(self, k, v, batch, cos=None, sin=None, q=None):
         """Writes the rows' keys and values [rows, kv_heads, head_dim] behind their
         sequences.  With ``cos``/``sin`` [rows, head_dim] the keys are rotated on the
         way (x * cos + rotate_half(x) * sin, in float32 and rounded once), and so are
         the queries ``q`` [rows, heads, head_dim], which are returned."""
-        stream = self._stream(batch)
-        _need((cos is None) == (sin is None), "cos and sin belong together")
-        _need(q is None or cos is not None, "q is given to be rotated: cos and sin are missing")
+        self._check(batch)
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin belong together")
+        if q is not None and cos is None:
+            raise ValueError("q is given to be rotated: cos and sin are missing")
         k = self._rows(k, self.kv_heads, batch, "k")
         v = self._rows(v, self.kv_heads, batch, "v")
-        out, heads = None, 0
         if cos is not None:
-            from .layers import table
-            cos, sin = (table(t, batch.rows, self.head_dim, k) for t in (cos, sin))
-            cos, sin = (t.clone() if t.data_ptr() % 16 else t for t in (cos, sin))
+            cos, sin = self._table(cos, batch, k), self._table(sin, batch, k)
+        out, heads, ldq = None, 0, 0
         if q is not None:
             q = self._rows(q, None, batch, "q")
-            heads = q.shape[1]
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        with torch.cuda.device(self.device):
-            call("alodlm_paged_append", self._ref, batch.ref(self), ptr(k), k.stride(0), ptr(v),
-                 v.stride(0), ptr(q), q.stride(0) if heads else 0, ptr(out), heads, ptr(cos),
-                 ptr(sin), stream)
+            heads, ldq = q.shape[1], q.stride(0)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        call_on(self.device, "alodlm_paged_append", self._ref, batch.ref(self), ptr(k), k.stride(0),
+                ptr(v), v.stride(0), ptr(q), ldq, ptr(out), heads, ptr(cos), ptr(sin))
         return out
 
     def retire(self, batch, counts):
         """Keeps the first ``counts[b]`` rows (int32 [sequences]) of a batch that is
         not final; the program then adds them to its lengths."""
-        stream = self._stream(batch)
+        self._check(batch)
         _need(not batch.final, "the batch's rows are kept already")
         counts = batch.per_sequence(counts, "counts")
-        with torch.cuda.device(self.device):
-            call("alodlm_paged_retire", self._ref, batch.ref(self), ptr(counts), stream)
+        call_on(self.device, "alodlm_paged_retire", self._ref, batch.ref(self), ptr(counts))
 
 
 class PagedBatch:
@@ -268,23 +277,21 @@ def paged_attention(q, cache, batch, scale=None, out=None):
     written the batch's own.  ``scale`` is head_dim^-0.5 unless given.  A row that
     sees no token is zero.  Rows behind the last sequence are zero, or left as they
     were in a caller's ``out``.  No gradient: this is the decoder's side."""
-    stream = cache._stream(batch)
+    cache._check(batch)
     q = cache._rows(q, None, batch, "q")
     heads = q.shape[1]
-    _need(heads > 0 and heads % cache.kv_heads == 0,
-          f"{heads} query heads do not share {cache.kv_heads} key/value heads")
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} query heads do not share {cache.kv_heads} key/value heads")
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
     fresh = out is None
     if fresh:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _need(out.dtype == q.dtype and out.shape == q.shape and out.device == q.device
-              and out.is_contiguous() and out.data_ptr() % 16 == 0,
-              f"out must be a contiguous, 16-byte aligned {q.dtype} tensor of q's shape")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif (out.dtype != q.dtype or out.shape != q.shape or out.device != q.device
+          or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} tensor of q's shape")
     ref = batch.ref(cache)
     need = query("alodlm_paged_attention_workspace", cache._ref, ref, heads)
     workspace = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-    with torch.cuda.device(cache.device):
-        call("alodlm_paged_attention", cache._ref, ref, ptr(q), q.stride(0), ptr(out), heads, scale,
-             int(fresh), ptr(workspace), stream)
+    call_on(q.device, "alodlm_paged_attention", cache._ref, ref, ptr(q), q.stride(0), ptr(out), heads,
+            scale, int(fresh), ptr(workspace))
     return out
