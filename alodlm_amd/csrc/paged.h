@@ -103,21 +103,22 @@ __device__ __forceinline__ int given_rows(const PagedBatch& bt, int b) {
   return min(min(max(bt.offsets[b + 1], r0), bt.rows) - r0, bt.max_rows);
 }
 
-// How a call is cut up.
-struct AttendPlan {
-  int64_t chunk_keys, chunks;
-  // matrix-core kernels: whether the waves split the query columns (else the keys),
-  // 16-column tiles a wave, workgroups along a sequence's columns
-  bool split_columns;
-  int column_tiles, query_tiles;
+// How a call is cut up, and which kernel takes it.
+enum PagedKernel {
+  PAGED_ROWS,         // csrc/paged_attention.hip: a wavefront per row and head
+  PAGED_SPLIT,        // csrc/paged_split.hip: bf16 matrix cores, the keys over the waves
+  PAGED_TILES,        // csrc/paged_tiles.hip: bf16 matrix cores, the query columns over the waves
+  PAGED_F32_KEYS,     // csrc/paged_f32.hip: float32 matrix cores, the keys over the waves
+  PAGED_F32_COLUMNS,  // csrc/paged_f32.hip: the query columns over the waves
 };
-
-// Matrix-core kernels, bf16 with head_dim 64 or 128: the keys (csrc/paged_split.hip) or
-// the query columns (csrc/paged_tiles.hip) over the waves of a workgroup.
-void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
-                        const AttendPlan& p, unsigned blocks, hipStream_t st);
-void paged_tiles_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
-                        const AttendPlan& p, unsigned blocks, hipStream_t st);
+struct AttendPlan {
+  PagedKernel kernel;
+  int column_tiles, query_tiles;  // 16-column tiles a wave, workgroups along a sequence's columns
+  int64_t chunk_keys, chunks;
+};
+typedef void paged_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
+                          const AttendPlan& p, unsigned blocks, hipStream_t st);
+paged_launch paged_split_launch, paged_tiles_launch, paged_f32_launch;
 
 // Host: checks of the two structs shared by the entry points (abi errors), and
 // their device forms.

@@ -5,8 +5,7 @@
 // carries log2 e).  The keys of a sequence are cut into chunks that run apart; their
 // (m, sum, unnormalised o) in float32 are joined by a second launch, in chunk order.
 //
-// paged_rows_kernel (float32, and head sizes that the matrix-core kernels do not
-// take): one wavefront per query row, head and chunk; 64 keys at a time, one per
+// paged_rows_kernel (head sizes that the matrix-core kernels do not take): one wavefront per query row, head and chunk; 64 keys at a time, one per
 // lane for the scores, then one output column per lane for the values, which lie
 // token by token.
 #include "paged.h"
@@ -274,9 +273,6 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 // ----------------------------------------------------------------------------
 // Host
 // ----------------------------------------------------------------------------
-#ifndef ROWS_LEAST
-#define ROWS_LEAST 128
-#endif
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Keys per chunk, in whole 64-key tiles: `want` workgroups or wavefronts in all where
@@ -290,17 +286,24 @@ static void cut_keys(AttendPlan& p, int64_t max_keys, int64_t units, int64_t wan
 
 static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_batch* b, int64_t heads) {
   AttendPlan p = {};
-  if (c->dtype != ALODLM_BF16 || (c->head_dim != 64 && c->head_dim != 128)) {
-    cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, ROWS_LEAST);
+  const int64_t columns = max(b->max_rows * (heads / c->kv_heads), (int64_t)1);
+  if (c->head_dim != 64 && c->head_dim != 128) {
+    p.kernel = PAGED_ROWS;
+    cut_keys(p, b->max_keys, b->sequences * b->max_rows * heads, 8192, 128);
     return p;
   }
-  const int64_t columns = max(b->max_rows * (heads / c->kv_heads), (int64_t)1);
-  p.split_columns = columns > 32;
-  const int waves = p.split_columns ? 4 : 1;
-  p.column_tiles = columns <= 16 * waves ? 1 : 2;
+  const bool f32 = c->dtype == ALODLM_F32;
+  // Few columns: the keys over the waves, whose outputs are joined; else the columns.
+  const bool keys = columns <= (f32 ? 16 : 32);
+  p.kernel = f32 ? (keys ? PAGED_F32_KEYS : PAGED_F32_COLUMNS) : keys ? PAGED_SPLIT : PAGED_TILES;
+  const int waves = keys ? 1 : 4;
+  p.column_tiles = f32 || columns <= 16 * waves ? 1 : 2;
   p.query_tiles = (int)ceil_div(columns, 16 * p.column_tiles * waves);
-  cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles, p.split_columns || b->sequences == 1 ? 1024 : 2048,
-           512 * p.column_tiles);
+  // One sequence fills the chip evenly with two workgroups a compute unit twice over;
+  // several of different lengths with smaller chunks.  Below 512 keys (256 in float32) a
+  // chunk's own start and join weigh more than its keys.
+  cut_keys(p, b->max_keys, b->sequences * c->kv_heads * p.query_tiles,
+           keys && b->sequences > 1 ? 2048 : 1024, (f32 ? 256 : 512) * p.column_tiles);
   return p;
 }
 
@@ -321,13 +324,14 @@ static int attend_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* 
   const PagedCache dc = paged_cache(c);
   const PagedBatch db = paged_batch(b);
   const int64_t units = b->sequences * b->max_rows * a.heads;
-  const int64_t main = plan.query_tiles ? b->sequences * c->kv_heads * plan.query_tiles * a.chunks
+  const int64_t main = plan.kernel != PAGED_ROWS ? b->sequences * c->kv_heads * plan.query_tiles * a.chunks
                                         : ceil_div(units * a.chunks, ROWS_WAVES);
   const int64_t blocks = (units ? main : 0) + a.zero_blocks;
   ALODLM_CHECK_ARG(blocks < (1ll << 31) && units < (1ll << 31), "paged_attention: too many rows in one call");
   if (blocks == 0) return ALODLM_OK;
-  if (plan.split_columns) paged_tiles_launch(c, b, a, plan, (unsigned)blocks, st);
-  else if (plan.query_tiles) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
+  if (plan.kernel == PAGED_SPLIT) paged_split_launch(c, b, a, plan, (unsigned)blocks, st);
+  else if (plan.kernel == PAGED_TILES) paged_tiles_launch(c, b, a, plan, (unsigned)blocks, st);
+  else if (plan.kernel != PAGED_ROWS) paged_f32_launch(c, b, a, plan, (unsigned)blocks, st);
   else paged_rows_kernel<T, EIGHT><<<(unsigned)blocks, 64 * ROWS_WAVES, 0, st>>>(dc, db, a);
   if (a.chunks > 1 && units) {
     const int quads = (int)c->head_dim / 4;

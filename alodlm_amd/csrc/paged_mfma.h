@@ -111,7 +111,7 @@ struct Span {
 // the place of values that are inf or NaN: 0 times one of them would not be 0 for the
 // rows that do not see it.  Those that do get them afterwards: the sum of dimension d's
 // inf and NaN over keys [from, to) (a probability is positive, and inf times it is inf).
-template <int DH, bool EIGHT>
+template <int DH, bool EIGHT, typename T>
 __device__ __forceinline__ float special_sum(const PagedCache& c, const PagedBatch& bt, const Span& sp,
                                              int d, int from, int to) {
   float sum = 0.f;
@@ -121,7 +121,7 @@ __device__ __forceinline__ float special_sum(const PagedCache& c, const PagedBat
     if (page < 0) continue;
     const int64_t at = sp.block(c, page, c.page * DH) + (int64_t)d * c.page + (key & (c.page - 1));
     const float v = EIGHT && pool ? __builtin_amdgcn_cvt_f32_fp8(((const e4m3_t*)c.values)[at], 0)
-                                  : bf16_to_float(((const bf16_t*)(EIGHT ? c.open_values : c.values))[at]);
+                                  : Elem<T>::load((const T*)(EIGHT ? c.open_values : c.values), at);
     if (!(fabsf(v) < INFINITY)) sum += v;
   }
   return sum;
@@ -286,5 +286,93 @@ template <int DH, int CT> struct Columns {
       __builtin_amdgcn_sched_group_barrier(0x8, 4 * CT, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+  }
+};
+
+// Four outputs in their type.
+__device__ __forceinline__ void store_four(bf16_t* p, f32x4 x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+}
+__device__ __forceinline__ void store_four(float* p, f32x4 x) { *reinterpret_cast<f32x4*>(p) = x; }
+
+// Writes column x of a tile: its outputs `o` over dims d0 .. + 4 N in strides of `step`,
+// maximum m and sum; the call's own or a chunk's part of them.  `whole`: where the keys
+// begin that not every row of the tile sees, [whole, k1) holding inf or NaN if `special`.
+template <int DH, bool EIGHT, typename T, int N>
+__device__ __forceinline__ void write_column(const PagedCache& c, const PagedBatch& bt, const AttendArgs& a,
+                                             const Span& sp, int x, int chunk, int k0, int k1, int whole,
+                                             bool special, f32x4 (&o)[N], float m, float sum, int d0,
+                                             int step, bool states) {
+  const int i = x / a.group;
+  if (i >= sp.given) return;
+  const int limit = sp.limit(i);
+  const int64_t T_heads = (int64_t)bt.rows * a.heads;
+  const int64_t to = (sp.row0 + i) * a.heads + sp.h * a.group + x % a.group;
+  if (special)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        o[n][k] += special_sum<DH, EIGHT, T>(c, bt, sp, d0 + n * step + k, whole, min(limit, k1));
+  if (limit == 0) {  // a row that sees no key is zero
+    m = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (a.chunks == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int n = 0; n < N; ++n) store_four((T*)a.out + to * DH + d0 + n * step, o[n] * inv);
+    return;
+  }
+  if (limit <= k0 && chunk > 0) return;  // the join knows which chunks a row has
+#pragma unroll
+  for (int n = 0; n < N; ++n) store_four(a.part + (chunk * T_heads + to) * DH + d0 + n * step, o[n]);
+  if (states) a.stat[chunk * T_heads + to] = make_float2(m, sum);
+}
+
+// LDS in which the waves of a workgroup, each of which went over keys of its own, are
+// joined 16 columns at a time.
+template <int DH> struct WaveJoin {
+  float o[PAGED_WAVES][16 * (DH + 4)], m[PAGED_WAVES][16], sum[PAGED_WAVES][16];
+  int special[PAGED_WAVES];
+
+  template <bool EIGHT, typename T, int CT, int DT>
+  __device__ __forceinline__ void write(const PagedCache& c, const PagedBatch& bt, const AttendArgs& a,
+                                        const Span& sp, int first, int chunk, int k0, int k1, int whole,
+                                        bool odd, const f32x4 (&out)[CT][DT], const float (&top)[CT],
+                                        const float (&total)[CT]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+    if (lane == 0) special[wave] = odd;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&o[wave][col * (DH + 4) + d * 16 + grp * 4]) = out[t][d];
+      if (grp == 0) {
+        m[wave][col] = top[t];
+        sum[wave][col] = total[t];
+      }
+      __syncthreads();
+      const int x = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (DH / 16);
+      float M = m[0][x];
+#pragma unroll
+      for (int w = 1; w < PAGED_WAVES; ++w) M = fmaxf(M, m[w][x]);
+      const float base = M == -INFINITY ? 0.f : M;
+      float all = 0.f;
+      f32x4 r[DH / 64] = {};
+#pragma unroll
+      for (int w = 0; w < PAGED_WAVES; ++w) {
+        const float f = __builtin_amdgcn_exp2f(m[w][x] - base);
+        all = fmaf(sum[w][x], f, all);
+#pragma unroll
+        for (int n = 0; n < DH / 64; ++n)
+          r[n] += *reinterpret_cast<const f32x4*>(&o[w][x * (DH + 4) + d0 + n * 4]) * f;
+      }
+      write_column<DH, EIGHT, T>(c, bt, a, sp, first + t * 16 + x, chunk, k0, k1, whole,
+                                 special[0] | special[1] | special[2] | special[3], r, M, all, d0, 4,
+                                 (threadIdx.x & 15) == 0);
+    }
   }
 };

@@ -19,9 +19,7 @@ template <int DH, int CT, bool EIGHT>
 __global__ void __launch_bounds__(64 * PAGED_WAVES, CT == 1 ? 3 : 1)
 paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   constexpr int DT = DH / 16;
-  __shared__ __attribute__((aligned(16))) float buf[PAGED_WAVES][16 * (DH + 4)];
-  __shared__ float m_of[PAGED_WAVES][16], l_of[PAGED_WAVES][16];
-  __shared__ int special_of[PAGED_WAVES];
+  __shared__ __attribute__((aligned(16))) WaveJoin<DH> join;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
   if (blockIdx.x >= gridDim.x - a.zero_blocks) {
@@ -201,59 +199,10 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     plain_tiles(whole, hi, k0, false, std::true_type());
   }
 
-  // join the waves, 16 columns at a time
-  const int64_t T_heads = (int64_t)bt.rows * a.heads;
-  const bool any = __any(odd);
-  if (lane == 0) special_of[wave] = any;
+  float sum[CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f32x4*>(&buf[wave][col * (DH + 4) + d * 16 + grp * 4]) = cols.o[t][d];
-    if (grp == 0) { m_of[wave][col] = cols.m[t]; l_of[wave][col] = cols.l[t][0]; }
-    __syncthreads();
-    const int x = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (DH / 16);
-    float M = m_of[0][x];
-#pragma unroll
-    for (int w = 1; w < PAGED_WAVES; ++w) M = fmaxf(M, m_of[w][x]);
-    const float base_m = M == -INFINITY ? 0.f : M;
-    float sum = 0.f, r[DH / 16] = {};
-#pragma unroll
-    for (int w = 0; w < PAGED_WAVES; ++w) {
-      const float f = __builtin_amdgcn_exp2f(m_of[w][x] - base_m);
-      sum = fmaf(l_of[w][x], f, sum);
-#pragma unroll
-      for (int i = 0; i < DH / 16; ++i) r[i] = fmaf(buf[w][x * (DH + 4) + d0 + i], f, r[i]);
-    }
-    const int y = first_col + t * 16 + x, i = y / a.group;
-    if (i >= sp.given) continue;
-    const int64_t to = (sp.row0 + i) * a.heads + sp.h * a.group + y % a.group;
-    if (special_of[0] | special_of[1] | special_of[2] | special_of[3])
-      for (int k = 0; k < DH / 16; ++k)
-        r[k] += special_sum<DH, EIGHT>(c, bt, sp, d0 + k, whole, min(sp.limit(i), k1));
-    if (sp.limit(i) == 0) {  // a row that sees no key is zero
-      M = -INFINITY;
-      sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < DH / 16; ++k) r[k] = 0.f;
-    }
-    if (a.chunks == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      bf16_t* out = (bf16_t*)a.out + to * DH + d0;
-#pragma unroll
-      for (int k = 0; k < DH / 16; k += 4)
-        *reinterpret_cast<uint2*>(out + k) = make_uint2(pack_bf16x2(r[k] * inv, r[k + 1] * inv),
-                                                        pack_bf16x2(r[k + 2] * inv, r[k + 3] * inv));
-      continue;
-    }
-    if (sp.limit(i) <= k0 && chunk > 0) continue;  // the join knows which chunks a row has
-    float* part = a.part + (chunk * T_heads + to) * DH + d0;
-#pragma unroll
-    for (int k = 0; k < DH / 16; k += 4)
-      *reinterpret_cast<f32x4*>(part + k) = f32x4{r[k], r[k + 1], r[k + 2], r[k + 3]};
-    if ((threadIdx.x & 15) == 0) a.stat[chunk * T_heads + to] = make_float2(M, sum);
-  }
+  for (int t = 0; t < CT; ++t) sum[t] = cols.l[t][0];
+  join.template write<EIGHT, bf16_t>(c, bt, a, sp, first_col, chunk, k0, k1, whole, __any(odd), cols.o, cols.m, sum);
 }
 
 template <int DH, int CT>

@@ -215,46 +215,15 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   }
 
   // every wave writes its own columns
-  const int64_t T_heads = (int64_t)bt.rows * a.heads;
   const bool any = __any(odd);
   if (lane == 0) special_of[wave] = any;
   __syncthreads();
   const int whole = max(min(hi, least) / PAGED_TILE * PAGED_TILE, k0);
   const bool special = special_of[0] | special_of[1] | special_of[2] | special_of[3];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    const int x = my_col + t * 16 + col, i = x / a.group;
-    if (i >= sp.given) continue;
-    const int64_t to = (sp.row0 + i) * a.heads + sp.h * a.group + x % a.group;
-    if (special) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          cols.o[t][d][k] += special_sum<DH, EIGHT>(c, bt, sp, d * 16 + grp * 4 + k, whole, min(sp.limit(i), k1));
-    }
-    if (sp.limit(i) == 0) {  // a row that sees no key is zero
-      cols.m[t] = -INFINITY;
-      cols.l[t][0] = 0.f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) cols.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    if (a.chunks == 1) {
-      const float sum = cols.l[t][0], inv = sum == 0.f ? 0.f : 1.f / sum;
-      bf16_t* out = (bf16_t*)a.out + to * DH + grp * 4;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-        *reinterpret_cast<uint2*>(out + d * 16) =
-            make_uint2(pack_bf16x2(cols.o[t][d][0] * inv, cols.o[t][d][1] * inv),
-                       pack_bf16x2(cols.o[t][d][2] * inv, cols.o[t][d][3] * inv));
-      continue;
-    }
-    if (sp.limit(i) <= k0 && chunk > 0) continue;  // the join knows which chunks a row has
-    float* part = a.part + (chunk * T_heads + to) * DH + grp * 4;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(part + d * 16) = cols.o[t][d];
-    if (grp == 0) a.stat[chunk * T_heads + to] = make_float2(cols.m[t], cols.l[t][0]);
-  }
+  for (int t = 0; t < CT; ++t)
+    write_column<DH, EIGHT, bf16_t>(c, bt, a, sp, my_col + t * 16 + col, chunk, k0, k1, whole, special, cols.o[t],
+                                    cols.m[t], cols.l[t][0], grp * 4, 16, grp == 0);
 }
 
 template <int DH, int CT>
