@@ -92,21 +92,20 @@ paged_f32_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[i] = mfma16_f32(k[i][e], q[j][e], s[i]);
       }
-      float v_scale[4] = {1.f, 1.f, 1.f, 1.f};
+      float k_scale[4], v_scale[4] = {1.f, 1.f, 1.f, 1.f};
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float scale = a.scale2;
+        k_scale[i] = a.scale2;
         if (E && id[i] >= 0) {
-          scale *= exp2_int(sp.exponent(c, id[i], 0));
+          k_scale[i] *= exp2_int(sp.exponent(c, id[i], 0));
           v_scale[i] = exp2_int(sp.exponent(c, id[i], 1));
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = base + 16 * i + 4 * grp + r;
-          s[i][r] *= scale;
           if (id[i] < 0 || (!whole && !(key >= lo && key < min(to, limit)))) s[i][r] = -INFINITY;
-          top = fmaxf(top, s[i][r]);
+          top = fmaxf(top, s[i][r] * k_scale[i]);
         }
       }
       if (__any(top > m + 8.f)) {  // the reference follows the maximum in steps
@@ -125,7 +124,7 @@ paged_f32_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         f32x4 p;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(s[i][r] - base_m);
+          p[r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], k_scale[i], -base_m));
           sum += p[r];
         }
         if (id[i] < 0) continue;

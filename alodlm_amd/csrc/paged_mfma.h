@@ -9,9 +9,13 @@
 // multiples of 16, each lane's 16 keys lie in one page.
 //
 // 8-bit codes become bf16 times the page's power of two in one instruction a pair
-// (v_cvt_scalef32_pk_bf16_fp8), exactly.  Scores, maxima, sums and outputs are float32;
-// the probabilities are rounded to bf16 for the second product, and the sum is that of
-// the rounded ones (one more product with ones), so that the weights add up to one.
+// (v_cvt_scalef32_pk_bf16_fp8), exactly.  Scores, maxima, sums and outputs are float32.
+// The second product takes the probabilities in bf16.  Where many columns share a tile
+// that is one rounding (2^-8 of a probability, as much again as the output's own), and the
+// sum is that of the rounded ones (one more product with ones), so that the weights add
+// up to one.  Decoding steps and small windows, which wait for memory, multiply
+// the rounding errors as well: the probabilities then have 16 bits, and only the
+// output's rounding is left.
 #pragma once
 
 #include "paged.h"
@@ -215,7 +219,10 @@ template <int DH, int CT> struct Columns {
   // running maximum, but follows it only when that has grown by more than 2^8: until
   // then the probabilities stay below 2^8 of what they would be, which costs float32
   // sums and bf16 factors nothing, and no output is rescaled.
-  __device__ __forceinline__ void softmax(const f32x4 (&s)[CT][4], bf16x8 (&p)[CT][2], float scale2) {
+  // With `low` the rounding errors of the probabilities are kept as bf16 too.
+  template <bool LOW>
+  __device__ __forceinline__ void softmax(const f32x4 (&s)[CT][4], bf16x8 (&p)[CT][2], bf16x8 (&low)[CT][2],
+                                          float scale2) {
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       float top = s[t][0][0];
@@ -234,31 +241,35 @@ template <int DH, int CT> struct Columns {
       }
       const float base = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        p[t][i / 8][i % 8] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale2, -base));
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale2, -base));
+        p[t][i / 8][i % 8] = (__bf16)e;
+        if (LOW) low[t][i / 8][i % 8] = (__bf16)(e - (float)p[t][i / 8][i % 8]);
+      }
     }
   }
   // value(d, j): dimension d * 16 + lane % 16, keys (lane / 16) * 16 + 8 j .. + 8.
   template <typename Value>
-  __device__ __forceinline__ void add_values(const bf16x8 (&p)[CT][2], Value value) {
+  __device__ __forceinline__ void add_values(const bf16x8 (&p)[CT][2], const bf16x8 (&low)[CT][2], Value value) {
     bf16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int t = 0; t < CT; ++t) l[t] = mfma16(ones, p[t][j], l[t]);
+      for (int t = 0; t < CT; ++t) l[t] = mfma16(ones, low[t][j], mfma16(ones, p[t][j], l[t]));
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const bf16x8 v = value(d, j);
 #pragma unroll
-        for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v, p[t][j], o[t][d]);
+        for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v, low[t][j], mfma16(v, p[t][j], o[t][d]));
       }
     }
   }
   // The same four fragments at a time, the next four read meanwhile.
-  template <typename Value>
-  __device__ __forceinline__ void add_values_ahead(const bf16x8 (&p)[CT][2], Value value) {
+  template <bool LOW, typename Value>
+  __device__ __forceinline__ void add_values_ahead(const bf16x8 (&p)[CT][2], const bf16x8 (&low)[CT][2],
+                                                   Value value) {
     bf16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
@@ -268,7 +279,10 @@ template <int DH, int CT> struct Columns {
 #pragma unroll
     for (int k = 0; k < 4; ++k) now[k] = value(k, 0);
 #pragma unroll
-    for (int t = 0; t < CT; ++t) l[t] = mfma16(ones, p[t][1], mfma16(ones, p[t][0], l[t]));
+    for (int t = 0; t < CT; ++t) {
+      l[t] = mfma16(ones, p[t][1], mfma16(ones, p[t][0], l[t]));
+      if (LOW) l[t] = mfma16(ones, low[t][1], mfma16(ones, low[t][0], l[t]));
+    }
 #pragma unroll
     for (int g = 0; g < STEPS; ++g) {
       __builtin_amdgcn_sched_barrier(0);
@@ -278,12 +292,15 @@ template <int DH, int CT> struct Columns {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int t = 0; t < CT; ++t)
-          o[t][g * 4 % DT + k] = mfma16(now[k], p[t][g * 4 / DT], o[t][g * 4 % DT + k]);
+        for (int t = 0; t < CT; ++t) {
+          f32x4& to = o[t][g * 4 % DT + k];
+          to = mfma16(now[k], p[t][g * 4 / DT], to);
+          if (LOW) to = mfma16(now[k], low[t][g * 4 / DT], to);
+        }
 #pragma unroll
       for (int k = 0; k < 4; ++k) now[k] = next[k];
       if (g + 1 < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, 4 * CT, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 4 * CT * (LOW ? 2 : 1), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   }

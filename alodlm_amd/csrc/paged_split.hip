@@ -89,9 +89,9 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       return f % 2 ? widen(w.z, w.w, scale) : widen(w.x, w.y, scale);
     });
   };
-  auto add_values = [&](const CodeTile<DH>& t, const bf16x8 (&p)[CT][2]) {
+  auto add_values = [&](const CodeTile<DH>& t, const bf16x8 (&p)[CT][2], const bf16x8 (&low)[CT][2]) {
     const float scale = exp2_int(t.v_exponent);
-    cols.add_values(p, [&](int d, int j) {
+    cols.add_values(p, low, [&](int d, int j) {
       const uint4 w = t.v[d];
       return j ? widen(w.z, w.w, scale) : widen(w.x, w.y, scale);
     });
@@ -116,15 +116,15 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     while (true) {
       const bool more = base + STEP < to;
       f32x4 s[CT][4];
-      bf16x8 p[CT][2];
+      bf16x8 p[CT][2], low[CT][2];
       scores(tile, s);
       if (more) load_key_codes(tile, base + STEP, sp.page_in(c, k_next, base + STEP, 0, to));
       if (!__all(tile.there)) {
         cols.hide(s, base, 0, to, tile.there);
         clear_values(tile);
       }
-      cols.softmax(s, p, a.scale2);
-      add_values(tile, p);
+      cols.template softmax<true>(s, p, low, a.scale2);
+      add_values(tile, p, low);
       if (!more) break;
       base += STEP;
       load_value_codes(tile, base, sp.page_in(c, v_next, base, 0, to));
@@ -139,11 +139,11 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       load_key_codes(tile, base, sp.page<true>(c, bt, base + (col >> 2) * 16, k0, to));
       load_value_codes(tile, base, sp.page<true>(c, bt, base + grp * 16, k0, to));
       f32x4 s[CT][4];
-      bf16x8 p[CT][2];
+      bf16x8 p[CT][2], low[CT][2];
       scores(tile, s);
       cols.hide(s, base, k0, to, tile.there);
       clear_values(tile);
-      cols.softmax(s, p, a.scale2);
+      cols.template softmax<true>(s, p, low, a.scale2);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         uint32_t* w = &tile.v[d].x;
@@ -153,7 +153,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
           w[i] = without_special<true>(w[i]);
         }
       }
-      add_values(tile, p);
+      add_values(tile, p, low);
     }
   };
   // Tiles [from, to) of keys [lo, to) in 16 bits, loaded as the products take them
@@ -168,13 +168,13 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       const bf16_t* kp = keys + key_place(base, max(k_page, 0));
       const bf16_t* vp = values + value_place(base, max(v_page, 0));
       f32x4 s[CT][4];
-      bf16x8 p[CT][2];
+      bf16x8 p[CT][2], low[CT][2];
       cols.scores(s, [&](int i, int f) {
         return *reinterpret_cast<const bf16x8*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
       });
       if (!whole || !__all(v_page >= 0)) cols.hide(s, base, lo, to, v_page >= 0);
-      cols.softmax(s, p, a.scale2);
-      cols.add_values(p, [&](int d, int j) {
+      cols.template softmax<true>(s, p, low, a.scale2);
+      cols.add_values(p, low, [&](int d, int j) {
         uint4 w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
         if (v_page < 0) w = make_uint4(0, 0, 0, 0);
         if (!whole) {

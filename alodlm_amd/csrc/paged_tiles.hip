@@ -198,15 +198,16 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     if (base < my_most) {
       const TileBuffer<DH>& t = tiles[i & 1];
       f32x4 s[CT][4];
-      bf16x8 p[CT][2];
+      constexpr bool LOW = CT == 1;
+      bf16x8 p[CT][2], low[CT][2];
       cols.scores_ahead(s, [&](int sub, int f) {
         const int key = (col >> 2) * 16 + 4 * sub + (col & 3);
         return *reinterpret_cast<const bf16x8*>(t.k + key_piece<DH>(key, f * 4 + grp));
       });
       const bool mine = there[i & 1][grp];
       if (base < lo || base + PAGED_TILE > min(end, my_least) || !__all(mine)) cols.hide(s, base, lo, end, mine);
-      cols.softmax(s, p, a.scale2);
-      cols.add_values_ahead(p, [&](int d, int j) {
+      cols.template softmax<LOW>(s, p, low, a.scale2);
+      cols.template add_values_ahead<LOW>(p, low, [&](int d, int j) {
         return *reinterpret_cast<const bf16x8*>(t.v + value_piece<DH>(d * 16 + col, grp, j));
       });
     }
