@@ -72,7 +72,7 @@ paged_f32_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     for (; base < to; base += step) {
       int id[4];
       const S *kp[4], *vp[4];
-      f32x4 s[4];
+      f32x4 s[4], s_odd[4];  // two sums each: half the roundings in a row
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = base + 16 * i;
@@ -80,7 +80,7 @@ paged_f32_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
         const int64_t block = sp.block(c, max(id[i], 0), head_block);
         kp[i] = keys + block + (((key & (page - 1)) + col) * DH + grp * 4);
         vp[i] = values + block + (col * page + (key & (page - 1)) + grp * 4);
-        s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s[i] = s_odd[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
       for (int j = 0; j < DT; ++j) {
@@ -90,8 +90,13 @@ paged_f32_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[i] = mfma16_f32(k[i][e], q[j][e], s[i]);
+          for (int i = 0; i < 4; ++i) {
+            f32x4& to = j % 2 ? s_odd[i] : s[i];
+            to = mfma16_f32(k[i][e], q[j][e], to);
+          }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += s_odd[i];
       float k_scale[4], v_scale[4] = {1.f, 1.f, 1.f, 1.f};
       float top = -INFINITY;
 #pragma unroll
