@@ -16,6 +16,7 @@ the vocabulary.
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, call_on, ptr, query
@@ -112,14 +113,22 @@ MAX_TOP = 64
 
 
 def _vocabulary_rows(logits):
-    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+    """The logits with a vocabulary in a row, and the rows' stride."""
+    R, V = logits.shape
+    row, column = logits.stride()
+    if V == 1 or column == 1:
+        if R < 2:  # one row's stride says nothing
+            return logits, V
+        if row >= V:
+            return logits, row
+    return logits.contiguous(), V
 
 
 def _log_probs(logits, targets, top, inv_temperature, ignore_index):
     """The four results and the buffer that starts with the backward's statistics."""
     R, V = logits.shape
     dev = logits.device
-    x = _vocabulary_rows(logits)
+    x, ld = _vocabulary_rows(logits)
     log_prob = torch.empty(R, dtype=torch.float32, device=dev)
     entropy = torch.empty_like(log_prob)
     top_log_prob = torch.empty(R, top, dtype=torch.float32, device=dev)
@@ -128,7 +137,7 @@ def _log_probs(logits, targets, top, inv_temperature, ignore_index):
     buf = torch.empty(2 * R + query("alodlm_token_log_probs_workspace", R, V, top),
                       dtype=torch.float32, device=dev)
     stats = buf.data_ptr()
-    call_on(dev, "alodlm_token_log_probs", x.data_ptr(), x.stride(0), targets.data_ptr(), R, V, top,
+    call_on(dev, "alodlm_token_log_probs", x.data_ptr(), ld, targets.data_ptr(), R, V, top,
             inv_temperature, ignore_index, log_prob.data_ptr(), entropy.data_ptr(), stats,
             top_log_prob.data_ptr(), top_ids.data_ptr(), stats + 8 * R, _lib.dtype_code(x.dtype))
     return log_prob, entropy, top_log_prob, top_ids, buf
@@ -145,15 +154,16 @@ class _TokenLogProbs(torch.autograd.Function):
         return tuple(outs)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_log_prob, d_entropy, d_top, _d_ids):
         logits, targets, top_ids, entropy, buf = ctx.saved_tensors
         top, inv_temperature, ignore_index = ctx.args
         R, V = logits.shape
-        x = _vocabulary_rows(logits)
+        x, ld = _vocabulary_rows(logits)
         out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
         grads = [g if g is None or (g.dtype == torch.float32 and g.is_contiguous())
                  else g.to(torch.float32).contiguous() for g in (d_log_prob, d_entropy, d_top)]
-        call_on(x.device, "alodlm_token_log_probs_bwd", ptr(x), x.stride(0), ptr(targets), ptr(top_ids),
+        call_on(x.device, "alodlm_token_log_probs_bwd", ptr(x), ld, ptr(targets), ptr(top_ids),
                 ptr(buf), ptr(entropy), *map(ptr, grads), R, V, top, inv_temperature, ignore_index,
                 ptr(out), _lib.dtype_code(x.dtype))
         return out, None, None, None, None

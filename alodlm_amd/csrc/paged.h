@@ -21,7 +21,7 @@ struct PagedBatch {
   const int32_t* lengths;
   const int32_t* offsets;
   const int32_t* slot_of;
-  int sequences, width, rows, max_rows, final_rows;
+  int sequences, width, rows, max_rows, max_keys, final_rows;
 
   // Row range of sequence b, inside the batch's rows.
   __device__ __forceinline__ int first_row(int b) const {
@@ -90,10 +90,13 @@ __device__ __forceinline__ int sealed_keys(const PagedCache& c, const PagedBatch
   return (bt.final_rows ? end : held) >> c.shift << c.shift;
 }
 
-// The first key whose place in the open pages another one has taken (windows longer
-// than the open pages are refused by the host; this bounds what is read).
-__device__ __forceinline__ int open_end(const PagedCache& c, int sealed, int end) {
-  return (int)min((int64_t)end, (int64_t)sealed + (int64_t)c.open_pages * c.page);
+// The end of the keys that are attended to: the tokens, as far as max_keys goes and open
+// pages hold them (windows longer than those are refused by the host; this bounds what is
+// read).
+__device__ __forceinline__ int key_end(const PagedCache& c, const PagedBatch& bt, int sealed, int end,
+                                       bool eight) {
+  end = min(end, bt.max_keys);
+  return eight ? (int)min((int64_t)end, (int64_t)sealed + (int64_t)c.open_pages * c.page) : end;
 }
 
 // Rows of sequence b that results are written for: those of the batch, up to max_rows,

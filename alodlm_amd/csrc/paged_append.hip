@@ -313,7 +313,7 @@ PagedCache paged_cache(const alodlm_paged_cache* c) {
 
 PagedBatch paged_batch(const alodlm_paged_batch* b) {
   return {b->table, b->lengths, b->offsets, b->slots, (int)b->sequences, (int)b->width,
-          (int)b->rows, (int)b->max_rows, (int)b->final_rows};
+          (int)b->rows, (int)b->max_rows, (int)b->max_keys, (int)b->final_rows};
 }
 
 template <typename T>

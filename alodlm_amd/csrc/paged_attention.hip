@@ -116,7 +116,7 @@ paged_rows_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     if (i < n) {
       const int end = held + n;
       sealed = sealed_keys(c, bt, held, end, EIGHT);
-      last = EIGHT ? open_end(c, sealed, end) : end;
+      last = key_end(c, bt, sealed, end, EIGHT);
       limit = min(held + i + 1, last);
       if (EIGHT) slot = bt.slot(b, c.slots);
     }
@@ -224,7 +224,7 @@ paged_join_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     int limit = 0;
     if (i < n) {
       const int end = held + n, sealed = sealed_keys(c, bt, held, end, EIGHT);
-      limit = min(held + i + 1, EIGHT ? open_end(c, sealed, end) : end);
+      limit = min(held + i + 1, key_end(c, bt, sealed, end, EIGHT));
     }
     const int count = max((limit + a.chunk_keys - 1) / a.chunk_keys, 1);
     at = ((int64_t)bt.first_row(b) + i) * a.heads + head;

@@ -75,7 +75,7 @@ struct Span {
     s.held = max(held, 0);
     const int end = s.held + s.n;
     s.sealed = EIGHT ? sealed_keys(c, bt, s.held, end, true) : end;
-    s.reach = EIGHT ? open_end(c, s.sealed, end) : end;
+    s.reach = key_end(c, bt, s.sealed, end, EIGHT);
     s.slot = EIGHT ? bt.slot(b, c.slots) : 0;
     s.row0 = bt.first_row(b);
     return s;

@@ -20,9 +20,12 @@ into calls.  A decoding window, whose rows the next pass rewrites, is a batch wi
 ``final=False``; ``retire`` keeps the first of its rows, as
 ``PrefixCache.retire`` does.
 
-Nothing here reads the device from the host, and every call can be captured into a
-graph.  The kernels follow no entry that is out of range: such tokens are neither
-written nor attended to (``PagedBatch.check`` finds them, for debugging).
+No call reads the device from the host (only a batch made without ``rows`` does, and
+``PagedBatch.check``), and every call can be captured into a graph; the batch's tensors
+are read when a call runs, so a program may change them in place between replays.  The
+kernels follow no entry that is out of range: such tokens are neither written nor
+attended to (``check`` finds them, for debugging).  Sequences may share whole pages (a
+common prefix); a page that is still being written, and a slot, belong to one.
 """
 
 import ctypes
@@ -132,8 +135,8 @@ class PagedCache:
 
     # ------------------------------------------------------------------ calls
     def _rows(self, t, heads, batch, what):
-        """``t`` as the kernels read it: rows [heads, head_dim] behind one another,
-        the row stride free, 16-byte aligned (copied where it is not)."""
+        """``t`` as the kernels read it, and its row stride: rows [heads, head_dim], the
+        stride free, 16-byte aligned (copied where it is not)."""
         if t.dtype != self.dtype:
             raise ValueError(f"{what} must be {self.dtype}, got {t.dtype}")
         if t.device != self.device:
@@ -144,10 +147,13 @@ class PagedCache:
             raise ValueError(f"{what} must be [{batch.rows}, {heads or 'heads'}, {dh}], "
                              f"got {list(shape)}")
         row, head, dim = t.stride()
+        if shape[0] < 2:  # one row's stride says nothing
+            row = shape[1] * dh
         if (dim != 1 or head != dh or row < shape[1] * dh or row * t.element_size() % 16
                 or t.data_ptr() % 16):
             t = t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()
-        return t
+            row = shape[1] * dh
+        return t, row
 
     def _table(self, t, batch, like):
         """A rotary table as the kernels read it (``layers.table``), 16-byte aligned."""
@@ -162,6 +168,9 @@ class PagedCache:
                              "device")
         if batch.device != self.device:
             raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        if self.eight_bit and batch.slots is None and batch.sequences > self.open_keys.shape[0]:
+            raise ValueError(f"{batch.sequences} sequences without slots of their own, and "
+                             f"{self.open_keys.shape[0]} slots")
 
     def append(self, k, v, batch, cos=None, sin=None, q=None):
         """Writes the rows' keys and values [rows, kv_heads, head_dim] behind their
@@ -173,17 +182,17 @@ class PagedCache:
             raise ValueError("cos and sin belong together")
         if q is not None and cos is None:
             raise ValueError("q is given to be rotated: cos and sin are missing")
-        k = self._rows(k, self.kv_heads, batch, "k")
-        v = self._rows(v, self.kv_heads, batch, "v")
+        k, ldk = self._rows(k, self.kv_heads, batch, "k")
+        v, ldv = self._rows(v, self.kv_heads, batch, "v")
         if cos is not None:
             cos, sin = self._table(cos, batch, k), self._table(sin, batch, k)
         out, heads, ldq = None, 0, 0
         if q is not None:
-            q = self._rows(q, None, batch, "q")
-            heads, ldq = q.shape[1], q.stride(0)
+            q, ldq = self._rows(q, None, batch, "q")
+            heads = q.shape[1]
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        call_on(self.device, "alodlm_paged_append", self._ref, batch.ref(self), ptr(k), k.stride(0),
-                ptr(v), v.stride(0), ptr(q), ldq, ptr(out), heads, ptr(cos), ptr(sin))
+        call_on(self.device, "alodlm_paged_append", self._ref, batch.ref(self), ptr(k), ldk,
+                ptr(v), ldv, ptr(q), ldq, ptr(out), heads, ptr(cos), ptr(sin))
         return out
 
     def retire(self, batch, counts):
@@ -205,9 +214,10 @@ class PagedBatch:
     ``rows`` (default: offsets[-1], read from the device) is the number of rows that
     the step's tensors have; rows behind the last sequence are padding.  ``max_rows``
     bounds a sequence's rows (default: ``rows``) and ``max_keys`` its tokens with
-    them (default: what the table holds): they size the launches, and a sequence's
-    rows and tokens past them are left out.  ``final``: the rows are kept, else they
-    are a window that ``retire`` shortens."""
+    them (default: what the table holds): they size the launches.  A sequence's rows
+    past max_rows are left out (their results are not written), and its tokens past
+    max_keys are not attended to.  ``final``: the rows are kept, else they are a window
+    that ``retire`` shortens."""
 
     def __init__(self, table, lengths, offsets, rows=None, max_rows=None, max_keys=None, slots=None,
                  final=True):
@@ -226,10 +236,11 @@ class PagedBatch:
         self._refs = {}
 
     def _ints(self, t, shape, what):
-        _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.device == self.device,
-              f"{what} must be int32 {list(shape)} on {self.device}, got {t.dtype} "
-              f"{list(t.shape)} on {t.device}")
-        return t.contiguous()
+        if (t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device
+                or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous int32 {list(shape)} on {self.device}, got "
+                             f"{t.dtype} {list(t.shape)} on {t.device}")
+        return t
 
     def per_sequence(self, t, what):
         return self._ints(t, (self.sequences,), what)
@@ -268,6 +279,7 @@ class PagedBatch:
             slots = range(self.sequences) if self.slots is None else self.slots.tolist()
             _need(all(0 <= s < cache.open_keys.shape[0] for s in slots),
                   "a sequence names a slot outside the cache")
+            _need(len(set(slots)) == self.sequences, "two sequences name one slot")
 
 
 def paged_attention(q, cache, batch, scale=None, out=None):
@@ -278,7 +290,7 @@ def paged_attention(q, cache, batch, scale=None, out=None):
     sees no token is zero.  Rows behind the last sequence are zero, or left as they
     were in a caller's ``out``.  No gradient: this is the decoder's side."""
     cache._check(batch)
-    q = cache._rows(q, None, batch, "q")
+    q, ldq = cache._rows(q, None, batch, "q")
     heads = q.shape[1]
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads do not share {cache.kv_heads} key/value heads")
@@ -292,6 +304,6 @@ def paged_attention(q, cache, batch, scale=None, out=None):
     ref = batch.ref(cache)
     need = query("alodlm_paged_attention_workspace", cache._ref, ref, heads)
     workspace = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-    call_on(q.device, "alodlm_paged_attention", cache._ref, ref, ptr(q), q.stride(0), ptr(out), heads,
+    call_on(q.device, "alodlm_paged_attention", cache._ref, ref, ptr(q), ldq, ptr(out), heads,
             scale, int(fresh), ptr(workspace))
     return out

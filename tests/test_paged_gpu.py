@@ -305,6 +305,8 @@ def test_refusals():
             (lambda: run.cache.append(k, k, batch, cos=cos), "belong together"),
             (lambda: run.cache.append(k, k, batch, q=q), "rotated"),
             (lambda: run.cache.append(k, k, batch, cos=cos[:, :32], sin=cos), "cos/sin"),
+            (lambda: run.cache.append(k, k, PagedBatch(run.table.expand(2, -1).contiguous().repeat(3, 1), run.slots.repeat(3),
+                                                       torch.zeros(7, dtype=torch.int32, device=DEV), rows=3)), "slots"),
             (lambda: run.cache.retire(batch, run.slots), "kept already"),
             (lambda: run.cache.retire(run.batch([1, 1], final=False), run.slots[:1]), "counts"),
             (lambda: run.cache.append(k[:2], k[:2], run.batch([2, 0], final=False)), "window"),
@@ -450,6 +452,65 @@ def test_scale_and_max_keys():
         run.plain.k[b].append(k[b])
         run.plain.v[b].append(v[b])
         run.compare(got[b:b + 1], q[b:b + 1], *run.plain.tokens(b), [n + 1], scale=0.5)
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, BF16, 64, True), (20, 2, 64, BF16, 16, False),
+                                   (4, 2, 128, F32, 64, True), (2, 1, 24, BF16, 64, True)])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_tokens_past_max_keys_take_no_part(shape, rows):
+    """A bound below the lengths: attention over the tokens within it, for rows over one
+    chunk of keys and over many."""
+    log(f"paged max_keys {shape} {rows}")
+    run = Run(2, *shape, tokens=12800)
+    counts = [6000, 90]
+    k, v = (run.randn(6090, shape[1], shape[2]) for _ in range(2))
+    run.cache.append(k.to(DEV), v.to(DEV), run.batch(counts))
+    run.lengths = counts
+    run.plain.k, run.plain.v = [list(k[:6000]), list(k[6000:])], [list(v[:6000]), list(v[6000:])]
+    q, more = run.randn(2 * rows, shape[0], shape[2]), run.randn(2 * rows, shape[1], shape[2])
+    for bound in (5200, 70, 65, 1, 0):
+        batch = run.batch([rows, rows], max_keys=bound)
+        run.cache.append(more.to(DEV), more.to(DEV), batch)
+        got = paged_attention(q.to(DEV), run.cache, batch).cpu()
+        if bound == 0:
+            assert not bool(got.any())
+            continue
+        for b, n in enumerate(counts):
+            mine = [more[b * rows + i] for i in range(rows)]
+            plain = OracleCache(1, run.page, run.eight_bit)
+            plain.k[0], plain.v[0] = run.plain.k[b] + mine, run.plain.v[b] + mine
+            K, V = plain.tokens(0)
+            run.compare(got[b * rows:(b + 1) * rows], q[b * rows:(b + 1) * rows], K, V,
+                        [min(n + i + 1, bound) for i in range(rows)])
+
+
+def test_single_rows_of_any_stride():
+    """One row, whose stride may be anything."""
+    log("paged single rows")
+    run = Run(1, 4, 2, 128, BF16, 64, True, tokens=64)
+    k, q = run.randn(1, 2, 128).to(DEV), run.randn(1, 4, 128).to(DEV)
+    batch = run.batch([1])
+    odd = [t.as_strided(t.shape, (1, 128, 1)) for t in (k, q)]
+    cos = torch.ones(1, 128, dtype=BF16, device=DEV)
+    turned = run.cache.append(odd[0], odd[0], batch, cos=cos, sin=torch.zeros_like(cos), q=odd[1])
+    assert torch.equal(turned, q)
+    out = paged_attention(turned, run.cache, batch)
+    assert torch.equal(out, k.repeat_interleave(2, 1))
+
+
+def test_shared_pages():
+    """Two sequences on the pages of one prefix, each with tokens of its own behind it."""
+    log("paged shared prefix")
+    for shape in ((4, 2, 128, BF16, 64, True), (4, 2, 64, F32, 16, False)):
+        run = Run(2, *shape, tokens=320)
+        run.table[1, :2 * 64 // shape[4]] = run.table[0, :2 * 64 // shape[4]]
+        k, v = (run.randn(128, 2, shape[2]) for _ in range(2))
+        run.cache.append(k.to(DEV), v.to(DEV), run.batch([128, 0]))
+        run.lengths = [128, 128]
+        run.plain.k, run.plain.v = [list(k), list(k)], [list(v), list(v)]
+        run.step([70, 3])
+        run.step([1, 1])
+        run.check_cache()
 
 
 def test_streams():

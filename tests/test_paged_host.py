@@ -96,6 +96,8 @@ def test_batch_refusals():
         batch(slots=ints(0))
     with pytest.raises(ValueError, match="negative"):
         batch(rows=-1)
+    with pytest.raises(ValueError, match="contiguous"):  # a copy would not follow changes in place
+        batch(slots=torch.arange(4, dtype=torch.int32)[::2])
     b = batch()
     assert (b.rows, b.max_rows, b.sequences, b.width) == (3, 3, 2, 2)
     assert batch(rows=7, max_rows=9).max_rows == 7
@@ -107,7 +109,7 @@ def test_checks_find_entries_out_of_range():
     for bad in (dict(table=((0, 8), (2, 3)), lengths=(16, 0)), dict(table=((-1, 0), (2, 3))),
                 dict(lengths=(-1, 0)), dict(lengths=(32, 0)), dict(offsets=(0, 3, 1), rows=3),
                 dict(offsets=(0, 1, 3), rows=2), dict(max_rows=1), dict(max_keys=5),
-                dict(slots=ints(0, 2)), dict(slots=ints(-1, 0)), dict(offsets=(-1, 1, 3))):
+                dict(slots=ints(0, 2)), dict(slots=ints(-1, 0)), dict(slots=ints(1, 1)), dict(offsets=(-1, 1, 3))):
         with pytest.raises(ValueError):
             batch(**bad).check(c)
     # a page that no token lies in may be named anyhow

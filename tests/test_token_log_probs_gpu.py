@@ -188,6 +188,19 @@ def test_strides(dtype):
             assert bool(((a - b).abs() <= 60 * EPS * (1 + b.abs())).all())
         check(view, t, 4)
     check(wide[::2][:, ::3], targets[:3] % 1000, 3)
+    for view in (wide.as_strided((1, 3001), (0, 1)), wide.as_strided((1, 1), (0, 0)), wide[:, 5:6],
+                 wide[2:3, 1:4]):
+        check(view, targets[:view.shape[0]].clamp(max=view.shape[1] - 1), 1)
+
+
+def test_no_second_derivative():
+    log("token_log_probs second derivative")
+    logits, targets = make(3, 40, F32)
+    x = logits.requires_grad_()
+    up = torch.ones(3, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(token_log_probs(x, targets).entropy, x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum(), up)
 
 
 def test_rows_and_targets_left_alone():
