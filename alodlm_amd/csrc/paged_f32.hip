@@ -10,6 +10,9 @@
 // Every value that a wave reads feeds 16 columns at the float32 rate, 32 cycles for 64
 // bytes a lane group: the caches keep up, so nothing is staged.  With few columns the
 // keys are split over the waves, else the columns.
+//
+// Measured: five sequences of 1 to 3 rows over 30 to 903 float32 tokens, 16 heads over 8,
+// 23 MB: 14 us and 4 for the join, two tiles a wave one after the other.
 #include "paged_mfma.h"
 
 __device__ __forceinline__ f32x4 mfma16_f32(float a, float b, f32x4 c) {

@@ -8,6 +8,15 @@
 // the buffer: one barrier a tile.  The limits are then the matrix instructions, the
 // LDS reads (32 KB a wave and tile against 32 columns) and the exponentials, which
 // two workgroups a compute unit overlap.
+//
+// Measured: four prompts of 700 to 4100 rows, 16 heads over 8 of 128: 178 to 208 us (the
+// clock goes with the card), 675 to 790 TFLOP/s of 1198 for a large library product;
+// matrix instructions busy 33 % of the cycles, vector instructions 48 %, LDS 27 %.  16
+// windows of 16 to 27 rows behind 300 to 3100 tokens, 32 heads over 8: 40 us and 8 for the
+// join, the time of the longest chunk.  On the way: integer divisions per tile cost 10 %,
+// page numbers checked and scales computed where they are loaded 18 %, outputs rescaled
+// at every new maximum 7 %, LDS reads left behind the products before them 4 %; bank
+// conflicts (27 % of the LDS cycles, none now) cost no time.
 #include "paged_mfma.h"
 
 template <int DH> struct TileBuffer {

@@ -15,6 +15,11 @@
 //
 // Split: one workgroup per row where there are rows enough, else a row is cut into
 // chunks whose sums and ordered candidates a second launch joins.
+//
+// Measured: 4096 rows of 151936 bf16 logits 214 to 238 us (5.2 to 5.8 TB/s) and their
+// gradient 405 us (6.1 TB/s read and written); eight rows with 20 alternatives 11 us and 7
+// for the join, both a chain of waits: a chunk's loads, the sums, the threshold by 256
+// comparisons a thread, the ranks.
 #include "common.h"
 
 #define LP_THREADS 256
