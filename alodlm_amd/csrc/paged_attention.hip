@@ -295,11 +295,14 @@ static AttendPlan attend_plan(const alodlm_paged_cache* c, const alodlm_paged_ba
     return p;
   }
   const bool f32 = c->dtype == ALODLM_F32;
-  // Few columns: the keys over the waves, whose outputs are joined; else the columns.
-  const bool keys = columns <= (f32 ? 16 : 32);
+  // Few columns: the keys over the waves, whose outputs are joined; else the columns, which
+  // reads a tile once for 64 of them.  16 sequences of up to 3100 tokens, 32 columns: codes
+  // 38 us with the keys over the waves and 41 with the columns, pages in bf16 55 and 45;
+  // 33 to 64 columns: codes 45 and 44, bf16 66 and 48.
+  const bool keys = columns <= (c->eight_bit && !f32 ? 32 : 16);
   p.kernel = f32 ? (keys ? PAGED_F32_KEYS : PAGED_F32_COLUMNS) : keys ? PAGED_SPLIT : PAGED_TILES;
   const int waves = keys ? 1 : 4;
-  p.column_tiles = f32 || columns <= 16 * waves ? 1 : 2;
+  p.column_tiles = f32 || keys || columns <= 16 * waves ? 1 : 2;
   p.query_tiles = (int)ceil_div(columns, 16 * p.column_tiles * waves);
   // One sequence fills the chip evenly with two workgroups a compute unit twice over;
   // several of different lengths with smaller chunks.  Below 512 keys (256 in float32) a

@@ -1,5 +1,5 @@
 // Attention over paged keys on the matrix cores, the keys split over the waves: bf16,
-// head_dim 64 and 128, few rows a sequence (decoding steps).
+// head_dim 64 and 128, few rows a sequence (decoding steps, small windows).
 //
 // A decoding step reads every key and value once and does a few operations with each:
 // it is bound by the bytes.  So nothing is staged: every wave takes 64-key tiles of its
@@ -10,7 +10,9 @@
 // Measured: 64 sequences of 200 to 8000 tokens, one row of 32 heads over 8 each, 585 MB:
 // 120 us and 5 for the join (4.7 TB/s; a large copy runs at 5.08).  One sequence of 130001
 // tokens, 16 heads over 8, 266 MB: 48 and 9 us.  One of 300 tokens: 11 us, two tiles and
-// an open page one after the other.  On the way: spilled registers cost 2.4 times (their
+// an open page one after the other.  16 windows of 16 rows, 16 heads over 8, behind 300 to
+// 3100 tokens: 38 us; both of a window's column tiles in one wave made it 42 (one wave a
+// SIMD instead of three).  On the way: spilled registers cost 2.4 times (their
 // reloads wait for the tile on its way), chunk numbers that pick the die 1.4 (eight
 // chunks, eight dies, and few sequences reach the last), a scale computed where its
 // exponent is loaded, or a page number checked there, 1.1 (both wait for what was loaded
@@ -24,10 +26,10 @@ template <int DH> struct CodeTile {
   bool there;
 };
 
-template <int DH, int CT, bool EIGHT>
-__global__ void __launch_bounds__(64 * PAGED_WAVES, CT == 1 ? 3 : 1)
+template <int DH, bool EIGHT>
+__global__ void __launch_bounds__(64 * PAGED_WAVES, 3)
 paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
-  constexpr int DT = DH / 16;
+  constexpr int DT = DH / 16, CT = 1;  // more columns: more workgroups
   __shared__ __attribute__((aligned(16))) WaveJoin<DH> join;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -36,14 +38,14 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     return;
   }
   const int page = c.page;
-  // Neighbouring workgroups go to different dies.  Heads side by side, then sequences,
-  // turned on by one per chunk, then chunks: every die gets long and short sequences, and
-  // the chunks that few sequences reach come last.  Query tiles lie a multiple of all
-  // that apart, so that they tend to meet on one die's cache.
-  const int per_chunk = bt.sequences * c.kv_heads, per_tile = per_chunk * a.chunks;
-  const int qt = blockIdx.x / per_tile, rest = blockIdx.x % per_tile;
-  const int chunk = rest / per_chunk;
-  const Span sp = Span::of<EIGHT>(c, bt, (rest % per_chunk / c.kv_heads + chunk) % bt.sequences,
+  // Neighbouring workgroups go to different dies.  Heads side by side, then a sequence's
+  // query tiles (eight heads on, so that they tend to meet on one die's cache), then
+  // sequences, turned on by one per chunk, then chunks: every die gets long and short
+  // sequences, and the chunks that few sequences reach come last.
+  const int per_chunk = bt.sequences * a.query_tiles * c.kv_heads;
+  const int chunk = blockIdx.x / per_chunk, rest = blockIdx.x % per_chunk;
+  const int qt = rest / c.kv_heads % a.query_tiles;
+  const Span sp = Span::of<EIGHT>(c, bt, (rest / (c.kv_heads * a.query_tiles) + chunk) % bt.sequences,
                                   rest % c.kv_heads);
   const int first_col = qt * 16 * CT;
   if (first_col >= sp.given * a.group) return;
@@ -214,22 +216,17 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   join.template write<EIGHT, bf16_t>(c, bt, a, sp, first_col, chunk, k0, k1, whole, __any(odd), cols.o, cols.m, sum);
 }
 
-template <int DH, int CT>
+template <int DH>
 static void launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
                    unsigned grid, hipStream_t st) {
   if (c->eight_bit)
-    paged_split_kernel<DH, CT, true><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
+    paged_split_kernel<DH, true><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
   else
-    paged_split_kernel<DH, CT, false><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
+    paged_split_kernel<DH, false><<<grid, 64 * PAGED_WAVES, 0, st>>>(paged_cache(c), paged_batch(b), a);
 }
 
 void paged_split_launch(const alodlm_paged_cache* c, const alodlm_paged_batch* b, const AttendArgs& a,
-                        const AttendPlan& p, unsigned grid, hipStream_t st) {
-  if (c->head_dim == 64) {
-    if (p.column_tiles == 1) launch<64, 1>(c, b, a, grid, st);
-    else launch<64, 2>(c, b, a, grid, st);
-  } else {
-    if (p.column_tiles == 1) launch<128, 1>(c, b, a, grid, st);
-    else launch<128, 2>(c, b, a, grid, st);
-  }
+                        const AttendPlan&, unsigned grid, hipStream_t st) {
+  if (c->head_dim == 64) launch<64>(c, b, a, grid, st);
+  else launch<128>(c, b, a, grid, st);
 }
