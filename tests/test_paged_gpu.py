@@ -440,6 +440,30 @@ def test_long_contexts(shape):
     run.step([2, 5, 3])
 
 
+@pytest.mark.parametrize("shape", [(2, 1, 128, BF16, 64, True), (2, 1, 64, BF16, 32, False), (2, 1, 64, F32, 64, False),
+                                   (1, 1, 24, BF16, 64, True), (1, 1, 256, F32, 64, True)])
+def test_many_chunks(shape):
+    """One row of few heads over more chunks than the join's ways take at once, and windows
+    whose columns end inside the first, second and ninth of their 16-column tiles."""
+    log(f"paged many chunks {shape}")
+    heads, kv, dh, dtype, page, eight_bit = shape
+    run = Run(2, *shape, tokens=36100, window=160)
+    counts = [36001, 5000]
+    T = sum(counts)
+    k, v = (run.randn(T, kv, dh) for _ in range(2))
+    run.cache.append(k.to(DEV), v.to(DEV), run.batch(counts))
+    run.lengths = counts
+    r = 0
+    for b, n in enumerate(counts):
+        run.plain.k[b], run.plain.v[b] = list(k[r:r + n]), list(v[r:r + n])
+        r += n
+    run.step([1, 0], final=False)
+    run.step([1, 1], final=False)
+    if dh in (64, 128):
+        run.step([13, 9], final=False)
+        run.step([67, 1], final=False)
+
+
 def test_scale_and_max_keys():
     log("paged scale")
     run = Run(2, 4, 2, 128, BF16, 64, True, tokens=640)
