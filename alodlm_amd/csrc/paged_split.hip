@@ -9,7 +9,7 @@
 //
 // Measured: 64 sequences of 200 to 8000 tokens, one row of 32 heads over 8 each, 585 MB:
 // 120 us and 5 for the join (4.7 TB/s; a large copy runs at 5.08).  One sequence of 130001
-// tokens, 16 heads over 8, 266 MB: 48 and 9 us.  One of 300 tokens: 11 us, two tiles and
+// tokens, 16 heads over 8, 266 MB: 48 and 7 us.  One of 300 tokens: 11 us, two tiles and
 // an open page one after the other.  16 windows of 16 rows, 16 heads over 8, behind 300 to
 // 3100 tokens: 38 us; both of a window's column tiles in one wave made it 42 (one wave a
 // SIMD instead of three).  On the way: spilled registers cost 2.4 times (their

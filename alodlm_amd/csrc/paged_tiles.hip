@@ -12,8 +12,9 @@
 // Measured: four prompts of 700 to 4100 rows, 16 heads over 8 of 128: 178 to 208 us (the
 // clock goes with the card), 675 to 790 TFLOP/s of 1198 for a large library product;
 // matrix instructions busy 33 % of the cycles, vector instructions 48 %, LDS 27 %.  16
-// windows of 16 to 27 rows behind 300 to 3100 tokens, 32 heads over 8: 40 us and 8 for the
-// join, the time of the longest chunk.  On the way: integer divisions per tile cost 10 %,
+// windows of 16 to 27 rows behind 300 to 3100 tokens, 32 heads over 8: 39 us and 8 for the
+// join, the time of a tile's instructions one after the other (2.7 us, in a cache or not)
+// with too few workgroups to fill the gaps.  On the way: integer divisions per tile cost 10 %,
 // page numbers checked and scales computed where they are loaded 18 %, outputs rescaled
 // at every new maximum 7 %, LDS reads left behind the products before them 4 %; bank
 // conflicts (27 % of the LDS cycles, none now) cost no time.
