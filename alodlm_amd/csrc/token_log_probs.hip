@@ -463,7 +463,8 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogProbGrad a, T* __res
   const float m = a.stats[2 * row], log_s = a.stats[2 * row + 1];
   const bool empty = m == -INFINITY && log_s == -INFINITY;
   const int64_t tg = a.targets[row];
-  const float gt = a.d_log_prob && tg != a.ignore ? a.d_log_prob[row] : 0.f;
+  float gt = a.d_log_prob && tg != a.ignore ? a.d_log_prob[row] : 0.f;
+  if (gt != 0.f && (tg < 0 || tg >= a.V)) gt = NAN;  // as the log probability is
   const float gh = a.d_entropy ? a.d_entropy[row] : 0.f;
   float all = gt;
   if (a.d_top)

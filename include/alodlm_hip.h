@@ -753,7 +753,8 @@ int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_b
  * log_prob -inf, entropy 0 and zero gradient.  The workspace (floats; none for many
  * rows) is 8-byte aligned.
  * The backward writes dlogits [rows, vocab] for the upstream gradients d_log_prob,
- * d_entropy [rows] and d_top [rows, top] (each may be NULL).
+ * d_entropy [rows] and d_top [rows, top] (each may be NULL): NaN in a row whose target
+ * is outside the vocabulary and whose d_log_prob is not zero.
  * ------------------------------------------------------------------------ */
 int64_t alodlm_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top);
 int alodlm_token_log_probs(const void* logits, int64_t ld, const int64_t* targets, int64_t rows,

@@ -175,6 +175,23 @@ def test_nan_inf_and_bad_targets(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_of_bad_targets(dtype):
+    """NaN where a log probability that is NaN takes part, else the other outputs' own."""
+    log(f"token_log_probs bad targets' gradient {dtype}")
+    logits, targets = make(5, 700, dtype, seed=8)
+    targets[:] = torch.tensor([3, 700, -1, -100, 699])
+    x = logits.clone().requires_grad_()
+    out = token_log_probs(x, targets)
+    every, = torch.autograd.grad(out.log_prob.sum(), x, retain_graph=True)
+    assert every.isnan().all(1).tolist() == [False, True, True, False, False]
+    assert bool(every[[0, 3, 4]].isfinite().all()) and not bool(every[3].any())
+    known = (targets >= 0) & (targets < 700)
+    some, = torch.autograd.grad(torch.where(known, out.log_prob, 0).sum() + out.entropy.sum(), x, retain_graph=True)
+    entropy, = torch.autograd.grad(out.entropy.sum(), x)
+    assert bool(some.isfinite().all()) and torch.equal(some[[1, 2, 3]], entropy[[1, 2, 3]])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_strides(dtype):
     """A slice of a wider buffer, a row start off every alignment, a transpose."""
     log(f"token_log_probs strides {dtype}")
