@@ -479,7 +479,9 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogProbGrad a, T* __res
   // parts by the gradient's alignment; logits that lie otherwise are read one by one
   const RowParts parts = RowParts::of(out, a.V);
   const bool together = ((uintptr_t)(x + parts.head) & 15) == 0;
-  const int g0 = chunk * LP_BWD_GRANULES, g1 = min(g0 + LP_BWD_GRANULES, parts.granules);
+  // chunks are counted for the most granules a row can have: the last one may start behind
+  // this row's, and its elements are then the tail alone
+  const int g0 = min(chunk * LP_BWD_GRANULES, parts.granules), g1 = min(g0 + LP_BWD_GRANULES, parts.granules);
 #pragma unroll 2
   for (int g = g0 + threadIdx.x; g < g1; g += LP_THREADS) {
     const int at = parts.head + g * N;
