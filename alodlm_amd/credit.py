@@ -179,7 +179,8 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
     A target of ``ignore_index`` has log probability 0 and no gradient; any other
     target outside the vocabulary gives NaN, in the gradient too unless the log
     probability takes no part.  A logit of -inf is a token that cannot
-    be; in a row of nothing else log_prob is -inf, the entropy 0 and the gradient 0.
+    be; in a row of nothing else the log_prob of a target in the vocabulary is -inf, the
+    entropy 0 and, unless that is NaN as above, the gradient 0.
     A NaN in a row makes its results NaN."""
     if logits.ndim != 2 or logits.shape[1] < 1:
         raise ValueError('Logits must be [rows, vocabulary]')

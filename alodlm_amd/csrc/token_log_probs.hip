@@ -464,7 +464,9 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogProbGrad a, T* __res
   const bool empty = m == -INFINITY && log_s == -INFINITY;
   const int64_t tg = a.targets[row];
   float gt = a.d_log_prob && tg != a.ignore ? a.d_log_prob[row] : 0.f;
-  if (gt != 0.f && (tg < 0 || tg >= a.V)) gt = NAN;  // as the log probability is
+  const bool bad = gt != 0.f && (tg < 0 || tg >= a.V);
+  if (bad) gt = NAN;  // as the log probability is
+  const float none = bad ? NAN : 0.f;  // the gradient of a row in which no token can be
   const float gh = a.d_entropy ? a.d_entropy[row] : 0.f;
   float all = gt;
   if (a.d_top)
@@ -491,12 +493,12 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogProbGrad a, T* __res
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = Elem<T>::load(x, at + i);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = empty ? 0.f : gradient(v[i]);
+    for (int i = 0; i < N; ++i) v[i] = empty ? none : gradient(v[i]);
     if constexpr (N == 8) Vec8<T>::store_nt(out + at, v);
     else __builtin_nontemporal_store(nt_f32x4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<nt_f32x4_t*>(out + at));
   }
   const bool last = chunk == a.chunks - 1;
-  auto single = [&](int at) { Elem<T>::store(out, at, empty ? 0.f : gradient(Elem<T>::load(x, at))); };
+  auto single = [&](int at) { Elem<T>::store(out, at, empty ? none : gradient(Elem<T>::load(x, at))); };
   if (chunk == 0 && (int)threadIdx.x < parts.head) single(threadIdx.x);
   if (last && parts.tail + (int)threadIdx.x < a.V) single(parts.tail + threadIdx.x);
   if (empty) return;

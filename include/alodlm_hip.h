@@ -750,8 +750,8 @@ int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_b
  *                 lower index first among equal ones
  * and stats [rows, 2], the largest logit and log sum exp(x - max x), which the
  * backward takes.  A logit of -inf has probability zero; a row of nothing else has
- * log_prob -inf, entropy 0 and zero gradient.  The workspace (floats; none for many
- * rows) is 8-byte aligned.
+ * log_prob -inf (of a target in the vocabulary), entropy 0 and, but for the NaN below,
+ * zero gradient.  The workspace (floats; none for many rows) is 8-byte aligned.
  * The backward writes dlogits [rows, vocab] for the upstream gradients d_log_prob,
  * d_entropy [rows] and d_top [rows, top] (each may be NULL): NaN in a row whose target
  * is outside the vocabulary and whose d_log_prob is not zero.

@@ -40,3 +40,20 @@ def test_gradient_beside_borders(dtype, V, own):
             x[:, c] = 9.0
             targets[:] = 1
         check(x, targets, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_of_no_token_and_bad_targets(dtype):
+    """Rows of -inf: the gradient is NaN where the log probability is (a target outside
+    the vocabulary that takes part), else zero."""
+    log(f"token_log_probs rows of no token {dtype}")
+    targets = torch.tensor([3, 700, -1, -100, 699], device=DEV)
+    bad = [False, True, True, False, False]
+    x = torch.full((5, 700), -math.inf, dtype=dtype, device=DEV).requires_grad_()
+    out = token_log_probs(x, targets, top=2)
+    assert out.log_prob.isnan().tolist() == bad
+    every, = torch.autograd.grad(out.log_prob.sum() + out.entropy.sum(), x, retain_graph=True)
+    assert every.isnan().all(1).tolist() == bad and not bool(every[[0, 3, 4]].any())
+    known = (targets >= 0) & (targets < 700)
+    some, = torch.autograd.grad(torch.where(known, out.log_prob, 0).sum() + out.entropy.sum(), x)
+    assert not bool(some.any())
