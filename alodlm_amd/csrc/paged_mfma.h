@@ -248,8 +248,10 @@ template <int DH, int CT> struct Columns {
       }
     }
   }
-  // value(d, j): dimension d * 16 + lane % 16, keys (lane / 16) * 16 + 8 j .. + 8.
-  template <typename Value>
+  // value(d, j): dimension d * 16 + lane % 16, keys (lane / 16) * 16 + 8 j .. + 8.  PLAIN:
+  // 16-bit values, which can be inf: a low part, which has either sign or is zero, would
+  // make NaN of it, so the low parts are multiplied with zeros in the place of inf and NaN.
+  template <bool PLAIN, typename Value>
   __device__ __forceinline__ void add_values(const bf16x8 (&p)[CT][2], const bf16x8 (&low)[CT][2], Value value) {
     bf16x8 ones;
 #pragma unroll
@@ -261,8 +263,15 @@ template <int DH, int CT> struct Columns {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const bf16x8 v = value(d, j);
+        bf16x8 v_low = v;
+        if constexpr (PLAIN) {
+          uint4 w = __builtin_bit_cast(uint4, v);
+          w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
+                         without_special<false>(w.w));
+          v_low = __builtin_bit_cast(bf16x8, w);
+        }
 #pragma unroll
-        for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v, low[t][j], mfma16(v, p[t][j], o[t][d]));
+        for (int t = 0; t < CT; ++t) o[t][d] = mfma16(v_low, low[t][j], mfma16(v, p[t][j], o[t][d]));
       }
     }
   }

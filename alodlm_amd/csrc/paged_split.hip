@@ -102,7 +102,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
   auto add_values = [&](const CodeTile<DH>& t, const bf16x8 (&p)[CT][2], const bf16x8 (&low)[CT][2]) {
     const float scale = exp2_int(t.v_exponent);
-    cols.add_values(p, low, [&](int d, int j) {
+    cols.template add_values<false>(p, low, [&](int d, int j) {
       const uint4 w = t.v[d];
       return j ? widen(w.z, w.w, scale) : widen(w.x, w.y, scale);
     });
@@ -169,8 +169,8 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   };
   // Tiles [from, to) of keys [lo, to) in 16 bits, loaded as the products take them
   // (keys and values of a tile at once do not fit the registers of two waves a SIMD).
-  auto plain_tiles = [&](int from, int to, int lo, bool whole, auto pool) {
-    constexpr bool POOL = decltype(pool)::value;
+  auto plain_tiles = [&](int from, int to, int lo, auto whole, auto pool) {
+    constexpr bool WHOLE = decltype(whole)::value, POOL = decltype(pool)::value;
     const bf16_t* keys = (const bf16_t*)(POOL ? c.keys : c.open_keys);
     const bf16_t* values = (const bf16_t*)(POOL ? c.values : c.open_values);
     for (int base = first_tile(from); base < to; base += STEP) {
@@ -183,12 +183,12 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       cols.scores(s, [&](int i, int f) {
         return *reinterpret_cast<const bf16x8*>(kp + 4 * i * DH + (f / 2) * 64 + (f % 2) * 8);
       });
-      if (!whole || !__all(v_page >= 0)) cols.hide(s, base, lo, to, v_page >= 0);
+      if (!WHOLE || !__all(v_page >= 0)) cols.hide(s, base, lo, to, v_page >= 0);
       cols.template softmax<true>(s, p, low, a.scale2);
-      cols.add_values(p, low, [&](int d, int j) {
+      cols.template add_values<WHOLE>(p, low, [&](int d, int j) {
         uint4 w = *reinterpret_cast<const uint4*>(vp + d * 16 * page + j * 8);
         if (v_page < 0) w = make_uint4(0, 0, 0, 0);
-        if (!whole) {
+        if (!WHOLE) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) |
                  special_bits<false>(w.w);
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y),
@@ -204,10 +204,10 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     whole_code_tiles(whole);
     edge_code_tiles(whole, hi);
     const int lo = max(k0, sp.sealed);
-    if (lo < k1) plain_tiles(lo / PAGED_TILE * PAGED_TILE, k1, lo, false, std::false_type());
+    if (lo < k1) plain_tiles(lo / PAGED_TILE * PAGED_TILE, k1, lo, std::false_type(), std::false_type());
   } else {
-    plain_tiles(k0, whole, k0, true, std::true_type());
-    plain_tiles(whole, hi, k0, false, std::true_type());
+    plain_tiles(k0, whole, k0, std::true_type(), std::true_type());
+    plain_tiles(whole, hi, k0, std::false_type(), std::true_type());
   }
 
   float sum[CT];

@@ -43,8 +43,9 @@ template <int DH, int CT, bool EIGHT>
 __global__ void __launch_bounds__(64 * PAGED_WAVES, 2)
 paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
   constexpr int DT = DH / 16, COLS = 16 * CT * PAGED_WAVES;
+  constexpr bool LOW = CT == 1;
   __shared__ __attribute__((aligned(16))) TileBuffer<DH> tiles[2];
-  __shared__ int there[2][4], special_of[PAGED_WAVES];
+  __shared__ int there[2][4], special_of[PAGED_WAVES], low_special[2][PAGED_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   if (blockIdx.x >= gridDim.x - a.zero_blocks) {
@@ -161,6 +162,7 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     const bool pool = i < pool_tiles, edge = !pool || base_of(i) + PAGED_TILE > min(hi, least);
     const int64_t kp = key_at(i, max(ahead.k, 0)), vp = value_at(i, max(ahead.v, 0));
     const bf16_t* values = (const bf16_t*)(EIGHT ? c.open_values : c.values);
+    uint32_t seen = 0;  // inf or NaN that stays
     uint4 wv[VR][2];
 #pragma unroll
     for (int r = 0; r < VR; ++r)
@@ -183,10 +185,16 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
           odd |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
           w = make_uint4(without_special<false>(w.x), without_special<false>(w.y), without_special<false>(w.z),
                          without_special<false>(w.w));
+        } else if (LOW) {
+          seen |= special_bits<false>(w.x) | special_bits<false>(w.y) | special_bits<false>(w.z) | special_bits<false>(w.w);
         }
         *reinterpret_cast<uint4*>(t.v + value_piece<DH>(t_dim + 64 * r, t_part, j)) = w;
       }
     if (tid < 4) there[i & 1][tid] = ahead.v >= 0;
+    if (LOW && !EIGHT) {
+      const bool any = __any(seen);
+      if (lane == 0) low_special[i & 1][wave] = any;
+    }
   };
   auto stage = [&](int i) {
     if (EIGHT && i < pool_tiles) stage_codes(i);
@@ -208,7 +216,6 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     if (base < my_most) {
       const TileBuffer<DH>& t = tiles[i & 1];
       f32x4 s[CT][4];
-      constexpr bool LOW = CT == 1;
       bf16x8 p[CT][2], low[CT][2];
       cols.scores_ahead(s, [&](int sub, int f) {
         const int key = (col >> 2) * 16 + 4 * sub + (col & 3);
@@ -217,9 +224,16 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       const bool mine = there[i & 1][grp];
       if (base < lo || base + PAGED_TILE > min(end, my_least) || !__all(mine)) cols.hide(s, base, lo, end, mine);
       cols.template softmax<LOW>(s, p, low, a.scale2);
-      cols.template add_values_ahead<LOW>(p, low, [&](int d, int j) {
+      auto value = [&](int d, int j) {
         return *reinterpret_cast<const bf16x8*>(t.v + value_piece<DH>(d * 16 + col, grp, j));
-      });
+      };
+      bool special = false;
+      if constexpr (LOW && !EIGHT) {
+        const int* w = low_special[i & 1];
+        special = w[0] | w[1] | w[2] | w[3];
+        if (special) cols.template add_values<true>(p, low, value);
+      }
+      if (!special) cols.template add_values_ahead<LOW>(p, low, value);
     }
     if (more) stage(i + 1);
     __syncthreads();
