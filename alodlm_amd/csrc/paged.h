@@ -71,16 +71,33 @@ struct AttendArgs {
   float2* stat;  // (maximum in base 2, sum) [chunks][rows * heads]
   int heads, group, chunk_keys, chunks, query_tiles, join_ways;
   float scale2;  // softmax scale * log2 e
-  int zero_blocks;  // workgroups behind the launch's others that clear the rows behind the last sequence
+  int zero_blocks;  // workgroups behind the launch's others that clear the rows without a result
 };
 
-// Zeros in the rows behind the last sequence, by `blocks` workgroups of 256 threads.
+// Zeros in the rows that no sequence has a result in, by `blocks` workgroups of 256
+// threads: before the first sequence, behind the last, and past max_rows.
 template <typename T>
 __device__ __forceinline__ void zero_rest(const PagedBatch& bt, T* out, int64_t width, int block, int blocks) {
-  const int64_t from = (int64_t)min(max(bt.offsets[bt.sequences], 0), bt.rows) * width;
-  const int64_t to = (int64_t)bt.rows * width;
-  for (int64_t i = from + (int64_t)block * 256 + threadIdx.x; i < to; i += (int64_t)blocks * 256)
-    Elem<T>::store(out, i, 0.f);
+  auto clear = [&](int64_t from, int64_t to, int thread, int threads) {
+    for (int64_t i = from * width + thread; i < to * width; i += threads) Elem<T>::store(out, i, 0.f);
+  };
+  const int thread = block * 256 + threadIdx.x, lane = threadIdx.x & 63;
+  clear(0, bt.first_row(0), thread, blocks * 256);
+  clear(bt.first_row(bt.sequences), bt.rows, thread, blocks * 256);
+  if (bt.max_rows == bt.rows) return;
+  // a sequence a lane; those with rows past max_rows one after the other by the wave
+  for (int b0 = thread - lane; b0 < bt.sequences; b0 += blocks * 256) {
+    const int b = b0 + lane;
+    int from = 0, to = 0;
+    if (b < bt.sequences) {
+      from = bt.first_row(b) + bt.max_rows;
+      to = min(bt.offsets[b + 1], bt.rows);
+    }
+    for (uint64_t left = __ballot(from < to); left; left &= left - 1) {
+      const int which = __builtin_ctzll(left);
+      clear(__shfl(from, which, 64), __shfl(to, which, 64), lane, 64);
+    }
+  }
 }
 
 // Where the 8-bit pages of a sequence end (keys before it are sealed).

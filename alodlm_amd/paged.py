@@ -212,11 +212,11 @@ class PagedBatch:
     int32 [sequences + 1]: sequence b has the rows [offsets[b], offsets[b + 1]).
     ``slots`` int32 [sequences]: the slot of its open pages (8 bits; default: b).
     ``rows`` (default: offsets[-1], read from the device) is the number of rows that
-    the step's tensors have; rows behind the last sequence are padding.  ``max_rows``
-    bounds a sequence's rows (default: ``rows``) and ``max_keys`` its tokens with
-    them (default: what the table holds): they size the launches.  A sequence's rows
-    past max_rows are left out (their results are not written), and its tokens past
-    max_keys are not attended to.  ``final``: the rows are kept, else they are a window
+    the step's tensors have; rows before the first sequence and behind the last one are
+    padding.  ``max_rows`` bounds a sequence's rows (default: ``rows``) and ``max_keys``
+    its tokens with them (default: what the table holds): they size the launches.  A
+    sequence's rows past max_rows are padding too, and its tokens past max_keys are not
+    attended to.  ``final``: the rows are kept, else they are a window
     that ``retire`` shortens."""
 
     def __init__(self, table, lengths, offsets, rows=None, max_rows=None, max_keys=None, slots=None,
@@ -287,8 +287,8 @@ def paged_attention(q, cache, batch, scale=None, out=None):
     [rows, heads, head_dim] (grouped-query heads), result [rows, heads, head_dim].
     Row i of sequence b sees the first lengths[b] + i + 1 tokens; ``append`` has
     written the batch's own.  ``scale`` is head_dim^-0.5 unless given.  A row that
-    sees no token is zero.  Rows behind the last sequence are zero, or left as they
-    were in a caller's ``out``.  No gradient: this is the decoder's side."""
+    sees no token is zero.  Rows that are padding are zero, or left as they were in a
+    caller's ``out``.  No gradient: this is the decoder's side."""
     cache._check(batch)
     q, ldq = cache._rows(q, None, batch, "q")
     heads = q.shape[1]

@@ -730,9 +730,10 @@ int alodlm_paged_retire(const alodlm_paged_cache* cache, const alodlm_paged_batc
  * sequence's tokens up to its own position (row i of sequence b: the first
  * lengths[b] + i + 1; the batch's tokens are in the cache).  Grouped-query heads:
  * query head h reads key/value head h / (heads / kv_heads).  A row that sees no
- * key is zero.  Rows behind the last sequence are left as they were, or set to
- * zero with zero_rest.  The workspace query (floats) depends on the shapes and
- * bounds of the two structs, not on device data. */
+ * key is zero.  Rows that no sequence has a result in (before the first, behind the
+ * last, past max_rows) are left as they were, or set to zero with zero_rest.  The
+ * workspace query (floats) depends on the shapes and bounds of the two structs, not on
+ * device data. */
 int64_t alodlm_paged_attention_workspace(const alodlm_paged_cache* cache,
                                          const alodlm_paged_batch* batch, int64_t heads);
 int alodlm_paged_attention(const alodlm_paged_cache* cache, const alodlm_paged_batch* batch,

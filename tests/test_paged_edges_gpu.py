@@ -62,3 +62,43 @@ def test_infinite_values(shape, rows, tokens):
         assert torch.equal(got[mine].where(ref.isinf(), 0.0), ref.where(ref.isinf(), 0.0))
         tol = attention_tolerance(ref, mag, size, max(limits), dtype, dh)
         assert bool(((got[mine] - ref).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("shape,tokens,limit", [
+    ((4, 2, 128, BF16, 64, True), 300, 1), ((4, 2, 128, BF16, 64, True), 300, 20), ((4, 2, 64, BF16, 16, False), 90, 70),
+    ((4, 2, 128, F32, 64, False), 300, 5), ((4, 2, 128, F32, 64, True), 40, 40), ((2, 1, 24, BF16, 64, True), 300, 3),
+    ((4, 2, 128, BF16, 64, True), 6000, 1), ((4, 2, 128, F32, 64, False), 6000, 2)])
+def test_rows_that_no_sequence_is_given(shape, tokens, limit):
+    """Rows before the first sequence, past max_rows and behind the last one: zero in a
+    fresh result, left alone in a caller's."""
+    log(f"paged rows of nobody {shape} {tokens} {limit}")
+    heads, kv, dh, dtype = shape[:4]
+    run = Run(4, *shape, tokens=tokens + 100)
+    held = [tokens, 1, 0, tokens]
+    T = sum(held)
+    k, v = (run.randn(T, kv, dh).to(DEV) for _ in range(2))
+    run.cache.append(k, v, run.batch(held))
+    counts = [limit + 7, limit, 0, limit + 300]
+    offsets = [3]
+    for n in counts:
+        offsets.append(offsets[-1] + n)
+    rows = offsets[-1] + 5
+    q, k, v = (run.randn(rows, n, dh).to(DEV) for n in (heads, kv, kv))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    batch = PagedBatch(run.table, ints(held), ints(offsets), rows=rows, max_rows=limit, slots=run.slots)
+    run.cache.append(k, v, batch)
+    mine = torch.zeros(rows, dtype=torch.bool)
+    for at, n in zip(offsets, counts):
+        mine[at:at + min(n, limit)] = True
+    out = torch.full(q.shape, 7.0, dtype=dtype, device=DEV)
+    paged_attention(q, run.cache, batch, out=out)
+    assert bool((out[~mine] == 7.0).all()) and bool((out[mine] != 7.0).any(-1).any(-1).all())
+    for _ in range(3):
+        # a fresh result tends to lie where the last tensor of its size was
+        used = torch.full(q.shape, math.nan, dtype=dtype, device=DEV)
+        del used
+        fresh = paged_attention(q, run.cache, batch)
+        assert not bool(fresh[~mine].any()) and torch.equal(fresh[mine], out[mine])
+        fresh = paged_attention(q, run.cache, PagedBatch(run.table, ints(held), ints([rows] * 5), rows=rows,
+                                                         max_rows=limit, slots=run.slots))
+        assert not bool(fresh.any())
