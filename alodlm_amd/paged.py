@@ -62,7 +62,29 @@ def _need(condition, message):
         raise ValueError(message)
 
 
-class PagedCache:
+class _Fixed:
+    """An object whose fields stay what ``__init__`` made of its arguments: the kernels
+    are given a struct of them, which would not follow."""
+    _fixed = frozenset()
+
+    def _fix(self):
+        object.__setattr__(self, "_fixed", frozenset(vars(self)))
+
+    def _free(self, name):
+        if name in self._fixed:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: change a tensor in place, "
+                                 f"or make another {type(self).__name__}")
+
+    def __setattr__(self, name, value):
+        self._free(name)
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        self._free(name)
+        object.__delattr__(self, name)
+
+
+class PagedCache(_Fixed):
     """One layer's pages.
 
     ``keys`` [pages, kv_heads, page_size, head_dim] and ``values`` [pages, kv_heads,
@@ -70,7 +92,7 @@ class PagedCache:
     int8 [pages, 2, kv_heads] and the open pages ``open_keys`` [slots, open_pages,
     kv_heads, page_size, head_dim] and ``open_values`` (the last two dimensions
     exchanged) in float32 or bfloat16, the type of the rows that are appended.
-    ``allocate`` makes them."""
+    ``allocate`` makes them.  The fields are fixed; the tensors' contents are not."""
 
     def __init__(self, keys, values, exponents=None, open_keys=None, open_values=None):
         _need(keys.ndim == 4 and values.ndim == 4, "keys and values must have four dimensions")
@@ -114,6 +136,7 @@ class PagedCache:
                                     ptr(open_values), pages, page, heads, dh, slots, opened, code,
                                     int(self.eight_bit))
         self._ref = ctypes.byref(self._struct)
+        self._fix()
 
     @classmethod
     def allocate(cls, pages, kv_heads, head_dim, dtype, device, page_size=64, eight_bit=True,
@@ -204,7 +227,7 @@ class PagedCache:
         call_on(self.device, "alodlm_paged_retire", self._ref, batch.ref(self), ptr(counts))
 
 
-class PagedBatch:
+class PagedBatch(_Fixed):
     """One step's rows.
 
     ``table`` int32 [sequences, width]: the pages of each sequence in order;
@@ -217,7 +240,8 @@ class PagedBatch:
     its tokens with them (default: what the table holds): they size the launches.  A
     sequence's rows past max_rows are padding too, and its tokens past max_keys are not
     attended to.  ``final``: the rows are kept, else they are a window
-    that ``retire`` shortens."""
+    that ``retire`` shortens.  The fields are fixed: a step with other tensors or bounds is
+    another batch; the tensors' contents may change."""
 
     def __init__(self, table, lengths, offsets, rows=None, max_rows=None, max_keys=None, slots=None,
                  final=True):
@@ -234,6 +258,7 @@ class PagedBatch:
         _need(self.rows >= 0 and self.max_rows >= 0 and (max_keys is None or max_keys >= 0),
               "rows, max_rows and max_keys must not be negative")
         self._refs = {}
+        self._fix()
 
     def _ints(self, t, shape, what):
         if (t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device

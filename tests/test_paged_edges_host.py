@@ -1,0 +1,38 @@
+"""What a paged cache and its batch refuse besides shapes and types, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tests.test_paged_host import batch, cache, ints
+
+
+def test_fields_are_fixed():
+    """The kernels take what a cache and a batch were made of: another tensor, bound or
+    flag needs another object; tensors may change in place."""
+    c, b = cache(slots=2), batch()
+    made = ctypes.string_at(b.ref(c), ctypes.sizeof(b._refs[c.page_size][1]))
+    for name, value in (("table", b.table.clone()), ("lengths", ints(7, 7)), ("offsets", ints(0, 0, 0)),
+                        ("slots", ints(1, 0)), ("rows", 2), ("max_rows", 1), ("max_keys", 3), ("final", False),
+                        ("sequences", 1), ("width", 1)):
+        before = getattr(b, name)
+        with pytest.raises(AttributeError, match=name):
+            setattr(b, name, value)
+        with pytest.raises(AttributeError, match=name):
+            delattr(b, name)
+        assert getattr(b, name) is before
+    for name in ("keys", "values", "exponents", "open_keys", "open_values"):
+        before = getattr(c, name)
+        with pytest.raises(AttributeError, match=name):
+            setattr(c, name, before.clone())
+        assert getattr(c, name) is before
+    for name, value in (("page_size", 32), ("kv_heads", 1), ("head_dim", 8), ("eight_bit", False),
+                        ("dtype", torch.float32), ("device", torch.device("cpu"))):
+        with pytest.raises(AttributeError, match=name):
+            setattr(c, name, value)
+    b.lengths.copy_(ints(9, 9))
+    assert ctypes.string_at(b.ref(c), len(made)) == made
+    c.layer = 3  # a program's own names are free
+    c.layer = b.step = 4
+    assert c.layer == b.step == 4
