@@ -298,7 +298,8 @@ int paged_check(const alodlm_paged_cache* c, const alodlm_paged_batch* b) {
   ALODLM_CHECK_ARG(b->sequences >= 0 && b->sequences < (1ll << 24) && b->rows >= 0 &&
                        b->rows < (1ll << 30) && b->max_rows >= 0 && b->max_rows <= b->rows,
                    "paged: sequences, rows or max_rows out of range");
-  ALODLM_CHECK_ARG(b->width >= 1 && b->width * ps < (1ll << 31) - ps,
+  // keys are counted in 32 bits, by the attention up to 8192 chunks' rounding to 64 past them
+  ALODLM_CHECK_ARG(b->width >= 1 && b->width < (1ll << 31) && b->width * ps < (1ll << 31) - (1ll << 20),
                    "paged: the table's width is out of range");
   ALODLM_CHECK_ARG(b->max_keys >= 0 && b->max_keys <= b->width * ps,
                    "paged: max_keys exceeds the table's pages");

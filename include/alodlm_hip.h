@@ -688,6 +688,7 @@ int alodlm_check_finite(const void* x, int64_t n, int dtype, int32_t* flag, void
  * rows [offsets[b], offsets[b + 1]) (at most max_rows), whose positions follow
  * them; with `final` the rows are kept, else only alodlm_paged_retire keeps the
  * first of them (a decoding window).  max_keys bounds lengths[b] plus its rows.
+ * A table has room for fewer than 2^31 - 2^20 tokens a sequence.
  * Arrays are on the device: entries out of range (a page outside the pool, a
  * slot outside the slots, a length below zero or past the table) are never
  * followed - such tokens are not written and not attended to.

@@ -5,7 +5,8 @@ import ctypes
 import pytest
 import torch
 
-from tests.test_paged_host import batch, cache, ints
+from alodlm_amd import _lib
+from tests.test_paged_host import batch, cache, ints, library, structs
 
 
 def test_fields_are_fixed():
@@ -36,3 +37,20 @@ def test_fields_are_fixed():
     c.layer = 3  # a program's own names are free
     c.layer = b.step = 4
     assert c.layer == b.step == 4
+
+
+@pytest.mark.parametrize("page,head_dim", [(16, 64), (128, 64), (64, 24)])
+def test_key_counts_next_to_2_to_the_31(page, head_dim):
+    """The kernels count keys in 32 bits, a chunk and a few tiles past the last: tables of
+    2^31 - 2^20 keys or more are refused."""
+    library()
+    c, b = cache(pages=2, page_size=page, head_dim=head_dim, slots=2), batch()
+    for width, fine in (((2 ** 31 - 2 ** 20) // page - 1, True), ((2 ** 31 - 2 ** 20) // page, False),
+                        (2 ** 31 // page - 2, False)):
+        cs, bs = structs(c, b, width=width, max_keys=width * page)
+        # nothing is launched: the rows are missing
+        with pytest.raises(ValueError, match="no rows" if fine else "width"):
+            _lib.call("alodlm_paged_attention", cs, bs, None, 2 * head_dim, None, 2, 0.25, 0, None, None)
+        with pytest.raises(ValueError, match="no rows" if fine else "width"):
+            _lib.call("alodlm_paged_append", cs, bs, None, 2 * head_dim, None, 2 * head_dim, None, 0, None, 0,
+                      None, None, None)
