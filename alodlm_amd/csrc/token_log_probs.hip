@@ -529,7 +529,8 @@ static int check_shape(int64_t rows, int64_t vocab, int64_t top, int64_t ld, flo
                    "token_log_probs: vocabulary or row stride out of range");
   ALODLM_CHECK_ARG(top >= 0 && top <= LP_MAX_TOP && top <= vocab,
                    "token_log_probs: top must be 0 to 64 and at most the vocabulary");
-  ALODLM_CHECK_ARG(inv_t > 0.f && inv_t < INFINITY, "token_log_probs: the temperature must be positive");
+  ALODLM_CHECK_ARG(inv_t > 0.f && inv_t * LP_LOG2E < INFINITY,
+                   "token_log_probs: the temperature must be positive, its inverse times log2 e finite");
   return ALODLM_OK;
 }
 

@@ -54,3 +54,18 @@ def test_key_counts_next_to_2_to_the_31(page, head_dim):
         with pytest.raises(ValueError, match="no rows" if fine else "width"):
             _lib.call("alodlm_paged_append", cs, bs, None, 2 * head_dim, None, 2 * head_dim, None, 0, None, 0,
                       None, None, None)
+
+
+def test_temperatures_whose_base_2_form_is_infinite():
+    """The exponentials are in base 2: a temperature whose inverse log2 e takes past float32
+    is refused.  The calls lack arrays: nothing is launched."""
+    library()
+    for inverse, match in ((3.4028234e38 * 0.6931471, "alternatives"), (2.4e38, "temperature"),
+                           (3.4e38, "temperature")):
+        with pytest.raises(ValueError, match=match):
+            _lib.call("alodlm_token_log_probs", None, 5, None, 1, 5, 2, inverse, -100, None, None, None, None, None,
+                      None, 1, None)
+        upstream = 16  # of the alternatives, whose ids are missing
+        with pytest.raises(ValueError, match=match):
+            _lib.call("alodlm_token_log_probs_bwd", None, 5, None, None, None, None, None, None, upstream, 1, 5, 2,
+                      inverse, -100, None, 1, None)
