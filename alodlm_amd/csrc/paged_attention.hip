@@ -386,7 +386,8 @@ extern "C" int alodlm_paged_attention(const alodlm_paged_cache* cache, const alo
   ALODLM_CHECK_ARG(heads >= 1 && heads <= 65536 && heads % cache->kv_heads == 0,
                    "paged_attention: heads must be a multiple of the cache's kv_heads");
   ALODLM_CHECK_ARG(ldq >= heads * cache->head_dim, "paged_attention: row stride below the row width");
-  ALODLM_CHECK_ARG(scale > 0.f && scale < INFINITY, "paged_attention: scale must be positive");
+  ALODLM_CHECK_ARG(scale > 0.f && scale * LOG2E < INFINITY,
+                   "paged_attention: scale must be positive, and finite times log2 e");
   ALODLM_CHECK_ARG((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
                        ldq * es % 16 == 0,
                    "paged_attention: rows must be 16-byte aligned");

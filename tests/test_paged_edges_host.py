@@ -69,3 +69,12 @@ def test_temperatures_whose_base_2_form_is_infinite():
         with pytest.raises(ValueError, match=match):
             _lib.call("alodlm_token_log_probs_bwd", None, 5, None, None, None, None, None, None, upstream, 1, 5, 2,
                       inverse, -100, None, 1, None)
+
+
+def test_scales_whose_base_2_form_is_infinite():
+    """The same for the attention's scale."""
+    library()
+    c, b = structs(cache(slots=2), batch())
+    for scale, match in ((3.4028234e38 * 0.6931471, "no rows"), (2.4e38, "scale")):
+        with pytest.raises(ValueError, match=match):
+            _lib.call("alodlm_paged_attention", c, b, None, 32, None, 2, scale, 0, None, None)
