@@ -559,6 +559,7 @@ extern "C" int alodlm_token_log_probs(const void* logits, int64_t ld, const int6
   if (rc) return rc;
   if (rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(top == 0 || (top_log_prob && top_ids), "token_log_probs: no room for the alternatives");
+  ALODLM_CHECK_ARG(logits && targets && log_prob && entropy && stats, "token_log_probs: the call lacks an array");
   const int64_t chunks = row_chunks(rows, vocab);
   ALODLM_CHECK_ARG(chunks == 1 || workspace, "token_log_probs: no workspace");
   ALODLM_CHECK_ARG(chunks == 1 || (uintptr_t)workspace % 8 == 0, "token_log_probs: workspace not 8-byte aligned");
@@ -591,6 +592,7 @@ extern "C" int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const 
   if (rc) return rc;
   if (rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(!d_top || top == 0 || top_ids, "token_log_probs_bwd: no alternatives");
+  ALODLM_CHECK_ARG(logits && targets && stats && entropy && dlogits, "token_log_probs_bwd: the call lacks an array");
   ALODLM_DISPATCH(dtype, T, {
     const int64_t granules = (vocab * (int64_t)sizeof(T) + 15) / 16;
     const int64_t chunks = (granules + LP_BWD_GRANULES - 1) / LP_BWD_GRANULES;

@@ -78,3 +78,17 @@ def test_scales_whose_base_2_form_is_infinite():
     for scale, match in ((3.4028234e38 * 0.6931471, "no rows"), (2.4e38, "scale")):
         with pytest.raises(ValueError, match=match):
             _lib.call("alodlm_paged_attention", c, b, None, 32, None, 2, scale, 0, None, None)
+
+
+@pytest.mark.parametrize("missing", ["logits", "targets", "log_prob", "entropy", "stats"])
+def test_log_probabilities_need_their_arrays(missing):
+    """The library's own checks: a missing array is refused before anything is launched."""
+    library()
+    at = {name: None if name == missing else 16 for name in ("logits", "targets", "log_prob", "entropy", "stats")}
+    with pytest.raises(ValueError, match="lacks"):
+        _lib.call("alodlm_token_log_probs", at["logits"], 5, at["targets"], 1, 5, 0, 1.0, -100, at["log_prob"],
+                  at["entropy"], at["stats"], None, None, None, 1, None)
+    at["dlogits"] = at.pop("log_prob")
+    with pytest.raises(ValueError, match="lacks"):
+        _lib.call("alodlm_token_log_probs_bwd", at["logits"], 5, at["targets"], None, at["stats"], at["entropy"], None,
+                  None, None, 1, 5, 0, 1.0, -100, at["dlogits"], 1, None)
