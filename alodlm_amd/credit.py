@@ -181,7 +181,10 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
     probability takes no part.  A logit of -inf is a token that cannot
     be; in a row of nothing else the log_prob of a target in the vocabulary is -inf, the
     entropy 0 and, unless that is NaN as above, the gradient 0.
-    A NaN in a row makes its results NaN."""
+    A NaN in a row makes its results NaN.
+
+    A backward that is captured into a graph must not find an eager autograd graph of the
+    same logits alive (its nodes are tied to the eager stream): drop its outputs first."""
     if logits.ndim != 2 or logits.shape[1] < 1:
         raise ValueError('Logits must be [rows, vocabulary]')
     _lib.dtype_code(logits.dtype)

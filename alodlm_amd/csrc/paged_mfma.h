@@ -15,7 +15,9 @@
 // sum is that of the rounded ones (one more product with ones), so that the weights add
 // up to one.  Decoding steps and small windows, which wait for memory, multiply
 // the rounding errors as well: the probabilities then have 16 bits, and only the
-// output's rounding is left.
+// output's rounding is left.  64 rows over 585 MB of codes take 118 us so; the values of
+// 16-bit pages, which can be inf, are cleared of it for the low parts' products (see
+// add_values), which costs a windows' kernel of one column tile 5 % (48 -> 50 us).
 #pragma once
 
 #include "paged.h"

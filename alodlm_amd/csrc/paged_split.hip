@@ -9,8 +9,9 @@
 //
 // Measured: 64 sequences of 200 to 8000 tokens, one row of 32 heads over 8 each, 585 MB:
 // 120 us and 5 for the join (4.7 TB/s; a large copy runs at 5.08).  One sequence of 130001
-// tokens, 16 heads over 8, 266 MB: 48 and 7 us.  One of 300 tokens: 11 us, two tiles and
-// an open page one after the other.  16 windows of 16 rows, 16 heads over 8, behind 300 to
+// tokens, 16 heads over 8, 266 MB: 48 and 7 us.  One of 300 tokens: 11 us, a tile of codes
+// a wave and behind one of them the open page.  Pages in bf16: the 64 sequences 235 us for
+// 1.07 GB (4.5 TB/s), the long one 109.  16 windows of 16 rows, 16 heads over 8, behind 300 to
 // 3100 tokens: 38 us; both of a window's column tiles in one wave made it 42 (one wave a
 // SIMD instead of three).  On the way: spilled registers cost 2.4 times (their
 // reloads wait for the tile on its way), chunk numbers that pick the die 1.4 (eight
@@ -168,7 +169,7 @@ paged_split_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
     }
   };
   // Tiles [from, to) of keys [lo, to) in 16 bits, loaded as the products take them
-  // (keys and values of a tile at once do not fit the registers of two waves a SIMD).
+  // (keys and values of a tile at once do not fit the registers of three waves a SIMD).
   auto plain_tiles = [&](int from, int to, int lo, auto whole, auto pool) {
     constexpr bool WHOLE = decltype(whole)::value, POOL = decltype(pool)::value;
     const bf16_t* keys = (const bf16_t*)(POOL ? c.keys : c.open_keys);

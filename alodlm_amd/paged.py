@@ -237,11 +237,11 @@ class PagedBatch(_Fixed):
     ``rows`` (default: offsets[-1], read from the device) is the number of rows that
     the step's tensors have; rows before the first sequence and behind the last one are
     padding.  ``max_rows`` bounds a sequence's rows (default: ``rows``) and ``max_keys``
-    its tokens with them (default: what the table holds): they size the launches.  A
-    sequence's rows past max_rows are padding too, and its tokens past max_keys are not
-    attended to.  ``final``: the rows are kept, else they are a window
-    that ``retire`` shortens.  The fields are fixed: a step with other tensors or bounds is
-    another batch; the tensors' contents may change."""
+    its tokens with them (default: what the table holds): they size the launches, so a
+    table much wider than its tokens wants ``max_keys``.  A sequence's rows past max_rows
+    are padding too, and its tokens past max_keys are not attended to.  ``final``: the rows
+    are kept, else they are a window that ``retire`` shortens.  The fields are fixed: a
+    step with other tensors or bounds is another batch; the tensors' contents may change."""
 
     def __init__(self, table, lengths, offsets, rows=None, max_rows=None, max_keys=None, slots=None,
                  final=True):
@@ -313,7 +313,9 @@ def paged_attention(q, cache, batch, scale=None, out=None):
     Row i of sequence b sees the first lengths[b] + i + 1 tokens; ``append`` has
     written the batch's own.  ``scale`` is head_dim^-0.5 unless given.  A row that
     sees no token is zero.  Rows that are padding are zero, or left as they were in a
-    caller's ``out``.  No gradient: this is the decoder's side."""
+    caller's ``out``.  Weights are summed relative to 2^-8 of the row's largest or more: a
+    result is finite while the tokens times the largest value stay below 2^119.  No
+    gradient: this is the decoder's side."""
     cache._check(batch)
     q, ldq = cache._rows(q, None, batch, "q")
     heads = q.shape[1]
