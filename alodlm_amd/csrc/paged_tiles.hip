@@ -230,7 +230,8 @@ paged_tiles_kernel(PagedCache c, PagedBatch bt, AttendArgs a) {
       bool special = false;
       if constexpr (LOW && !EIGHT) {
         const int* w = low_special[i & 1];
-        special = w[0] | w[1] | w[2] | w[3];
+        // a scalar: matrix instructions run whatever lanes a branch leaves on
+        special = __builtin_amdgcn_readfirstlane(w[0] | w[1] | w[2] | w[3]);
         if (special) cols.template add_values<true>(p, low, value);
       }
       if (!special) cols.template add_values_ahead<LOW>(p, low, value);
