@@ -1,0 +1,99 @@
+// Losses over a large vocabulary against a few known tokens a row.
+//
+// A row knows tokens id_k with probabilities q_k: one of probability 1 (cross entropy) or
+// a teacher's most likely ones.  With z the row's logits over T, p = softmax(z),
+//   loss = sum_k q_k (ln q_k - ln p[id_k])  [+ q_r (ln q_r - ln p_r)],
+// q_r = max(0, 1 - sum_k q_k) and p_r the probability of all tokens that are not known.
+// The known tokens are kept out of the sum over the vocabulary and joined to it at the
+// end, so p_r is a sum of its own and never a difference from 1.  With Q = sum_k q_k [+ q_r]
+// and s_r the softmax over the other tokens,
+//   dloss / dz = Q p - [q at the known] - [q_r s_r elsewhere]
+//              = (Q p_r - q_r) s_r   at a token that is not known: one factor a row,
+//                Q p - q             at a known one: one value a row and known token.
+// Sums are in base 2, relative to the largest logit: 2^((z - m) c) of raw logits z, c =
+// log2 e / T.
+#pragma once
+
+#include "common.h"
+
+#define VL_MAX_KNOWN 256
+#define VL_LOG2E 1.44269504088896341f
+#define VL_LN2 0.69314718055994531f
+#define VL_NONE 0x7fffffff  // no known token
+
+// What is kept of a call for its backward, in floats: 4 of the call, 8 of a row, and per
+// row and place its known tokens in ascending order (each once, VL_NONE behind them).
+struct KnownRows {
+  float* call;    // [0]: what an upstream gradient of the reduced loss is times
+  float* info;    // [rows][8]
+  int* ids;       // [rows][known]
+  float* weight;  // [rows][known]: q, then Q p - q
+  float* log_q;   // [rows][known]: the mean of ln q over an id's occurrences
+  float* logit;   // [rows][known]: raw logits
+  int known;
+};
+enum { RI_MASS = 0, RI_REST = 1, RI_BAD = 2, RI_COUNTED = 3, RI_M = 4, RI_LOG = 5, RI_FACTOR = 6, RI_LOSS = 7 };
+
+static inline int64_t known_rows_floats(int64_t rows, int64_t known) { return 4 + rows * (8 + 4 * known); }
+static inline KnownRows known_rows(float* state, int64_t rows, int64_t known) {
+  KnownRows r;
+  r.call = state;
+  r.info = state + 4;
+  r.ids = reinterpret_cast<int*>(r.info + 8 * rows);
+  r.weight = reinterpret_cast<float*>(r.ids + rows * known);
+  r.log_q = r.weight + rows * known;
+  r.logit = r.log_q + rows * known;
+  r.known = (int)known;
+  return r;
+}
+
+// A part of a row's sum over the tokens that are not known: its largest raw logit m and
+// sum 2^((z - m) c); -inf and 0 where no token can be (or none is there).
+struct Part {
+  float m, sum;
+};
+__device__ __forceinline__ Part part_join(const Part& a, const Part& b, float c) {
+  const float to = fmaxf(a.m, b.m), base = to == -INFINITY ? 0.f : to;
+  // what is -inf weighs 0 (NaN stays)
+  return {to, a.sum * __builtin_amdgcn_exp2f((a.m - base) * c) + b.sum * __builtin_amdgcn_exp2f((b.m - base) * c)};
+}
+
+enum { VL_NONE_REDUCED = 0, VL_SUM = 1, VL_MEAN = 2 };
+
+// Launches (vocab_loss.hip).
+void known_prepare_launch(const KnownRows& k, const int64_t* targets, const int64_t* ids,
+                          const float* log_q, int64_t rows, int64_t vocab, int64_t ignore,
+                          bool rest, hipStream_t st);
+// The row sums of logits [rows, width] that are columns first .. of the vocabulary, in
+// `chunks` parts a row at part[chunk * rows + row], and the known tokens' logits.
+int64_t row_stats_chunks(int64_t rows, int64_t width);
+template <typename T>
+void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, int64_t chunks, Part* part, hipStream_t st);
+// Losses and the gradient's factors from `parts` parts a row; the reduced loss.
+void known_finish_launch(const KnownRows& k, const Part* part, int64_t parts, int64_t rows,
+                         float c, bool cross, int reduction, float* loss,
+                         hipStream_t st);
+// dlogits (TO, row stride ldo, columns [width, padded) and rows [rows, padded_rows) zero) of logits
+// [rows, width], columns first .. of the vocabulary; may be in place.
+template <typename TI, typename TO>
+void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, float inv_t, const float* d_loss, int reduction,
+                      TO* out, int64_t ldo, int64_t padded_rows, int64_t padded, hipStream_t st);
+
+// What a row's gradient is times: the upstream gradient over the temperature.
+__device__ __forceinline__ float row_upstream(const float* call, const float* d_loss, int reduction,
+                                              int64_t row, float inv_t) {
+  return (reduction == VL_NONE_REDUCED ? d_loss[row] : d_loss[0] * call[0]) * inv_t;
+}
+
+static inline int check_vocab_loss(const char* what, int64_t rows, int64_t vocab, int64_t known,
+                                   float inv_t, int reduction) {
+  ALODLM_CHECK_ARG(rows >= 0 && rows < (1ll << 24), "%s: rows out of range", what);
+  ALODLM_CHECK_ARG(vocab >= 1 && vocab < (1ll << 30), "%s: vocabulary out of range", what);
+  ALODLM_CHECK_ARG(known >= 1 && known <= VL_MAX_KNOWN, "%s: 1 to 256 known tokens a row", what);
+  ALODLM_CHECK_ARG(inv_t > 0.f && inv_t * VL_LOG2E < INFINITY,
+                   "%s: the temperature must be positive, its inverse times log2 e finite", what);
+  ALODLM_CHECK_ARG(reduction >= 0 && reduction <= 2, "%s: bad reduction", what);
+  return ALODLM_OK;
+}

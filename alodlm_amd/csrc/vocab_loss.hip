@@ -1,0 +1,496 @@
+// Losses against a few known tokens a row over logits in memory: the rows' known tokens,
+// sums over the vocabulary, losses, gradients; and a teacher's divergence from a student's
+// logits (vocab_loss.h has the mathematics).  linear_loss.hip has the same without logits.
+//
+// The known tokens are marked in a bit map of the row's part in LDS, whose bytes lie as the
+// 16-byte pieces of the row do: one byte read a piece says whether any of its logits has to
+// be left out, so the pass over the row stays a stream.
+#include "vocab_loss.h"
+
+namespace {
+
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int MAP_WORDS = 8192 + 4;    // bits of a part: 2^18 tokens, and the row's ragged ends
+constexpr int64_t MAX_PART = 1 << 18;  // tokens of a part
+
+// ---------------------------------------------------------------------------
+// A row's known tokens, a wave each: ascending, every id once with its occurrences'
+// probabilities added up.  Ranks come from comparisons with all others (LDS broadcasts).
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(THREADS)
+known_prepare_kernel(KnownRows k, const int64_t* __restrict__ targets, const int64_t* __restrict__ ids,
+                     const float* __restrict__ log_q, int64_t rows, int vocab, int64_t ignore, int rest) {
+  __shared__ int s_id[WAVES][VL_MAX_KNOWN];
+  __shared__ float s_lq[WAVES][VL_MAX_KNOWN];
+  __shared__ int s_first[WAVES][VL_MAX_KNOWN];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = k.known;
+  const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
+  const bool live = row < rows;
+  bool bad = false, any = false;
+  double mass = 0.0;
+  if (live) {
+    for (int i = lane; i < K; i += 64) {
+      const int64_t id = targets ? targets[row] : ids[row * K + i];
+      const bool none = targets ? id == ignore : id < 0;
+      const bool known = !none && id >= 0 && id < vocab;
+      const float lq = known ? (log_q ? log_q[row * K + i] : 0.f) : -INFINITY;
+      bad |= !none && !known;
+      any |= !none;
+      s_id[wave][i] = known ? (int)id : VL_NONE;
+      s_lq[wave][i] = lq;
+      mass += exp((double)lq);
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  mass = wave_sum_d(mass);
+  bad = __any(bad);
+  any = __any(any);
+  for (int i = lane; i < K; i += 64) {
+    const int id = s_id[wave][i];
+    bool first = id != VL_NONE;
+    for (int j = 0; j < i; ++j) first &= s_id[wave][j] != id;
+    s_first[wave][i] = first;
+    k.ids[row * K + i] = VL_NONE;
+  }
+  // (a wave's LDS stores and loads stay in order)
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  for (int i = lane; i < K; i += 64) {
+    if (!s_first[wave][i]) continue;
+    const int id = s_id[wave][i];
+    int rank = 0;
+    double q = 0.0, terms = 0.0;
+    for (int j = 0; j < K; ++j) {
+      rank += s_first[wave][j] && s_id[wave][j] < id;
+      if (s_id[wave][j] == id) {
+        const double lq = s_lq[wave][j], one = exp(lq);
+        q += one;
+        if (one != 0.0) terms += one * lq;  // 0 ln 0 = 0; NaN stays
+      }
+    }
+    const int64_t at = row * K + rank;
+    k.ids[at] = id;
+    k.weight[at] = (float)q;
+    k.log_q[at] = q != 0.0 ? (float)(terms / q) : 0.f;
+  }
+  if (lane == 0) {
+    float* info = k.info + 8 * row;
+    info[RI_MASS] = (float)mass;
+    info[RI_REST] = rest && any ? (float)fmax(1.0 - mass, 0.0) : 0.f;
+    info[RI_BAD] = bad ? 1.f : 0.f;
+    info[RI_COUNTED] = any ? 1.f : 0.f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Row sums
+// ---------------------------------------------------------------------------
+// 16 bytes of a row.
+template <typename T> struct Piece;
+template <> struct Piece<bf16_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const bf16_t* p, float* v) { Vec8<bf16_t>::load(p, v); }
+  static __device__ __forceinline__ void store(bf16_t* p, const float* v) { Vec8<bf16_t>::store_nt(p, v); }
+};
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const float* p, float* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float* v) {
+    __builtin_nontemporal_store(nt_f32x4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<nt_f32x4_t*>(p));
+  }
+};
+
+struct Running {
+  float m, sum;
+  template <int N>
+  __device__ __forceinline__ void add(const float* x, float c) {
+    float g = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) g = fmaxf(g, x[i]);
+    if (g > m) {
+      if (m > -INFINITY) sum *= __builtin_amdgcn_exp2f((m - g) * c);
+      m = g;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f((x[i] - base) * c);
+  }
+};
+
+// Part blockIdx.x % chunks of row blockIdx.x / chunks: the tokens [lo, hi) of a
+// row's `width`.  Marks: bit col - lo + 8 - (the part's first piece's offset) ...
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int width, int64_t first,
+                 KnownRows k, float c, int chunks, int chunk_width, Part* __restrict__ part) {
+  constexpr int N = Piece<T>::N;
+  extern __shared__ uint32_t map[];
+  __shared__ float red[2][WAVES];
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x % chunks);
+  const int lo = min(chunk * chunk_width, width), hi = min(lo + chunk_width, width);
+  const T* x = logits + row * ld + lo;
+  const int n = hi - lo;
+  // up to N - 1 tokens before the first 16-byte boundary, whole pieces, the rest
+  const int head = min((int)(-(intptr_t)x & 15) / (int)sizeof(T), n);
+  const int pieces = (n - head) / N, tail = head + pieces * N;
+  // token t of the part has bit t - head + N: a piece has its own N bits
+  const int words = (n + 2 * N + 31) / 32;
+  for (int i = threadIdx.x; i < words; i += THREADS) map[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < k.known; i += THREADS) {
+    const int64_t id = k.ids[row * k.known + i];
+    const int64_t t = id - first - lo;
+    if (id == VL_NONE || t < 0 || t >= n) continue;
+    const int bit = (int)t - head + N;
+    atomicOr(&map[bit >> 5], 1u << (bit & 31));
+    k.logit[row * k.known + i] = Elem<T>::load(x, t);
+  }
+  __syncthreads();
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(map);
+  auto marks = [&](int p) -> uint32_t {  // of piece p
+    if constexpr (N == 8) return bytes[p + 1];
+    else return bytes[(p + 1) >> 1] >> (4 * ((p + 1) & 1)) & 15u;
+  };
+  Running r = {-INFINITY, 0.f};
+  constexpr int HELD = 4;
+  float v[HELD][N];
+  int p = threadIdx.x;
+  auto leave_out = [&](float* v, uint32_t bits) {
+    if (bits)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = bits >> i & 1 ? -INFINITY : v[i];
+  };
+  for (; p + (HELD - 1) * THREADS < pieces; p += HELD * THREADS) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) Piece<T>::load(x + head + (p + j * THREADS) * N, v[j]);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) leave_out(v[j], marks(p + j * THREADS));
+    r.add<HELD * N>(v[0], c);
+  }
+  for (; p < pieces; p += THREADS) {
+    Piece<T>::load(x + head + p * N, v[0]);
+    leave_out(v[0], marks(p));
+    r.add<N>(v[0], c);
+  }
+  auto single = [&](int t) {
+    const int bit = t - head + N;
+    const float v = map[bit >> 5] >> (bit & 31) & 1 ? -INFINITY : Elem<T>::load(x, t);
+    r.add<1>(&v, c);
+  };
+  if ((int)threadIdx.x < head) single(threadIdx.x);
+  if (tail + (int)threadIdx.x < n) single(tail + threadIdx.x);
+  // one rescaling, then sums
+  const float m = wave_max(r.m), base = m == -INFINITY ? 0.f : m;
+  const float s = wave_sum(r.sum * __builtin_amdgcn_exp2f((r.m - base) * c));
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = m; red[1][threadIdx.x >> 6] = s; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Part a = {red[0][0], red[1][0]};
+    for (int w = 1; w < WAVES; ++w) a = part_join(a, {red[0][w], red[1][w]}, c);
+    part[(int64_t)chunk * rows + row] = a;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Losses: 16 rows a workgroup.  Its threads first take the parts of 16 neighbouring rows
+// together, then a wave a row.
+// ---------------------------------------------------------------------------
+constexpr int FIN_ROWS = 16, FIN_LANES = 64;
+
+__global__ void __launch_bounds__(FIN_ROWS * FIN_LANES)
+known_finish_kernel(KnownRows k, const Part* __restrict__ part, int64_t parts, int64_t rows, float c,
+                    int cross, float* __restrict__ loss) {
+  __shared__ Part red[FIN_ROWS][FIN_LANES + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = k.known;
+  {
+    const int r = threadIdx.x % FIN_ROWS, l = threadIdx.x / FIN_ROWS;
+    const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + r;
+    Part a = {-INFINITY, 0.f};
+    if (row < rows)
+      for (int64_t p = l; p < parts; p += FIN_LANES) a = part_join(a, part[p * rows + row], c);
+    red[r][l] = a;
+  }
+  __syncthreads();
+  const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + wave;
+  if (row >= rows) return;
+  const Part mine = red[wave][lane];
+  float m = wave_max(mine.m);
+  const float base = m == -INFINITY ? 0.f : m;
+  const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * c));
+  const bool others = !(s_rest == 0.f);  // a token that is not known can be
+  const float m_rest = m;
+  // the known tokens join
+  float z[VL_MAX_KNOWN / 64], q[VL_MAX_KNOWN / 64];
+  bool known[VL_MAX_KNOWN / 64];
+#pragma unroll
+  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j) {
+    const int i = lane + 64 * j;
+    known[j] = i < K && k.ids[row * K + i] != VL_NONE;
+    z[j] = known[j] ? k.logit[row * K + i] : -INFINITY;
+    q[j] = known[j] ? k.weight[row * K + i] : 0.f;
+    m = fmaxf(m, z[j]);
+  }
+  m = wave_max(m);
+  const bool none = m == -INFINITY;  // no token can be (or NaN)
+  const float top = none ? 0.f : m;
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j)
+    if (known[j]) s += __builtin_amdgcn_exp2f((z[j] - top) * c);
+  s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * c) : 0.f);
+  const float log_s = log2f(s);
+  const float log_rest = others ? (m_rest - top) * c + log2f(s_rest) : -INFINITY;
+  float* info = k.info + 8 * row;
+  const bool empty = none && s == 0.f, bad = info[RI_BAD] != 0.f, counted = info[RI_COUNTED] != 0.f;
+  const float p_rest = others ? __builtin_amdgcn_exp2f(log_rest - log_s) : 0.f;
+  const float q_rest = others ? info[RI_REST] : 0.f;
+  const float mass = info[RI_MASS] + q_rest;
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j) {
+    if (!known[j]) continue;
+    const int64_t at = row * K + lane + 64 * j;
+    const float log_p = (z[j] - top) * c - log_s;
+    if (cross) {
+      // -ln p = ln(1 + others / own): small losses keep their digits
+      const float x = VL_LN2 * (log_rest - (z[j] - top) * c);
+      sum = !others ? (z[j] < INFINITY ? 0.f : NAN) : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
+      if (!(z[j] < INFINITY)) sum = NAN;
+    } else if (q[j] != 0.f) {
+      sum += q[j] * (k.log_q[at] - VL_LN2 * log_p);
+    }
+    const float p = __builtin_amdgcn_exp2f(log_p);
+    k.weight[at] = bad ? NAN : empty ? 0.f : cross ? -p_rest : fmaf(mass, p, -q[j]);
+  }
+  sum = wave_sum(sum);
+  if (q_rest != 0.f) sum += q_rest * (logf(q_rest) - VL_LN2 * (log_rest - log_s));
+  if (empty) sum = info[RI_MASS] != 0.f ? INFINITY : 0.f;
+  if (!counted) sum = 0.f;
+  if (bad) sum = NAN;
+  if (lane == 0) {
+    info[RI_M] = top;
+    info[RI_LOG] = log_rest;
+    info[RI_FACTOR] = bad ? NAN : !counted || !others ? 0.f : fmaf(mass, p_rest, -q_rest);
+    info[RI_LOSS] = sum;
+    if (loss) loss[row] = sum;
+  }
+}
+
+// The sum or mean of the rows' losses, in a fixed order.
+__global__ void __launch_bounds__(1024)
+known_reduce_kernel(KnownRows k, int64_t rows, int mean, float* __restrict__ loss) {
+  __shared__ double total[16], count[16];
+  double t = 0.0, n = 0.0;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    t += (double)k.info[8 * r + RI_LOSS];
+    n += (double)k.info[8 * r + RI_COUNTED];
+  }
+  t = wave_sum_d(t);
+  n = wave_sum_d(n);
+  if ((threadIdx.x & 63) == 0) { total[threadIdx.x >> 6] = t; count[threadIdx.x >> 6] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) { t += total[w]; n += count[w]; }
+    const double by = mean ? fmax(n, 1.0) : 1.0;
+    loss[0] = (float)(t / by);
+    k.call[0] = (float)(1.0 / by);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gradients: a stream.  The known tokens' are written again behind a barrier.
+// ---------------------------------------------------------------------------
+constexpr int GRAD_PIECES = THREADS * 4;
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(THREADS)
+row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t first, KnownRows k,
+                 float c, float inv_t, const float* __restrict__ d_loss, int reduction, TO* out,
+                 int64_t ldo, int padded, int chunks) {
+  constexpr int N = 8;  // tokens a thread takes at a time
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x % chunks);
+  TO* o = out + row * ldo;
+  // pieces by the gradient's 16-byte (bf16) or 32-byte (float) alignment
+  const int head = min((int)(-(intptr_t)o & (8 * (int)sizeof(TO) - 1)) / (int)sizeof(TO), padded);
+  const int pieces = (padded - head) / N, tail = head + pieces * N;
+  const int p0 = min(chunk * GRAD_PIECES, pieces), p1 = min(p0 + GRAD_PIECES, pieces);
+  const bool last = chunk == chunks - 1;
+  const bool live = row < rows;
+  const TI* x = logits + (live ? row : 0) * ld;
+  float g = 0.f, factor = 0.f, m = 0.f, log_rest = 0.f;
+  if (live) {
+    const float* info = k.info + 8 * row;
+    g = row_upstream(k.call, d_loss, reduction, row, inv_t);
+    m = info[RI_M];
+    log_rest = info[RI_LOG];
+    factor = g == 0.f && info[RI_BAD] != 0.f ? 0.f : g * info[RI_FACTOR];
+  }
+  const bool flat = factor == 0.f;  // nothing but the known tokens has a gradient
+  auto gradient = [&](float v) { return factor * __builtin_amdgcn_exp2f((v - m) * c - log_rest); };
+  const bool together = ((uintptr_t)(x + head) & 15) == 0;
+#pragma unroll 2
+  for (int p = p0 + threadIdx.x; p < p1; p += THREADS) {
+    const int at = head + p * N;
+    float v[N];
+    if (flat) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.f;
+    } else {
+      if (together && at + N <= width) {
+#pragma unroll
+        for (int i = 0; i < N; i += Piece<TI>::N) Piece<TI>::load(x + at + i, v + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = at + i < width ? Elem<TI>::load(x, at + i) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = at + i < width ? gradient(v[i]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += Piece<TO>::N) Piece<TO>::store(o + at + i, v + i);
+  }
+  auto single = [&](int at) {
+    Elem<TO>::store(o, at, flat || at >= width ? 0.f : gradient(Elem<TI>::load(x, at)));
+  };
+  if (chunk == 0 && (int)threadIdx.x < head) single(threadIdx.x);
+  if (last && tail + (int)threadIdx.x < padded) single(tail + threadIdx.x);
+  if (!live) return;
+  __syncthreads();
+  const int lo = chunk == 0 ? 0 : head + p0 * N, hi = min(last ? padded : head + p1 * N, width);
+  for (int i = threadIdx.x; i < k.known; i += THREADS) {
+    const int id = k.ids[row * k.known + i];
+    const int64_t at = (int64_t)id - first;
+    if (id == VL_NONE || at < lo || at >= hi) continue;
+    Elem<TO>::store(o, at, g == 0.f ? 0.f : g * k.weight[row * k.known + i]);
+  }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+void known_prepare_launch(const KnownRows& k, const int64_t* targets, const int64_t* ids,
+                          const float* log_q, int64_t rows, int64_t vocab, int64_t ignore,
+                          bool rest, hipStream_t st) {
+  known_prepare_kernel<<<ceil_div_u(rows, WAVES), THREADS, 0, st>>>(k, targets, ids, log_q, rows,
+                                                                    (int)vocab, ignore, rest);
+}
+
+// Parts of a row: one where the rows alone give every compute unit two workgroups, else as
+// many as make 256 workgroups (few rows) or 1024, of 2048 tokens at least.
+int64_t row_stats_chunks(int64_t rows, int64_t width) {
+  const int64_t least = (width + MAX_PART - 1) / MAX_PART;
+  if (rows >= 512) return least;
+  const int64_t want = ((rows < 32 ? 256 : 1024) + rows - 1) / rows;
+  const int64_t most = width / 2048 > 1 ? width / 2048 : 1;
+  const int64_t n = want < most ? want : most;
+  return n > least ? n : least;
+}
+
+template <typename T>
+void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, int64_t chunks, Part* part, hipStream_t st) {
+  // parts of whole 64 tokens: their 16-byte pieces lie alike
+  const int64_t chunk_width = ((width + chunks - 1) / chunks + 63) / 64 * 64;
+  const size_t lds = 4 * (size_t)((chunk_width + 2 * Piece<T>::N + 31) / 32 + 1);
+  row_stats_kernel<T><<<(unsigned)(rows * chunks), THREADS, lds, st>>>(
+      logits, ld, rows, (int)width, first, k, c, (int)chunks, (int)chunk_width, part);
+}
+template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
+                                      float, int64_t, Part*, hipStream_t);
+template void row_stats_launch<bf16_t>(const bf16_t*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
+                                       float, int64_t, Part*, hipStream_t);
+
+void known_finish_launch(const KnownRows& k, const Part* part, int64_t parts, int64_t rows, float c,
+                         bool cross, int reduction, float* loss, hipStream_t st) {
+  const bool each = reduction == VL_NONE_REDUCED;
+  if (rows > 0)
+    known_finish_kernel<<<ceil_div_u(rows, FIN_ROWS), FIN_ROWS * FIN_LANES, 0, st>>>(
+        k, part, parts, rows, c, cross, each ? loss : nullptr);
+  if (!each) known_reduce_kernel<<<1, 1024, 0, st>>>(k, rows, reduction == VL_MEAN, loss);
+}
+
+template <typename TI, typename TO>
+void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, float inv_t, const float* d_loss, int reduction,
+                      TO* out, int64_t ldo, int64_t padded_rows, int64_t padded, hipStream_t st) {
+  const int64_t chunks = (padded / 8 + GRAD_PIECES) / GRAD_PIECES;
+  row_grads_kernel<TI, TO><<<(unsigned)(padded_rows * chunks), THREADS, 0, st>>>(
+      logits, ld, rows, (int)width, first, k, c, inv_t, d_loss, reduction, out, ldo, (int)padded,
+      (int)chunks);
+}
+template void row_grads_launch<float, float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
+                                             float, float, const float*, int, float*, int64_t, int64_t, int64_t,
+                                             hipStream_t);
+template void row_grads_launch<float, bf16_t>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
+                                              float, float, const float*, int, bf16_t*, int64_t, int64_t, int64_t,
+                                              hipStream_t);
+
+// ---------------------------------------------------------------------------
+// Distillation from logits
+// ---------------------------------------------------------------------------
+extern "C" int64_t alodlm_vocab_loss_state(int64_t rows, int64_t known) { return known_rows_floats(rows, known); }
+
+extern "C" int64_t alodlm_distillation_workspace(int64_t rows, int64_t vocab) {
+  return rows > 0 ? 2 * rows * row_stats_chunks(rows, vocab) : 0;
+}
+
+extern "C" int alodlm_distillation(const void* logits, int64_t ld, const int64_t* ids, const float* log_q,
+                                   int64_t rows, int64_t vocab, int64_t known, float inv_temperature,
+                                   int rest, int reduction, float* loss, float* state,
+                                   float* workspace, int dtype, void* stream) {
+  const int rc = check_vocab_loss("distillation", rows, vocab, known, inv_temperature, reduction);
+  if (rc) return rc;
+  ALODLM_CHECK_ARG(ld >= vocab, "distillation: rows overlap");
+  if (rows == 0 && reduction == VL_NONE_REDUCED) return ALODLM_OK;
+  ALODLM_CHECK_ARG(loss && state && (rows == 0 || (logits && ids && log_q && workspace)),
+                   "distillation: the call lacks an array");
+  const hipStream_t st = as_stream(stream);
+  const KnownRows k = known_rows(state, rows, known);
+  const float c = inv_temperature * VL_LOG2E;
+  if (rows > 0) {
+    const int64_t chunks = row_stats_chunks(rows, vocab);
+    ALODLM_CHECK_ARG(rows * chunks < (1ll << 31), "distillation: too many rows in one call");
+    known_prepare_launch(k, nullptr, ids, log_q, rows, vocab, 0, rest != 0, st);
+    Part* part = reinterpret_cast<Part*>(workspace);
+    ALODLM_DISPATCH(dtype, T, {
+      row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, k, c, chunks, part, st);
+    });
+    known_finish_launch(k, part, chunks, rows, c, false, reduction, loss, st);
+  } else {
+    known_finish_launch(k, nullptr, 0, 0, c, false, reduction, loss, st);
+  }
+  ALODLM_CHECK_LAUNCH("distillation");
+  return ALODLM_OK;
+}
+
+extern "C" int alodlm_distillation_bwd(const void* logits, int64_t ld, const float* state, const float* d_loss,
+                                       int64_t rows, int64_t vocab, int64_t known,
+                                       float inv_temperature, int reduction, void* dlogits, int dtype,
+                                       void* stream) {
+  const int rc = check_vocab_loss("distillation_bwd", rows, vocab, known, inv_temperature, reduction);
+  if (rc) return rc;
+  ALODLM_CHECK_ARG(ld >= vocab, "distillation_bwd: rows overlap");
+  if (rows == 0) return ALODLM_OK;
+  ALODLM_CHECK_ARG(logits && state && d_loss && dlogits, "distillation_bwd: the call lacks an array");
+  ALODLM_CHECK_ARG(rows * ((vocab / 8 + GRAD_PIECES) / GRAD_PIECES) < (1ll << 31),
+                   "distillation_bwd: too many rows in one call");
+  const KnownRows k = known_rows(const_cast<float*>(state), rows, known);  // read only
+  const float c = inv_temperature * VL_LOG2E;
+  ALODLM_DISPATCH(dtype, T, {
+    const int64_t chunks = (vocab / 8 + GRAD_PIECES) / GRAD_PIECES;
+    row_grads_kernel<T, T><<<(unsigned)(rows * chunks), THREADS, 0, as_stream(stream)>>>(
+        (const T*)logits, ld, rows, (int)vocab, 0, k, c, inv_temperature, d_loss, reduction, (T*)dlogits,
+        vocab, (int)vocab, (int)chunks);
+  });
+  ALODLM_CHECK_LAUNCH("distillation_bwd");
+  return ALODLM_OK;
+}

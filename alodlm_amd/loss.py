@@ -9,16 +9,24 @@ segment's clean stream (alodlm/loss.py:12-32).  Both are differentiable:
 outcome_loss in ``ce`` (through the detached truncated stick) and in the gate
 logits (through log q), autoregressive_loss in ``logits``.
 
+``linear_cross_entropy(hidden, weight, targets)`` is the cross entropy of hidden states
+times the output projection without the logits being kept;
+``distillation_loss(logits, teacher_ids, teacher_log_probs)`` and
+``linear_distillation_loss(hidden, weight, ...)`` the divergence from a teacher of which
+each row's most likely tokens are known (``credit.token_log_probs(..., top=k)`` of the
+teacher's logits), from the student's logits or from its hidden states.
+
 The objective kernel accumulates in float32 where the reference's bf16 run
 keeps the stick and the denoising sum in bf16; sums run in one workgroup in a
 fixed order.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, query
-from .credit import _require_gpu, check_sequence_boundaries
+from ._lib import call, call_on, ptr, query
+from .credit import _require_gpu, _vocabulary_rows, check_sequence_boundaries
 
 METRIC_KEYS = ("denoising", "actor", "sampled_mean_depth", "prediction_cost",
                "regularization_cost", "profile_mean_depth", "first_pass_halt_probability")
@@ -128,3 +136,214 @@ def autoregressive_loss(logits, labels, packed_boundaries):
     if R == 0:
         return torch.tensor(0.0, device=logits.device, requires_grad=True)
     return _AutoregressiveLoss.apply(logits, sel, target, n_rows, R)
+
+
+MAX_KNOWN = 256
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _aligned_rows(t):
+    """A matrix whose rows the kernels can take, and their stride: elements of a row next
+    to each other, and 16-byte aligned rows where a row is a whole number of 16 bytes."""
+    rows, width = t.shape
+    step = 16 // t.element_size()
+    if width == 1 or t.stride(1) == 1:
+        stride = width if rows < 2 else t.stride(0)
+        if stride >= width and (width % step or (stride % step == 0 and t.data_ptr() % 16 == 0)):
+            return t, stride
+    t = t.contiguous()
+    return (t if t.data_ptr() % 16 == 0 or width % step else t.clone()), width
+
+
+def _upstream(d_loss):
+    if d_loss.dtype == torch.float32 and d_loss.is_contiguous():
+        return d_loss
+    return d_loss.to(torch.float32).contiguous()
+
+
+def _state(rows, known, reduction, device):
+    """The result of a call and what its backward takes."""
+    loss = torch.empty(() if reduction else rows, dtype=torch.float32, device=device)
+    return loss, torch.empty(query("alodlm_vocab_loss_state", rows, known), dtype=torch.float32,
+                             device=device)
+
+
+def _distill(logits, ids, log_q, inv_temperature, rest, reduction):
+    R, V = logits.shape
+    dev = logits.device
+    x, ld = _vocabulary_rows(logits)
+    loss, state = _state(R, ids.shape[1], reduction, dev)
+    ws = torch.empty(query("alodlm_distillation_workspace", R, V), dtype=torch.float32, device=dev)
+    call_on(dev, "alodlm_distillation", x.data_ptr(), ld, ids.data_ptr(), log_q.data_ptr(), R, V,
+            ids.shape[1], inv_temperature, rest, reduction, loss.data_ptr(), state.data_ptr(),
+            ws.data_ptr(), _lib.dtype_code(x.dtype))
+    return loss, state
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, log_q, inv_temperature, rest, reduction):
+        loss, state = _distill(logits, ids, log_q, inv_temperature, rest, reduction)
+        ctx.save_for_backward(logits, state)
+        ctx.args = ids.shape[1], inv_temperature, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_loss):
+        logits, state = ctx.saved_tensors
+        R, V = logits.shape
+        x, ld = _vocabulary_rows(logits)
+        out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+        up = _upstream(d_loss)
+        call_on(x.device, "alodlm_distillation_bwd", x.data_ptr(), ld, state.data_ptr(), up.data_ptr(),
+                R, V, *ctx.args, out.data_ptr(), _lib.dtype_code(x.dtype))
+        return out, None, None, None, None, None
+
+
+def _linear(hidden, weight, targets, ids, log_q, inv_temperature, ignore_index, rest, reduction):
+    R, H = hidden.shape
+    V, dev = weight.shape[0], hidden.device
+    known = 1 if ids is None else ids.shape[1]
+    h, ldh = _aligned_rows(hidden)
+    w, ldw = _aligned_rows(weight)
+    code = _lib.dtype_code(h.dtype)
+    loss, state = _state(R, known, reduction, dev)
+    ws = torch.empty(query("alodlm_linear_loss_workspace", R, V, H, code), dtype=torch.float32, device=dev)
+    call_on(dev, "alodlm_linear_loss", h.data_ptr(), ldh, w.data_ptr(), ldw, ptr(targets), ptr(ids),
+            ptr(log_q), R, V, H, known, inv_temperature, ignore_index, rest, reduction, loss.data_ptr(),
+            state.data_ptr(), ws.data_ptr(), code)
+    return loss, state
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, *args):
+        loss, state = _linear(hidden, weight, *args)
+        ctx.save_for_backward(hidden, weight, state)
+        ids = args[1]
+        ctx.args = 1 if ids is None else ids.shape[1], args[3], args[6]
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_loss):
+        hidden, weight, state = ctx.saved_tensors
+        (R, H), V, dev = hidden.shape, weight.shape[0], hidden.device
+        h, ldh = _aligned_rows(hidden)
+        w, ldw = _aligned_rows(weight)
+        code = _lib.dtype_code(h.dtype)
+        dh = torch.empty(R, H, dtype=h.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            dw = (torch.empty if R else torch.zeros)(V, H, dtype=h.dtype, device=dev)
+        ws = torch.empty(query("alodlm_linear_loss_bwd_workspace", R, V, H, dh is not None, dw is not None,
+                               code), dtype=torch.float32, device=dev)
+        up = _upstream(d_loss)
+        call_on(dev, "alodlm_linear_loss_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, state.data_ptr(),
+                up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
+        return (dh, dw) + (None,) * 7
+
+
+def _check_options(temperature, reduction):
+    if not 0 < temperature < float("inf"):
+        raise ValueError('temperature must be positive and finite')
+    if reduction not in _REDUCTIONS:
+        raise ValueError('reduction must be "none", "sum" or "mean"')
+
+
+def _check_factors(hidden, weight):
+    if hidden.ndim != 2 or weight.ndim != 2 or min(weight.shape) < 1 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError('Hidden states must be [rows, width] and the weight [vocabulary, width]')
+    _lib.dtype_code(hidden.dtype)
+    if weight.dtype != hidden.dtype or weight.device != hidden.device:
+        raise ValueError('Hidden states and weight must share a dtype and a device')
+
+
+def _check_teacher(x, teacher_ids, teacher_log_probs):
+    if (teacher_ids.dtype != torch.int64 or teacher_ids.ndim != 2
+            or teacher_ids.shape[0] != x.shape[0] or not 1 <= teacher_ids.shape[1] <= MAX_KNOWN):
+        raise ValueError(f'Teacher ids must be int64 [rows, 1 to {MAX_KNOWN}]')
+    if teacher_log_probs.dtype != torch.float32 or teacher_log_probs.shape != teacher_ids.shape:
+        raise ValueError('Teacher log probabilities must be float32, one per id')
+    if not teacher_ids.device == teacher_log_probs.device == x.device:
+        raise ValueError('The teacher\'s tensors and the student\'s must share a device')
+    if teacher_log_probs.requires_grad and torch.is_grad_enabled():
+        raise ValueError('Teacher log probabilities have no gradient here: detach them')
+
+
+def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the tokens ``targets`` (int64 [rows]) under the logits
+    ``hidden`` [rows, width] times ``weight`` [vocabulary, width] transposed, over
+    ``temperature``: float32, the mean over the rows whose target is not ``ignore_index``
+    (0 if there is none), their sum, or with ``reduction="none"`` the rows' own.  The logits
+    are not rounded and never kept: the backward computes them again, a piece of the
+    vocabulary at a time, in at most about half a GiB for up to 2^20 rows.  Differentiable
+    in ``hidden`` and ``weight`` (either may be without gradient, which saves its product).
+
+    A row of ``ignore_index`` has loss 0 and no gradient; any other target outside the
+    vocabulary makes its loss NaN, and its gradients where the loss takes part.
+
+    A backward that is captured into a graph must not find an eager autograd graph of the
+    same leaves alive (its nodes are tied to the eager stream): drop its outputs first."""
+    _check_factors(hidden, weight)
+    if targets.dtype != torch.int64 or targets.shape != hidden.shape[:1]:
+        raise ValueError('Targets must be int64, one per row of hidden states')
+    if targets.device != hidden.device:
+        raise ValueError('Targets and hidden states must share a device')
+    _check_options(temperature, reduction)
+    _require_gpu(hidden, "linear_cross_entropy")
+    args = (hidden, weight, targets.contiguous(), None, None, 1.0 / temperature, int(ignore_index), False,
+            _REDUCTIONS[reduction])
+    if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        return _Linear.apply(*args)
+    return _linear(*args)[0]
+
+
+def distillation_loss(logits, teacher_ids, teacher_log_probs, temperature=1.0, rest=True, reduction="mean"):
+    """Divergence of the student p = softmax(``logits`` / ``temperature``) ([rows,
+    vocabulary]) from a teacher whose most likely tokens a row are ``teacher_ids`` (int64
+    [rows, up to 256]) with log probabilities ``teacher_log_probs`` (float32, taken at the
+    same temperature):
+
+        sum_k q_k (log q_k - log p[id_k])  and with ``rest``  + q_r (log q_r - log p_r),
+
+    all other tokens taken as one, q_r = max(0, 1 - sum_k q_k); where no other token can be
+    (all are known, or their logits -inf) it takes no part.  float32, the mean over the rows
+    that have a teacher's token (0 if none has), their sum, or each row's with
+    ``reduction="none"``.  Differentiable in ``logits``.
+
+    An id below 0 is no token (rows of fewer, down to none: loss 0 and no gradient); one
+    given twice counts twice; one outside the vocabulary makes the row's loss NaN, and its
+    gradient where the loss takes part.  A logit of -inf is a token that cannot be: the
+    loss is inf where the teacher gives it probability.
+
+    A backward that is captured into a graph must not find an eager autograd graph of the
+    same logits alive (its nodes are tied to the eager stream): drop its outputs first."""
+    if logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError('Logits must be [rows, vocabulary]')
+    _lib.dtype_code(logits.dtype)
+    _check_teacher(logits, teacher_ids, teacher_log_probs)
+    _check_options(temperature, reduction)
+    _require_gpu(logits, "distillation_loss")
+    args = (logits, teacher_ids.contiguous(), teacher_log_probs.contiguous(), 1.0 / temperature, bool(rest),
+            _REDUCTIONS[reduction])
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distillation.apply(*args)
+    return _distill(*args)[0]
+
+
+def linear_distillation_loss(hidden, weight, teacher_ids, teacher_log_probs, temperature=1.0, rest=True,
+                             reduction="mean"):
+    """``distillation_loss`` of the logits ``hidden`` [rows, width] times ``weight``
+    [vocabulary, width] transposed, without keeping them, as ``linear_cross_entropy``:
+    differentiable in ``hidden`` and ``weight``."""
+    _check_factors(hidden, weight)
+    _check_teacher(hidden, teacher_ids, teacher_log_probs)
+    _check_options(temperature, reduction)
+    _require_gpu(hidden, "linear_distillation_loss")
+    args = (hidden, weight, None, teacher_ids.contiguous(), teacher_log_probs.contiguous(), 1.0 / temperature,
+            0, bool(rest), _REDUCTIONS[reduction])
+    if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        return _Linear.apply(*args)
+    return _linear(*args)[0]

@@ -769,6 +769,51 @@ int alodlm_token_log_probs_bwd(const void* logits, int64_t ld, const int64_t* ta
                                int64_t rows, int64_t vocab, int64_t top, float inv_temperature,
                                int64_t ignore, void* dlogits, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Losses against a few known tokens a row: cross entropy (one of probability 1, as in
+ * alodlm/loss.py:12-32) and distillation from a teacher's most likely tokens (no
+ * counterpart in the reference).  With p = softmax(logits * inv_temperature) and q =
+ * exp(log_q) [rows, known] the probabilities of the tokens ids [rows, known],
+ *   loss[r] = sum_k q_k (log q_k - log p[id_k])
+ *             (+ q_r (log q_r - log p_r) with `rest`: all other tokens as one event,
+ *              q_r = max(0, 1 - sum_k q_k); where none of them can be it takes no part).
+ * An id < 0 is no token, one given twice counts twice, one outside the vocabulary makes the
+ * row's loss NaN and, where its upstream gradient is not 0, its gradient.  A row of no
+ * tokens has loss 0 and no gradient.  A logit of -inf is a token that cannot be.
+ * 1 to 256 known tokens a row.  `reduction`: 0 loss [rows], 1 their sum, 2 their mean over
+ * the rows that have a token (0 if none has): loss [1].  `state` (alodlm_vocab_loss_state
+ * floats) is what the backward takes, with d_loss [rows] or [1].
+ * ------------------------------------------------------------------------ */
+int64_t alodlm_vocab_loss_state(int64_t rows, int64_t known);
+/* From logits [rows, vocab] (dtype, row stride ld); the backward writes dlogits [rows,
+ * vocab].  The workspace (floats) is 8-byte aligned. */
+int64_t alodlm_distillation_workspace(int64_t rows, int64_t vocab);
+int alodlm_distillation(const void* logits, int64_t ld, const int64_t* ids, const float* log_q,
+                        int64_t rows, int64_t vocab, int64_t known, float inv_temperature, int rest,
+                        int reduction, float* loss, float* state, float* workspace, int dtype,
+                        void* stream);
+int alodlm_distillation_bwd(const void* logits, int64_t ld, const float* state, const float* d_loss,
+                            int64_t rows, int64_t vocab, int64_t known, float inv_temperature,
+                            int reduction, void* dlogits, int dtype, void* stream);
+/* From hidden [rows, width] and the output projection weight [vocab, width] (dtype, row
+ * strides ldh, ldw), whose product the logits are; they are never kept.  `targets` int64
+ * [rows] in place of ids and log_q: cross entropy (known 1, rest 0), `ignore` no token.  The
+ * backward writes d_hidden [rows, width] and d_weight [vocab, width] (each may be NULL).
+ * bfloat16 rows of a width that is a multiple of 64 are 16-byte aligned, and so are the
+ * workspaces (floats). */
+int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int dtype);
+int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                       const int64_t* targets, const int64_t* ids, const float* log_q, int64_t rows,
+                       int64_t vocab, int64_t width, int64_t known, float inv_temperature,
+                       int64_t ignore, int rest, int reduction, float* loss, float* state,
+                       float* workspace, int dtype, void* stream);
+int64_t alodlm_linear_loss_bwd_workspace(int64_t rows, int64_t vocab, int64_t width, int d_hidden,
+                                         int d_weight, int dtype);
+int alodlm_linear_loss_bwd(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                           const float* state, const float* d_loss, int64_t rows, int64_t vocab,
+                           int64_t width, int64_t known, float inv_temperature, int reduction,
+                           void* d_hidden, void* d_weight, float* workspace, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
