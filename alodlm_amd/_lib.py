@@ -119,11 +119,12 @@ SIGNATURES = {
     "alodlm_distillation_workspace": [I64, I64],
     "alodlm_distillation": [P, I64, P, P, I64, I64, I64, F32, I32, I32, P, P, P, I32, P],
     "alodlm_distillation_bwd": [P, I64, P, P, I64, I64, I64, F32, I32, P, I32, P],
-    "alodlm_linear_loss_workspace": [I64, I64, I64, I32],
-    "alodlm_linear_loss": [P, I64, P, I64, P, P, P, I64, I64, I64, I64, F32, I64, I32, I32, P, P, P,
+    "alodlm_linear_loss_kept": [I64, I64, I64, I32],
+    "alodlm_linear_loss_workspace": [I64, I64, I64, I32, I32],
+    "alodlm_linear_loss": [P, I64, P, I64, P, P, P, I64, I64, I64, I64, F32, I64, I32, I32, P, P, P, P,
                            I32, P],
-    "alodlm_linear_loss_bwd_workspace": [I64, I64, I64, I32, I32, I32],
-    "alodlm_linear_loss_bwd": [P, I64, P, I64, P, P, I64, I64, I64, I64, F32, I32, P, P, P, I32, P],
+    "alodlm_linear_loss_bwd_workspace": [I64, I64, I64, I32, I32, I32, I32],
+    "alodlm_linear_loss_bwd": [P, I64, P, I64, P, P, P, I64, I64, I64, I64, F32, I32, P, P, P, I32, P],
 }
 _RESTYPE = {
     "alodlm_last_error": ctypes.c_char_p,
@@ -145,6 +146,7 @@ _RESTYPE = {
     "alodlm_token_log_probs_workspace": I64,
     "alodlm_vocab_loss_state": I64,
     "alodlm_distillation_workspace": I64,
+    "alodlm_linear_loss_kept": I64,
     "alodlm_linear_loss_workspace": I64,
     "alodlm_linear_loss_bwd_workspace": I64,
 }

@@ -7,14 +7,21 @@
 // tile leaves one part (largest logit, sum) a row.  Nothing of the size of the logits is
 // written.  Backward: a piece of the vocabulary at a time, the tiles are computed once more
 // and leave the piece's gradient D = dloss / dlogits in bf16, from which two products give
-// its share of d_hidden (D W, summed in float32 over the pieces) and its rows of d_weight
-// (D^T hidden, written once).  Four products of 2 rows vocab width operations in all, of
-// which the second computation of the logits is what not keeping them costs.
+// its share of d_hidden (D W, in float32 planes that one pass adds up) and its rows of
+// d_weight (D^T hidden, written once).  Four products of 2 rows vocab width operations in
+// all, of which the second computation of the logits is what not keeping them costs.
 //
-// D is rounded to bf16 (half a step, 2^-9 of a value at most), as a bf16 model's logits'
-// gradient is anywhere: it is an operand of the bf16 matrix cores.  Float32 models, and
-// widths that are no multiple of 64, take a piece's logits in float32 through memory.
+// Logits of at most 2^25 values are cheaper to keep, in float32, than to compute again (and
+// the products of few rows read the weight, which a tile of 256 rows would wait for): they
+// go through memory and the row kernels of vocab_loss.hip, as those of float32 models and
+// of 64 rows or fewer do, piece by piece where they are more.
+//
+// D is rounded to bf16 (half a step, 2^-8 of a value at most), as a bf16 model's logits'
+// gradient is anywhere: it is an operand of the bf16 matrix cores.  A reduced loss's upstream
+// gradient is applied to the products, not to D: of a row far from its target, D is then -1
+// there, which is exact.
 #include "gemm_dl_tile.h"
+#include "gemm_mid.h"
 #include "vocab_loss.h"
 
 namespace {
@@ -81,10 +88,11 @@ struct SumHooks {
   static constexpr int EXTRA_LDS = TileMarks::BYTES + 2 * TB * (int)sizeof(Part);
   KnownRows k;
   float c;
-  Part* part;  // [tiles][rows]
+  Part* part;     // [tiles][rows], of the piece
+  int64_t first;  // the piece's first token
 
   __device__ __forceinline__ void before(char* extra, int64_t M, int64_t m0, int64_t n0) const {
-    TileMarks::fill(extra, k, m0 + threadIdx.x, M, n0);
+    TileMarks::fill(extra, k, m0 + threadIdx.x, M, first + n0);
   }
   template <typename Quad>
   __device__ __forceinline__ void after(char*, char* extra, Quad quad, void*, int64_t, int64_t M,
@@ -145,9 +153,8 @@ struct GradHooks {
   static constexpr bool Epilogue = true;
   static constexpr int EXTRA_LDS = TileMarks::BYTES + TB * 16;
   KnownRows k;
-  float c, inv_t;
-  const float* d_loss;
-  int reduction;
+  float c;
+  Upstream up;
   int64_t first;          // the piece's first token
   int64_t rows, columns;  // of D, padding included
 
@@ -156,7 +163,7 @@ struct GradHooks {
     float4 r = make_float4(0.f, 1e30f, 0.f, 0.f);  // 2^-1e30: nothing
     if (row < M) {
       const float* info = k.info + 8 * row;
-      const float g = row_upstream(k.call, d_loss, reduction, row, inv_t);
+      const float g = up.row(row);
       const float f = info[RI_FACTOR];
       r.z = g;
       if (g != 0.f && f != 0.f) {
@@ -196,13 +203,13 @@ struct GradHooks {
     __syncthreads();
     const int64_t row = m0 + threadIdx.x;
     if (row >= M) return;
-    const float up = consts[threadIdx.x].z;
+    const float own_up = consts[threadIdx.x].z;
     const uint32_t* bits = reinterpret_cast<const uint32_t*>(extra) + 8 * threadIdx.x;
     const float* own = k.weight + row * k.known + TileMarks::before(extra, threadIdx.x);
     for (int w = 0; w < 8; ++w)
       for (uint32_t b = bits[w]; b; b &= b - 1, ++own)
         reinterpret_cast<bf16_t*>(D)[row * ldd + n0 + 32 * w + __builtin_ctz(b)] =
-            float_to_bf16(up == 0.f ? 0.f : up * *own);
+            float_to_bf16(own_up == 0.f ? 0.f : own_up * *own);
   }
 };
 
@@ -215,101 +222,232 @@ void tiles_launch(const bf16_t* hidden, int64_t ldh, const bf16_t* weight, int64
       hidden, ldh, weight, ldw, out, ldo, nullptr, 0, rows, tokens, width, 1.f, width, nullptr, 0, hooks);
 }
 
-// dst [padded, width] = src's first `rows` rows, zeros behind them.
+// Rows of d_weight straight from the tiles: times the upstream gradient, rounded once.
+struct ScaleHooks {
+  static constexpr bool Epilogue = true;
+  Upstream up;
+  template <typename Quad>
+  __device__ __forceinline__ void after(char* lds, Quad quad, void* C, int64_t ldc, int64_t M, int64_t N,
+                                        int64_t m0, int64_t n0) const {
+    tile_epilogue<ALODLM_EPI_STORE, 256, true>(lds, quad, C, ldc, nullptr, 0, M, N, m0, n0, up.all(),
+                                               nullptr, 0);
+  }
+};
+
+// dst [padded, padded_width] = src [rows, width], zeros around it.
 template <typename T>
 __global__ void __launch_bounds__(256)
-copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, T* __restrict__ dst, int64_t ldd,
-                 int64_t width) {
-  const int64_t row = blockIdx.y, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at < width) dst[row * ldd + at] = row < rows ? src[row * lds + at] : T(0);
+copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, int64_t width, T* __restrict__ dst,
+                 int64_t padded, int64_t padded_width) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= padded_width) return;
+  for (int64_t row = blockIdx.y; row < padded; row += gridDim.y)
+    dst[row * padded_width + at] = row < rows && at < width ? src[row * lds + at] : T(0);
 }
-template <typename T>
-void copy_rows(const T* src, int64_t lds, int64_t rows, T* dst, int64_t ldd, int64_t padded, int64_t width,
-               hipStream_t st) {
-  for (int64_t r = 0; r < padded; r += 65535) {  // rows of a launch
-    const int64_t n = padded - r < 65535 ? padded - r : 65535;
-    copy_rows_kernel<T><<<dim3(ceil_div_u(width, 256), (unsigned)n), 256, 0, st>>>(
-        src + r * lds, lds, rows - r, dst + r * ldd, ldd, width);
+
+// out [rows, width] = up.all() * (the planes' sum + D's last `rest` columns times the
+// weight's last `rest` rows, which no product took), rounded once.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t rows, int64_t width,
+                      Upstream up, const T* __restrict__ D, int64_t ldd, const T* __restrict__ weight,
+                      int64_t ldw, int rest, T* __restrict__ out) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (at >= width) return;
+  const float scale = up.all();
+  const int64_t plane = rows * width;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float* src = planes + row * width + at;
+    float s[VEC] = {};
+#pragma unroll 4
+    for (int64_t p = 0; p < count; ++p) {
+      if constexpr (VEC == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src + p * plane);
+        s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+      } else {
+        s[0] += src[p * plane];
+      }
+    }
+    for (int t = 0; t < rest; ++t) {
+      const float d = Elem<T>::load(D, row * ldd + t);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] = fmaf(d, Elem<T>::load(weight, t * ldw + at + e), s[e]);
+    }
+    T* dst = out + row * width + at;
+    if constexpr (VEC == 4 && sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(scale * s[0], scale * s[1]),
+                                                  pack_bf16x2(scale * s[2], scale * s[3]));
+    else if constexpr (VEC == 4)
+      *reinterpret_cast<float4*>(dst) = make_float4(scale * s[0], scale * s[1], scale * s[2], scale * s[3]);
+    else
+      Elem<T>::store(dst, 0, scale * s[0]);
   }
 }
 
-int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t ceil_div(int64_t x, int64_t by) { return (x + by - 1) / by; }
+int64_t up_to(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
+dim3 row_grid(int64_t width, int64_t rows) {
+  return dim3((unsigned)ceil_div(width, 256), (unsigned)(rows < 65535 ? rows : 65535));
+}
 
-// Bytes of a piece: what is held of the vocabulary at a time.
-constexpr int64_t PIECE_BYTES = 512ll << 20;
+template <typename T>
+void finish_product(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
+                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, T* out,
+                    hipStream_t st) {
+  const bool vec = width % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
+  if (vec)
+    finish_product_kernel<T, 4><<<row_grid(width / 4, rows), 256, 0, st>>>(planes, count, rows, width, up, D, ldd,
+                                                                           weight, ldw, rest, out);
+  else
+    finish_product_kernel<T, 1><<<row_grid(width, rows), 256, 0, st>>>(planes, count, rows, width, up, D, ldd,
+                                                                       weight, ldw, rest, out);
+}
 
+// Which bf16 tiles a product [M, N] over K runs on and how its K is split: the least of
+// the times that gemm.hip's rule is made of (a 32-deep step of a round of 256 workgroups:
+// 0.58 to 0.78 us on 256x256 tiles, 0.28 us on 128x128 ones and 0.3 on 32 or 64 rows), and
+// the float planes, written and read at 5.5 TB/s; `direct`: 256x256 tiles need none.
+struct Split {
+  bool large;
+  int64_t planes;
+};
+Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct, bool few) {
+  const int64_t steps = ceil_div(K, 32);
+  Split best = {true, 1};
+  double least = 1e30;
+  auto offer = [&](bool large, int64_t s, int64_t tiles, double each) {
+    double t = (double)ceil_div(tiles * s, 256) * (double)ceil_div(steps, s) * each;
+    if (!(large && direct)) t += 4.0 + 4e-6 / 5.5 * (double)(2 * s) * (double)M * (double)N;
+    if (t < least) {
+      least = t;
+      best = {large, s};
+    }
+  };
+  if (large_ok) {
+    const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
+    for (int64_t s = 1; s <= (direct ? 1 : 8) && (s == 1 || steps / s >= 16); ++s) {
+      const double fill = tiles * s < 256 ? (double)(tiles * s) / 256.0 : 1.0;
+      offer(true, s, tiles, 0.58 + 0.2 * fill);
+    }
+  }
+  const int64_t rows = !few ? 128 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int64_t tiles = ceil_div(M, rows) * ceil_div(N, 128);
+  for (int64_t s = 1; s <= 64 && (s == 1 || steps / s >= 8); ++s) offer(false, s, tiles, rows == 128 ? 0.28 : 0.3);
+  return best;
+}
+
+constexpr int64_t KEPT = 1 << 25;                // logits that a forward keeps for its backward
+constexpr int64_t PIECE_BYTES = 512ll << 20;     // of what is held of the vocabulary at a time
+constexpr int64_t FEW = ALODLM_FEW_ROWS;
+
+// How a call runs, from its sizes alone.
 struct Plan {
-  bool tiles;             // logits stay on chip
+  bool half, regular;     // bf16; rows of whole 16 bytes, on the tile kernels
+  bool small, keep, tiles;  // few enough logits to keep; kept; never in memory
   int64_t piece, pieces;  // tokens of a piece (a multiple of 256), pieces
-  int64_t parts, part_chunks;
-  int64_t padded_rows, contributions;
-  bool pad, accumulate;
+  int64_t deep, deep_rows;  // width and rows as the tile kernels take them
+  bool copy_hidden, copy_weight;
+  int64_t chunks, parts;    // of a piece's rows, of all
+  int64_t planes;           // of d_hidden, most
+  bool direct;              // d_hidden needs no planes
+  Split hidden_split, last_split;
   // workspace, in floats
-  int64_t part, logits, D, hidden, sums, tail, d_tail, gemm, total;
+  int64_t part, logits, D, hidden, weight, sums, rows, gemm, total;
 };
 
-Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool backward, bool d_hidden, bool d_weight) {
+// Whether a piece's logits come from the 128-column tiles of few rows, which leave rows of
+// the piece's own length, and the row stride of logits in memory.
+bool few_logits(const Plan& p, int64_t R, int64_t n) {
+  return p.regular && R <= FEW && n >= 128 * 256 && (!p.small || p.pieces == 1);
+}
+int64_t logits_stride(const Plan& p, int64_t R, int64_t V, int64_t n) {
+  return few_logits(p, R, n) ? n : up_to(p.keep ? V : n, 8);
+}
+
+Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backward, bool d_hidden,
+               bool d_weight) {
   Plan p = {};
-  const int64_t es = dtype == ALODLM_BF16 ? 2 : 4;
-  p.tiles = dtype == ALODLM_BF16 && H % 64 == 0;
-  p.padded_rows = dtype == ALODLM_BF16 ? up(R, 32) : R;
-  const int64_t token = p.padded_rows * (p.tiles ? 2 : 4);  // bytes
-  const int64_t most = PIECE_BYTES / token / 256 * 256 > 256 ? PIECE_BYTES / token / 256 * 256 : 256;
-  p.pieces = (V + most - 1) / most;
-  p.piece = up((V + p.pieces - 1) / p.pieces, 256);
-  p.pieces = (V + p.piece - 1) / p.piece;
-  int64_t at = 0;
+  p.half = dtype == ALODLM_BF16;
+  p.regular = p.half && H % 8 == 0;
+  // (a loss has the same bits whether or not a backward will want the logits)
+  p.small = R * up_to(V, 8) <= KEPT;
+  p.keep = keep && p.small;
+  p.tiles = p.regular && !p.small && R > FEW;
+  p.deep = p.regular ? up_to(H, 64) : H;
+  p.deep_rows = p.half ? up_to(R, 32) : R;
+  const int64_t es = p.half ? 2 : 4;
+  const bool computes = !(backward && p.keep);  // the logits
+  p.copy_weight = p.regular && computes && p.deep != H;
+  p.copy_hidden = p.regular && ((computes && p.deep != H) || (backward && d_weight && p.deep_rows != R));
+  // bytes of a token
+  int64_t most = V;
+  auto limit = [&](int64_t bytes) {
+    const int64_t n = PIECE_BYTES / bytes / 256 * 256;
+    most = n < most ? (n > 256 ? n : 256) : most;
+  };
+  if (backward && p.half) limit(2 * p.deep_rows);
+  if (computes && !p.tiles && !p.small) limit(4 * R);
+  if (p.copy_weight) limit(2 * p.deep);
+  if (backward && d_weight && p.half && !p.regular) limit(4 * H);
+  if (p.regular) {  // the 128x128 tiles' operands stay below 2 GiB
+    const int64_t n = (1ll << 30) / up_to(H, 64) / 256 * 256;
+    most = n < most ? n : most;
+  }
+  p.pieces = ceil_div(V, most);
+  p.piece = up_to(ceil_div(V, p.pieces), 256);
+  p.pieces = ceil_div(V, p.piece);
+  const int64_t last = V - (p.pieces - 1) * p.piece, whole = last / 32 * 32, rest = last - whole;
+  int64_t at = 0, gemm = 0;
   auto room = [&](int64_t floats) {
     const int64_t here = at;
-    at += up(floats, 64);
+    at += up_to(floats, 64);
     return here;
   };
-  int64_t gemm = 0;
   auto product = [&](int64_t M, int64_t N, int64_t K, int epi) {
     if (M < 1 || K < 1) return;
     const int64_t n = alodlm_gemm_workspace(M, N, K, epi, dtype);
     gemm = n > gemm ? n : gemm;
   };
-  const int store_f32 = dtype == ALODLM_F32 ? ALODLM_EPI_STORE : ALODLM_EPI_STORE_F32;
-  const int64_t last = V - (p.pieces - 1) * p.piece;
-  if (!p.tiles) {
-    p.logits = room(R * p.piece);
-    if (p.pieces > 1) product(R, p.piece, H, store_f32);
-    product(R, last, H, store_f32);
+  const int f32_out = p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
+  if (p.copy_hidden) p.hidden = room(ceil_div(p.deep_rows * p.deep * es, 4));
+  if (p.copy_weight) p.weight = room(ceil_div(p.piece * p.deep * es, 4));
+  if (computes && !p.tiles) {
+    if (!p.keep) p.logits = room(R * (p.pieces > 1 ? p.piece : up_to(V, 8)));
+    if (p.pieces > 1) product(R, p.piece, p.deep, f32_out);
+    product(R, last, p.deep, f32_out);
   }
   if (!backward) {
-    p.part_chunks = p.tiles ? 0 : row_stats_chunks(R, p.piece);
-    p.parts = p.tiles ? (V + TB - 1) / TB : p.part_chunks * p.pieces;
+    p.chunks = p.tiles ? p.piece / TB : row_stats_chunks(R, p.piece);
+    p.parts = p.tiles ? ceil_div(V, TB) : p.chunks * p.pieces;
     p.part = room(2 * R * p.parts);
   } else {
-    // float32: D takes the logits' place
-    if (dtype == ALODLM_BF16) p.D = room((p.padded_rows * p.piece * es + 3) / 4);
+    // float32: D takes the place of logits that are not kept
+    if (p.half || p.keep) p.D = room(ceil_div(p.deep_rows * p.piece * es, 4));
     else p.D = p.logits;
-    const int64_t whole = last / 32 * 32, rest = last - whole;
-    p.pad = d_weight && p.padded_rows != R;
-    if (p.pad) p.hidden = room((p.padded_rows * H * es + 3) / 4);
-    if (rest) {
-      p.tail = room((32 * H * es + 3) / 4);
-      p.d_tail = room((32 * H * es + 3) / 4);
-    }
-    p.contributions = p.pieces - 1 + (whole > 0) + (rest > 0);
-    p.accumulate = d_hidden && p.contributions > 1;
-    if (p.accumulate && dtype == ALODLM_BF16) p.sums = room(R * H);
     if (d_hidden) {
-      if (p.accumulate) {
-        for (int epi : {store_f32, (int)ALODLM_EPI_ACCUM}) {
-          if (p.pieces > 1) product(R, H, p.piece, epi);
-          product(R, H, whole, epi);
-          if (rest) product(R, H, 32, epi);
-        }
-      } else {
-        product(R, H, whole ? whole : 32, ALODLM_EPI_STORE);
+      const bool large = R >= 256 && H >= 256;
+      p.hidden_split = p.regular ? split_product(R, H, p.piece, large, false, true) : Split{true, 1};
+      p.last_split = p.regular && whole ? split_product(R, H, whole, large, false, true) : Split{true, 1};
+      p.planes = (p.pieces - 1) * p.hidden_split.planes + (whole ? p.last_split.planes : 0);
+      p.direct = !p.half && p.planes == 1 && rest == 0;
+      if (!p.direct) p.sums = room(p.planes * R * H);
+      if (!p.regular) {
+        if (p.pieces > 1) product(R, H, p.piece, f32_out);
+        product(R, H, whole, f32_out);
       }
     }
     if (d_weight) {
-      if (p.pieces > 1) product(p.piece, H, p.padded_rows, ALODLM_EPI_STORE);
-      product(whole, H, p.padded_rows, ALODLM_EPI_STORE);
-      if (rest) product(32, H, p.padded_rows, ALODLM_EPI_STORE);
+      int64_t floats = 0;
+      for (const int64_t n : {p.piece, up_to(last, 32)}) {
+        if (p.regular) {
+          const Split s = split_product(n, H, R, true, true, false);
+          if (!s.large && s.planes * n * H > floats) floats = s.planes * n * H;
+        } else {
+          product(p.half ? n : up_to(n == p.piece ? n : last, 8), H, R, f32_out);
+          if (p.half && n * H > floats) floats = n * H;
+        }
+      }
+      p.rows = room(floats);
     }
   }
   p.gemm = room(gemm);
@@ -328,7 +466,7 @@ int check_linear(const char* what, const void* hidden, int64_t ldh, const void* 
                    "%s: row strides out of range", what);
   if (R > 0)
     ALODLM_CHECK_ARG(hidden && weight, "%s: the call lacks an array", what);
-  if (R > 0 && dtype == ALODLM_BF16 && H % 64 == 0)
+  if (R > 0 && dtype == ALODLM_BF16 && H % 8 == 0)
     ALODLM_CHECK_ARG((((uintptr_t)hidden | (uintptr_t)weight) & 15) == 0 && ldh % 8 == 0 && ldw % 8 == 0,
                      "%s: rows must be 16-byte aligned", what);
   return ALODLM_OK;
@@ -340,149 +478,260 @@ int check_linear(const char* what, const void* hidden, int64_t ldh, const void* 
     if (_rc) return _rc;         \
   } while (0)
 
-template <typename T>
-int backward(const T* hidden, int64_t ldh, const T* weight, int64_t ldw, const KnownRows& k,
-             const float* d_loss, int64_t R, int64_t V, int64_t H, float inv_t, int reduction,
-             T* d_hidden, T* d_weight, float* ws, int dtype, hipStream_t st) {
-  const Plan p = make_plan(R, V, H, dtype, true, d_hidden != nullptr, d_weight != nullptr);
-  constexpr bool half = sizeof(T) == 2;
-  const float c = inv_t * VL_LOG2E;
-  float* gemm = p.gemm < 0 ? nullptr : ws + p.gemm;
-  T* D = reinterpret_cast<T*>(ws + p.D);
-  T* tail = reinterpret_cast<T*>(ws + p.tail);
-  T* d_tail = reinterpret_cast<T*>(ws + p.d_tail);
-  const T* h = hidden;
-  int64_t ldp = ldh;
-  if (p.pad) {
-    T* padded = reinterpret_cast<T*>(ws + p.hidden);
-    copy_rows(hidden, ldh, R, padded, H, p.padded_rows, H, st);
-    h = padded;
-    ldp = H;
+// What the calls below take of the plan and the caller's arrays.
+template <typename T> struct Call {
+  Plan p;
+  const T* hidden;
+  int64_t ldh;
+  const T* weight;
+  int64_t ldw;
+  int64_t R, V, H;
+  float* ws;
+  int dtype;
+  hipStream_t st;
+  const T* deep_hidden;  // as the tile kernels take it
+  int64_t deep_ldh;
+
+  float* gemm() const { return p.gemm < 0 ? nullptr : ws + p.gemm; }
+  void copy_hidden() {
+    deep_hidden = hidden;
+    deep_ldh = ldh;
+    if (!p.copy_hidden) return;
+    T* to = reinterpret_cast<T*>(ws + p.hidden);
+    copy_rows_kernel<T><<<row_grid(p.deep, p.deep_rows), 256, 0, st>>>(hidden, ldh, R, H, to, p.deep_rows, p.deep);
+    deep_hidden = to;
+    deep_ldh = p.deep;
   }
-  float* sums = half ? ws + p.sums : reinterpret_cast<float*>(d_hidden);
-  bool begun = false;
-  auto to_hidden = [&](const T* d, const T* w, int64_t ld, int64_t tokens) {
-    if (!p.accumulate)
-      return alodlm_gemm(d, p.piece, 1, w, ld, 0, d_hidden, H, nullptr, 0, R, H, tokens, 1.f,
-                         ALODLM_EPI_STORE, dtype, gemm, st);
-    const int epi = begun ? ALODLM_EPI_ACCUM : half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
-    begun = true;
-    return alodlm_gemm(d, p.piece, 1, w, ld, 0, sums, H, nullptr, 0, R, H, tokens, 1.f, epi, dtype, gemm,
-                       st);
-  };
-  for (int64_t first = 0; first < V; first += p.piece) {
-    const int64_t n = V - first < p.piece ? V - first : p.piece;
-    const int64_t whole = n / 32 * 32, rest = n - whole, padded = up(n, 32);
+  // the piece's rows of the weight for the products that compute logits
+  const T* piece_weight(int64_t first, int64_t n, int64_t& ld) const {
     const T* w = weight + first * ldw;
+    ld = ldw;
+    if (!p.copy_weight) return w;
+    T* to = reinterpret_cast<T*>(ws + p.weight);
+    copy_rows_kernel<T><<<row_grid(p.deep, n), 256, 0, st>>>(w, ldw, n, H, to, n, p.deep);
+    ld = p.deep;
+    return to;
+  }
+  int64_t logits_ld(int64_t n) const { return logits_stride(p, R, V, n); }
+  // float logits of a piece, row stride logits_ld(n)
+  int logits(int64_t first, int64_t n, float* out) const {
+    int64_t ld;
+    const T* w = piece_weight(first, n, ld);
+    const int64_t to = logits_ld(n);
+    if constexpr (sizeof(T) == 2)
+      if (few_logits(p, R, n) && n * ld < (1ll << 30)) {
+        gemm_mid_planes(deep_hidden, deep_ldh, 1, w, ld, 1, R, n, p.deep, 1, out, st);
+        ALODLM_CHECK_LAUNCH("linear_loss_logits");
+        return ALODLM_OK;
+      }
+    return alodlm_gemm(deep_hidden, deep_ldh, 1, w, ld, 1, out, to, nullptr, 0, R, n, p.deep, 1.f,
+                       p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE, dtype, gemm(), st);
+  }
+};
+
+template <typename T>
+int forward(Call<T>& a, const KnownRows& k, const GivenRows& given, float c, int reduction, float* loss,
+            float* kept) {
+  const Plan& p = a.p;
+  Part* part = reinterpret_cast<Part*>(a.ws + p.part);
+  a.copy_hidden();
+  // whole logits in memory need no prepared tokens
+  const bool whole = !p.tiles && p.pieces == 1;
+  if (!whole) known_prepare_launch(k, given, a.R, a.st);
+  float* logits = p.keep ? kept : a.ws + p.logits;
+  int64_t ld = 0;
+  for (int64_t first = 0, i = 0; first < a.V; first += p.piece, ++i) {
+    const int64_t n = a.V - first < p.piece ? a.V - first : p.piece;
     if (p.tiles) {
-      if constexpr (half) {
-        const GradHooks hooks = {k, c, inv_t, d_loss, reduction, first, p.padded_rows, padded};
-        tiles_launch(hidden, ldh, w, ldw, R, n, H, D, p.piece, hooks, st);
+      if constexpr (sizeof(T) == 2) {
+        const SumHooks hooks = {k, c, part + i * p.chunks * a.R, first};
+        int64_t ldw;
+        const T* w = a.piece_weight(first, n, ldw);
+        tiles_launch(a.deep_hidden, a.deep_ldh, w, ldw, a.R, n, p.deep, nullptr, 0, hooks, a.st);
       }
     } else {
-      float* logits = ws + p.logits;
-      LL_CALL(alodlm_gemm(hidden, ldh, 1, w, ldw, 1, logits, p.piece, nullptr, 0, R, n, H, 1.f,
-                          half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE, dtype, gemm, st));
-      row_grads_launch<float, T>(logits, p.piece, R, n, first, k, c, inv_t, d_loss, reduction, D, p.piece,
-                                 p.padded_rows, padded, st);
+      float* to = p.keep ? logits + first : logits;
+      LL_CALL(a.logits(first, n, to));
+      ld = a.logits_ld(n);
+      row_stats_launch<float>(to, ld, a.R, n, first, whole ? nullptr : &k, given, c, p.chunks,
+                              part + i * p.chunks * a.R, a.st);
+    }
+    ALODLM_CHECK_LAUNCH("linear_loss");
+  }
+  known_finish_launch<float>(k, given, whole ? logits : nullptr, ld, part, p.parts, a.R, c, reduction, loss, a.st);
+  ALODLM_CHECK_LAUNCH("linear_loss");
+  return ALODLM_OK;
+}
+
+template <typename T>
+int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const float* kept, T* d_hidden,
+             T* d_weight) {
+  const Plan& p = a.p;
+  constexpr bool half = sizeof(T) == 2;
+  const int64_t R = a.R, V = a.V, H = a.H;
+  const int f32_out = half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
+  T* D = reinterpret_cast<T*>(a.ws + p.D);
+  float* sums = a.ws + p.sums;
+  int64_t planes = 0, rest = 0;
+  const T* rest_weight = nullptr;
+  a.copy_hidden();
+  for (int64_t first = 0; first < V; first += p.piece) {
+    const int64_t n = V - first < p.piece ? V - first : p.piece, padded = up_to(n, 32);
+    const bool last = first + n == V;
+    // D of the piece; zeros from column n to `columns`
+    const bool own = half || p.keep;  // D has a place of its own
+    const int64_t ldd = own ? p.piece : a.logits_ld(n), columns = own ? padded : ldd;
+    if (p.tiles) {
+      if constexpr (half) {
+        const GradHooks hooks = {k, c, up, first, p.deep_rows, columns};
+        int64_t ldw;
+        const T* w = a.piece_weight(first, n, ldw);
+        tiles_launch(a.deep_hidden, a.deep_ldh, w, ldw, R, n, p.deep, D, p.piece, hooks, a.st);
+      }
+    } else {
+      const float* logits = p.keep ? kept + first : a.ws + p.logits;
+      if (!p.keep) LL_CALL(a.logits(first, n, a.ws + p.logits));
+      row_grads_launch<float, T>(logits, a.logits_ld(n), R, n, first, k, c, up, D, ldd, p.deep_rows, columns,
+                                 a.st);
     }
     ALODLM_CHECK_LAUNCH("linear_loss_bwd");
-    if (rest) copy_rows(w + whole * ldw, ldw, rest, tail, H, 32, H, st);
+    const T* w = a.weight + first * a.ldw;
     if (d_hidden) {
-      if (whole) LL_CALL(to_hidden(D, w, ldw, whole));
-      if (rest) LL_CALL(to_hidden(D + whole, tail, H, 32));
+      const int64_t take = n / 32 * 32;
+      rest = n - take;  // 0 but in the last piece
+      rest_weight = w + take * a.ldw;
+      if (take) {
+        const Split s = last ? p.last_split : p.hidden_split;
+        float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * R * H;
+        bool done = false;
+        if constexpr (half) {
+          if (p.regular && s.large) {
+            int64_t count = 1;
+            gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, R, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
+                           s.planes, &count, 0, a.st);
+            planes += count;
+            done = true;
+          } else if (p.regular && take * a.ldw < (1ll << 30)) {
+            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, 0, R, H, take, s.planes, to, a.st);
+            done = true;
+          }
+        }
+        if (!done) {
+          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, R, H, take, 1.f, f32_out, a.dtype,
+                              p.regular ? nullptr : a.gemm(), a.st));
+          ++planes;
+        }
+        ALODLM_CHECK_LAUNCH("linear_loss_bwd");
+      }
+      if (last && !p.direct)
+        finish_product<T>(sums, planes, R, H, up, D + take, ldd, rest_weight, a.ldw, (int)rest, d_hidden, a.st);
     }
     if (d_weight) {
-      if (whole)
-        LL_CALL(alodlm_gemm(D, p.piece, 0, h, ldp, 0, d_weight + first * H, H, nullptr, 0, whole, H,
-                            p.padded_rows, 1.f, ALODLM_EPI_STORE, dtype, gemm, st));
-      if (rest) {
-        LL_CALL(alodlm_gemm(D + whole, p.piece, 0, h, ldp, 0, d_tail, H, nullptr, 0, 32, H, p.padded_rows,
-                            1.f, ALODLM_EPI_STORE, dtype, gemm, st));
-        copy_rows(d_tail, H, rest, d_weight + (first + whole) * H, H, rest, H, st);
+      T* to = d_weight + first * H;  // (up to 31 rows behind the last: the caller's room)
+      if constexpr (half) {
+        float* rows = a.ws + p.rows;
+        const Split s = p.regular ? split_product(padded, H, R, true, true, false) : Split{false, 1};
+        int64_t count = 1;
+        if (s.large) {
+          const int64_t tiles = ceil_div(padded, TB) * ceil_div(H, TB);
+          gemm_dl_kernel<false, false, ALODLM_EPI_STORE, 4, true, false, ScaleHooks>
+              <<<dim3((unsigned)tiles, 1), 256, 0, a.st>>>(D, ldd, a.deep_hidden, a.deep_ldh, to, H, nullptr, 0,
+                                                           padded, H, p.deep_rows, 1.f, p.deep_rows, nullptr, 0,
+                                                           KSegs{}, ScaleHooks{up});
+        } else {
+          if (p.regular && R * a.deep_ldh < (1ll << 30))
+            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, 0, padded, H, R, s.planes, rows, a.st);
+          else
+            LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, rows, H, nullptr, 0, padded, H, R, 1.f, f32_out,
+                                a.dtype, p.regular ? nullptr : a.gemm(), a.st));
+          finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, to, a.st);
+        }
+      } else {
+        LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, to, H, nullptr, 0, up_to(n, 8), H, R, 1.f, f32_out, a.dtype,
+                            a.gemm(), a.st));
       }
+      ALODLM_CHECK_LAUNCH("linear_loss_bwd");
     }
-    ALODLM_CHECK_LAUNCH("linear_loss_bwd");
   }
-  if (p.accumulate && half) LL_CALL(alodlm_cast_f32(sums, nullptr, d_hidden, R * H, dtype, st));
+  ALODLM_CHECK_LAUNCH("linear_loss_bwd");
   return ALODLM_OK;
 }
 
 }  // namespace
 
-extern "C" int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int dtype) {
+extern "C" int64_t alodlm_linear_loss_kept(int64_t rows, int64_t vocab, int64_t width, int dtype) {
   if (rows < 1 || vocab < 1 || width < 1) return 0;
-  return make_plan(rows, vocab, width, dtype, false, false, false).total;
+  return make_plan(rows, vocab, width, dtype, true, false, false, false).keep ? rows * up_to(vocab, 8) : 0;
 }
 
-extern "C" int64_t alodlm_linear_loss_bwd_workspace(int64_t rows, int64_t vocab, int64_t width,
+extern "C" int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int keep,
+                                                int dtype) {
+  if (rows < 1 || vocab < 1 || width < 1) return 0;
+  return make_plan(rows, vocab, width, dtype, keep != 0, false, false, false).total;
+}
+
+extern "C" int64_t alodlm_linear_loss_bwd_workspace(int64_t rows, int64_t vocab, int64_t width, int keep,
                                                     int d_hidden, int d_weight, int dtype) {
   if (rows < 1 || vocab < 1 || width < 1) return 0;
-  return make_plan(rows, vocab, width, dtype, true, d_hidden != 0, d_weight != 0).total;
+  return make_plan(rows, vocab, width, dtype, keep != 0, true, d_hidden != 0, d_weight != 0).total;
 }
 
 extern "C" int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                                   const int64_t* targets, const int64_t* ids, const float* log_q,
                                   int64_t rows, int64_t vocab, int64_t width, int64_t known,
                                   float inv_temperature, int64_t ignore, int rest, int reduction,
-                                  float* loss, float* state, float* workspace, int dtype, void* stream) {
+                                  float* loss, float* state, float* kept, float* workspace, int dtype,
+                                  void* stream) {
   LL_CALL(check_linear("linear_loss", hidden, ldh, weight, ldw, rows, vocab, width, known, inv_temperature,
                        reduction, dtype));
   ALODLM_CHECK_ARG(!targets || (known == 1 && !rest), "linear_loss: a target is one known token");
-  if (rows == 0 && reduction == VL_NONE_REDUCED) return ALODLM_OK;
+  if (rows == 0 && reduction == VL_EACH) return ALODLM_OK;
   ALODLM_CHECK_ARG(loss && state && (rows == 0 || (workspace && (targets || (ids && log_q)))),
                    "linear_loss: the call lacks an array");
-  ALODLM_CHECK_ARG((uintptr_t)workspace % 16 == 0, "linear_loss: workspace not 16-byte aligned");
+  ALODLM_CHECK_ARG((((uintptr_t)workspace | (uintptr_t)kept) & 15) == 0, "linear_loss: workspace not 16-byte aligned");
   const hipStream_t st = as_stream(stream);
   const KnownRows k = known_rows(state, rows, known);
+  const GivenRows given = {targets, ids, log_q, ignore, (int)known, (int)vocab, rest != 0};
+  const float c = inv_temperature * VL_LOG2E;
   if (rows == 0) {
-    known_finish_launch(k, nullptr, 0, 0, 1.f, false, reduction, loss, st);
+    known_finish_launch<float>(k, given, nullptr, 0, nullptr, 0, 0, c, reduction, loss, st);
     ALODLM_CHECK_LAUNCH("linear_loss");
     return ALODLM_OK;
   }
-  const Plan p = make_plan(rows, vocab, width, dtype, false, false, false);
-  const float c = inv_temperature * VL_LOG2E;
-  Part* part = reinterpret_cast<Part*>(workspace + p.part);
-  known_prepare_launch(k, targets, ids, log_q, rows, vocab, ignore, rest != 0, st);
-  if (p.tiles) {
-    const SumHooks hooks = {k, c, part};
-    tiles_launch((const bf16_t*)hidden, ldh, (const bf16_t*)weight, ldw, rows, vocab, width, nullptr, 0,
-                 hooks, st);
-  } else {
-    float* logits = workspace + p.logits;
-    const int64_t es = dtype == ALODLM_BF16 ? 2 : 4;
-    ALODLM_CHECK_ARG(rows * p.part_chunks < (1ll << 31), "linear_loss: too many rows in one call");
-    for (int64_t first = 0, i = 0; first < vocab; first += p.piece, ++i) {
-      const int64_t n = vocab - first < p.piece ? vocab - first : p.piece;
-      LL_CALL(alodlm_gemm(hidden, ldh, 1, (const char*)weight + first * ldw * es, ldw, 1, logits, p.piece,
-                          nullptr, 0, rows, n, width, 1.f,
-                          dtype == ALODLM_F32 ? ALODLM_EPI_STORE : ALODLM_EPI_STORE_F32, dtype,
-                          p.gemm < 0 ? nullptr : workspace + p.gemm, stream));
-      row_stats_launch<float>(logits, p.piece, rows, n, first, k, c, p.part_chunks,
-                              part + i * p.part_chunks * rows, st);
-    }
+  const Plan p = make_plan(rows, vocab, width, dtype, kept != nullptr, false, false, false);
+  ALODLM_CHECK_ARG(!kept || p.keep, "linear_loss: logits of this size are not kept");
+  ALODLM_CHECK_ARG(rows * p.chunks < (1ll << 31), "linear_loss: too many rows in one call");
+  if (dtype == ALODLM_BF16) {
+    Call<bf16_t> a = {p, (const bf16_t*)hidden, ldh, (const bf16_t*)weight, ldw, rows, vocab, width, workspace,
+                      dtype, st};
+    return forward(a, k, given, c, reduction, loss, kept);
   }
-  known_finish_launch(k, part, p.parts, rows, c, targets != nullptr, reduction, loss, st);
-  ALODLM_CHECK_LAUNCH("linear_loss");
-  return ALODLM_OK;
+  Call<float> a = {p, (const float*)hidden, ldh, (const float*)weight, ldw, rows, vocab, width, workspace, dtype, st};
+  return forward(a, k, given, c, reduction, loss, kept);
 }
 
 extern "C" int alodlm_linear_loss_bwd(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
-                                      const float* state, const float* d_loss, int64_t rows, int64_t vocab,
-                                      int64_t width, int64_t known, float inv_temperature, int reduction,
-                                      void* d_hidden, void* d_weight, float* workspace, int dtype,
+                                      const float* state, const float* kept, const float* d_loss, int64_t rows,
+                                      int64_t vocab, int64_t width, int64_t known, float inv_temperature,
+                                      int reduction, void* d_hidden, void* d_weight, float* workspace, int dtype,
                                       void* stream) {
   LL_CALL(check_linear("linear_loss_bwd", hidden, ldh, weight, ldw, rows, vocab, width, known,
                        inv_temperature, reduction, dtype));
   if (rows == 0 || (!d_hidden && !d_weight)) return ALODLM_OK;
   ALODLM_CHECK_ARG(state && d_loss && workspace, "linear_loss_bwd: the call lacks an array");
-  ALODLM_CHECK_ARG((uintptr_t)workspace % 16 == 0, "linear_loss_bwd: workspace not 16-byte aligned");
+  ALODLM_CHECK_ARG((((uintptr_t)workspace | (uintptr_t)kept | (uintptr_t)d_hidden | (uintptr_t)d_weight) & 15) == 0,
+                   "linear_loss_bwd: an array is not 16-byte aligned");
+  const hipStream_t st = as_stream(stream);
   const KnownRows k = known_rows(const_cast<float*>(state), rows, known);  // read only
-  if (dtype == ALODLM_BF16)
-    return backward((const bf16_t*)hidden, ldh, (const bf16_t*)weight, ldw, k, d_loss, rows, vocab, width,
-                    inv_temperature, reduction, (bf16_t*)d_hidden, (bf16_t*)d_weight, workspace, dtype,
-                    as_stream(stream));
-  return backward((const float*)hidden, ldh, (const float*)weight, ldw, k, d_loss, rows, vocab, width,
-                  inv_temperature, reduction, (float*)d_hidden, (float*)d_weight, workspace, dtype,
-                  as_stream(stream));
+  const float c = inv_temperature * VL_LOG2E;
+  const Plan p = make_plan(rows, vocab, width, dtype, kept != nullptr, true, d_hidden != nullptr, d_weight != nullptr);
+  ALODLM_CHECK_ARG(!kept || p.keep, "linear_loss_bwd: logits of this size are not kept");
+  const Upstream up = {k.call, d_loss, reduction, p.half, inv_temperature};
+  if (dtype == ALODLM_BF16) {
+    Call<bf16_t> a = {p, (const bf16_t*)hidden, ldh, (const bf16_t*)weight, ldw, rows, vocab, width, workspace,
+                      dtype, st};
+    return backward(a, k, c, up, kept, (bf16_t*)d_hidden, (bf16_t*)d_weight);
+  }
+  Call<float> a = {p, (const float*)hidden, ldh, (const float*)weight, ldw, rows, vocab, width, workspace, dtype, st};
+  return backward(a, k, c, up, kept, (float*)d_hidden, (float*)d_weight);
 }

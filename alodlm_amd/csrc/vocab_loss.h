@@ -22,7 +22,8 @@
 #define VL_NONE 0x7fffffff  // no known token
 
 // What is kept of a call for its backward, in floats: 4 of the call, 8 of a row, and per
-// row and place its known tokens in ascending order (each once, VL_NONE behind them).
+// row and place its known tokens, each id once (VL_NONE elsewhere).  known_prepare puts
+// them in ascending order.
 struct KnownRows {
   float* call;    // [0]: what an upstream gradient of the reduced loss is times
   float* info;    // [rows][8]
@@ -47,6 +48,16 @@ static inline KnownRows known_rows(float* state, int64_t rows, int64_t known) {
   return r;
 }
 
+// The known tokens as the caller has them: targets [rows] (one token of probability 1,
+// `ignore` none), or ids and log_q [rows][known].
+struct GivenRows {
+  const int64_t* targets;
+  const int64_t* ids;
+  const float* log_q;
+  int64_t ignore;
+  int known, vocab, rest;
+};
+
 // A part of a row's sum over the tokens that are not known: its largest raw logit m and
 // sum 2^((z - m) c); -inf and 0 where no token can be (or none is there).
 struct Part {
@@ -58,34 +69,49 @@ __device__ __forceinline__ Part part_join(const Part& a, const Part& b, float c)
   return {to, a.sum * __builtin_amdgcn_exp2f((a.m - base) * c) + b.sum * __builtin_amdgcn_exp2f((b.m - base) * c)};
 }
 
-enum { VL_NONE_REDUCED = 0, VL_SUM = 1, VL_MEAN = 2 };
+enum { VL_EACH = 0, VL_SUM = 1, VL_MEAN = 2 };
+
+// The upstream gradient over the temperature.  `apart`: a reduced loss's, which all rows
+// share, is left to the end (all()), so that a row's gradient is Q p - q itself and loses
+// nothing to another factor's mantissa when it is rounded; a row's is then 1, or 0 where
+// the whole is.
+struct Upstream {
+  const float* call;
+  const float* d_loss;
+  int reduction, apart;
+  float inv_t;
+  __device__ __forceinline__ float shared() const { return d_loss[0] * call[0] * inv_t; }
+  __device__ __forceinline__ float row(int64_t r) const {
+    if (reduction == VL_EACH) return d_loss[r] * inv_t;
+    return apart ? (shared() != 0.f ? 1.f : 0.f) : shared();
+  }
+  __device__ __forceinline__ float all() const { return apart && reduction != VL_EACH ? shared() : 1.f; }
+};
 
 // Launches (vocab_loss.hip).
-void known_prepare_launch(const KnownRows& k, const int64_t* targets, const int64_t* ids,
-                          const float* log_q, int64_t rows, int64_t vocab, int64_t ignore,
-                          bool rest, hipStream_t st);
-// The row sums of logits [rows, width] that are columns first .. of the vocabulary, in
-// `chunks` parts a row at part[chunk * rows + row], and the known tokens' logits.
+//
+// The rows' known tokens into k, in ascending order.
+void known_prepare_launch(const KnownRows& k, const GivenRows& given, int64_t rows, hipStream_t st);
+// The row sums of logits [rows, width], columns first .. of the vocabulary, in `chunks`
+// parts a row at part[chunk * rows + row].  With known tokens that are prepared, their
+// logits go to k; else `given` names them.
 int64_t row_stats_chunks(int64_t rows, int64_t width);
 template <typename T>
 void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows& k, float c, int64_t chunks, Part* part, hipStream_t st);
-// Losses and the gradient's factors from `parts` parts a row; the reduced loss.
-void known_finish_launch(const KnownRows& k, const Part* part, int64_t parts, int64_t rows,
-                         float c, bool cross, int reduction, float* loss,
-                         hipStream_t st);
-// dlogits (TO, row stride ldo, columns [width, padded) and rows [rows, padded_rows) zero) of logits
-// [rows, width], columns first .. of the vocabulary; may be in place.
+                      const KnownRows* k, const GivenRows& given, float c, int64_t chunks, Part* part,
+                      hipStream_t st);
+// Losses and the gradient's factors from `parts` parts a row, and the reduced loss.  With
+// whole logits [rows, vocab] in memory (else NULL) the known tokens need no preparation.
+template <typename T>
+void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* logits, int64_t ld,
+                         const Part* part, int64_t parts, int64_t rows, float c, int reduction,
+                         float* loss, hipStream_t st);
+// dlogits (TO, row stride ldo; columns [width, padded) and rows [rows, padded_rows) zero) of
+// logits [rows, width], columns first .. of the vocabulary; may be in place.
 template <typename TI, typename TO>
 void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows& k, float c, float inv_t, const float* d_loss, int reduction,
-                      TO* out, int64_t ldo, int64_t padded_rows, int64_t padded, hipStream_t st);
-
-// What a row's gradient is times: the upstream gradient over the temperature.
-__device__ __forceinline__ float row_upstream(const float* call, const float* d_loss, int reduction,
-                                              int64_t row, float inv_t) {
-  return (reduction == VL_NONE_REDUCED ? d_loss[row] : d_loss[0] * call[0]) * inv_t;
-}
+                      const KnownRows& k, float c, const Upstream& up, TO* out, int64_t ldo,
+                      int64_t padded_rows, int64_t padded, hipStream_t st);
 
 static inline int check_vocab_loss(const char* what, int64_t rows, int64_t vocab, int64_t known,
                                    float inv_t, int reduction) {

@@ -14,73 +14,144 @@ constexpr int MAP_WORDS = 8192 + 4;    // bits of a part: 2^18 tokens, and the r
 constexpr int64_t MAX_PART = 1 << 18;  // tokens of a part
 
 // ---------------------------------------------------------------------------
-// A row's known tokens, a wave each: ascending, every id once with its occurrences'
-// probabilities added up.  Ranks come from comparisons with all others (LDS broadcasts).
+// A row's known tokens, a wave a row: lane l has the places l + 64 j.
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(THREADS)
-known_prepare_kernel(KnownRows k, const int64_t* __restrict__ targets, const int64_t* __restrict__ ids,
-                     const float* __restrict__ log_q, int64_t rows, int vocab, int64_t ignore, int rest) {
-  __shared__ int s_id[WAVES][VL_MAX_KNOWN];
-  __shared__ float s_lq[WAVES][VL_MAX_KNOWN];
-  __shared__ int s_first[WAVES][VL_MAX_KNOWN];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = k.known;
-  const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
-  const bool live = row < rows;
+constexpr int HELD = VL_MAX_KNOWN / 64;
+
+struct RowKnown {
+  int id[HELD];          // VL_NONE: none
+  float q[HELD], log_q[HELD];
+  int place[HELD];       // where it is kept: the ids in ascending order, each once
+  float mass, q_rest;
+  bool bad, counted;
+};
+
+// Ranks come from comparisons with all others (LDS broadcasts of four).  `ids`: this wave's,
+// room for the known tokens rounded up to four.
+__device__ __forceinline__ void known_of_row(const GivenRows& given, int64_t row, int* ids, RowKnown& r) {
+  const int lane = threadIdx.x & 63, K = given.known;
   bool bad = false, any = false;
   double mass = 0.0;
-  if (live) {
-    for (int i = lane; i < K; i += 64) {
-      const int64_t id = targets ? targets[row] : ids[row * K + i];
-      const bool none = targets ? id == ignore : id < 0;
-      const bool known = !none && id >= 0 && id < vocab;
-      const float lq = known ? (log_q ? log_q[row * K + i] : 0.f) : -INFINITY;
-      bad |= !none && !known;
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) {
+    const int i = lane + 64 * j;
+    r.id[j] = VL_NONE;
+    r.q[j] = r.log_q[j] = 0.f;
+    r.place[j] = i;
+    if (64 * j >= K) continue;
+    if (i < K) {
+      const int64_t id = given.targets ? given.targets[row] : given.ids[row * K + i];
+      const bool none = given.targets ? id == given.ignore : id < 0;
+      bad |= !none && !(id >= 0 && id < given.vocab);
       any |= !none;
-      s_id[wave][i] = known ? (int)id : VL_NONE;
-      s_lq[wave][i] = lq;
-      mass += exp((double)lq);
-    }
-  }
-  __syncthreads();
-  if (!live) return;
-  mass = wave_sum_d(mass);
-  bad = __any(bad);
-  any = __any(any);
-  for (int i = lane; i < K; i += 64) {
-    const int id = s_id[wave][i];
-    bool first = id != VL_NONE;
-    for (int j = 0; j < i; ++j) first &= s_id[wave][j] != id;
-    s_first[wave][i] = first;
-    k.ids[row * K + i] = VL_NONE;
-  }
-  // (a wave's LDS stores and loads stay in order)
-  __builtin_amdgcn_wave_barrier();
-  __threadfence_block();
-  for (int i = lane; i < K; i += 64) {
-    if (!s_first[wave][i]) continue;
-    const int id = s_id[wave][i];
-    int rank = 0;
-    double q = 0.0, terms = 0.0;
-    for (int j = 0; j < K; ++j) {
-      rank += s_first[wave][j] && s_id[wave][j] < id;
-      if (s_id[wave][j] == id) {
-        const double lq = s_lq[wave][j], one = exp(lq);
-        q += one;
-        if (one != 0.0) terms += one * lq;  // 0 ln 0 = 0; NaN stays
+      if (!none && id >= 0 && id < given.vocab) {
+        r.id[j] = (int)id;
+        const double q = given.targets ? 1.0 : exp((double)given.log_q[row * K + i]);
+        mass += q;
+        r.q[j] = (float)q;
+        // 0 ln 0 = 0; NaN stays
+        r.log_q[j] = given.targets || q == 0.0 ? 0.f : given.log_q[row * K + i];
       }
     }
-    const int64_t at = row * K + rank;
-    k.ids[at] = id;
-    k.weight[at] = (float)q;
-    k.log_q[at] = q != 0.0 ? (float)(terms / q) : 0.f;
+    if (i < (K + 3) / 4 * 4) ids[i] = r.id[j];
   }
-  if (lane == 0) {
-    float* info = k.info + 8 * row;
-    info[RI_MASS] = (float)mass;
-    info[RI_REST] = rest && any ? (float)fmax(1.0 - mass, 0.0) : 0.f;
-    info[RI_BAD] = bad ? 1.f : 0.f;
-    info[RI_COUNTED] = any ? 1.f : 0.f;
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  r.mass = (float)wave_sum_d(mass);
+  r.counted = __any(any);
+  r.bad = __any(bad);
+  r.q_rest = given.rest && r.counted ? (float)fmax(1.0 - wave_sum_d(mass), 0.0) : 0.f;
+  bool twice = false;
+  const int4* four = reinterpret_cast<const int4*>(ids);
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) {
+    const int i = lane + 64 * j, id = r.id[j];
+    if (64 * j >= K) continue;
+    int rank = 0;
+#pragma unroll 4
+    for (int n = 0; n < (K + 3) / 4; ++n) {
+      const int4 o = four[n];
+      const int other[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool before = 4 * n + e < i;
+        rank += other[e] < id || (other[e] == id && before);
+        twice |= other[e] == id && before && id != VL_NONE;
+      }
+    }
+    r.place[j] = rank;  // the absent behind the others
   }
+  if (!__any(twice)) return;
+  // an id given more than once: its first place takes the others' probabilities
+#pragma unroll 1
+  for (int j = 0; j < HELD; ++j) {
+    const int i = lane + 64 * j;
+    if (i >= K) continue;
+    const int id = i < 64 ? r.id[0] : i < 128 ? r.id[1] : i < 192 ? r.id[2] : r.id[3];
+    bool first = true;
+    int place = 0;
+    double q = 0.0, terms = 0.0;
+    for (int n = 0; n < K; ++n) {
+      const int other = ids[n];
+      bool leads = other != VL_NONE;  // the first of its id
+      for (int m = 0; m < n; ++m) leads &= ids[m] != other;
+      if (other == id && n < i) first = false;
+      if (leads) place += other < id;
+      else place += id == VL_NONE && n < i;  // places that are left over, behind the others
+      if (other == id && id != VL_NONE) {
+        const double lq = given.log_q[row * K + n], one = exp(lq);
+        q += one;
+        if (one != 0.0) terms += one * lq;
+      }
+    }
+    int distinct = 0;
+    if (id != VL_NONE && !first) {  // a place that is left over, too
+      int over = 0;
+      for (int n = 0; n < K; ++n) {
+        bool leads = ids[n] != VL_NONE;
+        for (int m = 0; m < n; ++m) leads &= ids[m] != ids[n];
+        distinct += leads;
+        over += !leads && n < i;
+      }
+      place = distinct + over;
+    }
+    const bool known = id != VL_NONE && first;
+    const float qf = known ? (float)q : 0.f, lf = known && q != 0.0 ? (float)(terms / q) : 0.f;
+#pragma unroll
+    for (int t = 0; t < HELD; ++t)
+      if (t == j) {
+        r.id[t] = known ? id : VL_NONE;
+        r.q[t] = qf;
+        r.log_q[t] = lf;
+        r.place[t] = place;
+      }
+  }
+}
+
+__device__ __forceinline__ void write_info(float* info, const RowKnown& r) {
+  info[RI_MASS] = r.mass;
+  info[RI_REST] = r.q_rest;
+  info[RI_BAD] = r.bad ? 1.f : 0.f;
+  info[RI_COUNTED] = r.counted ? 1.f : 0.f;
+}
+
+__global__ void __launch_bounds__(THREADS)
+known_prepare_kernel(KnownRows k, GivenRows given, int64_t rows) {
+  __shared__ __attribute__((aligned(16))) int ids[WAVES][VL_MAX_KNOWN];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * WAVES + wave;
+  if (row >= rows) return;
+  RowKnown r;
+  known_of_row(given, row, ids[wave], r);
+#pragma unroll
+  for (int j = 0; j < HELD; ++j)
+    if (lane + 64 * j < k.known) {
+      const int64_t at = row * k.known + r.place[j];
+      k.ids[at] = r.id[j];
+      k.weight[at] = r.q[j];
+      k.log_q[at] = r.log_q[j];
+    }
+  if (lane == 0) write_info(k.info + 8 * row, r);
 }
 
 // ---------------------------------------------------------------------------
@@ -121,12 +192,13 @@ struct Running {
   }
 };
 
-// Part blockIdx.x % chunks of row blockIdx.x / chunks: the tokens [lo, hi) of a
-// row's `width`.  Marks: bit col - lo + 8 - (the part's first piece's offset) ...
-template <typename T>
+// Part blockIdx.x % chunks of row blockIdx.x / chunks: the tokens [lo, hi) of a row's
+// `width`.  PREPARED: the known tokens are in k, and their logits go there.
+template <typename T, bool PREPARED>
 __global__ void __launch_bounds__(THREADS)
 row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int width, int64_t first,
-                 KnownRows k, float c, int chunks, int chunk_width, Part* __restrict__ part) {
+                 KnownRows k, GivenRows given, float c, int chunks, int chunk_width,
+                 Part* __restrict__ part) {
   constexpr int N = Piece<T>::N;
   extern __shared__ uint32_t map[];
   __shared__ float red[2][WAVES];
@@ -142,13 +214,22 @@ row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int wid
   const int words = (n + 2 * N + 31) / 32;
   for (int i = threadIdx.x; i < words; i += THREADS) map[i] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < k.known; i += THREADS) {
-    const int64_t id = k.ids[row * k.known + i];
-    const int64_t t = id - first - lo;
-    if (id == VL_NONE || t < 0 || t >= n) continue;
-    const int bit = (int)t - head + N;
+  const int known = PREPARED ? k.known : given.known;
+  for (int i = threadIdx.x; i < known; i += THREADS) {
+    int64_t id;
+    bool none;
+    if constexpr (PREPARED) {
+      id = k.ids[row * known + i];
+      none = id == VL_NONE;
+    } else {
+      id = given.targets ? given.targets[row] : given.ids[row * known + i];
+      none = given.targets && id == given.ignore;
+    }
+    // (an id that is none, or outside the vocabulary, is not of any part)
+    if (none || id < first + lo || id >= first + hi) continue;
+    const int t = (int)(id - first - lo), bit = t - head + N;
     atomicOr(&map[bit >> 5], 1u << (bit & 31));
-    k.logit[row * k.known + i] = Elem<T>::load(x, t);
+    if constexpr (PREPARED) k.logit[row * known + i] = Elem<T>::load(x, t);
   }
   __syncthreads();
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(map);
@@ -157,20 +238,20 @@ row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int wid
     else return bytes[(p + 1) >> 1] >> (4 * ((p + 1) & 1)) & 15u;
   };
   Running r = {-INFINITY, 0.f};
-  constexpr int HELD = 4;
-  float v[HELD][N];
+  constexpr int AHEAD = 4;
+  float v[AHEAD][N];
   int p = threadIdx.x;
   auto leave_out = [&](float* v, uint32_t bits) {
     if (bits)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = bits >> i & 1 ? -INFINITY : v[i];
   };
-  for (; p + (HELD - 1) * THREADS < pieces; p += HELD * THREADS) {
+  for (; p + (AHEAD - 1) * THREADS < pieces; p += AHEAD * THREADS) {
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) Piece<T>::load(x + head + (p + j * THREADS) * N, v[j]);
+    for (int j = 0; j < AHEAD; ++j) Piece<T>::load(x + head + (p + j * THREADS) * N, v[j]);
 #pragma unroll
-    for (int j = 0; j < HELD; ++j) leave_out(v[j], marks(p + j * THREADS));
-    r.add<HELD * N>(v[0], c);
+    for (int j = 0; j < AHEAD; ++j) leave_out(v[j], marks(p + j * THREADS));
+    r.add<AHEAD * N>(v[0], c);
   }
   for (; p < pieces; p += THREADS) {
     Piece<T>::load(x + head + p * N, v[0]);
@@ -202,80 +283,108 @@ row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int wid
 // ---------------------------------------------------------------------------
 constexpr int FIN_ROWS = 16, FIN_LANES = 64;
 
+// GIVEN: the known tokens come from the caller, their logits from `logits`.
+template <typename T, bool GIVEN>
 __global__ void __launch_bounds__(FIN_ROWS * FIN_LANES)
-known_finish_kernel(KnownRows k, const Part* __restrict__ part, int64_t parts, int64_t rows, float c,
-                    int cross, float* __restrict__ loss) {
+known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, int64_t ld,
+                    const Part* __restrict__ part, int64_t parts, int64_t rows, float c,
+                    float* __restrict__ loss) {
   __shared__ Part red[FIN_ROWS][FIN_LANES + 1];
+  __shared__ __attribute__((aligned(16))) int ids[GIVEN ? FIN_ROWS : 1][VL_MAX_KNOWN];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = k.known;
+  const bool cross = given.targets != nullptr;
+  const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + wave;
+  RowKnown r;
+  float z[HELD];
+  if (row < rows) {
+    float* info = k.info + 8 * row;
+    if constexpr (GIVEN) {
+      known_of_row(given, row, ids[wave], r);
+#pragma unroll
+      for (int j = 0; j < HELD; ++j)
+        z[j] = r.id[j] != VL_NONE ? Elem<T>::load(logits, row * ld + r.id[j]) : -INFINITY;
+      if (lane == 0) write_info(info, r);
+    } else {
+#pragma unroll
+      for (int j = 0; j < HELD; ++j) {
+        const int i = lane + 64 * j;
+        const int64_t at = row * K + i;
+        r.id[j] = i < K ? k.ids[at] : VL_NONE;
+        const bool known = r.id[j] != VL_NONE;
+        z[j] = known ? k.logit[at] : -INFINITY;
+        r.q[j] = known ? k.weight[at] : 0.f;
+        r.log_q[j] = known ? k.log_q[at] : 0.f;
+        r.place[j] = i;
+      }
+      r.mass = info[RI_MASS];
+      r.q_rest = info[RI_REST];
+      r.bad = info[RI_BAD] != 0.f;
+      r.counted = info[RI_COUNTED] != 0.f;
+    }
+  }
   {
-    const int r = threadIdx.x % FIN_ROWS, l = threadIdx.x / FIN_ROWS;
-    const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + r;
+    const int n = threadIdx.x % FIN_ROWS, l = threadIdx.x / FIN_ROWS;
+    const int64_t at = (int64_t)blockIdx.x * FIN_ROWS + n;
     Part a = {-INFINITY, 0.f};
-    if (row < rows)
-      for (int64_t p = l; p < parts; p += FIN_LANES) a = part_join(a, part[p * rows + row], c);
-    red[r][l] = a;
+    if (at < rows)
+#pragma unroll 4
+      for (int64_t p = l; p < parts; p += FIN_LANES) a = part_join(a, part[p * rows + at], c);
+    red[n][l] = a;
   }
   __syncthreads();
-  const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + wave;
   if (row >= rows) return;
   const Part mine = red[wave][lane];
   float m = wave_max(mine.m);
   const float base = m == -INFINITY ? 0.f : m;
   const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * c));
-  const bool others = !(s_rest == 0.f);  // a token that is not known can be
+  const bool others = !(s_rest == 0.f);  // a token that is not known can be (or NaN)
   const float m_rest = m;
   // the known tokens join
-  float z[VL_MAX_KNOWN / 64], q[VL_MAX_KNOWN / 64];
-  bool known[VL_MAX_KNOWN / 64];
 #pragma unroll
-  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j) {
-    const int i = lane + 64 * j;
-    known[j] = i < K && k.ids[row * K + i] != VL_NONE;
-    z[j] = known[j] ? k.logit[row * K + i] : -INFINITY;
-    q[j] = known[j] ? k.weight[row * K + i] : 0.f;
-    m = fmaxf(m, z[j]);
-  }
+  for (int j = 0; j < HELD; ++j) m = fmaxf(m, z[j]);
   m = wave_max(m);
-  const bool none = m == -INFINITY;  // no token can be (or NaN)
+  const bool none = m == -INFINITY;
   const float top = none ? 0.f : m;
   float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j)
-    if (known[j]) s += __builtin_amdgcn_exp2f((z[j] - top) * c);
+  for (int j = 0; j < HELD; ++j)
+    if (r.id[j] != VL_NONE) s += __builtin_amdgcn_exp2f((z[j] - top) * c);
   s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * c) : 0.f);
   const float log_s = log2f(s);
   const float log_rest = others ? (m_rest - top) * c + log2f(s_rest) : -INFINITY;
-  float* info = k.info + 8 * row;
-  const bool empty = none && s == 0.f, bad = info[RI_BAD] != 0.f, counted = info[RI_COUNTED] != 0.f;
+  const bool empty = none && s == 0.f;  // no token can be
   const float p_rest = others ? __builtin_amdgcn_exp2f(log_rest - log_s) : 0.f;
-  const float q_rest = others ? info[RI_REST] : 0.f;
-  const float mass = info[RI_MASS] + q_rest;
+  const float q_rest = others ? r.q_rest : 0.f;
+  const float mass = r.mass + q_rest;
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < VL_MAX_KNOWN / 64; ++j) {
-    if (!known[j]) continue;
-    const int64_t at = row * K + lane + 64 * j;
+  for (int j = 0; j < HELD; ++j) {
+    if (lane + 64 * j >= K) continue;
+    const int64_t at = row * K + r.place[j];
+    if constexpr (GIVEN) k.ids[at] = r.id[j];
+    if (r.id[j] == VL_NONE) continue;
     const float log_p = (z[j] - top) * c - log_s;
     if (cross) {
       // -ln p = ln(1 + others / own): small losses keep their digits
       const float x = VL_LN2 * (log_rest - (z[j] - top) * c);
-      sum = !others ? (z[j] < INFINITY ? 0.f : NAN) : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
+      sum = !others ? 0.f : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
       if (!(z[j] < INFINITY)) sum = NAN;
-    } else if (q[j] != 0.f) {
-      sum += q[j] * (k.log_q[at] - VL_LN2 * log_p);
+    } else if (r.q[j] != 0.f) {
+      sum += r.q[j] * (r.log_q[j] - VL_LN2 * log_p);
     }
     const float p = __builtin_amdgcn_exp2f(log_p);
-    k.weight[at] = bad ? NAN : empty ? 0.f : cross ? -p_rest : fmaf(mass, p, -q[j]);
+    k.weight[at] = r.bad ? NAN : empty ? 0.f : cross ? -p_rest : fmaf(mass, p, -r.q[j]);
   }
   sum = wave_sum(sum);
   if (q_rest != 0.f) sum += q_rest * (logf(q_rest) - VL_LN2 * (log_rest - log_s));
-  if (empty) sum = info[RI_MASS] != 0.f ? INFINITY : 0.f;
-  if (!counted) sum = 0.f;
-  if (bad) sum = NAN;
+  if (empty) sum = r.mass != 0.f ? INFINITY : 0.f;
+  if (!r.counted) sum = 0.f;
+  if (r.bad) sum = NAN;
   if (lane == 0) {
+    float* info = k.info + 8 * row;
     info[RI_M] = top;
     info[RI_LOG] = log_rest;
-    info[RI_FACTOR] = bad ? NAN : !counted || !others ? 0.f : fmaf(mass, p_rest, -q_rest);
+    info[RI_FACTOR] = r.bad ? NAN : !r.counted || !others ? 0.f : fmaf(mass, p_rest, -q_rest);
     info[RI_LOSS] = sum;
     if (loss) loss[row] = sum;
   }
@@ -311,8 +420,7 @@ constexpr int GRAD_PIECES = THREADS * 4;
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(THREADS)
 row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t first, KnownRows k,
-                 float c, float inv_t, const float* __restrict__ d_loss, int reduction, TO* out,
-                 int64_t ldo, int padded, int chunks) {
+                 float c, Upstream up, TO* out, int64_t ldo, int padded, int chunks) {
   constexpr int N = 8;  // tokens a thread takes at a time
   const int64_t row = blockIdx.x / chunks;
   const int chunk = (int)(blockIdx.x % chunks);
@@ -327,7 +435,7 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
   float g = 0.f, factor = 0.f, m = 0.f, log_rest = 0.f;
   if (live) {
     const float* info = k.info + 8 * row;
-    g = row_upstream(k.call, d_loss, reduction, row, inv_t);
+    g = up.row(row);
     m = info[RI_M];
     log_rest = info[RI_LOG];
     factor = g == 0.f && info[RI_BAD] != 0.f ? 0.f : g * info[RI_FACTOR];
@@ -377,11 +485,8 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-void known_prepare_launch(const KnownRows& k, const int64_t* targets, const int64_t* ids,
-                          const float* log_q, int64_t rows, int64_t vocab, int64_t ignore,
-                          bool rest, hipStream_t st) {
-  known_prepare_kernel<<<ceil_div_u(rows, WAVES), THREADS, 0, st>>>(k, targets, ids, log_q, rows,
-                                                                    (int)vocab, ignore, rest);
+void known_prepare_launch(const KnownRows& k, const GivenRows& given, int64_t rows, hipStream_t st) {
+  known_prepare_kernel<<<ceil_div_u(rows, WAVES), THREADS, 0, st>>>(k, given, rows);
 }
 
 // Parts of a row: one where the rows alone give every compute unit two workgroups, else as
@@ -397,41 +502,49 @@ int64_t row_stats_chunks(int64_t rows, int64_t width) {
 
 template <typename T>
 void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows& k, float c, int64_t chunks, Part* part, hipStream_t st) {
-  // parts of whole 64 tokens: their 16-byte pieces lie alike
+                      const KnownRows* k, const GivenRows& given, float c, int64_t chunks, Part* part,
+                      hipStream_t st) {
   const int64_t chunk_width = ((width + chunks - 1) / chunks + 63) / 64 * 64;
   const size_t lds = 4 * (size_t)((chunk_width + 2 * Piece<T>::N + 31) / 32 + 1);
-  row_stats_kernel<T><<<(unsigned)(rows * chunks), THREADS, lds, st>>>(
-      logits, ld, rows, (int)width, first, k, c, (int)chunks, (int)chunk_width, part);
+  const unsigned grid = (unsigned)(rows * chunks);
+  if (k)
+    row_stats_kernel<T, true><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, *k, given, c,
+                                                          (int)chunks, (int)chunk_width, part);
+  else
+    row_stats_kernel<T, false><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, KnownRows{},
+                                                           given, c, (int)chunks, (int)chunk_width, part);
 }
-template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
-                                      float, int64_t, Part*, hipStream_t);
-template void row_stats_launch<bf16_t>(const bf16_t*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
-                                       float, int64_t, Part*, hipStream_t);
+template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows*,
+                                      const GivenRows&, float, int64_t, Part*, hipStream_t);
 
-void known_finish_launch(const KnownRows& k, const Part* part, int64_t parts, int64_t rows, float c,
-                         bool cross, int reduction, float* loss, hipStream_t st) {
-  const bool each = reduction == VL_NONE_REDUCED;
-  if (rows > 0)
-    known_finish_kernel<<<ceil_div_u(rows, FIN_ROWS), FIN_ROWS * FIN_LANES, 0, st>>>(
-        k, part, parts, rows, c, cross, each ? loss : nullptr);
+template <typename T>
+void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* logits, int64_t ld,
+                         const Part* part, int64_t parts, int64_t rows, float c, int reduction,
+                         float* loss, hipStream_t st) {
+  float* each = reduction == VL_EACH ? loss : nullptr;
+  const unsigned grid = ceil_div_u(rows, FIN_ROWS), threads = FIN_ROWS * FIN_LANES;
+  if (rows > 0 && logits)
+    known_finish_kernel<T, true><<<grid, threads, 0, st>>>(k, given, logits, ld, part, parts, rows, c, each);
+  else if (rows > 0)
+    known_finish_kernel<T, false><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
   if (!each) known_reduce_kernel<<<1, 1024, 0, st>>>(k, rows, reduction == VL_MEAN, loss);
 }
+template void known_finish_launch<float>(const KnownRows&, const GivenRows&, const float*, int64_t, const Part*,
+                                         int64_t, int64_t, float, int, float*, hipStream_t);
 
 template <typename TI, typename TO>
 void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows& k, float c, float inv_t, const float* d_loss, int reduction,
-                      TO* out, int64_t ldo, int64_t padded_rows, int64_t padded, hipStream_t st) {
+                      const KnownRows& k, float c, const Upstream& up, TO* out, int64_t ldo,
+                      int64_t padded_rows, int64_t padded, hipStream_t st) {
   const int64_t chunks = (padded / 8 + GRAD_PIECES) / GRAD_PIECES;
   row_grads_kernel<TI, TO><<<(unsigned)(padded_rows * chunks), THREADS, 0, st>>>(
-      logits, ld, rows, (int)width, first, k, c, inv_t, d_loss, reduction, out, ldo, (int)padded,
-      (int)chunks);
+      logits, ld, rows, (int)width, first, k, c, up, out, ldo, (int)padded, (int)chunks);
 }
 template void row_grads_launch<float, float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
-                                             float, float, const float*, int, float*, int64_t, int64_t, int64_t,
+                                             float, const Upstream&, float*, int64_t, int64_t, int64_t,
                                              hipStream_t);
 template void row_grads_launch<float, bf16_t>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
-                                              float, float, const float*, int, bf16_t*, int64_t, int64_t, int64_t,
+                                              float, const Upstream&, bf16_t*, int64_t, int64_t, int64_t,
                                               hipStream_t);
 
 // ---------------------------------------------------------------------------
@@ -450,24 +563,22 @@ extern "C" int alodlm_distillation(const void* logits, int64_t ld, const int64_t
   const int rc = check_vocab_loss("distillation", rows, vocab, known, inv_temperature, reduction);
   if (rc) return rc;
   ALODLM_CHECK_ARG(ld >= vocab, "distillation: rows overlap");
-  if (rows == 0 && reduction == VL_NONE_REDUCED) return ALODLM_OK;
+  if (rows == 0 && reduction == VL_EACH) return ALODLM_OK;
   ALODLM_CHECK_ARG(loss && state && (rows == 0 || (logits && ids && log_q && workspace)),
                    "distillation: the call lacks an array");
+  ALODLM_CHECK_ARG((uintptr_t)workspace % 8 == 0, "distillation: workspace not 8-byte aligned");
+  const int64_t chunks = rows > 0 ? row_stats_chunks(rows, vocab) : 0;
+  ALODLM_CHECK_ARG(rows * chunks < (1ll << 31), "distillation: too many rows in one call");
   const hipStream_t st = as_stream(stream);
   const KnownRows k = known_rows(state, rows, known);
+  const GivenRows given = {nullptr, ids, log_q, 0, (int)known, (int)vocab, rest != 0};
   const float c = inv_temperature * VL_LOG2E;
-  if (rows > 0) {
-    const int64_t chunks = row_stats_chunks(rows, vocab);
-    ALODLM_CHECK_ARG(rows * chunks < (1ll << 31), "distillation: too many rows in one call");
-    known_prepare_launch(k, nullptr, ids, log_q, rows, vocab, 0, rest != 0, st);
-    Part* part = reinterpret_cast<Part*>(workspace);
-    ALODLM_DISPATCH(dtype, T, {
-      row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, k, c, chunks, part, st);
-    });
-    known_finish_launch(k, part, chunks, rows, c, false, reduction, loss, st);
-  } else {
-    known_finish_launch(k, nullptr, 0, 0, c, false, reduction, loss, st);
-  }
+  Part* part = reinterpret_cast<Part*>(workspace);
+  ALODLM_DISPATCH(dtype, T, {
+    if (rows > 0) row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, nullptr, given, c, chunks, part, st);
+    known_finish_launch<T>(k, given, rows > 0 ? (const T*)logits : nullptr, ld, part, chunks, rows, c, reduction,
+                           loss, st);
+  });
   ALODLM_CHECK_LAUNCH("distillation");
   return ALODLM_OK;
 }
@@ -484,12 +595,10 @@ extern "C" int alodlm_distillation_bwd(const void* logits, int64_t ld, const flo
   ALODLM_CHECK_ARG(rows * ((vocab / 8 + GRAD_PIECES) / GRAD_PIECES) < (1ll << 31),
                    "distillation_bwd: too many rows in one call");
   const KnownRows k = known_rows(const_cast<float*>(state), rows, known);  // read only
-  const float c = inv_temperature * VL_LOG2E;
+  const Upstream up = {k.call, d_loss, reduction, 0, inv_temperature};
   ALODLM_DISPATCH(dtype, T, {
-    const int64_t chunks = (vocab / 8 + GRAD_PIECES) / GRAD_PIECES;
-    row_grads_kernel<T, T><<<(unsigned)(rows * chunks), THREADS, 0, as_stream(stream)>>>(
-        (const T*)logits, ld, rows, (int)vocab, 0, k, c, inv_temperature, d_loss, reduction, (T*)dlogits,
-        vocab, (int)vocab, (int)chunks);
+    row_grads_launch<T, T>((const T*)logits, ld, rows, vocab, 0, k, inv_temperature * VL_LOG2E, up, (T*)dlogits,
+                           vocab, rows, vocab, as_stream(stream));
   });
   ALODLM_CHECK_LAUNCH("distillation_bwd");
   return ALODLM_OK;

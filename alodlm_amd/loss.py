@@ -21,6 +21,8 @@ keeps the stick and the denoising sum in bf16; sums run in one workgroup in a
 fixed order.
 """
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -155,29 +157,34 @@ def _aligned_rows(t):
     return (t if t.data_ptr() % 16 == 0 or width % step else t.clone()), width
 
 
+def _floats(n, device):
+    return torch.empty(n, dtype=torch.float32, device=device)
+
+
 def _upstream(d_loss):
     if d_loss.dtype == torch.float32 and d_loss.is_contiguous():
         return d_loss
     return d_loss.to(torch.float32).contiguous()
 
 
-def _state(rows, known, reduction, device):
-    """The result of a call and what its backward takes."""
-    loss = torch.empty(() if reduction else rows, dtype=torch.float32, device=device)
-    return loss, torch.empty(query("alodlm_vocab_loss_state", rows, known), dtype=torch.float32,
-                             device=device)
+@functools.lru_cache(maxsize=256)
+def _distill_sizes(R, V, known):
+    return query("alodlm_vocab_loss_state", R, known), query("alodlm_distillation_workspace", R, V)
 
 
 def _distill(logits, ids, log_q, inv_temperature, rest, reduction):
     R, V = logits.shape
     dev = logits.device
     x, ld = _vocabulary_rows(logits)
-    loss, state = _state(R, ids.shape[1], reduction, dev)
-    ws = torch.empty(query("alodlm_distillation_workspace", R, V), dtype=torch.float32, device=dev)
+    state, ws = _distill_sizes(R, V, ids.shape[1])
+    loss = _floats(() if reduction else R, dev)
+    # the state, then the workspace (8-byte aligned: the state's floats are even)
+    buf = _floats(state + ws, dev)
+    at = buf.data_ptr()
     call_on(dev, "alodlm_distillation", x.data_ptr(), ld, ids.data_ptr(), log_q.data_ptr(), R, V,
-            ids.shape[1], inv_temperature, rest, reduction, loss.data_ptr(), state.data_ptr(),
-            ws.data_ptr(), _lib.dtype_code(x.dtype))
-    return loss, state
+            ids.shape[1], inv_temperature, rest, reduction, loss.data_ptr(), at, at + 4 * state,
+            _lib.dtype_code(x.dtype))
+    return loss, buf
 
 
 class _Distillation(torch.autograd.Function):
@@ -201,26 +208,37 @@ class _Distillation(torch.autograd.Function):
         return out, None, None, None, None, None
 
 
-def _linear(hidden, weight, targets, ids, log_q, inv_temperature, ignore_index, rest, reduction):
+@functools.lru_cache(maxsize=256)
+def _linear_sizes(R, V, H, known, code, keep, dh, dw):
+    """Floats of a call's state, kept logits, forward and backward workspaces."""
+    kept = query("alodlm_linear_loss_kept", R, V, H, code) if keep else 0
+    return (query("alodlm_vocab_loss_state", R, known), kept,
+            query("alodlm_linear_loss_workspace", R, V, H, kept > 0, code),
+            query("alodlm_linear_loss_bwd_workspace", R, V, H, kept > 0, dh, dw, code))
+
+
+def _linear(hidden, weight, targets, ids, log_q, inv_temperature, ignore_index, rest, reduction, keep=False):
     R, H = hidden.shape
     V, dev = weight.shape[0], hidden.device
     known = 1 if ids is None else ids.shape[1]
     h, ldh = _aligned_rows(hidden)
     w, ldw = _aligned_rows(weight)
     code = _lib.dtype_code(h.dtype)
-    loss, state = _state(R, known, reduction, dev)
-    ws = torch.empty(query("alodlm_linear_loss_workspace", R, V, H, code), dtype=torch.float32, device=dev)
+    state, kept, ws, _ = _linear_sizes(R, V, H, known, code, keep, True, True)
+    loss = _floats(() if reduction else R, dev)
+    state, ws = _floats(state, dev), _floats(ws, dev)
+    kept = _floats(kept, dev) if kept else None
     call_on(dev, "alodlm_linear_loss", h.data_ptr(), ldh, w.data_ptr(), ldw, ptr(targets), ptr(ids),
             ptr(log_q), R, V, H, known, inv_temperature, ignore_index, rest, reduction, loss.data_ptr(),
-            state.data_ptr(), ws.data_ptr(), code)
-    return loss, state
+            state.data_ptr(), ptr(kept), ws.data_ptr(), code)
+    return loss, state, kept
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, *args):
-        loss, state = _linear(hidden, weight, *args)
-        ctx.save_for_backward(hidden, weight, state)
+        loss, *saved = _linear(hidden, weight, *args, keep=True)
+        ctx.save_for_backward(hidden, weight, *saved)
         ids = args[1]
         ctx.args = 1 if ids is None else ids.shape[1], args[3], args[6]
         return loss
@@ -228,21 +246,20 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        hidden, weight, state = ctx.saved_tensors
+        hidden, weight, state, kept = ctx.saved_tensors
         (R, H), V, dev = hidden.shape, weight.shape[0], hidden.device
         h, ldh = _aligned_rows(hidden)
         w, ldw = _aligned_rows(weight)
         code = _lib.dtype_code(h.dtype)
-        dh = torch.empty(R, H, dtype=h.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = None
-        if ctx.needs_input_grad[1]:
-            dw = (torch.empty if R else torch.zeros)(V, H, dtype=h.dtype, device=dev)
-        ws = torch.empty(query("alodlm_linear_loss_bwd_workspace", R, V, H, dh is not None, dw is not None,
-                               code), dtype=torch.float32, device=dev)
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dh = torch.empty(R, H, dtype=h.dtype, device=dev) if need_h else None
+        # room for whole 32 rows: the kernels' tiles
+        dw = (torch.empty if R else torch.zeros)(-(-V // 32) * 32, H, dtype=h.dtype, device=dev) if need_w else None
+        ws = _floats(_linear_sizes(R, V, H, ctx.args[0], code, kept is not None, need_h, need_w)[3], dev)
         up = _upstream(d_loss)
         call_on(dev, "alodlm_linear_loss_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, state.data_ptr(),
-                up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
-        return (dh, dw) + (None,) * 7
+                ptr(kept), up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
+        return (dh, None if dw is None else dw[:V]) + (None,) * 7
 
 
 def _check_options(temperature, reduction):
@@ -277,9 +294,10 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     ``hidden`` [rows, width] times ``weight`` [vocabulary, width] transposed, over
     ``temperature``: float32, the mean over the rows whose target is not ``ignore_index``
     (0 if there is none), their sum, or with ``reduction="none"`` the rows' own.  The logits
-    are not rounded and never kept: the backward computes them again, a piece of the
-    vocabulary at a time, in at most about half a GiB for up to 2^20 rows.  Differentiable
-    in ``hidden`` and ``weight`` (either may be without gradient, which saves its product).
+    are not rounded, and more than 2^25 of them are not kept: the backward computes them
+    again, a piece of the vocabulary at a time, in workspaces of half a GiB each.
+    Differentiable in ``hidden`` and ``weight`` (either may be without gradient, which saves
+    its product).
 
     A row of ``ignore_index`` has loss 0 and no gradient; any other target outside the
     vocabulary makes its loss NaN, and its gradients where the loss takes part.

@@ -796,23 +796,27 @@ int alodlm_distillation_bwd(const void* logits, int64_t ld, const float* state, 
                             int64_t rows, int64_t vocab, int64_t known, float inv_temperature,
                             int reduction, void* dlogits, int dtype, void* stream);
 /* From hidden [rows, width] and the output projection weight [vocab, width] (dtype, row
- * strides ldh, ldw), whose product the logits are; they are never kept.  `targets` int64
- * [rows] in place of ids and log_q: cross entropy (known 1, rest 0), `ignore` no token.  The
- * backward writes d_hidden [rows, width] and d_weight [vocab, width] (each may be NULL).
- * bfloat16 rows of a width that is a multiple of 64 are 16-byte aligned, and so are the
- * workspaces (floats). */
-int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int dtype);
+ * strides ldh, ldw), whose product the logits are.  `targets` int64 [rows] in place of ids
+ * and log_q: cross entropy (known 1, rest 0), `ignore` no token.  Where
+ * alodlm_linear_loss_kept (floats) is not 0, few enough logits may be kept for the backward
+ * in `kept` (else NULL; `keep` says so to the workspace queries); others are never kept.  The
+ * backward writes d_hidden [rows, width] and d_weight [vocab, width], which has room for
+ * vocab rounded up to 32 rows (each may be NULL).  bfloat16 rows of a width that is a
+ * multiple of 8 are 16-byte aligned; the workspaces (floats), kept and the gradients are. */
+int64_t alodlm_linear_loss_kept(int64_t rows, int64_t vocab, int64_t width, int dtype);
+int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int keep, int dtype);
 int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                        const int64_t* targets, const int64_t* ids, const float* log_q, int64_t rows,
                        int64_t vocab, int64_t width, int64_t known, float inv_temperature,
                        int64_t ignore, int rest, int reduction, float* loss, float* state,
-                       float* workspace, int dtype, void* stream);
-int64_t alodlm_linear_loss_bwd_workspace(int64_t rows, int64_t vocab, int64_t width, int d_hidden,
-                                         int d_weight, int dtype);
+                       float* kept, float* workspace, int dtype, void* stream);
+int64_t alodlm_linear_loss_bwd_workspace(int64_t rows, int64_t vocab, int64_t width, int keep,
+                                         int d_hidden, int d_weight, int dtype);
 int alodlm_linear_loss_bwd(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
-                           const float* state, const float* d_loss, int64_t rows, int64_t vocab,
-                           int64_t width, int64_t known, float inv_temperature, int reduction,
-                           void* d_hidden, void* d_weight, float* workspace, int dtype, void* stream);
+                           const float* state, const float* kept, const float* d_loss, int64_t rows,
+                           int64_t vocab, int64_t width, int64_t known, float inv_temperature,
+                           int reduction, void* d_hidden, void* d_weight, float* workspace, int dtype,
+                           void* stream);
 
 #ifdef __cplusplus
 }
