@@ -20,6 +20,7 @@
 // gradient is anywhere: it is an operand of the bf16 matrix cores.  A reduced loss's upstream
 // gradient is applied to the products, not to D: of a row far from its target, D is then -1
 // there, which is exact.
+#include "few_f32.h"
 #include "gemm_dl_tile.h"
 #include "gemm_mid.h"
 #include "vocab_loss.h"
@@ -234,15 +235,19 @@ struct ScaleHooks {
   }
 };
 
-// dst [padded, padded_width] = src [rows, width], zeros around it.
+// dst [padded, padded_width] = src [rows, width], zeros around it, 16 bytes a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
 copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, int64_t width, T* __restrict__ dst,
                  int64_t padded, int64_t padded_width) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr int N = 16 / (int)sizeof(T);
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
   if (at >= padded_width) return;
-  for (int64_t row = blockIdx.y; row < padded; row += gridDim.y)
-    dst[row * padded_width + at] = row < rows && at < width ? src[row * lds + at] : T(0);
+  for (int64_t row = blockIdx.y; row < padded; row += gridDim.y) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < rows && at < width) v = *reinterpret_cast<const uint4*>(src + row * lds + at);
+    *reinterpret_cast<uint4*>(dst + row * padded_width + at) = v;
+  }
 }
 
 // out [rows, width] = up.all() * (the planes' sum + D's last `rest` columns times the
@@ -325,7 +330,7 @@ Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct,
   };
   if (large_ok) {
     const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
-    for (int64_t s = 1; s <= (direct ? 1 : 8) && (s == 1 || steps / s >= 16); ++s) {
+    for (int64_t s = 1; s <= (direct ? 1 : 32) && (s == 1 || steps / s >= 16); ++s) {
       const double fill = tiles * s < 256 ? (double)(tiles * s) / 256.0 : 1.0;
       offer(true, s, tiles, 0.58 + 0.2 * fill);
     }
@@ -344,6 +349,7 @@ constexpr int64_t FEW = ALODLM_FEW_ROWS;
 struct Plan {
   bool half, regular;     // bf16; rows of whole 16 bytes, on the tile kernels
   bool small, keep, tiles;  // few enough logits to keep; kept; never in memory
+  bool few;                 // float32 products of few rows (few_f32.hip)
   int64_t piece, pieces;  // tokens of a piece (a multiple of 256), pieces
   int64_t deep, deep_rows;  // width and rows as the tile kernels take them
   bool copy_hidden, copy_weight;
@@ -373,6 +379,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   p.small = R * up_to(V, 8) <= KEPT;
   p.keep = keep && p.small;
   p.tiles = p.regular && !p.small && R > FEW;
+  p.few = !p.half && R <= FEW_F32_ROWS && H % 4 == 0 && V * H >= (1 << 20);
   p.deep = p.regular ? up_to(H, 64) : H;
   p.deep_rows = p.half ? up_to(R, 32) : R;
   const int64_t es = p.half ? 2 : 4;
@@ -422,9 +429,13 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
     p.part = room(2 * R * p.parts);
   } else {
     // float32: D takes the place of logits that are not kept
-    if (p.half || p.keep) p.D = room(ceil_div(p.deep_rows * p.piece * es, 4));
+    if (p.few) p.D = room(p.piece * few_f32_pad(R));
+    else if (p.half || p.keep) p.D = room(ceil_div(p.deep_rows * p.piece * es, 4));
     else p.D = p.logits;
-    if (d_hidden) {
+    if (p.few) {
+      p.planes = (p.pieces - 1) * few_f32_planes(p.piece, H) + few_f32_planes(last, H);
+      if (d_hidden) p.sums = room(p.planes * R * H);
+    } else if (d_hidden) {
       const bool large = R >= 256 && H >= 256;
       p.hidden_split = p.regular ? split_product(R, H, p.piece, large, false, true) : Split{true, 1};
       p.last_split = p.regular && whole ? split_product(R, H, whole, large, false, true) : Split{true, 1};
@@ -436,7 +447,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
         product(R, H, whole, f32_out);
       }
     }
-    if (d_weight) {
+    if (d_weight && !p.few) {
       int64_t floats = 0;
       for (const int64_t n : {p.piece, up_to(last, 32)}) {
         if (p.regular) {
@@ -466,8 +477,9 @@ int check_linear(const char* what, const void* hidden, int64_t ldh, const void* 
                    "%s: row strides out of range", what);
   if (R > 0)
     ALODLM_CHECK_ARG(hidden && weight, "%s: the call lacks an array", what);
-  if (R > 0 && dtype == ALODLM_BF16 && H % 8 == 0)
-    ALODLM_CHECK_ARG((((uintptr_t)hidden | (uintptr_t)weight) & 15) == 0 && ldh % 8 == 0 && ldw % 8 == 0,
+  const int64_t step = dtype == ALODLM_BF16 ? 8 : 4;  // elements of 16 bytes
+  if (R > 0 && H % step == 0)
+    ALODLM_CHECK_ARG((((uintptr_t)hidden | (uintptr_t)weight) & 15) == 0 && ldh % step == 0 && ldw % step == 0,
                      "%s: rows must be 16-byte aligned", what);
   return ALODLM_OK;
 }
@@ -498,7 +510,7 @@ template <typename T> struct Call {
     deep_ldh = ldh;
     if (!p.copy_hidden) return;
     T* to = reinterpret_cast<T*>(ws + p.hidden);
-    copy_rows_kernel<T><<<row_grid(p.deep, p.deep_rows), 256, 0, st>>>(hidden, ldh, R, H, to, p.deep_rows, p.deep);
+    copy_rows_kernel<T><<<row_grid(p.deep / 8, p.deep_rows), 256, 0, st>>>(hidden, ldh, R, H, to, p.deep_rows, p.deep);
     deep_hidden = to;
     deep_ldh = p.deep;
   }
@@ -508,7 +520,7 @@ template <typename T> struct Call {
     ld = ldw;
     if (!p.copy_weight) return w;
     T* to = reinterpret_cast<T*>(ws + p.weight);
-    copy_rows_kernel<T><<<row_grid(p.deep, n), 256, 0, st>>>(w, ldw, n, H, to, n, p.deep);
+    copy_rows_kernel<T><<<row_grid(p.deep / 8, n), 256, 0, st>>>(w, ldw, n, H, to, n, p.deep);
     ld = p.deep;
     return to;
   }
@@ -591,6 +603,19 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
     } else {
       const float* logits = p.keep ? kept + first : a.ws + p.logits;
       if (!p.keep) LL_CALL(a.logits(first, n, a.ws + p.logits));
+      if constexpr (!half)
+        if (p.few) {
+          const T* w = a.weight + first * a.ldw;
+          few_grads_launch(logits, a.logits_ld(n), R, n, first, k, c, up, D, few_f32_pad(R), a.st);
+          if (d_hidden) {
+            few_f32_hidden(D, w, a.ldw, R, n, H, sums + planes * R * H, a.st);
+            planes += few_f32_planes(n, H);
+            if (last) finish_product<T>(sums, planes, R, H, up, nullptr, 0, nullptr, 0, 0, d_hidden, a.st);
+          }
+          if (d_weight) few_f32_weight(D, a.hidden, a.ldh, R, n, H, d_weight + first * H, a.st);
+          ALODLM_CHECK_LAUNCH("linear_loss_bwd");
+          continue;
+        }
       row_grads_launch<float, T>(logits, a.logits_ld(n), R, n, first, k, c, up, D, ldd, p.deep_rows, columns,
                                  a.st);
     }

@@ -113,6 +113,11 @@ void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width,
                       const KnownRows& k, float c, const Upstream& up, TO* out, int64_t ldo,
                       int64_t padded_rows, int64_t padded, hipStream_t st);
 
+// The same of few rows in float32, tokens first: out [width][pad], zeros behind the rows.
+void few_grads_launch(const float* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, const Upstream& up, float* out, int64_t pad,
+                      hipStream_t st);
+
 static inline int check_vocab_loss(const char* what, int64_t rows, int64_t vocab, int64_t known,
                                    float inv_t, int reduction) {
   ALODLM_CHECK_ARG(rows >= 0 && rows < (1ll << 24), "%s: rows out of range", what);

@@ -480,6 +480,47 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
   }
 }
 
+// Few rows, tokens first: a thread a token, which reads its logits of all rows.
+constexpr int MAX_FEW = 32;
+
+__global__ void __launch_bounds__(THREADS)
+few_grads_kernel(const float* __restrict__ logits, int64_t ld, int rows, int width, int64_t first, KnownRows k,
+                 float c, Upstream up, float* __restrict__ out, int pad) {
+  __shared__ float s_m[MAX_FEW], s_log[MAX_FEW], s_factor[MAX_FEW], s_up[MAX_FEW];
+  if ((int)threadIdx.x < rows) {
+    const float* info = k.info + 8 * threadIdx.x;
+    const float g = up.row(threadIdx.x);
+    s_m[threadIdx.x] = info[RI_M];
+    s_log[threadIdx.x] = info[RI_LOG];
+    s_factor[threadIdx.x] = g == 0.f && info[RI_BAD] != 0.f ? 0.f : g * info[RI_FACTOR];
+    s_up[threadIdx.x] = g;
+  }
+  __syncthreads();
+  const int lo = blockIdx.x * THREADS, at = lo + threadIdx.x;
+  if (at < width) {
+    float* o = out + (int64_t)at * pad;
+    for (int r = 0; r < pad; r += 4) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = r + e < rows ? s_factor[r + e] : 0.f;
+        v[e] = 0.f;
+        if (f != 0.f)  // (or NaN)
+          v[e] = f * __builtin_amdgcn_exp2f((logits[(r + e) * ld + at] - s_m[r + e]) * c - s_log[r + e]);
+      }
+      *reinterpret_cast<float4*>(o + r) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  __syncthreads();
+  // the known tokens' own
+  for (int i = threadIdx.x; i < rows * k.known; i += THREADS) {
+    const int r = i / k.known;
+    const int64_t t = (int64_t)k.ids[i] - first - lo;
+    if (k.ids[i] == VL_NONE || t < 0 || t >= THREADS || lo + t >= width) continue;
+    out[(lo + t) * pad + r] = s_up[r] == 0.f ? 0.f : s_up[r] * k.weight[i];
+  }
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -546,6 +587,13 @@ template void row_grads_launch<float, float>(const float*, int64_t, int64_t, int
 template void row_grads_launch<float, bf16_t>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
                                               float, const Upstream&, bf16_t*, int64_t, int64_t, int64_t,
                                               hipStream_t);
+
+void few_grads_launch(const float* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
+                      const KnownRows& k, float c, const Upstream& up, float* out, int64_t pad,
+                      hipStream_t st) {
+  few_grads_kernel<<<ceil_div_u(width, THREADS), THREADS, 0, st>>>(logits, ld, (int)rows, (int)width, first, k, c,
+                                                                  up, out, (int)pad);
+}
 
 // ---------------------------------------------------------------------------
 // Distillation from logits

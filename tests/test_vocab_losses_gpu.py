@@ -318,7 +318,7 @@ def check_linear(hidden, weight, targets=None, ids=None, log_q=None, temperature
 
 
 SMALL = [(1, 1, 8), (1, 31, 40), (3, 5, 64), (5, 33, 40), (7, 1000, 72), (64, 1003, 64), (65, 700, 64), (33, 300, 8),
-         (300, 264, 128), (257, 2049, 192), (1000, 40, 256), (5, 40000, 64), (40, 33000, 136), (64, 151936, 64)]
+         (300, 264, 128), (3, 9001, 132), (8, 20000, 64), (16, 1100, 1028), (24, 2051, 640), (32, 1200, 2052), (257, 2049, 192), (1000, 40, 256), (5, 40000, 64), (40, 33000, 136), (64, 151936, 64)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -332,7 +332,7 @@ def test_linear_cross_entropy(R, V, H, dtype):
 
 @pytest.mark.parametrize("R,V,H,dtype", [
     (257, 131101, 64, BF16), (300, 151936, 128, BF16), (1000, 33601, 72, BF16), (4100, 70001, 64, BF16),
-    (64, 600001, 64, BF16), (65, 524321, 8, BF16), (4100, 40001, 32, F32), (3, 12000001, 4, F32)])
+    (64, 600001, 64, BF16), (65, 524321, 8, BF16), (4100, 40001, 32, F32), (3, 12000001, 4, F32), (31, 1200001, 12, F32)])
 def test_logits_that_are_not_kept(R, V, H, dtype):
     """More than 2^25 logits: computed twice, some in several pieces of the vocabulary."""
     log(f"linear not kept {R} x {V} x {H} {dtype}")

@@ -124,6 +124,7 @@ ALL = [distill, distill_bwd, linear, linear_bwd]
         dict(dtype=2), dict(width=0), dict(width=1 << 20), dict(ldh=7), dict(ldw=7), dict(ldh=1 << 22), dict(hidden=None),
         dict(weight=None), dict(hidden=24), dict(weight=24), dict(ldh=12), dict(ldw=12), dict(ws=None), dict(ws=24),
         dict(rows=1 << 20, vocab=1000, kept=16))]
+    + [(f, dict(dtype=0, **b)) for f in ALL[2:] for b in (dict(hidden=24), dict(weight=24), dict(ldh=10), dict(ldw=10))]
     + [(linear, dict(targets=None)), (linear, dict(known=2)), (linear, dict(rest=1)), (linear, dict(loss=None)),
        (linear_bwd, dict(d_loss=None)), (linear_bwd, dict(dh=24)), (linear_bwd, dict(dw=24))])
 def test_library_refusals(make, bad):
