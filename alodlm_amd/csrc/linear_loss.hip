@@ -83,7 +83,12 @@ struct TileMarks {
   }
 };
 
-// Forward tiles: parts of the rows' sums, and the known tokens' logits.
+// Forward tiles: parts of the rows' sums, and the known tokens' logits.  The parts' reference
+// is the largest exponent z c rounded up to a whole number K: 2^(z c - K) is one multiply-add
+// and one exponential, K is exact, and parts are joined by whole powers of two.  The values
+// of 16 rows that hold a known token, or columns past the vocabulary, go through LDS, where
+// single ones can be reached (a lane's own 32 values, so nothing waits for another lane);
+// selecting them in registers made the compiler spill 52 of them, 5 % of the kernel's time.
 struct SumHooks {
   static constexpr bool Epilogue = true;
   static constexpr int EXTRA_LDS = TileMarks::BYTES + 2 * TB * (int)sizeof(Part);
@@ -96,56 +101,62 @@ struct SumHooks {
     TileMarks::fill(extra, k, m0 + threadIdx.x, M, first + n0);
   }
   template <typename Quad>
-  __device__ __forceinline__ void after(char*, char* extra, Quad quad, void*, int64_t, int64_t M,
+  __device__ __forceinline__ void after(char* lds, char* extra, Quad quad, void*, int64_t, int64_t M,
                                         int64_t N, int64_t m0, int64_t n0) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave & 1, g = lane >> 4;
     Part* red = reinterpret_cast<Part*>(extra + TileMarks::BYTES);
+    // this lane's values: 16 bytes at own + 1024 j
+    char* own = lds + 8192 * wave + 16 * lane;
     const bool edge = n0 + TB > N;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stages are free
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float v[8][4];
       int row = 0, col = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        quad(8 * i + j, row, col, v[j]);
-        if (edge)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = n0 + col + e < N ? v[j][e] : -INFINITY;
-      }
+      for (int j = 0; j < 8; ++j) quad(8 * i + j, row, col, v[j]);
       const uint4 b = TileMarks::half(extra, row, wn);
-      if (__any((b.x | b.y | b.z | b.w) != 0)) {
-        // this lane's 32 columns, a bit each
-        uint32_t mine = 0;
+      if (edge || __any((b.x | b.y | b.z | b.w) != 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(own + 1024 * j) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+        uint32_t mine = 0;  // a bit a column of this lane
 #pragma unroll
         for (int j = 0; j < 8; ++j) mine |= TileMarks::nibble(b, j, g) << (4 * j);
-        for (uint32_t left = mine; left; left &= left - 1) {
-          const int at = __builtin_ctz(left);
-          float z = v[0][0];
-#pragma unroll
-          for (int n = 1; n < 32; ++n) z = at == n ? v[n >> 2][n & 3] : z;
-          const int tile_col = wn * 128 + 16 * (at >> 2) + 4 * g + (at & 3);
-          k.logit[(m0 + row) * k.known + TileMarks::place(extra, row, tile_col)] = z;
+        for (; mine; mine &= mine - 1) {
+          const int at = __builtin_ctz(mine), tile_col = wn * 128 + 16 * (at >> 2) + 4 * g + (at & 3);
+          float* z = reinterpret_cast<float*>(own + 1024 * (at >> 2)) + (at & 3);
+          k.logit[(m0 + row) * k.known + TileMarks::place(extra, row, tile_col)] = *z;
+          *z = -INFINITY;
         }
+        if (edge)
+#pragma unroll 1
+          for (int at = 0; at < 32; ++at)
+            if (n0 + wn * 128 + 16 * (at >> 2) + 4 * g + (at & 3) >= N)
+              *(reinterpret_cast<float*>(own + 1024 * (at >> 2)) + (at & 3)) = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < 32; ++n) v[n >> 2][n & 3] = mine >> n & 1 ? -INFINITY : v[n >> 2][n & 3];
+        for (int j = 0; j < 8; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(own + 1024 * j);
+          v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
+        }
       }
       float m = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         m = fmaxf(m, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
-      m = quad_max(m);
-      const float base = m == -INFINITY ? 0.f : m;
+      m = part_ref(quad_max(m), c);
+      const float minus = m == -INFINITY ? 0.f : -m;
       float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += __builtin_amdgcn_exp2f((v[j][e] - base) * c);
+        for (int e = 0; e < 4; ++e) s[e] += __builtin_amdgcn_exp2f(fmaf(v[j][e], c, minus));
       const float sum = quad_sum((s[0] + s[1]) + (s[2] + s[3]));
       if (g == 0) red[wn * TB + row] = {m, sum};
     }
     __syncthreads();
     const int t = threadIdx.x;
-    if (m0 + t < M) part[n0 / TB * M + m0 + t] = part_join(red[t], red[TB + t], c);
+    if (m0 + t < M) part[n0 / TB * M + m0 + t] = part_join(red[t], red[TB + t], 1.f);
   }
 };
 
@@ -169,7 +180,7 @@ struct GradHooks {
       r.z = g;
       if (g != 0.f && f != 0.f) {
         r.x = g * f;
-        r.y = fmaf(info[RI_M], c, info[RI_LOG]);
+        r.y = info[RI_M] + info[RI_LOG];
       }
     }
     reinterpret_cast<float4*>(extra + TileMarks::BYTES)[threadIdx.x] = r;
@@ -180,7 +191,6 @@ struct GradHooks {
                                         int64_t M, int64_t N, int64_t m0, int64_t n0) const {
     const int lane = threadIdx.x & 63, wm = threadIdx.x >> 7;
     const float4* consts = reinterpret_cast<const float4*>(extra + TileMarks::BYTES);
-    const bool edge = n0 + TB > N;
     float factor[8], log_rest[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -194,15 +204,14 @@ struct GradHooks {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         v[e] = factor[i] * __builtin_amdgcn_exp2f(fmaf(v[e], c, -log_rest[i]));
-      if (edge)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = n0 + col + e < N ? v[e] : 0.f;
     };
     tile_epilogue<ALODLM_EPI_STORE, 256, false>(lds, grad, D, ldd, nullptr, 0, rows, columns, m0, n0,
                                                 1.f, nullptr, 0);
-    // the known tokens' own, behind the tile's stores
+    // the known tokens' own and the padding, behind the tile's stores
     __syncthreads();
     const int64_t row = m0 + threadIdx.x;
+    if (n0 + TB > N && row < rows)
+      for (int64_t at = N; at < columns; ++at) reinterpret_cast<bf16_t*>(D)[row * ldd + at] = 0;
     if (row >= M) return;
     const float own_up = consts[threadIdx.x].z;
     const uint32_t* bits = reinterpret_cast<const uint32_t*>(extra) + 8 * threadIdx.x;
@@ -251,28 +260,45 @@ copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, int64_t w
 }
 
 // out [rows, width] = up.all() * (the planes' sum + D's last `rest` columns times the
-// weight's last `rest` rows, which no product took), rounded once.
-template <typename T, int VEC>
+// weight's last `rest` rows, which no product took), rounded once.  GROUPS of threads take
+// every GROUPS-th plane each (many planes of few rows: a thread would wait for one after the
+// other), their sums are added in order.
+template <typename T, int VEC, int GROUPS>
 __global__ void __launch_bounds__(256)
 finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t rows, int64_t width,
                       Upstream up, const T* __restrict__ D, int64_t ldd, const T* __restrict__ weight,
                       int64_t ldw, int rest, T* __restrict__ out) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
-  if (at >= width) return;
+  constexpr int LANES = 256 / GROUPS;
+  __shared__ float shared[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? LANES * VEC : 1];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int64_t at = ((int64_t)blockIdx.x * LANES + lane) * VEC;
+  const bool inside = at < width;
   const float scale = up.all();
   const int64_t plane = rows * width;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const float* src = planes + row * width + at;
     float s[VEC] = {};
-#pragma unroll 4
-    for (int64_t p = 0; p < count; ++p) {
-      if constexpr (VEC == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src + p * plane);
-        s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
-      } else {
-        s[0] += src[p * plane];
+    if (inside)
+#pragma unroll 8
+      for (int64_t p = group; p < count; p += GROUPS) {
+        if constexpr (VEC == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src + p * plane);
+          s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+        } else {
+          s[0] += src[p * plane];
+        }
       }
+    if constexpr (GROUPS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) shared[group][lane * VEC + e] = s[e];
+      __syncthreads();
+      if (group) continue;
+      for (int n = 1; n < GROUPS; ++n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += shared[n][lane * VEC + e];
     }
+    if (!inside) continue;
     for (int t = 0; t < rest; ++t) {
       const float d = Elem<T>::load(D, row * ldd + t);
 #pragma unroll
@@ -295,17 +321,26 @@ dim3 row_grid(int64_t width, int64_t rows) {
   return dim3((unsigned)ceil_div(width, 256), (unsigned)(rows < 65535 ? rows : 65535));
 }
 
+template <typename T, int VEC>
+void finish_columns(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
+                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, T* out,
+                    hipStream_t st) {
+  if (count >= 16)
+    finish_product_kernel<T, VEC, 16><<<row_grid(ceil_div(width, VEC) * 16, rows), 256, 0, st>>>(
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, out);
+  else
+    finish_product_kernel<T, VEC, 1><<<row_grid(ceil_div(width, VEC), rows), 256, 0, st>>>(
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, out);
+}
+
 template <typename T>
 void finish_product(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
                     const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, T* out,
                     hipStream_t st) {
-  const bool vec = width % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0;
-  if (vec)
-    finish_product_kernel<T, 4><<<row_grid(width / 4, rows), 256, 0, st>>>(planes, count, rows, width, up, D, ldd,
-                                                                           weight, ldw, rest, out);
+  if (width % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0)
+    finish_columns<T, 4>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, out, st);
   else
-    finish_product_kernel<T, 1><<<row_grid(width, rows), 256, 0, st>>>(planes, count, rows, width, up, D, ldd,
-                                                                       weight, ldw, rest, out);
+    finish_columns<T, 1>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, out, st);
 }
 
 // Which bf16 tiles a product [M, N] over K runs on and how its K is split: the least of
@@ -436,7 +471,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
       p.planes = (p.pieces - 1) * few_f32_planes(p.piece, H) + few_f32_planes(last, H);
       if (d_hidden) p.sums = room(p.planes * R * H);
     } else if (d_hidden) {
-      const bool large = R >= 256 && H >= 256;
+      const bool large = H >= 256;
       p.hidden_split = p.regular ? split_product(R, H, p.piece, large, false, true) : Split{true, 1};
       p.last_split = p.regular && whole ? split_product(R, H, whole, large, false, true) : Split{true, 1};
       p.planes = (p.pieces - 1) * p.hidden_split.planes + (whole ? p.last_split.planes : 0);
@@ -536,6 +571,15 @@ template <typename T> struct Call {
         ALODLM_CHECK_LAUNCH("linear_loss_logits");
         return ALODLM_OK;
       }
+    if constexpr (sizeof(T) == 2)
+      // 256 rows of tiles at once, where the dispatch would take two of 128
+      if (p.regular && R > 128 && R < 256 && n >= 256 * 128) {
+        int64_t count = 1;
+        gemm_dl_launch(deep_hidden, deep_ldh, 1, w, ld, 1, out, to, nullptr, 0, R, n, p.deep, 1.f,
+                       ALODLM_EPI_STORE_F32, nullptr, 1, &count, 0, st);
+        ALODLM_CHECK_LAUNCH("linear_loss_logits");
+        return ALODLM_OK;
+      }
     return alodlm_gemm(deep_hidden, deep_ldh, 1, w, ld, 1, out, to, nullptr, 0, R, n, p.deep, 1.f,
                        p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE, dtype, gemm(), st);
   }
@@ -570,7 +614,8 @@ int forward(Call<T>& a, const KnownRows& k, const GivenRows& given, float c, int
     }
     ALODLM_CHECK_LAUNCH("linear_loss");
   }
-  known_finish_launch<float>(k, given, whole ? logits : nullptr, ld, part, p.parts, a.R, c, reduction, loss, a.st);
+  known_finish_launch<float>(k, given, whole ? logits : nullptr, ld, part, p.parts, a.R, c, p.tiles,
+                             reduction, loss, a.st);
   ALODLM_CHECK_LAUNCH("linear_loss");
   return ALODLM_OK;
 }
@@ -719,7 +764,7 @@ extern "C" int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* w
   const GivenRows given = {targets, ids, log_q, ignore, (int)known, (int)vocab, rest != 0};
   const float c = inv_temperature * VL_LOG2E;
   if (rows == 0) {
-    known_finish_launch<float>(k, given, nullptr, 0, nullptr, 0, 0, c, reduction, loss, st);
+    known_finish_launch<float>(k, given, nullptr, 0, nullptr, 0, 0, c, false, reduction, loss, st);
     ALODLM_CHECK_LAUNCH("linear_loss");
     return ALODLM_OK;
   }

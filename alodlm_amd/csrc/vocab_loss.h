@@ -10,8 +10,8 @@
 //   dloss / dz = Q p - [q at the known] - [q_r s_r elsewhere]
 //              = (Q p_r - q_r) s_r   at a token that is not known: one factor a row,
 //                Q p - q             at a known one: one value a row and known token.
-// Sums are in base 2, relative to the largest logit: 2^((z - m) c) of raw logits z, c =
-// log2 e / T.
+// Sums are in base 2 with c = log2 e / T: 2^((z - m) c) of raw logits z relative to the largest
+// m, or, where logits come from the matrix cores, 2^(z c - K) relative to a whole number K.
 #pragma once
 
 #include "common.h"
@@ -59,10 +59,12 @@ struct GivenRows {
 };
 
 // A part of a row's sum over the tokens that are not known: its largest raw logit m and
-// sum 2^((z - m) c); -inf and 0 where no token can be (or none is there).
+// sum 2^((z - m) c), or K (in m) and sum 2^(z c - K); -inf and 0 where no token can be (or
+// none is there).  Joined with c, or 1 for the latter.
 struct Part {
   float m, sum;
 };
+__device__ __forceinline__ float part_ref(float largest, float c) { return ceilf(largest * c); }
 __device__ __forceinline__ Part part_join(const Part& a, const Part& b, float c) {
   const float to = fmaxf(a.m, b.m), base = to == -INFINITY ? 0.f : to;
   // what is -inf weighs 0 (NaN stays)
@@ -102,10 +104,11 @@ void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, 
                       hipStream_t st);
 // Losses and the gradient's factors from `parts` parts a row, and the reduced loss.  With
 // whole logits [rows, vocab] in memory (else NULL) the known tokens need no preparation.
+// `scaled`: the parts' reference is a whole number K, and RI_M is then one too.
 template <typename T>
 void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* logits, int64_t ld,
-                         const Part* part, int64_t parts, int64_t rows, float c, int reduction,
-                         float* loss, hipStream_t st);
+                         const Part* part, int64_t parts, int64_t rows, float c, bool scaled,
+                         int reduction, float* loss, hipStream_t st);
 // dlogits (TO, row stride ldo; columns [width, padded) and rows [rows, padded_rows) zero) of
 // logits [rows, width], columns first .. of the vocabulary; may be in place.
 template <typename TI, typename TO>

@@ -283,8 +283,9 @@ row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int wid
 // ---------------------------------------------------------------------------
 constexpr int FIN_ROWS = 16, FIN_LANES = 64;
 
-// GIVEN: the known tokens come from the caller, their logits from `logits`.
-template <typename T, bool GIVEN>
+// GIVEN: the known tokens come from the caller, their logits from `logits`.  SCALED: the
+// references are whole exponents.
+template <typename T, bool GIVEN, bool SCALED>
 __global__ void __launch_bounds__(FIN_ROWS * FIN_LANES)
 known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, int64_t ld,
                     const Part* __restrict__ part, int64_t parts, int64_t rows, float c,
@@ -293,6 +294,8 @@ known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, 
   __shared__ __attribute__((aligned(16))) int ids[GIVEN ? FIN_ROWS : 1][VL_MAX_KNOWN];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = k.known;
   const bool cross = given.targets != nullptr;
+  const float step = SCALED ? 1.f : c;  // of differences of references
+  auto exponent = [&](float z, float ref) { return SCALED ? fmaf(z, c, -ref) : (z - ref) * c; };
   const int64_t row = (int64_t)blockIdx.x * FIN_ROWS + wave;
   RowKnown r;
   float z[HELD];
@@ -328,7 +331,7 @@ known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, 
     Part a = {-INFINITY, 0.f};
     if (at < rows)
 #pragma unroll 4
-      for (int64_t p = l; p < parts; p += FIN_LANES) a = part_join(a, part[p * rows + at], c);
+      for (int64_t p = l; p < parts; p += FIN_LANES) a = part_join(a, part[p * rows + at], step);
     red[n][l] = a;
   }
   __syncthreads();
@@ -336,22 +339,22 @@ known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, 
   const Part mine = red[wave][lane];
   float m = wave_max(mine.m);
   const float base = m == -INFINITY ? 0.f : m;
-  const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * c));
+  const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * step));
   const bool others = !(s_rest == 0.f);  // a token that is not known can be (or NaN)
   const float m_rest = m;
   // the known tokens join
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) m = fmaxf(m, z[j]);
+  for (int j = 0; j < HELD; ++j) m = fmaxf(m, SCALED ? part_ref(z[j], c) : z[j]);
   m = wave_max(m);
   const bool none = m == -INFINITY;
   const float top = none ? 0.f : m;
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < HELD; ++j)
-    if (r.id[j] != VL_NONE) s += __builtin_amdgcn_exp2f((z[j] - top) * c);
-  s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * c) : 0.f);
+    if (r.id[j] != VL_NONE) s += __builtin_amdgcn_exp2f(exponent(z[j], top));
+  s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * step) : 0.f);
   const float log_s = log2f(s);
-  const float log_rest = others ? (m_rest - top) * c + log2f(s_rest) : -INFINITY;
+  const float log_rest = others ? (m_rest - top) * step + log2f(s_rest) : -INFINITY;
   const bool empty = none && s == 0.f;  // no token can be
   const float p_rest = others ? __builtin_amdgcn_exp2f(log_rest - log_s) : 0.f;
   const float q_rest = others ? r.q_rest : 0.f;
@@ -363,10 +366,10 @@ known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, 
     const int64_t at = row * K + r.place[j];
     if constexpr (GIVEN) k.ids[at] = r.id[j];
     if (r.id[j] == VL_NONE) continue;
-    const float log_p = (z[j] - top) * c - log_s;
+    const float own = exponent(z[j], top), log_p = own - log_s;
     if (cross) {
       // -ln p = ln(1 + others / own): small losses keep their digits
-      const float x = VL_LN2 * (log_rest - (z[j] - top) * c);
+      const float x = VL_LN2 * (log_rest - own);
       sum = !others ? 0.f : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
       if (!(z[j] < INFINITY)) sum = NAN;
     } else if (r.q[j] != 0.f) {
@@ -560,18 +563,20 @@ template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, i
 
 template <typename T>
 void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* logits, int64_t ld,
-                         const Part* part, int64_t parts, int64_t rows, float c, int reduction,
-                         float* loss, hipStream_t st) {
+                         const Part* part, int64_t parts, int64_t rows, float c, bool scaled,
+                         int reduction, float* loss, hipStream_t st) {
   float* each = reduction == VL_EACH ? loss : nullptr;
   const unsigned grid = ceil_div_u(rows, FIN_ROWS), threads = FIN_ROWS * FIN_LANES;
   if (rows > 0 && logits)
-    known_finish_kernel<T, true><<<grid, threads, 0, st>>>(k, given, logits, ld, part, parts, rows, c, each);
+    known_finish_kernel<T, true, false><<<grid, threads, 0, st>>>(k, given, logits, ld, part, parts, rows, c, each);
+  else if (rows > 0 && scaled)
+    known_finish_kernel<T, false, true><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
   else if (rows > 0)
-    known_finish_kernel<T, false><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
+    known_finish_kernel<T, false, false><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
   if (!each) known_reduce_kernel<<<1, 1024, 0, st>>>(k, rows, reduction == VL_MEAN, loss);
 }
 template void known_finish_launch<float>(const KnownRows&, const GivenRows&, const float*, int64_t, const Part*,
-                                         int64_t, int64_t, float, int, float*, hipStream_t);
+                                         int64_t, int64_t, float, bool, int, float*, hipStream_t);
 
 template <typename TI, typename TO>
 void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
@@ -624,8 +629,8 @@ extern "C" int alodlm_distillation(const void* logits, int64_t ld, const int64_t
   Part* part = reinterpret_cast<Part*>(workspace);
   ALODLM_DISPATCH(dtype, T, {
     if (rows > 0) row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, nullptr, given, c, chunks, part, st);
-    known_finish_launch<T>(k, given, rows > 0 ? (const T*)logits : nullptr, ld, part, chunks, rows, c, reduction,
-                           loss, st);
+    known_finish_launch<T>(k, given, rows > 0 ? (const T*)logits : nullptr, ld, part, chunks, rows, c, false,
+                           reduction, loss, st);
   });
   ALODLM_CHECK_LAUNCH("distillation");
   return ALODLM_OK;
