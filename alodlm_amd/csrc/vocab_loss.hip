@@ -416,17 +416,19 @@ known_reduce_kernel(KnownRows k, int64_t rows, int mean, float* __restrict__ los
 }
 
 // ---------------------------------------------------------------------------
-// Gradients: a stream.  The known tokens' are written again behind a barrier.
+// Gradients: a stream.  The known tokens' are written again behind a barrier.  The last rows
+// come first: the forward read them last, and the last-level cache may hold them.
 // ---------------------------------------------------------------------------
-constexpr int GRAD_PIECES = THREADS * 4;
+constexpr int GRAD_PIECES = THREADS * 2;
 
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(THREADS)
 row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t first, KnownRows k,
                  float c, Upstream up, TO* out, int64_t ldo, int padded, int chunks) {
   constexpr int N = 8;  // tokens a thread takes at a time
-  const int64_t row = blockIdx.x / chunks;
-  const int chunk = (int)(blockIdx.x % chunks);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = block / chunks;
+  const int chunk = (int)(block % chunks);
   TO* o = out + row * ldo;
   // pieces by the gradient's 16-byte (bf16) or 32-byte (float) alignment
   const int head = min((int)(-(intptr_t)o & (8 * (int)sizeof(TO) - 1)) / (int)sizeof(TO), padded);
