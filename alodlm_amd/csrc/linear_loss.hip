@@ -420,7 +420,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   const int64_t es = p.half ? 2 : 4;
   const bool computes = !(backward && p.keep);  // the logits
   p.copy_weight = p.regular && computes && p.deep != H;
-  p.copy_hidden = p.regular && ((computes && p.deep != H) || (backward && d_weight && p.deep_rows != R));
+  p.copy_hidden = p.copy_weight;
   // bytes of a token
   int64_t most = V;
   auto limit = [&](int64_t bytes) {
@@ -451,6 +451,8 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
     gemm = n > gemm ? n : gemm;
   };
   const int f32_out = p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
+  if (backward && d_weight && p.regular && p.deep_rows != R)  // whole 32 rows for the large tiles
+    for (const int64_t n : {p.piece, up_to(last, 32)}) p.copy_hidden |= split_product(n, H, R, true, true, false).large;
   if (p.copy_hidden) p.hidden = room(ceil_div(p.deep_rows * p.deep * es, 4));
   if (p.copy_weight) p.weight = room(ceil_div(p.piece * p.deep * es, 4));
   if (computes && !p.tiles) {
@@ -609,7 +611,7 @@ int forward(Call<T>& a, const KnownRows& k, const GivenRows& given, float c, int
       float* to = p.keep ? logits + first : logits;
       LL_CALL(a.logits(first, n, to));
       ld = a.logits_ld(n);
-      row_stats_launch<float>(to, ld, a.R, n, first, whole ? nullptr : &k, given, c, p.chunks,
+      row_stats_launch<float>(to, ld, a.R, n, first, k, given, !whole, c, p.chunks,
                               part + i * p.chunks * a.R, a.st);
     }
     ALODLM_CHECK_LAUNCH("linear_loss");

@@ -95,13 +95,13 @@ struct Upstream {
 // The rows' known tokens into k, in ascending order.
 void known_prepare_launch(const KnownRows& k, const GivenRows& given, int64_t rows, hipStream_t st);
 // The row sums of logits [rows, width], columns first .. of the vocabulary, in `chunks`
-// parts a row at part[chunk * rows + row].  With known tokens that are prepared, their
-// logits go to k; else `given` names them.
+// parts a row at part[chunk * rows + row].  `prepared`: k has the known tokens, and their
+// logits go there; else `given` names them.
 int64_t row_stats_chunks(int64_t rows, int64_t width);
 template <typename T>
 void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows* k, const GivenRows& given, float c, int64_t chunks, Part* part,
-                      hipStream_t st);
+                      const KnownRows& k, const GivenRows& given, bool prepared, float c, int64_t chunks,
+                      Part* part, hipStream_t st);
 // Losses and the gradient's factors from `parts` parts a row, and the reduced loss.  With
 // whole logits [rows, vocab] in memory (else NULL) the known tokens need no preparation.
 // `scaled`: the parts' reference is a whole number K, and RI_M is then one too.

@@ -283,12 +283,33 @@ row_stats_kernel(const T* __restrict__ logits, int64_t ld, int64_t rows, int wid
 // ---------------------------------------------------------------------------
 constexpr int FIN_ROWS = 16, FIN_LANES = 64;
 
+// The sum or mean of the rows' losses, by a workgroup of 1024 threads in a fixed order.
+__device__ __forceinline__ void reduce_losses(const KnownRows& k, int64_t rows, bool mean, float* loss) {
+  __shared__ double total[16], count[16];
+  double t = 0.0, n = 0.0;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    t += (double)k.info[8 * r + RI_LOSS];
+    n += (double)k.info[8 * r + RI_COUNTED];
+  }
+  t = wave_sum_d(t);
+  n = wave_sum_d(n);
+  if ((threadIdx.x & 63) == 0) { total[threadIdx.x >> 6] = t; count[threadIdx.x >> 6] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) { t += total[w]; n += count[w]; }
+    const double by = mean ? fmax(n, 1.0) : 1.0;
+    loss[0] = (float)(t / by);
+    k.call[0] = (float)(1.0 / by);
+  }
+}
+
 // GIVEN: the known tokens come from the caller, their logits from `logits`.  SCALED: the
 // references are whole exponents.
 template <typename T, bool GIVEN, bool SCALED>
 __global__ void __launch_bounds__(FIN_ROWS * FIN_LANES)
 known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, int64_t ld,
-                    const Part* __restrict__ part, int64_t parts, int64_t rows, float c,
+                    const Part* __restrict__ part, int64_t parts, int64_t rows, float c, int reduction,
                     float* __restrict__ loss) {
   __shared__ Part red[FIN_ROWS][FIN_LANES + 1];
   __shared__ __attribute__((aligned(16))) int ids[GIVEN ? FIN_ROWS : 1][VL_MAX_KNOWN];
@@ -335,84 +356,74 @@ known_finish_kernel(KnownRows k, GivenRows given, const T* __restrict__ logits, 
     red[n][l] = a;
   }
   __syncthreads();
-  if (row >= rows) return;
-  const Part mine = red[wave][lane];
-  float m = wave_max(mine.m);
-  const float base = m == -INFINITY ? 0.f : m;
-  const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * step));
-  const bool others = !(s_rest == 0.f);  // a token that is not known can be (or NaN)
-  const float m_rest = m;
-  // the known tokens join
+  if (row < rows) {
+    const Part mine = red[wave][lane];
+    float m = wave_max(mine.m);
+    const float base = m == -INFINITY ? 0.f : m;
+    const float s_rest = wave_sum(mine.sum * __builtin_amdgcn_exp2f((mine.m - base) * step));
+    const bool others = !(s_rest == 0.f);  // a token that is not known can be (or NaN)
+    const float m_rest = m;
+    // the known tokens join
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) m = fmaxf(m, SCALED ? part_ref(z[j], c) : z[j]);
-  m = wave_max(m);
-  const bool none = m == -INFINITY;
-  const float top = none ? 0.f : m;
-  float s = 0.f;
+    for (int j = 0; j < HELD; ++j) m = fmaxf(m, SCALED ? part_ref(z[j], c) : z[j]);
+    m = wave_max(m);
+    const bool none = m == -INFINITY;
+    const float top = none ? 0.f : m;
+    float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < HELD; ++j)
-    if (r.id[j] != VL_NONE) s += __builtin_amdgcn_exp2f(exponent(z[j], top));
-  s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * step) : 0.f);
-  const float log_s = log2f(s);
-  const float log_rest = others ? (m_rest - top) * step + log2f(s_rest) : -INFINITY;
-  const bool empty = none && s == 0.f;  // no token can be
-  const float p_rest = others ? __builtin_amdgcn_exp2f(log_rest - log_s) : 0.f;
-  const float q_rest = others ? r.q_rest : 0.f;
-  const float mass = r.mass + q_rest;
-  float sum = 0.f;
+    for (int j = 0; j < HELD; ++j)
+      if (r.id[j] != VL_NONE) s += __builtin_amdgcn_exp2f(exponent(z[j], top));
+    s = wave_sum(s) + (others ? s_rest * __builtin_amdgcn_exp2f((m_rest - top) * step) : 0.f);
+    const float log_s = log2f(s);
+    const float log_rest = others ? (m_rest - top) * step + log2f(s_rest) : -INFINITY;
+    const bool empty = none && s == 0.f;  // no token can be
+    const float p_rest = others ? __builtin_amdgcn_exp2f(log_rest - log_s) : 0.f;
+    const float q_rest = others ? r.q_rest : 0.f;
+    const float mass = r.mass + q_rest;
+    float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < HELD; ++j) {
-    if (lane + 64 * j >= K) continue;
-    const int64_t at = row * K + r.place[j];
-    if constexpr (GIVEN) k.ids[at] = r.id[j];
-    if (r.id[j] == VL_NONE) continue;
-    const float own = exponent(z[j], top), log_p = own - log_s;
-    if (cross) {
-      // -ln p = ln(1 + others / own): small losses keep their digits
-      const float x = VL_LN2 * (log_rest - own);
-      sum = !others ? 0.f : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
-      if (!(z[j] < INFINITY)) sum = NAN;
-    } else if (r.q[j] != 0.f) {
-      sum += r.q[j] * (r.log_q[j] - VL_LN2 * log_p);
+    for (int j = 0; j < HELD; ++j) {
+      if (lane + 64 * j >= K) continue;
+      const int64_t at = row * K + r.place[j];
+      if constexpr (GIVEN) k.ids[at] = r.id[j];
+      if (r.id[j] == VL_NONE) continue;
+      const float own = exponent(z[j], top), log_p = own - log_s;
+      if (cross) {
+        // -ln p = ln(1 + others / own): small losses keep their digits
+        const float x = VL_LN2 * (log_rest - own);
+        sum = !others ? 0.f : x > 0.f ? x + log1pf(expf(-x)) : log1pf(expf(x));
+        if (!(z[j] < INFINITY)) sum = NAN;
+      } else if (r.q[j] != 0.f) {
+        sum += r.q[j] * (r.log_q[j] - VL_LN2 * log_p);
+      }
+      const float p = __builtin_amdgcn_exp2f(log_p);
+      k.weight[at] = r.bad ? NAN : empty ? 0.f : cross ? -p_rest : fmaf(mass, p, -r.q[j]);
     }
-    const float p = __builtin_amdgcn_exp2f(log_p);
-    k.weight[at] = r.bad ? NAN : empty ? 0.f : cross ? -p_rest : fmaf(mass, p, -r.q[j]);
+    sum = wave_sum(sum);
+    if (q_rest != 0.f) sum += q_rest * (logf(q_rest) - VL_LN2 * (log_rest - log_s));
+    if (empty) sum = r.mass != 0.f ? INFINITY : 0.f;
+    if (!r.counted) sum = 0.f;
+    if (r.bad) sum = NAN;
+    if (lane == 0) {
+      float* info = k.info + 8 * row;
+      info[RI_M] = top;
+      info[RI_LOG] = log_rest;
+      info[RI_FACTOR] = r.bad ? NAN : !r.counted || !others ? 0.f : fmaf(mass, p_rest, -q_rest);
+      info[RI_LOSS] = sum;
+      if (reduction == VL_EACH) loss[row] = sum;
+    }
   }
-  sum = wave_sum(sum);
-  if (q_rest != 0.f) sum += q_rest * (logf(q_rest) - VL_LN2 * (log_rest - log_s));
-  if (empty) sum = r.mass != 0.f ? INFINITY : 0.f;
-  if (!r.counted) sum = 0.f;
-  if (r.bad) sum = NAN;
-  if (lane == 0) {
-    float* info = k.info + 8 * row;
-    info[RI_M] = top;
-    info[RI_LOG] = log_rest;
-    info[RI_FACTOR] = r.bad ? NAN : !r.counted || !others ? 0.f : fmaf(mass, p_rest, -q_rest);
-    info[RI_LOSS] = sum;
-    if (loss) loss[row] = sum;
+  // one workgroup's rows are all there are (more take a launch of their own: the last
+  // workgroup adding up the others' rows needs device-wide fences, which took 70 us of 256)
+  if (reduction != VL_EACH && gridDim.x == 1) {
+    __syncthreads();
+    reduce_losses(k, rows, reduction == VL_MEAN, loss);
   }
 }
 
-// The sum or mean of the rows' losses, in a fixed order.
 __global__ void __launch_bounds__(1024)
 known_reduce_kernel(KnownRows k, int64_t rows, int mean, float* __restrict__ loss) {
-  __shared__ double total[16], count[16];
-  double t = 0.0, n = 0.0;
-#pragma unroll 4
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-    t += (double)k.info[8 * r + RI_LOSS];
-    n += (double)k.info[8 * r + RI_COUNTED];
-  }
-  t = wave_sum_d(t);
-  n = wave_sum_d(n);
-  if ((threadIdx.x & 63) == 0) { total[threadIdx.x >> 6] = t; count[threadIdx.x >> 6] = n; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) { t += total[w]; n += count[w]; }
-    const double by = mean ? fmax(n, 1.0) : 1.0;
-    loss[0] = (float)(t / by);
-    k.call[0] = (float)(1.0 / by);
-  }
+  reduce_losses(k, rows, mean, loss);
 }
 
 // ---------------------------------------------------------------------------
@@ -548,34 +559,37 @@ int64_t row_stats_chunks(int64_t rows, int64_t width) {
 
 template <typename T>
 void row_stats_launch(const T* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
-                      const KnownRows* k, const GivenRows& given, float c, int64_t chunks, Part* part,
-                      hipStream_t st) {
+                      const KnownRows& k, const GivenRows& given, bool prepared, float c, int64_t chunks,
+                      Part* part, hipStream_t st) {
   const int64_t chunk_width = ((width + chunks - 1) / chunks + 63) / 64 * 64;
   const size_t lds = 4 * (size_t)((chunk_width + 2 * Piece<T>::N + 31) / 32 + 1);
   const unsigned grid = (unsigned)(rows * chunks);
-  if (k)
-    row_stats_kernel<T, true><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, *k, given, c,
+  if (prepared)
+    row_stats_kernel<T, true><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, k, given, c,
                                                           (int)chunks, (int)chunk_width, part);
   else
-    row_stats_kernel<T, false><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, KnownRows{},
-                                                           given, c, (int)chunks, (int)chunk_width, part);
+    row_stats_kernel<T, false><<<grid, THREADS, lds, st>>>(logits, ld, rows, (int)width, first, k, given, c,
+                                                           (int)chunks, (int)chunk_width, part);
 }
-template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows*,
-                                      const GivenRows&, float, int64_t, Part*, hipStream_t);
+template void row_stats_launch<float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
+                                      const GivenRows&, bool, float, int64_t, Part*, hipStream_t);
 
 template <typename T>
 void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* logits, int64_t ld,
                          const Part* part, int64_t parts, int64_t rows, float c, bool scaled,
                          int reduction, float* loss, hipStream_t st) {
-  float* each = reduction == VL_EACH ? loss : nullptr;
   const unsigned grid = ceil_div_u(rows, FIN_ROWS), threads = FIN_ROWS * FIN_LANES;
   if (rows > 0 && logits)
-    known_finish_kernel<T, true, false><<<grid, threads, 0, st>>>(k, given, logits, ld, part, parts, rows, c, each);
+    known_finish_kernel<T, true, false><<<grid, threads, 0, st>>>(k, given, logits, ld, part, parts, rows, c,
+                                                                  reduction, loss);
   else if (rows > 0 && scaled)
-    known_finish_kernel<T, false, true><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
+    known_finish_kernel<T, false, true><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c,
+                                                                  reduction, loss);
   else if (rows > 0)
-    known_finish_kernel<T, false, false><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c, each);
-  if (!each) known_reduce_kernel<<<1, 1024, 0, st>>>(k, rows, reduction == VL_MEAN, loss);
+    known_finish_kernel<T, false, false><<<grid, threads, 0, st>>>(k, given, nullptr, 0, part, parts, rows, c,
+                                                                  reduction, loss);
+  if (reduction != VL_EACH && grid != 1)
+    known_reduce_kernel<<<1, 1024, 0, st>>>(k, rows, reduction == VL_MEAN, loss);
 }
 template void known_finish_launch<float>(const KnownRows&, const GivenRows&, const float*, int64_t, const Part*,
                                          int64_t, int64_t, float, bool, int, float*, hipStream_t);
@@ -630,7 +644,7 @@ extern "C" int alodlm_distillation(const void* logits, int64_t ld, const int64_t
   const float c = inv_temperature * VL_LOG2E;
   Part* part = reinterpret_cast<Part*>(workspace);
   ALODLM_DISPATCH(dtype, T, {
-    if (rows > 0) row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, nullptr, given, c, chunks, part, st);
+    if (rows > 0) row_stats_launch<T>((const T*)logits, ld, rows, vocab, 0, k, given, false, c, chunks, part, st);
     known_finish_launch<T>(k, given, rows > 0 ? (const T*)logits : nullptr, ld, part, chunks, rows, c, false,
                            reduction, loss, st);
   });

@@ -225,20 +225,20 @@ def _linear(hidden, weight, targets, ids, log_q, inv_temperature, ignore_index, 
     w, ldw = _aligned_rows(weight)
     code = _lib.dtype_code(h.dtype)
     state, kept, ws, _ = _linear_sizes(R, V, H, known, code, keep, True, True)
-    loss = _floats(() if reduction else R, dev)
-    state, ws = _floats(state, dev), _floats(ws, dev)
-    kept = _floats(kept, dev) if kept else None
+    loss, ws = _floats(() if reduction else R, dev), _floats(ws, dev)
+    saved = _floats(state + kept, dev)  # (the state's floats are whole 16 bytes)
+    at = saved.data_ptr()
     call_on(dev, "alodlm_linear_loss", h.data_ptr(), ldh, w.data_ptr(), ldw, ptr(targets), ptr(ids),
             ptr(log_q), R, V, H, known, inv_temperature, ignore_index, rest, reduction, loss.data_ptr(),
-            state.data_ptr(), ptr(kept), ws.data_ptr(), code)
-    return loss, state, kept
+            at, at + 4 * state if kept else None, ws.data_ptr(), code)
+    return loss, saved
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, *args):
-        loss, *saved = _linear(hidden, weight, *args, keep=True)
-        ctx.save_for_backward(hidden, weight, *saved)
+        loss, saved = _linear(hidden, weight, *args, keep=True)
+        ctx.save_for_backward(hidden, weight, saved)
         ids = args[1]
         ctx.args = 1 if ids is None else ids.shape[1], args[3], args[6]
         return loss
@@ -246,7 +246,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        hidden, weight, state, kept = ctx.saved_tensors
+        hidden, weight, saved = ctx.saved_tensors
         (R, H), V, dev = hidden.shape, weight.shape[0], hidden.device
         h, ldh = _aligned_rows(hidden)
         w, ldw = _aligned_rows(weight)
@@ -255,10 +255,10 @@ class _Linear(torch.autograd.Function):
         dh = torch.empty(R, H, dtype=h.dtype, device=dev) if need_h else None
         # room for whole 32 rows: the kernels' tiles
         dw = (torch.empty if R else torch.zeros)(-(-V // 32) * 32, H, dtype=h.dtype, device=dev) if need_w else None
-        ws = _floats(_linear_sizes(R, V, H, ctx.args[0], code, kept is not None, need_h, need_w)[3], dev)
-        up = _upstream(d_loss)
-        call_on(dev, "alodlm_linear_loss_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, state.data_ptr(),
-                ptr(kept), up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
+        state, kept, _, ws = _linear_sizes(R, V, H, ctx.args[0], code, True, need_h, need_w)
+        ws, up, at = _floats(ws, dev), _upstream(d_loss), saved.data_ptr()
+        call_on(dev, "alodlm_linear_loss_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, at,
+                at + 4 * state if kept else None, up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
         return (dh, None if dw is None else dw[:V]) + (None,) * 7
 
 
