@@ -20,6 +20,7 @@
 // gradient is anywhere: it is an operand of the bf16 matrix cores.  A reduced loss's upstream
 // gradient is applied to the products, not to D: of a row far from its target, D is then -1
 // there, which is exact.
+#include "few_bf16.h"
 #include "few_f32.h"
 #include "gemm_dl_tile.h"
 #include "gemm_mid.h"
@@ -396,8 +397,8 @@ struct Plan {
   int64_t part, logits, D, hidden, weight, sums, rows, gemm, total;
 };
 
-// Whether a piece's logits come from the 128-column tiles of few rows, which leave rows of
-// the piece's own length, and the row stride of logits in memory.
+// Whether a piece's logits come from few_bf16.hip, which leaves rows of the piece's own
+// length, and the row stride of logits in memory.
 bool few_logits(const Plan& p, int64_t R, int64_t n) {
   return p.regular && R <= FEW && n >= 128 * 256 && (!p.small || p.pieces == 1);
 }
@@ -568,8 +569,8 @@ template <typename T> struct Call {
     const T* w = piece_weight(first, n, ld);
     const int64_t to = logits_ld(n);
     if constexpr (sizeof(T) == 2)
-      if (few_logits(p, R, n) && n * ld < (1ll << 30)) {
-        gemm_mid_planes(deep_hidden, deep_ldh, 1, w, ld, 1, R, n, p.deep, 1, out, st);
+      if (few_logits(p, R, n)) {
+        few_bf16_logits(deep_hidden, deep_ldh, w, ld, R, n, p.deep, out, st);
         ALODLM_CHECK_LAUNCH("linear_loss_logits");
         return ALODLM_OK;
       }
