@@ -149,6 +149,8 @@ def _aligned_rows(t):
     to each other, and 16-byte aligned rows where a row is a whole number of 16 bytes."""
     rows, width = t.shape
     step = 16 // t.element_size()
+    if t.is_contiguous() and (t.data_ptr() % 16 == 0 or width % step):
+        return t, width
     if width == 1 or t.stride(1) == 1:
         stride = width if rows < 2 else t.stride(0)
         if stride >= width and (width % step or (stride % step == 0 and t.data_ptr() % 16 == 0)):
