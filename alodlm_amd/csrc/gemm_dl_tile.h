@@ -388,10 +388,12 @@ __device__ __forceinline__ void tile_epilogue(char* tile, Quad quad, void* C, in
 // What a product with an epilogue of its own passes to a kernel (`Epilogue` true): after(..)
 // takes the tile's sums by quad() and may use the stages' LDS behind a barrier of its own.
 // gemm_dl2_kernel's have more: before(..) runs while the first loads are under way (what it
-// stores to LDS every wave sees behind the loop), and EXTRA_LDS bytes behind TILE_LDS.
+// stores to LDS every wave sees behind the loop), EXTRA_LDS bytes behind TILE_LDS, and the
+// tile rows that are swept together.
 struct NoHooks {
   static constexpr bool Epilogue = false;
   static constexpr int EXTRA_LDS = 0;
+  static constexpr __device__ int group(int) { return 3; }
 };
 
 // The kernel.  Each wave's 128x128 tile is 8 x 8 blocks of 16x16; the 64
@@ -612,7 +614,7 @@ gemm_dl2_kernel(const bf16_t* __restrict__ A, int64_t lda, const bf16_t* __restr
   const int T = tiles_m * tiles_n;
   int t = blockIdx.x;
   if (T % 8 == 0) t = (t % 8) * (T / 8) + t / 8;
-  const int group = 3, per_group = group * tiles_n;
+  const int group = Hooks::group(tiles_m), per_group = group * tiles_n;
   const int g = t / per_group, first_m = g * group;
   const int gsize = (tiles_m - first_m) < group ? (tiles_m - first_m) : group;
   const int tm = first_m + (t % per_group) % gsize, tn = (t % per_group) / gsize;

@@ -84,6 +84,11 @@ struct TileMarks {
   }
 };
 
+// Tile rows that are swept together: all of them up to six, else three, as gemm_dl.hip's
+// products (a lone fourth row took the weight once more: 777 rows 1.62 -> 1.59 ms, 1000 rows of
+// width 4096 4.41 -> 4.30; of 16 tile rows, three together take 7.92 ms, four 7.96, 16 8.04).
+__device__ __forceinline__ int swept_rows(int tiles_m) { return tiles_m <= 6 ? tiles_m : 3; }
+
 // Forward tiles: parts of the rows' sums, and the known tokens' logits.  The parts' reference
 // is the largest exponent z c rounded up to a whole number K: 2^(z c - K) is one multiply-add
 // and one exponential, K is exact, and parts are joined by whole powers of two.  The values
@@ -93,6 +98,7 @@ struct TileMarks {
 struct SumHooks {
   static constexpr bool Epilogue = true;
   static constexpr int EXTRA_LDS = TileMarks::BYTES + 2 * TB * (int)sizeof(Part);
+  static __device__ int group(int tiles_m) { return swept_rows(tiles_m); }
   KnownRows k;
   float c;
   Part* part;     // [tiles][rows], of the piece
@@ -165,6 +171,7 @@ struct SumHooks {
 struct GradHooks {
   static constexpr bool Epilogue = true;
   static constexpr int EXTRA_LDS = TileMarks::BYTES + TB * 16;
+  static __device__ int group(int tiles_m) { return swept_rows(tiles_m); }
   KnownRows k;
   float c;
   Upstream up;
