@@ -187,8 +187,10 @@ struct GradHooks {
       const float f = info[RI_FACTOR];
       r.z = g;
       if (g != 0.f && f != 0.f) {
-        r.x = g * f;
-        r.y = info[RI_M] + info[RI_LOG];
+        // the whole part of the exponent joins the whole reference, where it is exact
+        const float whole = floorf(info[RI_LOG]);
+        r.x = g * f * __builtin_amdgcn_exp2f(whole - info[RI_LOG]);
+        r.y = info[RI_M] + whole;
       }
     }
     reinterpret_cast<float4*>(extra + TileMarks::BYTES)[threadIdx.x] = r;
@@ -437,6 +439,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   };
   if (backward && p.half) limit(2 * p.deep_rows);
   if (computes && !p.tiles && !p.small) limit(4 * R);
+  if (backward && p.few) limit(4 * few_f32_pad(R));
   if (p.copy_weight) limit(2 * p.deep);
   if (backward && d_weight && p.half && !p.regular) limit(4 * H);
   if (p.regular) {  // the 128x128 tiles' operands stay below 2 GiB
@@ -522,6 +525,7 @@ int check_linear(const char* what, const void* hidden, int64_t ldh, const void* 
                    "%s: row strides out of range", what);
   if (R > 0)
     ALODLM_CHECK_ARG(hidden && weight, "%s: the call lacks an array", what);
+  ALODLM_CHECK_ARG((R + 255) / 256 * ((V + 255) / 256) < VL_MOST_GROUPS, "%s: too many rows in one call", what);
   const int64_t step = dtype == ALODLM_BF16 ? 8 : 4;  // elements of 16 bytes
   if (R > 0 && H % step == 0)
     ALODLM_CHECK_ARG((((uintptr_t)hidden | (uintptr_t)weight) & 15) == 0 && ldh % step == 0 && ldw % step == 0,
@@ -780,7 +784,7 @@ extern "C" int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* w
   }
   const Plan p = make_plan(rows, vocab, width, dtype, kept != nullptr, false, false, false);
   ALODLM_CHECK_ARG(!kept || p.keep, "linear_loss: logits of this size are not kept");
-  ALODLM_CHECK_ARG(rows * p.chunks < (1ll << 31), "linear_loss: too many rows in one call");
+  ALODLM_CHECK_ARG(p.tiles || rows * p.chunks < VL_MOST_GROUPS, "linear_loss: too many rows in one call");
   if (dtype == ALODLM_BF16) {
     Call<bf16_t> a = {p, (const bf16_t*)hidden, ldh, (const bf16_t*)weight, ldw, rows, vocab, width, workspace,
                       dtype, st};

@@ -20,6 +20,7 @@
 #define VL_LOG2E 1.44269504088896341f
 #define VL_LN2 0.69314718055994531f
 #define VL_NONE 0x7fffffff  // no known token
+#define VL_MOST_GROUPS (1ll << 24)  // workgroups of 256 threads in a launch: fewer than 2^32 threads
 
 // What is kept of a call for its backward, in floats: 4 of the call, 8 of a row, and per
 // row and place its known tokens, each id once (VL_NONE elsewhere).  known_prepare puts

@@ -637,7 +637,7 @@ extern "C" int alodlm_distillation(const void* logits, int64_t ld, const int64_t
                    "distillation: the call lacks an array");
   ALODLM_CHECK_ARG((uintptr_t)workspace % 8 == 0, "distillation: workspace not 8-byte aligned");
   const int64_t chunks = rows > 0 ? row_stats_chunks(rows, vocab) : 0;
-  ALODLM_CHECK_ARG(rows * chunks < (1ll << 31), "distillation: too many rows in one call");
+  ALODLM_CHECK_ARG(rows * chunks < VL_MOST_GROUPS, "distillation: too many rows in one call");
   const hipStream_t st = as_stream(stream);
   const KnownRows k = known_rows(state, rows, known);
   const GivenRows given = {nullptr, ids, log_q, 0, (int)known, (int)vocab, rest != 0};
@@ -661,7 +661,7 @@ extern "C" int alodlm_distillation_bwd(const void* logits, int64_t ld, const flo
   ALODLM_CHECK_ARG(ld >= vocab, "distillation_bwd: rows overlap");
   if (rows == 0) return ALODLM_OK;
   ALODLM_CHECK_ARG(logits && state && d_loss && dlogits, "distillation_bwd: the call lacks an array");
-  ALODLM_CHECK_ARG(rows * ((vocab / 8 + GRAD_PIECES) / GRAD_PIECES) < (1ll << 31),
+  ALODLM_CHECK_ARG(rows * ((vocab / 8 + GRAD_PIECES) / GRAD_PIECES) < VL_MOST_GROUPS,
                    "distillation_bwd: too many rows in one call");
   const KnownRows k = known_rows(const_cast<float*>(state), rows, known);  // read only
   const Upstream up = {k.call, d_loss, reduction, 0, inv_temperature};

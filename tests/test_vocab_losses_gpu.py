@@ -278,7 +278,7 @@ def check_linear(hidden, weight, targets=None, ids=None, log_q=None, temperature
     leaves = [x for x in (h, w) if x.requires_grad]
     found = torch.autograd.grad(got, leaves, up) if leaves else []
     row = upstream(ids, reduction, up)
-    h64, w64 = hidden.double(), weight.double()
+    h64, w64 = hidden.detach().double(), weight.detach().double()
     losses, masses, tols = [], [], []
     dh, dh_far, dh_rms = (torch.zeros(R, H, dtype=torch.float64, device=DEV) for _ in range(3))
     dw, dw_far, dw_rms = (torch.zeros(V, H, dtype=torch.float64, device=DEV) for _ in range(3))
@@ -340,6 +340,66 @@ def test_logits_that_are_not_kept(R, V, H, dtype):
     hidden, weight, targets = factors(R, V, H, dtype)
     check_linear(hidden, weight, targets, reduction="mean")
     check_linear(hidden, weight, targets, reduction="none", temperature=0.7, grads=(True, False))
+
+
+@pytest.mark.parametrize("temperature", [0.004, 0.05, 40.0])
+@pytest.mark.parametrize("R,V", [(300, 120001), (90, 3000)])
+def test_linear_temperatures(R, V, temperature):
+    """Exponents of up to some thousands, and nearly flat ones.  (Logits of few values: the
+    sums' own error over the temperature stays small.)"""
+    log(f"linear temperature {temperature} {R} x {V}")
+    gen = generator(R)
+    hidden = torch.randint(-2, 3, (R, 64), generator=gen, device=DEV).to(BF16)
+    weight = (torch.randint(-2, 3, (V, 64), generator=gen, device=DEV) / 16).to(BF16)
+    targets = torch.randint(0, V, (R,), generator=gen, device=DEV)
+    targets[::2] = (hidden[::2].float() @ weight.float().T).argmax(-1)
+    ids, log_q = tokens(R, V, 5, gen, DEV)
+    check_linear(hidden, weight, targets, temperature=temperature)
+    check_linear(hidden, weight, ids=ids, log_q=log_q, temperature=temperature, reduction="none")
+
+
+def test_more_than_2_to_the_31_elements():
+    """Logits whose offsets pass 32 bits, and a weight whose offsets do: the last rows as by
+    themselves."""
+    log("vocabulary losses, long offsets")
+    R, V = 14200, 151936
+    gen = generator(5)
+    logits = torch.empty(R, V, dtype=BF16, device=DEV)
+    for r in range(0, R, 1000):
+        logits[r:r + 1000] = (2.5 * torch.randn(min(1000, R - r), V, generator=gen, device=DEV)).to(BF16)
+    first = torch.randint(0, V - 9, (R, 1), generator=gen, device=DEV)
+    ids, log_q = first + 3 * torch.arange(3, device=DEV), torch.full((R, 3), -1.5, device=DEV)
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, ids, log_q, reduction="none")
+    g, = torch.autograd.grad(loss, x, torch.ones(R, device=DEV))
+    for part in (slice(0, 600), slice(R - 600, R)):
+        y = logits.detach()[part].clone().requires_grad_()
+        own = distillation_loss(y, ids[part], log_q[part], reduction="none")
+        assert torch.equal(own, loss[part])
+        assert torch.equal(torch.autograd.grad(own, y, torch.ones(600, device=DEV))[0], g[part])
+    del x, logits, loss, g, y, own
+    R, V, H = 70, 560001, 4096
+    hidden = torch.randn(R, H, generator=gen, device=DEV).to(BF16)
+    weight = torch.empty(V, H, dtype=BF16, device=DEV)
+    for v in range(0, V, 80000):
+        weight[v:v + 80000] = (0.03 * torch.randn(min(80000, V - v), H, generator=gen, device=DEV)).to(BF16)
+    targets = torch.randint(0, V, (R,), generator=gen, device=DEV)
+    targets[:4] = torch.tensor([V - 1, V - 2, 0, 524289], device=DEV)
+    # the same tokens in another order: the vocabulary's second half first
+    order = torch.arange(V, device=DEV).roll(V // 2)
+    h, w = hidden.clone().requires_grad_(), weight.requires_grad_()
+    loss = linear_cross_entropy(h, w, targets, reduction="none")
+    gh, gw = torch.autograd.grad(loss, (h, w), torch.ones(R, device=DEV))
+    other = weight.detach()[order].requires_grad_()
+    h2 = hidden.clone().requires_grad_()
+    loss2 = linear_cross_entropy(h2, other, (targets + V // 2) % V, reduction="none")
+    gh2, gw2 = torch.autograd.grad(loss2, (h2, other), torch.ones(R, device=DEV))
+    # sums in another order: the vocabulary's error, twice, and a rounding of the gradients
+    assert bool(((loss - loss2).abs() <= 2 * (V / 256 + 60) * EPS * (1 + loss.abs())).all())
+    assert float((gh.double() - gh2.double()).norm()) <= 2 * B * float(gh.double().norm())
+    for v in range(0, V, 80000):
+        a, b = gw[order[v:v + 80000]].float(), gw2[v:v + 80000].float()
+        assert float((a - b).norm()) <= B * float(a.norm())
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

@@ -117,13 +117,13 @@ ALL = [distill, distill_bwd, linear, linear_bwd]
     dict(rows=-1), dict(rows=1 << 24), dict(vocab=0), dict(vocab=1 << 30), dict(known=0), dict(known=257),
     dict(inv_t=0.0), dict(inv_t=-1.0), dict(inv_t=math.nan), dict(inv_t=math.inf), dict(inv_t=3e38), dict(reduction=3),
     dict(reduction=-1), dict(state=None))]
-    + [(f, b) for f in ALL[:2] for b in (dict(ld=8), dict(logits=None))]
+    + [(f, b) for f in ALL[:2] for b in (dict(ld=8), dict(logits=None), dict(rows=1 << 22, vocab=1 << 20, ld=1 << 20))]
     + [(distill, dict(ids=None)), (distill, dict(q=None)), (distill, dict(ws=None)), (distill, dict(loss=None)),
        (distill, dict(ws=20)), (distill_bwd, dict(d_loss=None)), (distill_bwd, dict(out=None))]
     + [(f, b) for f in ALL[2:] for b in (
         dict(dtype=2), dict(width=0), dict(width=1 << 20), dict(ldh=7), dict(ldw=7), dict(ldh=1 << 22), dict(hidden=None),
         dict(weight=None), dict(hidden=24), dict(weight=24), dict(ldh=12), dict(ldw=12), dict(ws=None), dict(ws=24),
-        dict(rows=1 << 20, vocab=1000, kept=16))]
+        dict(rows=1 << 20, vocab=1000, kept=16), dict(rows=1 << 23, vocab=1 << 20))]
     + [(f, dict(dtype=0, **b)) for f in ALL[2:] for b in (dict(hidden=24), dict(weight=24), dict(ldh=10), dict(ldw=10))]
     + [(linear, dict(targets=None)), (linear, dict(known=2)), (linear, dict(rest=1)), (linear, dict(loss=None)),
        (linear_bwd, dict(d_loss=None)), (linear_bwd, dict(dh=24)), (linear_bwd, dict(dw=24))])
