@@ -2,8 +2,9 @@
 //
 // Bound: the weight's bytes, and how memory is asked for them: every workgroup goes down the
 // rows of its tokens, and the longer the piece of a row that it takes at a time, the better.
-// 8 rows of width 2048 against 151936 tokens: 139 us with 64-byte pieces (gemm_mid.hip's
-// stages), 131 with 128, 122 with 256 and 114 with 512 (5.5 TB/s).  So a stage is 16 KB of
+// 4 rows of width 2048 against 151936 tokens, the weight not in a cache: 152 us with 64-byte
+// pieces (gemm_mid.hip's stages), 146 with 128, 138 with 256 and 133 with 512; 8 rows scored
+// again and again 119 (5.2 TB/s).  So a stage is 16 KB of
 // the weight: 64 KH deep for 128 / KH tokens, KH as large as the width divides and the hidden
 // states' part of a stage stays below the weight's.  Two workgroups a compute unit, each with
 // two or three stages under way, filled by direct loads to LDS; a wave has 16 or 32 tokens

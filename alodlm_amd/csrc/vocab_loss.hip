@@ -10,7 +10,6 @@
 namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-constexpr int MAP_WORDS = 8192 + 4;    // bits of a part: 2^18 tokens, and the row's ragged ends
 constexpr int64_t MAX_PART = 1 << 18;  // tokens of a part
 
 // ---------------------------------------------------------------------------
