@@ -34,7 +34,8 @@ __device__ __forceinline__ void load_slot(const char* origin, uint32_t off, uint
 template <int MB, int KH>
 __global__ void __launch_bounds__(KH == 4 ? 128 : 256, 2)
 few_logits_kernel(const bf16_t* __restrict__ hidden, int64_t ldh, const bf16_t* __restrict__ weight,
-                  int64_t ldw, int rows, int64_t tokens, int64_t share, int width, float* __restrict__ out) {
+                  int64_t ldw, int rows, int64_t tokens, int64_t share, int width, float* __restrict__ out,
+                  int64_t ldo) {
   // 1 KB blocks of a stage: the weight's, then the hidden states'
   constexpr int TOKENS = 128 / KH, DEEP = 64 * KH, NW = KH == 4 ? 2 : 4;
   constexpr int WT = TOKENS / 16 / NW;  // 16-token blocks a wave
@@ -105,8 +106,8 @@ few_logits_kernel(const bf16_t* __restrict__ hidden, int64_t ldh, const bf16_t* 
       for (int j = 0; j < WT; ++j) {
         const int64_t row = 16 * i + (lane & 15), token = first + 16 * WT * wave + 16 * j + 4 * (lane >> 4);
         if (row >= rows) continue;
-        float* o = out + row * tokens + token;
-        if (tokens % 4 == 0 && token < last)  // (a share is whole 16 tokens)
+        float* o = out + row * ldo + token;
+        if (token + 4 <= last)
           *reinterpret_cast<float4*>(o) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
         else
 #pragma unroll
@@ -153,14 +154,15 @@ few_logits_kernel(const bf16_t* __restrict__ hidden, int64_t ldh, const bf16_t* 
 }  // namespace
 
 void few_bf16_logits(const bf16_t* hidden, int64_t ldh, const bf16_t* weight, int64_t ldw, int64_t rows,
-                     int64_t tokens, int64_t width, float* out, hipStream_t st) {
+                     int64_t tokens, int64_t width, float* out, int64_t ldo, hipStream_t st) {
   const int kh = rows <= 16 && width % 256 == 0 ? 4 : width % 128 == 0 ? 2 : 1;
   const int64_t tiles = (tokens + 128 / kh - 1) / (128 / kh), most = 2 * device_cus();
   const int64_t units = (tokens + 15) / 16, groups = tiles < most ? tiles : most;
   const int64_t share = 16 * ((units + groups - 1) / groups);
   const unsigned grid = (unsigned)((tokens + share - 1) / share);
   auto launch = [&](auto kernel) {
-    kernel<<<grid, kh == 4 ? 128 : 256, 0, st>>>(hidden, ldh, weight, ldw, (int)rows, tokens, share, (int)width, out);
+    kernel<<<grid, kh == 4 ? 128 : 256, 0, st>>>(hidden, ldh, weight, ldw, (int)rows, tokens, share, (int)width, out,
+                                               ldo);
   };
   if (rows <= 16) launch(kh == 4 ? few_logits_kernel<1, 4> : kh == 2 ? few_logits_kernel<1, 2> : few_logits_kernel<1, 1>);
   else if (rows <= 32) launch(kh == 2 ? few_logits_kernel<2, 2> : few_logits_kernel<2, 1>);

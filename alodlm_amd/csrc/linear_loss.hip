@@ -406,14 +406,9 @@ struct Plan {
   int64_t part, logits, D, hidden, weight, sums, rows, gemm, total;
 };
 
-// Whether a piece's logits come from few_bf16.hip, which leaves rows of the piece's own
-// length, and the row stride of logits in memory.
-bool few_logits(const Plan& p, int64_t R, int64_t n) {
-  return p.regular && R <= FEW && n >= 128 * 256 && (!p.small || p.pieces == 1);
-}
-int64_t logits_stride(const Plan& p, int64_t R, int64_t V, int64_t n) {
-  return few_logits(p, R, n) ? n : up_to(p.keep ? V : n, 8);
-}
+// Row stride of a piece's logits in memory (a forward's and its backward's pieces differ, the
+// logits between them do not).
+int64_t logits_stride(const Plan& p, int64_t V, int64_t n) { return up_to(p.small ? V : n, 8); }
 
 Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backward, bool d_hidden,
                bool d_weight) {
@@ -467,7 +462,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   if (p.copy_hidden) p.hidden = room(ceil_div(p.deep_rows * p.deep * es, 4));
   if (p.copy_weight) p.weight = room(ceil_div(p.piece * p.deep * es, 4));
   if (computes && !p.tiles) {
-    if (!p.keep) p.logits = room(R * (p.pieces > 1 ? p.piece : up_to(V, 8)));
+    if (!p.keep) p.logits = room(R * up_to(p.small ? V : p.piece, 8));
     if (p.pieces > 1) product(R, p.piece, p.deep, f32_out);
     product(R, last, p.deep, f32_out);
   }
@@ -573,15 +568,15 @@ template <typename T> struct Call {
     ld = p.deep;
     return to;
   }
-  int64_t logits_ld(int64_t n) const { return logits_stride(p, R, V, n); }
+  int64_t logits_ld(int64_t n) const { return logits_stride(p, V, n); }
   // float logits of a piece, row stride logits_ld(n)
   int logits(int64_t first, int64_t n, float* out) const {
     int64_t ld;
     const T* w = piece_weight(first, n, ld);
     const int64_t to = logits_ld(n);
     if constexpr (sizeof(T) == 2)
-      if (few_logits(p, R, n)) {
-        few_bf16_logits(deep_hidden, deep_ldh, w, ld, R, n, p.deep, out, st);
+      if (p.regular && R <= FEW && n >= 128 * 256) {
+        few_bf16_logits(deep_hidden, deep_ldh, w, ld, R, n, p.deep, out, to, st);
         ALODLM_CHECK_LAUNCH("linear_loss_logits");
         return ALODLM_OK;
       }

@@ -342,6 +342,28 @@ def test_logits_that_are_not_kept(R, V, H, dtype):
     check_linear(hidden, weight, targets, reduction="none", temperature=0.7, grads=(True, False))
 
 
+@pytest.mark.parametrize("R,V,H,dtype", [(3, 10000001, 64, BF16), (2, 9000003, 40, BF16), (2, 8500001, 4, F32)])
+def test_kept_logits_of_several_pieces(R, V, H, dtype):
+    """Few rows against a vocabulary whose gradient is taken in pieces and whose logits are
+    kept whole, or computed in other pieces."""
+    log(f"linear kept, pieces {R} x {V} x {H} {dtype}")
+    assert R * V <= 1 << 25
+    hidden, weight, targets = factors(R, V, H, dtype)
+    check_linear(hidden, weight, targets, reduction="none", grads=(True, False))
+    h, w = hidden.clone().requires_grad_(), weight.requires_grad_()
+    loss = linear_cross_entropy(h, w, targets)
+    assert torch.equal(loss, linear_cross_entropy(hidden, weight.detach(), targets))
+    gw, = torch.autograd.grad(loss, w)
+    rows = torch.cat([torch.arange(0, V, V // 7, device=DEV), targets[targets >= 0], torch.arange(V - 40, V, device=DEV)])
+    lp = (hidden.double() @ weight.detach().double().T).log_softmax(-1)
+    n = int((targets >= 0).sum())
+    D = lp.exp()[:, rows] - (targets[:, None] == rows[None]).double()
+    ref = (D * (targets >= 0)[:, None] / n).T @ hidden.double()
+    one = B if dtype == BF16 else 64 * EPS
+    size = (D.abs() * (targets >= 0)[:, None] / n).T @ hidden.double().abs()
+    assert bool(((gw[rows].double() - ref).abs() <= 2 * one * size + 1e-30).all())
+
+
 @pytest.mark.parametrize("temperature", [0.004, 0.05, 40.0])
 @pytest.mark.parametrize("R,V", [(300, 120001), (90, 3000)])
 def test_linear_temperatures(R, V, temperature):
