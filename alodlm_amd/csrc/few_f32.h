@@ -7,7 +7,6 @@
 constexpr int64_t FEW_F32_ROWS = 32;
 // Rows of D as the kernels read it: D [tokens][few_f32_pad(rows)], tokens first.
 int64_t few_f32_pad(int64_t rows);
-bool few_f32_eligible(int64_t rows, int64_t tokens, int64_t width, const void* weight, int64_t ldw);
 // Parts of the tokens that few_f32_hidden leaves planes of.
 int64_t few_f32_planes(int64_t tokens, int64_t width);
 // planes [few_f32_planes][rows][width] whose sum is D^T weight.

@@ -122,11 +122,6 @@ template <typename F> void with_rows(int64_t rows, F f) {
 
 int64_t few_f32_pad(int64_t rows) { return rows <= 4 ? 4 : (rows + 7) / 8 * 8; }
 
-bool few_f32_eligible(int64_t rows, int64_t tokens, int64_t width, const void* weight, int64_t ldw) {
-  return rows <= FEW_F32_ROWS && tokens * width >= (1 << 20) && width % 4 == 0 && ldw % 4 == 0 &&
-         (reinterpret_cast<uintptr_t>(weight) & 15) == 0;
-}
-
 int64_t few_f32_planes(int64_t tokens, int64_t width) { return token_parts(tokens, width); }
 
 void few_f32_hidden(const float* D, const float* weight, int64_t ldw, int64_t rows, int64_t tokens,

@@ -60,13 +60,17 @@ __device__ __forceinline__ void known_of_row(const GivenRows& given, int64_t row
   r.counted = __any(any);
   r.bad = __any(bad);
   r.q_rest = given.rest && r.counted ? (float)fmax(1.0 - wave_sum_d(mass), 0.0) : 0.f;
+  // places whose id no earlier place has
+  uint64_t firsts[HELD];
   bool twice = false;
   const int4* four = reinterpret_cast<const int4*>(ids);
 #pragma unroll
   for (int j = 0; j < HELD; ++j) {
     const int i = lane + 64 * j, id = r.id[j];
+    firsts[j] = 0;
     if (64 * j >= K) continue;
     int rank = 0;
+    bool again = false;
 #pragma unroll 4
     for (int n = 0; n < (K + 3) / 4; ++n) {
       const int4 o = four[n];
@@ -75,55 +79,40 @@ __device__ __forceinline__ void known_of_row(const GivenRows& given, int64_t row
       for (int e = 0; e < 4; ++e) {
         const bool before = 4 * n + e < i;
         rank += other[e] < id || (other[e] == id && before);
-        twice |= other[e] == id && before && id != VL_NONE;
+        again |= other[e] == id && before;
       }
     }
     r.place[j] = rank;  // the absent behind the others
+    firsts[j] = __ballot(id != VL_NONE && !again);
+    twice |= id != VL_NONE && again;
   }
   if (!__any(twice)) return;
-  // an id given more than once: its first place takes the others' probabilities
-#pragma unroll 1
+  // an id given more than once: its first place takes the others' probabilities, and they
+  // go behind the known ones
+  auto is_first = [&](int n) {
+    return ((n < 64 ? firsts[0] : n < 128 ? firsts[1] : n < 192 ? firsts[2] : firsts[3]) >> (n & 63) & 1) != 0;
+  };
+#pragma unroll
   for (int j = 0; j < HELD; ++j) {
-    const int i = lane + 64 * j;
+    const int i = lane + 64 * j, id = r.id[j];
     if (i >= K) continue;
-    const int id = i < 64 ? r.id[0] : i < 128 ? r.id[1] : i < 192 ? r.id[2] : r.id[3];
-    bool first = true;
+    const bool known = (firsts[j] >> lane & 1) != 0;
     int place = 0;
     double q = 0.0, terms = 0.0;
+#pragma unroll 1
     for (int n = 0; n < K; ++n) {
       const int other = ids[n];
-      bool leads = other != VL_NONE;  // the first of its id
-      for (int m = 0; m < n; ++m) leads &= ids[m] != other;
-      if (other == id && n < i) first = false;
-      if (leads) place += other < id;
-      else place += id == VL_NONE && n < i;  // places that are left over, behind the others
-      if (other == id && id != VL_NONE) {
+      place += is_first(n) ? !known || other < id : !known && n < i;
+      if (known && other == id) {
         const double lq = given.log_q[row * K + n], one = exp(lq);
         q += one;
         if (one != 0.0) terms += one * lq;
       }
     }
-    int distinct = 0;
-    if (id != VL_NONE && !first) {  // a place that is left over, too
-      int over = 0;
-      for (int n = 0; n < K; ++n) {
-        bool leads = ids[n] != VL_NONE;
-        for (int m = 0; m < n; ++m) leads &= ids[m] != ids[n];
-        distinct += leads;
-        over += !leads && n < i;
-      }
-      place = distinct + over;
-    }
-    const bool known = id != VL_NONE && first;
-    const float qf = known ? (float)q : 0.f, lf = known && q != 0.0 ? (float)(terms / q) : 0.f;
-#pragma unroll
-    for (int t = 0; t < HELD; ++t)
-      if (t == j) {
-        r.id[t] = known ? id : VL_NONE;
-        r.q[t] = qf;
-        r.log_q[t] = lf;
-        r.place[t] = place;
-      }
+    r.id[j] = known ? id : VL_NONE;
+    r.q[j] = (float)q;
+    r.log_q[j] = q != 0.0 ? (float)(terms / q) : 0.f;
+    r.place[j] = place;
   }
 }
 
