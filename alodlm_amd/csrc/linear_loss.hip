@@ -191,6 +191,8 @@ struct GradHooks {
         const float whole = floorf(info[RI_LOG]);
         r.x = g * f * __builtin_amdgcn_exp2f(whole - info[RI_LOG]);
         r.y = info[RI_M] + whole;
+      } else if (!(info[RI_LOG] < INFINITY)) {
+        r.w = 1.f;  // NaN that takes no part
       }
     }
     reinterpret_cast<float4*>(extra + TileMarks::BYTES)[threadIdx.x] = r;
@@ -224,6 +226,8 @@ struct GradHooks {
       for (int64_t at = N; at < columns; ++at) reinterpret_cast<bf16_t*>(D)[row * ldd + at] = 0;
     if (row >= M) return;
     const float own_up = consts[threadIdx.x].z;
+    if (consts[threadIdx.x].w != 0.f)
+      for (int64_t at = n0; at < N && at < n0 + TB; ++at) reinterpret_cast<bf16_t*>(D)[row * ldd + at] = 0;
     const uint32_t* bits = reinterpret_cast<const uint32_t*>(extra) + 8 * threadIdx.x;
     const float* own = k.weight + row * k.known + TileMarks::before(extra, threadIdx.x);
     for (int w = 0; w < 8; ++w)

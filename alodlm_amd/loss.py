@@ -302,7 +302,9 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     its product).
 
     A row of ``ignore_index`` has loss 0 and no gradient; any other target outside the
-    vocabulary makes its loss NaN, and its gradients where the loss takes part.
+    vocabulary makes its loss NaN, and its gradients where the loss takes part.  A row that
+    takes no part (ignored, or of upstream gradient 0) may hold NaN where the weight has no
+    gradient; the weight's is a product that multiplies such a row by 0.
 
     A backward that is captured into a graph must not find an eager autograd graph of the
     same leaves alive (its nodes are tied to the eager stream): drop its outputs first."""

@@ -342,6 +342,44 @@ def test_logits_that_are_not_kept(R, V, H, dtype):
     check_linear(hidden, weight, targets, reduction="none", temperature=0.7, grads=(True, False))
 
 
+@pytest.mark.parametrize("R,V,H,dtype", [(300, 1500, 64, BF16), (300, 120001, 64, BF16), (40, 1500, 64, BF16),
+                                         (300, 1501, 60, F32), (20, 30000, 64, F32)])
+def test_rows_that_take_no_part_may_hold_nan(R, V, H, dtype):
+    """Rows of NaN or infinite hidden states that are ignored, or whose loss has no upstream
+    gradient, leave the others as they are and have no gradient themselves."""
+    log(f"linear no part {R} x {V} x {H} {dtype}")
+    hidden, weight, targets = factors(R, V, H, dtype)
+    up = torch.rand(R, device=DEV) + 0.5
+    bad = torch.tensor([0, 3, 7, R - 1], device=DEV)
+    targets[bad[:2]] = -100
+    targets[bad[2:]] = 5
+    up[bad[2:]] = 0.0
+    wild = hidden.clone()
+    wild[bad[0]], wild[bad[1], 3] = math.nan, math.inf
+    wild[bad[2], 1], wild[bad[3]] = math.nan, -math.inf
+    got = []
+    for x in (hidden, wild):
+        h = x.clone().requires_grad_()
+        loss = linear_cross_entropy(h, weight, targets, reduction="none")
+        g, = torch.autograd.grad(loss, h, up)
+        got.append((loss.detach(), g))
+    assert bool((got[1][0][bad[:2]] == 0).all())
+    keep = torch.ones(R, dtype=torch.bool, device=DEV)
+    keep[bad[2:]] = False
+    assert torch.equal(got[0][0][keep], got[1][0][keep])
+    assert torch.equal(got[0][1], got[1][1]) and bool((got[1][1][bad] == 0).all())
+    # a teacher without tokens, the mean
+    h = wild.clone()
+    h[bad[2:]] = hidden[bad[2:]]
+    h.requires_grad_()
+    ids = torch.randint(0, V, (R, 3), device=DEV)
+    ids[bad[:2]] = -1
+    log_q = torch.full((R, 3), -2.0, device=DEV)
+    out = linear_distillation_loss(h, weight, ids, log_q)
+    g, = torch.autograd.grad(out, h)
+    assert bool(out.isfinite()) and bool(g.isfinite().all()) and bool((g[bad[:2]] == 0).all())
+
+
 @pytest.mark.parametrize("R,V,H,dtype", [(3, 10000001, 64, BF16), (2, 9000003, 40, BF16), (2, 8500001, 4, F32)])
 def test_kept_logits_of_several_pieces(R, V, H, dtype):
     """Few rows against a vocabulary whose gradient is taken in pieces and whose logits are
