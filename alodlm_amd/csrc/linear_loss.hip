@@ -19,7 +19,10 @@
 // D is rounded to bf16 (half a step, 2^-8 of a value at most), as a bf16 model's logits'
 // gradient is anywhere: it is an operand of the bf16 matrix cores.  A reduced loss's upstream
 // gradient is applied to the products, not to D: of a row far from its target, D is then -1
-// there, which is exact.
+// there, which is exact.  Of few rows, whose D's rounding does not average out (13 rows: 1.5
+// times the error of the result's own), D is two bf16 parts that the products take as rows of
+// their own, waiting for the weight as before: 16 rows of width 4096 against 151936 tokens 782 ->
+// 793 us, 64 of width 2048 516 -> 587.
 #include "few_bf16.h"
 #include "few_f32.h"
 #include "gemm_dl_tile.h"
@@ -258,22 +261,24 @@ struct ScaleHooks {
   }
 };
 
-// dst [padded, padded_width] = src [rows, width], zeros around it, 16 bytes a thread.
+// dst [padded, padded_width] = src [rows, width] `times` below each other, zeros around them, 16
+// bytes a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
 copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, int64_t width, T* __restrict__ dst,
-                 int64_t padded, int64_t padded_width) {
+                 int64_t padded, int64_t padded_width, int times) {
   constexpr int N = 16 / (int)sizeof(T);
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
   if (at >= padded_width) return;
   for (int64_t row = blockIdx.y; row < padded; row += gridDim.y) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < rows && at < width) v = *reinterpret_cast<const uint4*>(src + row * lds + at);
+    if (row < rows * times && at < width)
+      v = *reinterpret_cast<const uint4*>(src + (row < rows ? row : row - rows) * lds + at);
     *reinterpret_cast<uint4*>(dst + row * padded_width + at) = v;
   }
 }
 
-// out [rows, width] = up.all() * (the planes' sum + D's last `rest` columns times the
+// out [rows, width] = up.all() * (the planes' sum + the last `rest` columns of D's parts times the
 // weight's last `rest` rows, which no product took), rounded once.  GROUPS of threads take
 // every GROUPS-th plane each (many planes of few rows: a thread would wait for one after the
 // other), their sums are added in order.
@@ -281,7 +286,7 @@ template <typename T, int VEC, int GROUPS>
 __global__ void __launch_bounds__(256)
 finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t rows, int64_t width,
                       Upstream up, const T* __restrict__ D, int64_t ldd, const T* __restrict__ weight,
-                      int64_t ldw, int rest, T* __restrict__ out) {
+                      int64_t ldw, int rest, int parts, T* __restrict__ out) {
   constexpr int LANES = 256 / GROUPS;
   __shared__ float shared[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? LANES * VEC : 1];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -314,7 +319,8 @@ finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t r
     }
     if (!inside) continue;
     for (int t = 0; t < rest; ++t) {
-      const float d = Elem<T>::load(D, row * ldd + t);
+      float d = Elem<T>::load(D, row * ldd + t);
+      if (parts > 1) d += Elem<T>::load(D, (rows + row) * ldd + t);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s[e] = fmaf(d, Elem<T>::load(weight, t * ldw + at + e), s[e]);
     }
@@ -337,24 +343,24 @@ dim3 row_grid(int64_t width, int64_t rows) {
 
 template <typename T, int VEC>
 void finish_columns(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
-                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, T* out,
+                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, int parts, T* out,
                     hipStream_t st) {
   if (count >= 16)
     finish_product_kernel<T, VEC, 16><<<row_grid(ceil_div(width, VEC) * 16, rows), 256, 0, st>>>(
-        planes, count, rows, width, up, D, ldd, weight, ldw, rest, out);
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
   else
     finish_product_kernel<T, VEC, 1><<<row_grid(ceil_div(width, VEC), rows), 256, 0, st>>>(
-        planes, count, rows, width, up, D, ldd, weight, ldw, rest, out);
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
 }
 
 template <typename T>
 void finish_product(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
-                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, T* out,
+                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, int parts, T* out,
                     hipStream_t st) {
   if (width % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0)
-    finish_columns<T, 4>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, out, st);
+    finish_columns<T, 4>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out, st);
   else
-    finish_columns<T, 1>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, out, st);
+    finish_columns<T, 1>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out, st);
 }
 
 // Which bf16 tiles a product [M, N] over K runs on and how its K is split: the least of
@@ -400,9 +406,10 @@ struct Plan {
   bool small, keep, tiles;  // few enough logits to keep; kept; never in memory
   bool few;                 // float32 products of few rows (few_f32.hip)
   int64_t piece, pieces;  // tokens of a piece (a multiple of 256), pieces
-  int64_t deep, deep_rows;  // width and rows as the tile kernels take them
+  int64_t deep, deep_rows;  // width and rows of D as the tile kernels take them
+  int parts;                // of D, each of as many rows as there are
   bool copy_hidden, copy_weight;
-  int64_t chunks, parts;    // of a piece's rows, of all
+  int64_t chunks, sum_parts;  // of a piece's rows, of all
   int64_t planes;           // of d_hidden, most
   bool direct;              // d_hidden needs no planes
   Split hidden_split, last_split;
@@ -425,7 +432,9 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   p.tiles = p.regular && !p.small && R > FEW;
   p.few = !p.half && R <= FEW_F32_ROWS && H % 4 == 0 && V * H >= (1 << 20);
   p.deep = p.regular ? up_to(H, 64) : H;
-  p.deep_rows = p.half ? up_to(R, 32) : R;
+  p.parts = backward && p.half && R <= FEW ? 2 : 1;
+  const int64_t d_rows = p.parts * R;
+  p.deep_rows = p.half ? up_to(d_rows, 32) : R;
   const int64_t es = p.half ? 2 : 4;
   const bool computes = !(backward && p.keep);  // the logits
   p.copy_weight = p.regular && computes && p.deep != H;
@@ -440,7 +449,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   if (computes && !p.tiles && !p.small) limit(4 * R);
   if (backward && p.few) limit(4 * few_f32_pad(R));
   if (p.copy_weight) limit(2 * p.deep);
-  if (backward && d_weight && p.half && !p.regular) limit(4 * H);
+  if (backward && d_weight && p.half && !p.regular) limit(4 * p.parts * H);
   if (p.regular) {  // the 128x128 tiles' operands stay below 2 GiB
     const int64_t n = (1ll << 30) / up_to(H, 64) / 256 * 256;
     most = n < most ? n : most;
@@ -461,8 +470,11 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
     gemm = n > gemm ? n : gemm;
   };
   const int f32_out = p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
-  if (backward && d_weight && p.regular && p.deep_rows != R)  // whole 32 rows for the large tiles
-    for (const int64_t n : {p.piece, up_to(last, 32)}) p.copy_hidden |= split_product(n, H, R, true, true, false).large;
+  // whole 32 rows for the large tiles; a row for each part of D
+  p.copy_hidden |= backward && d_weight && p.regular && p.parts > 1;
+  if (backward && d_weight && p.regular && p.deep_rows != R)
+    for (const int64_t n : {p.piece, up_to(last, 32)})
+      p.copy_hidden |= split_product(n, H, d_rows, true, true, false).large;
   if (p.copy_hidden) p.hidden = room(ceil_div(p.deep_rows * p.deep * es, 4));
   if (p.copy_weight) p.weight = room(ceil_div(p.piece * p.deep * es, 4));
   if (computes && !p.tiles) {
@@ -472,8 +484,8 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   }
   if (!backward) {
     p.chunks = p.tiles ? p.piece / TB : row_stats_chunks(R, p.piece);
-    p.parts = p.tiles ? ceil_div(V, TB) : p.chunks * p.pieces;
-    p.part = room(2 * R * p.parts);
+    p.sum_parts = p.tiles ? ceil_div(V, TB) : p.chunks * p.pieces;
+    p.part = room(2 * R * p.sum_parts);
   } else {
     // float32: D takes the place of logits that are not kept
     if (p.few) p.D = room(p.piece * few_f32_pad(R));
@@ -484,25 +496,25 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
       if (d_hidden) p.sums = room(p.planes * R * H);
     } else if (d_hidden) {
       const bool large = H >= 256;
-      p.hidden_split = p.regular ? split_product(R, H, p.piece, large, false, true) : Split{true, 1};
-      p.last_split = p.regular && whole ? split_product(R, H, whole, large, false, true) : Split{true, 1};
+      p.hidden_split = p.regular ? split_product(d_rows, H, p.piece, large, false, true) : Split{true, 1};
+      p.last_split = p.regular && whole ? split_product(d_rows, H, whole, large, false, true) : Split{true, 1};
       p.planes = (p.pieces - 1) * p.hidden_split.planes + (whole ? p.last_split.planes : 0);
       p.direct = !p.half && p.planes == 1 && rest == 0;
-      if (!p.direct) p.sums = room(p.planes * R * H);
+      if (!p.direct) p.sums = room(p.planes * d_rows * H);
       if (!p.regular) {
-        if (p.pieces > 1) product(R, H, p.piece, f32_out);
-        product(R, H, whole, f32_out);
+        if (p.pieces > 1) product(d_rows, H, p.piece, f32_out);
+        product(d_rows, H, whole, f32_out);
       }
     }
     if (d_weight && !p.few) {
       int64_t floats = 0;
       for (const int64_t n : {p.piece, up_to(last, 32)}) {
         if (p.regular) {
-          const Split s = split_product(n, H, R, true, true, false);
+          const Split s = split_product(n, H, d_rows, true, true, false);
           if (!s.large && s.planes * n * H > floats) floats = s.planes * n * H;
         } else {
           product(p.half ? n : up_to(n == p.piece ? n : last, 8), H, R, f32_out);
-          if (p.half && n * H > floats) floats = n * H;
+          if (p.half && p.parts * n * H > floats) floats = p.parts * n * H;
         }
       }
       p.rows = room(floats);
@@ -558,7 +570,8 @@ template <typename T> struct Call {
     deep_ldh = ldh;
     if (!p.copy_hidden) return;
     T* to = reinterpret_cast<T*>(ws + p.hidden);
-    copy_rows_kernel<T><<<row_grid(p.deep / 8, p.deep_rows), 256, 0, st>>>(hidden, ldh, R, H, to, p.deep_rows, p.deep);
+    copy_rows_kernel<T><<<row_grid(p.deep / 8, p.deep_rows), 256, 0, st>>>(hidden, ldh, R, H, to, p.deep_rows, p.deep,
+                                                                          p.parts);
     deep_hidden = to;
     deep_ldh = p.deep;
   }
@@ -568,7 +581,7 @@ template <typename T> struct Call {
     ld = ldw;
     if (!p.copy_weight) return w;
     T* to = reinterpret_cast<T*>(ws + p.weight);
-    copy_rows_kernel<T><<<row_grid(p.deep / 8, n), 256, 0, st>>>(w, ldw, n, H, to, n, p.deep);
+    copy_rows_kernel<T><<<row_grid(p.deep / 8, n), 256, 0, st>>>(w, ldw, n, H, to, n, p.deep, 1);
     ld = p.deep;
     return to;
   }
@@ -627,7 +640,7 @@ int forward(Call<T>& a, const KnownRows& k, const GivenRows& given, float c, int
     }
     ALODLM_CHECK_LAUNCH("linear_loss");
   }
-  known_finish_launch<float>(k, given, whole ? logits : nullptr, ld, part, p.parts, a.R, c, p.tiles,
+  known_finish_launch<float>(k, given, whole ? logits : nullptr, ld, part, p.sum_parts, a.R, c, p.tiles,
                              reduction, loss, a.st);
   ALODLM_CHECK_LAUNCH("linear_loss");
   return ALODLM_OK;
@@ -638,7 +651,7 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
              T* d_weight) {
   const Plan& p = a.p;
   constexpr bool half = sizeof(T) == 2;
-  const int64_t R = a.R, V = a.V, H = a.H;
+  const int64_t R = a.R, V = a.V, H = a.H, d_rows = p.parts * R;
   const int f32_out = half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
   T* D = reinterpret_cast<T*>(a.ws + p.D);
   float* sums = a.ws + p.sums;
@@ -668,14 +681,14 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
           if (d_hidden) {
             few_f32_hidden(D, w, a.ldw, R, n, H, sums + planes * R * H, a.st);
             planes += few_f32_planes(n, H);
-            if (last) finish_product<T>(sums, planes, R, H, up, nullptr, 0, nullptr, 0, 0, d_hidden, a.st);
+            if (last) finish_product<T>(sums, planes, R, H, up, nullptr, 0, nullptr, 0, 0, 1, d_hidden, a.st);
           }
           if (d_weight) few_f32_weight(D, a.hidden, a.ldh, R, n, H, d_weight + first * H, a.st);
           ALODLM_CHECK_LAUNCH("linear_loss_bwd");
           continue;
         }
       row_grads_launch<float, T>(logits, a.logits_ld(n), R, n, first, k, c, up, D, ldd, p.deep_rows, columns,
-                                 a.st);
+                                 a.st, p.parts > 1);
     }
     ALODLM_CHECK_LAUNCH("linear_loss_bwd");
     const T* w = a.weight + first * a.ldw;
@@ -685,35 +698,37 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
       rest_weight = w + take * a.ldw;
       if (take) {
         const Split s = last ? p.last_split : p.hidden_split;
-        float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * R * H;
+        float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * d_rows * H;
         bool done = false;
         if constexpr (half) {
           if (p.regular && s.large) {
             int64_t count = 1;
-            gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, R, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
+            gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
                            s.planes, &count, 0, a.st);
             planes += count;
             done = true;
           } else if (p.regular && take * a.ldw < (1ll << 30)) {
-            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, 0, R, H, take, s.planes, to, a.st);
+            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, 0, d_rows, H, take, s.planes, to, a.st);
             done = true;
           }
         }
         if (!done) {
-          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, R, H, take, 1.f, f32_out, a.dtype,
+          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, f32_out, a.dtype,
                               p.regular ? nullptr : a.gemm(), a.st));
           ++planes;
         }
         ALODLM_CHECK_LAUNCH("linear_loss_bwd");
       }
       if (last && !p.direct)
-        finish_product<T>(sums, planes, R, H, up, D + take, ldd, rest_weight, a.ldw, (int)rest, d_hidden, a.st);
+        // (a plane has the parts' rows one after the other: planes of their own)
+        finish_product<T>(sums, p.parts * planes, R, H, up, D + take, ldd, rest_weight, a.ldw, (int)rest, p.parts,
+                          d_hidden, a.st);
     }
     if (d_weight) {
       T* to = d_weight + first * H;  // (up to 31 rows behind the last: the caller's room)
       if constexpr (half) {
         float* rows = a.ws + p.rows;
-        const Split s = p.regular ? split_product(padded, H, R, true, true, false) : Split{false, 1};
+        const Split s = p.regular ? split_product(padded, H, d_rows, true, true, false) : Split{false, 1};
         int64_t count = 1;
         if (s.large) {
           const int64_t tiles = ceil_div(padded, TB) * ceil_div(H, TB);
@@ -722,12 +737,14 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
                                                            padded, H, p.deep_rows, 1.f, p.deep_rows, nullptr, 0,
                                                            KSegs{}, ScaleHooks{up});
         } else {
-          if (p.regular && R * a.deep_ldh < (1ll << 30))
-            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, 0, padded, H, R, s.planes, rows, a.st);
-          else
-            LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, rows, H, nullptr, 0, padded, H, R, 1.f, f32_out,
-                                a.dtype, p.regular ? nullptr : a.gemm(), a.st));
-          finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, to, a.st);
+          if (p.regular && (p.parts > 1 || R * a.deep_ldh < (1ll << 30))) {
+            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, 0, padded, H, d_rows, s.planes, rows, a.st);
+          } else {
+            for (count = 0; count < p.parts; ++count)
+              LL_CALL(alodlm_gemm(D + count * R * ldd, ldd, 0, a.hidden, a.ldh, 0, rows + count * padded * H, H, nullptr,
+                                  0, padded, H, R, 1.f, f32_out, a.dtype, p.regular ? nullptr : a.gemm(), a.st));
+          }
+          finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, 1, to, a.st);
         }
       } else {
         LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, to, H, nullptr, 0, up_to(n, 8), H, R, 1.f, f32_out, a.dtype,

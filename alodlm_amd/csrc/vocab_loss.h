@@ -111,11 +111,12 @@ void known_finish_launch(const KnownRows& k, const GivenRows& given, const T* lo
                          const Part* part, int64_t parts, int64_t rows, float c, bool scaled,
                          int reduction, float* loss, hipStream_t st);
 // dlogits (TO, row stride ldo; columns [width, padded) and rows [rows, padded_rows) zero) of
-// logits [rows, width], columns first .. of the vocabulary; may be in place.
+// logits [rows, width], columns first .. of the vocabulary; may be in place.  `parts` (bf16 of
+// float logits): in two parts, rows r and rows + r, which the padded rows take in.
 template <typename TI, typename TO>
 void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
                       const KnownRows& k, float c, const Upstream& up, TO* out, int64_t ldo,
-                      int64_t padded_rows, int64_t padded, hipStream_t st);
+                      int64_t padded_rows, int64_t padded, hipStream_t st, bool parts);
 
 // The same of few rows in float32, tokens first: out [width][pad], zeros behind the rows.
 void few_grads_launch(const float* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,

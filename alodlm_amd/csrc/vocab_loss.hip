@@ -5,6 +5,8 @@
 // The known tokens are marked in a bit map of the row's part in LDS, whose bytes lie as the
 // 16-byte pieces of the row do: one byte read a piece says whether any of its logits has to
 // be left out, so the pass over the row stays a stream.
+#include <type_traits>
+
 #include "vocab_loss.h"
 
 namespace {
@@ -420,21 +422,27 @@ known_reduce_kernel(KnownRows k, int64_t rows, int mean, float* __restrict__ los
 // ---------------------------------------------------------------------------
 constexpr int GRAD_PIECES = THREADS * 2;
 
-template <typename TI, typename TO>
+// PARTS: two bf16 parts of each, the value's rounding and what that leaves, in rows r and
+// rows + r.
+template <typename TI, typename TO, bool PARTS>
 __global__ void __launch_bounds__(THREADS)
 row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t first, KnownRows k,
                  float c, Upstream up, TO* out, int64_t ldo, int padded, int chunks) {
   constexpr int N = 8;  // tokens a thread takes at a time
   const unsigned block = gridDim.x - 1 - blockIdx.x;
-  const int64_t row = block / chunks;
+  int64_t row = block / chunks;
   const int chunk = (int)(block % chunks);
+  const bool live = row < rows;
+  if (PARTS && !live) row += rows;  // behind both parts
   TO* o = out + row * ldo;
+  // the second part
+  auto left = [](float v) { const float by = v - bf16_to_float(float_to_bf16(v)); return by - by == 0.f ? by : 0.f; };
+  TO* o2 = o + rows * ldo;
   // pieces by the gradient's 16-byte (bf16) or 32-byte (float) alignment
   const int head = min((int)(-(intptr_t)o & (8 * (int)sizeof(TO) - 1)) / (int)sizeof(TO), padded);
   const int pieces = (padded - head) / N, tail = head + pieces * N;
   const int p0 = min(chunk * GRAD_PIECES, pieces), p1 = min(p0 + GRAD_PIECES, pieces);
   const bool last = chunk == chunks - 1;
-  const bool live = row < rows;
   const TI* x = logits + (live ? row : 0) * ld;
   float g = 0.f, factor = 0.f, m = 0.f, log_rest = 0.f;
   if (live) {
@@ -467,9 +475,17 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
     }
 #pragma unroll
     for (int i = 0; i < N; i += Piece<TO>::N) Piece<TO>::store(o + at + i, v + i);
+    if (PARTS && live) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = left(v[i]);
+#pragma unroll
+      for (int i = 0; i < N; i += Piece<TO>::N) Piece<TO>::store(o2 + at + i, v + i);
+    }
   }
   auto single = [&](int at) {
-    Elem<TO>::store(o, at, flat || at >= width ? 0.f : gradient(Elem<TI>::load(x, at)));
+    const float v = flat || at >= width ? 0.f : gradient(Elem<TI>::load(x, at));
+    Elem<TO>::store(o, at, v);
+    if (PARTS && live) Elem<TO>::store(o2, at, left(v));
   };
   if (chunk == 0 && (int)threadIdx.x < head) single(threadIdx.x);
   if (last && tail + (int)threadIdx.x < padded) single(tail + threadIdx.x);
@@ -480,7 +496,9 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
     const int id = k.ids[row * k.known + i];
     const int64_t at = (int64_t)id - first;
     if (id == VL_NONE || at < lo || at >= hi) continue;
-    Elem<TO>::store(o, at, g == 0.f ? 0.f : g * k.weight[row * k.known + i]);
+    const float v = g == 0.f ? 0.f : g * k.weight[row * k.known + i];
+    Elem<TO>::store(o, at, v);
+    if (PARTS) Elem<TO>::store(o2, at, left(v));
   }
 }
 
@@ -585,17 +603,23 @@ template void known_finish_launch<float>(const KnownRows&, const GivenRows&, con
 template <typename TI, typename TO>
 void row_grads_launch(const TI* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
                       const KnownRows& k, float c, const Upstream& up, TO* out, int64_t ldo,
-                      int64_t padded_rows, int64_t padded, hipStream_t st) {
+                      int64_t padded_rows, int64_t padded, hipStream_t st, bool parts) {
   const int64_t chunks = (padded / 8 + GRAD_PIECES) / GRAD_PIECES;
-  row_grads_kernel<TI, TO><<<(unsigned)(padded_rows * chunks), THREADS, 0, st>>>(
+  if constexpr (!std::is_same<TI, TO>::value)
+    if (parts) {
+      row_grads_kernel<TI, TO, true><<<(unsigned)((padded_rows - rows) * chunks), THREADS, 0, st>>>(
+          logits, ld, rows, (int)width, first, k, c, up, out, ldo, (int)padded, (int)chunks);
+      return;
+    }
+  row_grads_kernel<TI, TO, false><<<(unsigned)(padded_rows * chunks), THREADS, 0, st>>>(
       logits, ld, rows, (int)width, first, k, c, up, out, ldo, (int)padded, (int)chunks);
 }
 template void row_grads_launch<float, float>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
                                              float, const Upstream&, float*, int64_t, int64_t, int64_t,
-                                             hipStream_t);
+                                             hipStream_t, bool);
 template void row_grads_launch<float, bf16_t>(const float*, int64_t, int64_t, int64_t, int64_t, const KnownRows&,
                                               float, const Upstream&, bf16_t*, int64_t, int64_t, int64_t,
-                                              hipStream_t);
+                                              hipStream_t, bool);
 
 void few_grads_launch(const float* logits, int64_t ld, int64_t rows, int64_t width, int64_t first,
                       const KnownRows& k, float c, const Upstream& up, float* out, int64_t pad,
@@ -655,7 +679,7 @@ extern "C" int alodlm_distillation_bwd(const void* logits, int64_t ld, const flo
   const Upstream up = {k.call, d_loss, reduction, 0, inv_temperature};
   ALODLM_DISPATCH(dtype, T, {
     row_grads_launch<T, T>((const T*)logits, ld, rows, vocab, 0, k, inv_temperature * VL_LOG2E, up, (T*)dlogits,
-                           vocab, rows, vocab, as_stream(stream));
+                           vocab, rows, vocab, as_stream(stream), false);
   });
   ALODLM_CHECK_LAUNCH("distillation_bwd");
   return ALODLM_OK;

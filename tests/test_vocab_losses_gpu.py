@@ -297,7 +297,9 @@ def check_linear(hidden, weight, targets=None, ids=None, log_q=None, temperature
         size = (p * mass[:, None] + q[:, :V] + mass[:, None] * torch.where(q[:, :V] > 0, 0.0, p)
                 / torch.where(q[:, :V] > 0, 0.0, p).sum(-1, keepdim=True).clamp(min=1e-300)) / temperature * row[part, None].abs()
         # errors of D in every term, all of one sign; its rounding
-        far = 8 * (tol[:, None] + 2 * EPS) * size + (B if hidden.dtype == BF16 else 0.0) * D.abs()
+        # (of up to 64 rows in two parts: the second's rounding)
+        step = 0.0 if hidden.dtype != BF16 else B if R > 64 else B * B
+        far = 8 * (tol[:, None] + 2 * EPS) * size + step * D.abs()
         far = far + (R + V) / 32 * EPS * D.abs()  # the products' sums
         dh[part] = D @ w64
         dh_far[part] = far @ w64.abs()
