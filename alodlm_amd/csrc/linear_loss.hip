@@ -282,12 +282,12 @@ copy_rows_kernel(const T* __restrict__ src, int64_t lds, int64_t rows, int64_t w
 // weight's last `rest` rows, which no product took), rounded once.  GROUPS of threads take
 // every GROUPS-th plane each (many planes of few rows: a thread would wait for one after the
 // other), their sums are added in order.
-template <typename T, int VEC, int GROUPS>
+template <typename T, int GROUPS>
 __global__ void __launch_bounds__(256)
 finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t rows, int64_t width,
                       Upstream up, const T* __restrict__ D, int64_t ldd, const T* __restrict__ weight,
                       int64_t ldw, int rest, int parts, T* __restrict__ out) {
-  constexpr int LANES = 256 / GROUPS;
+  constexpr int LANES = 256 / GROUPS, VEC = 4;
   __shared__ float shared[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? LANES * VEC : 1];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int64_t at = ((int64_t)blockIdx.x * LANES + lane) * VEC;
@@ -300,12 +300,8 @@ finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t r
     if (inside)
 #pragma unroll 8
       for (int64_t p = group; p < count; p += GROUPS) {
-        if constexpr (VEC == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + p * plane);
-          s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
-        } else {
-          s[0] += src[p * plane];
-        }
+        const float4 x = *reinterpret_cast<const float4*>(src + p * plane);
+        s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
       }
     if constexpr (GROUPS > 1) {
       __syncthreads();
@@ -325,13 +321,11 @@ finish_product_kernel(const float* __restrict__ planes, int64_t count, int64_t r
       for (int e = 0; e < VEC; ++e) s[e] = fmaf(d, Elem<T>::load(weight, t * ldw + at + e), s[e]);
     }
     T* dst = out + row * width + at;
-    if constexpr (VEC == 4 && sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2)
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(scale * s[0], scale * s[1]),
                                                   pack_bf16x2(scale * s[2], scale * s[3]));
-    else if constexpr (VEC == 4)
-      *reinterpret_cast<float4*>(dst) = make_float4(scale * s[0], scale * s[1], scale * s[2], scale * s[3]);
     else
-      Elem<T>::store(dst, 0, scale * s[0]);
+      *reinterpret_cast<float4*>(dst) = make_float4(scale * s[0], scale * s[1], scale * s[2], scale * s[3]);
   }
 }
 
@@ -341,26 +335,16 @@ dim3 row_grid(int64_t width, int64_t rows) {
   return dim3((unsigned)ceil_div(width, 256), (unsigned)(rows < 65535 ? rows : 65535));
 }
 
-template <typename T, int VEC>
-void finish_columns(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
-                    const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, int parts, T* out,
-                    hipStream_t st) {
-  if (count >= 16)
-    finish_product_kernel<T, VEC, 16><<<row_grid(ceil_div(width, VEC) * 16, rows), 256, 0, st>>>(
-        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
-  else
-    finish_product_kernel<T, VEC, 1><<<row_grid(ceil_div(width, VEC), rows), 256, 0, st>>>(
-        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
-}
-
 template <typename T>
 void finish_product(const float* planes, int64_t count, int64_t rows, int64_t width, const Upstream& up,
                     const T* D, int64_t ldd, const T* weight, int64_t ldw, int rest, int parts, T* out,
                     hipStream_t st) {
-  if (width % 4 == 0 && (uintptr_t)out % (4 * sizeof(T)) == 0)
-    finish_columns<T, 4>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out, st);
+  if (count >= 16)
+    finish_product_kernel<T, 16><<<row_grid(width / 4 * 16, rows), 256, 0, st>>>(
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
   else
-    finish_columns<T, 1>(planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out, st);
+    finish_product_kernel<T, 1><<<row_grid(width / 4, rows), 256, 0, st>>>(
+        planes, count, rows, width, up, D, ldd, weight, ldw, rest, parts, out);
 }
 
 // Which bf16 tiles a product [M, N] over K runs on and how its K is split: the least of
@@ -402,7 +386,7 @@ constexpr int64_t FEW = ALODLM_FEW_ROWS;
 
 // How a call runs, from its sizes alone.
 struct Plan {
-  bool half, regular;     // bf16; rows of whole 16 bytes, on the tile kernels
+  bool half;              // bf16
   bool small, keep, tiles;  // few enough logits to keep; kept; never in memory
   bool few;                 // float32 products of few rows (few_f32.hip)
   int64_t piece, pieces;  // tokens of a piece (a multiple of 256), pieces
@@ -425,19 +409,18 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
                bool d_weight) {
   Plan p = {};
   p.half = dtype == ALODLM_BF16;
-  p.regular = p.half && H % 8 == 0;
   // (a loss has the same bits whether or not a backward will want the logits)
   p.small = R * up_to(V, 8) <= KEPT;
   p.keep = keep && p.small;
-  p.tiles = p.regular && !p.small && R > FEW;
-  p.few = !p.half && R <= FEW_F32_ROWS && H % 4 == 0 && V * H >= (1 << 20);
-  p.deep = p.regular ? up_to(H, 64) : H;
+  p.tiles = p.half && !p.small && R > FEW;
+  p.few = !p.half && R <= FEW_F32_ROWS && V * H >= (1 << 20);
+  p.deep = p.half ? up_to(H, 64) : H;
   p.parts = backward && p.half && R <= FEW ? 2 : 1;
   const int64_t d_rows = p.parts * R;
   p.deep_rows = p.half ? up_to(d_rows, 32) : R;
   const int64_t es = p.half ? 2 : 4;
   const bool computes = !(backward && p.keep);  // the logits
-  p.copy_weight = p.regular && computes && p.deep != H;
+  p.copy_weight = p.half && computes && p.deep != H;
   p.copy_hidden = p.copy_weight;
   // bytes of a token
   int64_t most = V;
@@ -449,8 +432,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   if (computes && !p.tiles && !p.small) limit(4 * R);
   if (backward && p.few) limit(4 * few_f32_pad(R));
   if (p.copy_weight) limit(2 * p.deep);
-  if (backward && d_weight && p.half && !p.regular) limit(4 * p.parts * H);
-  if (p.regular) {  // the 128x128 tiles' operands stay below 2 GiB
+  if (p.half) {  // the 128x128 tiles' operands stay below 2 GiB
     const int64_t n = (1ll << 30) / up_to(H, 64) / 256 * 256;
     most = n < most ? n : most;
   }
@@ -471,8 +453,8 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   };
   const int f32_out = p.half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
   // whole 32 rows for the large tiles; a row for each part of D
-  p.copy_hidden |= backward && d_weight && p.regular && p.parts > 1;
-  if (backward && d_weight && p.regular && p.deep_rows != R)
+  p.copy_hidden |= backward && d_weight && p.parts > 1;
+  if (backward && d_weight && p.half && p.deep_rows != R)
     for (const int64_t n : {p.piece, up_to(last, 32)})
       p.copy_hidden |= split_product(n, H, d_rows, true, true, false).large;
   if (p.copy_hidden) p.hidden = room(ceil_div(p.deep_rows * p.deep * es, 4));
@@ -496,12 +478,12 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
       if (d_hidden) p.sums = room(p.planes * R * H);
     } else if (d_hidden) {
       const bool large = H >= 256;
-      p.hidden_split = p.regular ? split_product(d_rows, H, p.piece, large, false, true) : Split{true, 1};
-      p.last_split = p.regular && whole ? split_product(d_rows, H, whole, large, false, true) : Split{true, 1};
+      p.hidden_split = p.half ? split_product(d_rows, H, p.piece, large, false, true) : Split{true, 1};
+      p.last_split = p.half && whole ? split_product(d_rows, H, whole, large, false, true) : Split{true, 1};
       p.planes = (p.pieces - 1) * p.hidden_split.planes + (whole ? p.last_split.planes : 0);
       p.direct = !p.half && p.planes == 1 && rest == 0;
       if (!p.direct) p.sums = room(p.planes * d_rows * H);
-      if (!p.regular) {
+      if (!p.half) {
         if (p.pieces > 1) product(d_rows, H, p.piece, f32_out);
         product(d_rows, H, whole, f32_out);
       }
@@ -509,12 +491,11 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
     if (d_weight && !p.few) {
       int64_t floats = 0;
       for (const int64_t n : {p.piece, up_to(last, 32)}) {
-        if (p.regular) {
+        if (p.half) {
           const Split s = split_product(n, H, d_rows, true, true, false);
           if (!s.large && s.planes * n * H > floats) floats = s.planes * n * H;
         } else {
-          product(p.half ? n : up_to(n == p.piece ? n : last, 8), H, R, f32_out);
-          if (p.half && p.parts * n * H > floats) floats = p.parts * n * H;
+          product(up_to(n == p.piece ? n : last, 8), H, R, f32_out);
         }
       }
       p.rows = room(floats);
@@ -538,7 +519,8 @@ int check_linear(const char* what, const void* hidden, int64_t ldh, const void* 
     ALODLM_CHECK_ARG(hidden && weight, "%s: the call lacks an array", what);
   ALODLM_CHECK_ARG((R + 255) / 256 * ((V + 255) / 256) < VL_MOST_GROUPS, "%s: too many rows in one call", what);
   const int64_t step = dtype == ALODLM_BF16 ? 8 : 4;  // elements of 16 bytes
-  if (R > 0 && H % step == 0)
+  ALODLM_CHECK_ARG(H % step == 0, "%s: rows must be whole 16 bytes", what);
+  if (R > 0)
     ALODLM_CHECK_ARG((((uintptr_t)hidden | (uintptr_t)weight) & 15) == 0 && ldh % step == 0 && ldw % step == 0,
                      "%s: rows must be 16-byte aligned", what);
   return ALODLM_OK;
@@ -592,14 +574,14 @@ template <typename T> struct Call {
     const T* w = piece_weight(first, n, ld);
     const int64_t to = logits_ld(n);
     if constexpr (sizeof(T) == 2)
-      if (p.regular && R <= FEW && n >= 128 * 256) {
+      if (R <= FEW && n >= 128 * 256) {
         few_bf16_logits(deep_hidden, deep_ldh, w, ld, R, n, p.deep, out, to, st);
         ALODLM_CHECK_LAUNCH("linear_loss_logits");
         return ALODLM_OK;
       }
     if constexpr (sizeof(T) == 2)
       // 256 rows of tiles at once, where the dispatch would take two of 128
-      if (p.regular && R > 128 && R < 256 && n >= 256 * 128) {
+      if (R > 128 && R < 256 && n >= 256 * 128) {
         int64_t count = 1;
         gemm_dl_launch(deep_hidden, deep_ldh, 1, w, ld, 1, out, to, nullptr, 0, R, n, p.deep, 1.f,
                        ALODLM_EPI_STORE_F32, nullptr, 1, &count, 0, st);
@@ -701,20 +683,20 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
         float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * d_rows * H;
         bool done = false;
         if constexpr (half) {
-          if (p.regular && s.large) {
+          if (s.large) {
             int64_t count = 1;
             gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
                            s.planes, &count, 0, a.st);
             planes += count;
             done = true;
-          } else if (p.regular && take * a.ldw < (1ll << 30)) {
+          } else if (take * a.ldw < (1ll << 30)) {
             planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, 0, d_rows, H, take, s.planes, to, a.st);
             done = true;
           }
         }
         if (!done) {
           LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, f32_out, a.dtype,
-                              p.regular ? nullptr : a.gemm(), a.st));
+                              half ? nullptr : a.gemm(), a.st));
           ++planes;
         }
         ALODLM_CHECK_LAUNCH("linear_loss_bwd");
@@ -728,7 +710,7 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
       T* to = d_weight + first * H;  // (up to 31 rows behind the last: the caller's room)
       if constexpr (half) {
         float* rows = a.ws + p.rows;
-        const Split s = p.regular ? split_product(padded, H, d_rows, true, true, false) : Split{false, 1};
+        const Split s = split_product(padded, H, d_rows, true, true, false);
         int64_t count = 1;
         if (s.large) {
           const int64_t tiles = ceil_div(padded, TB) * ceil_div(H, TB);
@@ -737,13 +719,11 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
                                                            padded, H, p.deep_rows, 1.f, p.deep_rows, nullptr, 0,
                                                            KSegs{}, ScaleHooks{up});
         } else {
-          if (p.regular && (p.parts > 1 || R * a.deep_ldh < (1ll << 30))) {
+          if (p.parts > 1 || R * a.deep_ldh < (1ll << 30))
             count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, 0, padded, H, d_rows, s.planes, rows, a.st);
-          } else {
-            for (count = 0; count < p.parts; ++count)
-              LL_CALL(alodlm_gemm(D + count * R * ldd, ldd, 0, a.hidden, a.ldh, 0, rows + count * padded * H, H, nullptr,
-                                  0, padded, H, R, 1.f, f32_out, a.dtype, p.regular ? nullptr : a.gemm(), a.st));
-          }
+          else
+            LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, rows, H, nullptr, 0, padded, H, R, 1.f, f32_out,
+                                a.dtype, nullptr, a.st));
           finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, 1, to, a.st);
         }
       } else {

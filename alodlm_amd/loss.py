@@ -145,18 +145,22 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def _aligned_rows(t):
-    """A matrix whose rows the kernels can take, and their stride: elements of a row next
-    to each other, and 16-byte aligned rows where a row is a whole number of 16 bytes."""
+    """A matrix whose rows the kernels can take (elements of a row next to each other, whole
+    16 bytes, 16-byte aligned), and their stride; rows of other widths have zeros behind them."""
     rows, width = t.shape
     step = 16 // t.element_size()
-    if t.is_contiguous() and (t.data_ptr() % 16 == 0 or width % step):
-        return t, width
-    if width == 1 or t.stride(1) == 1:
+    if width % step:
+        out = torch.zeros(rows, -(-width // step) * step, dtype=t.dtype, device=t.device)
+        out[:, :width] = t
+        return out, out.shape[1]
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t, width
         stride = width if rows < 2 else t.stride(0)
-        if stride >= width and (width % step or (stride % step == 0 and t.data_ptr() % 16 == 0)):
+        if t.stride(1) == 1 and stride >= width and stride % step == 0:
             return t, stride
     t = t.contiguous()
-    return (t if t.data_ptr() % 16 == 0 or width % step else t.clone()), width
+    return (t if t.data_ptr() % 16 == 0 else t.clone()), width
 
 
 def _floats(n, device):
@@ -220,12 +224,11 @@ def _linear_sizes(R, V, H, known, code, keep, dh, dw):
 
 
 def _linear(hidden, weight, targets, ids, log_q, inv_temperature, ignore_index, rest, reduction, keep=False):
-    R, H = hidden.shape
     V, dev = weight.shape[0], hidden.device
     known = 1 if ids is None else ids.shape[1]
     h, ldh = _aligned_rows(hidden)
     w, ldw = _aligned_rows(weight)
-    code = _lib.dtype_code(h.dtype)
+    (R, H), code = h.shape, _lib.dtype_code(h.dtype)
     state, kept, ws, _ = _linear_sizes(R, V, H, known, code, keep, True, True)
     loss, ws = _floats(() if reduction else R, dev), _floats(ws, dev)
     saved = _floats(state + kept, dev)  # (the state's floats are whole 16 bytes)
@@ -249,10 +252,10 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_loss):
         hidden, weight, saved = ctx.saved_tensors
-        (R, H), V, dev = hidden.shape, weight.shape[0], hidden.device
+        width, V, dev = hidden.shape[1], weight.shape[0], hidden.device
         h, ldh = _aligned_rows(hidden)
         w, ldw = _aligned_rows(weight)
-        code = _lib.dtype_code(h.dtype)
+        (R, H), code = h.shape, _lib.dtype_code(h.dtype)
         need_h, need_w = ctx.needs_input_grad[:2]
         dh = torch.empty(R, H, dtype=h.dtype, device=dev) if need_h else None
         # room for whole 32 rows: the kernels' tiles
@@ -261,7 +264,11 @@ class _Linear(torch.autograd.Function):
         ws, up, at = _floats(ws, dev), _upstream(d_loss), saved.data_ptr()
         call_on(dev, "alodlm_linear_loss_bwd", h.data_ptr(), ldh, w.data_ptr(), ldw, at,
                 at + 4 * state if kept else None, up.data_ptr(), R, V, H, *ctx.args, ptr(dh), ptr(dw), ws.data_ptr(), code)
-        return (dh, None if dw is None else dw[:V]) + (None,) * 7
+        if dw is not None:
+            dw = dw[:V]
+        if H != width:
+            dh, dw = (g if g is None else g[:, :width].contiguous() for g in (dh, dw))
+        return (dh, dw) + (None,) * 7
 
 
 def _check_options(temperature, reduction):

@@ -801,8 +801,8 @@ int alodlm_distillation_bwd(const void* logits, int64_t ld, const float* state, 
  * alodlm_linear_loss_kept (floats) is not 0, few enough logits may be kept for the backward
  * in `kept` (else NULL; `keep` says so to the workspace queries); others are never kept.  The
  * backward writes d_hidden [rows, width] and d_weight [vocab, width], which has room for
- * vocab rounded up to 32 rows (each may be NULL).  Rows of whole 16 bytes
- * are 16-byte aligned; so are the workspaces (floats), kept and the gradients. */
+ * vocab rounded up to 32 rows (each may be NULL).  Rows are
+ * whole 16 bytes and 16-byte aligned; so are the workspaces (floats), kept and the gradients. */
 int64_t alodlm_linear_loss_kept(int64_t rows, int64_t vocab, int64_t width, int dtype);
 int64_t alodlm_linear_loss_workspace(int64_t rows, int64_t vocab, int64_t width, int keep, int dtype);
 int alodlm_linear_loss(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,

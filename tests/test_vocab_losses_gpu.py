@@ -382,6 +382,21 @@ def test_rows_that_take_no_part_may_hold_nan(R, V, H, dtype):
     assert bool(out.isfinite()) and bool(g.isfinite().all()) and bool((g[bad[:2]] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("R,V,H", [(3, 40, 1), (70, 900, 3), (20, 30000, 37), (90, 1003, 513), (300, 120001, 34)])
+def test_rows_of_any_width(R, V, H, dtype):
+    """Rows of any width, dense, in wider buffers and transposed; either gradient alone."""
+    log(f"linear odd widths {R} x {V} x {H} {dtype}")
+    hidden, weight, targets = factors(R, V, H, dtype)
+    _, (gh, gw) = check_linear(hidden, weight, targets)
+    assert gh.is_contiguous() and gw.is_contiguous()
+    wide = torch.full((V, H + 11), math.nan, dtype=dtype, device=DEV)
+    wide[:, 5:5 + H] = weight
+    for h, w, grads in ((hidden.t().contiguous().t(), wide[:, 5:5 + H], (True, False)), (hidden, weight, (False, True))):
+        _, (g,) = check_linear(h, w, targets, grads=grads)
+        assert torch.equal(g, gh if grads[0] else gw)
+
+
 @pytest.mark.parametrize("R,V,H,dtype", [(3, 10000001, 64, BF16), (2, 9000003, 40, BF16), (2, 8500001, 4, F32)])
 def test_kept_logits_of_several_pieces(R, V, H, dtype):
     """Few rows against a vocabulary whose gradient is taken in pieces and whose logits are

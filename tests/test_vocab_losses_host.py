@@ -158,3 +158,12 @@ def test_sizes():
     assert small <= (512 << 20) // 4 + 9 * 2 * planes
     assert q("alodlm_linear_loss_workspace", 4096, 151936, 2048, 0, 1) == 2 * 4096 * 594
     assert q("alodlm_vocab_loss_state", 10, 20) == 4 + 10 * (8 + 80)
+
+
+@pytest.mark.parametrize("make", [linear, linear_bwd])
+@pytest.mark.parametrize("bad", [dict(width=12, ldh=16, ldw=16), dict(width=6, ldh=8, ldw=8, dtype=0)])
+def test_library_takes_rows_of_whole_16_bytes(make, bad):
+    library()
+    name, args = make(**bad)
+    with pytest.raises(ValueError, match="16 bytes"):
+        _lib.call(name, *args)
