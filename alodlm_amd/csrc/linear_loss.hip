@@ -58,12 +58,34 @@ struct TileMarks {
     *reinterpret_cast<uint4*>(bits + 4) = make_uint4(0, 0, 0, 0);
     int before = 0;
     if (row < rows) {
-      const int* ids = k.ids + row * k.known;
-#pragma unroll 8
-      for (int i = 0; i < k.known; ++i) {
-        const int at = ids[i] - (int)token0;
-        before += at < 0;
-        if ((unsigned)at < (unsigned)TB) bits[at >> 5] |= 1u << (at & 31);
+      const int K = k.known, token = (int)token0;
+      const int* ids = k.ids + row * K;
+      // the first that is not before the tile: eight parts of what is left, seven loads at once
+      // (2048 rows of width 2048 against 151936 tokens, 64 known a row: 4.51 -> 4.34 ms, 256: 5.61 ->
+      // 4.43).
+      // Every loaded id is used, or the main loop would wait for those that are not.
+      for (int n = K; n > 8;) {
+        n = (n + 7) >> 3;
+        int parts = 0;
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+          const int at = before + j * n - 1;
+          parts += (int)(ids[at < K ? at : K - 1] < token) & (int)(at < K);
+        }
+        before += parts * n;
+      }
+      bool more = true;
+      for (int i = before; more && i < K; i += 8) {
+        int id[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) id[e] = ids[i + e < K ? i + e : K - 1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = (i + e < K ? id[e] : VL_NONE) - token;
+          before += at < 0;
+          if ((unsigned)at < (unsigned)TB) bits[at >> 5] |= 1u << (at & 31);
+          more = at < TB;
+        }
       }
     }
     reinterpret_cast<uint16_t*>(lds + TB * 32)[threadIdx.x] = (uint16_t)before;
