@@ -22,7 +22,6 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
 
 namespace {
 
-
 __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 3; }
 
 // 16 bytes a lane from the wave-uniform origin plus the lane's offset into LDS slot lane of m0v.
