@@ -16,6 +16,7 @@ the vocabulary.
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -25,6 +26,13 @@ from ._lib import call, call_on, ptr, query
 def _require_gpu(t, what):
     if t.device.type != "cuda":
         raise ValueError(f"{what} runs on the HIP kernels; move the tensors to a CUDA (ROCm) device")
+
+
+def _refuse_tangents(what, *tensors):
+    """Forward-mode derivatives are refused: a tensor with a tangent need not require a
+    gradient, and a result without one would count as constant."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def check_sequence_boundaries(masked_indices, cum_seqlens):

@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, call_on, ptr, query
-from .credit import _require_gpu, _vocabulary_rows, check_sequence_boundaries
+from .credit import _refuse_tangents, _require_gpu, _vocabulary_rows, check_sequence_boundaries
 
 METRIC_KEYS = ("denoising", "actor", "sampled_mean_depth", "prediction_cost",
                "regularization_cost", "profile_mean_depth", "first_pass_halt_probability")
@@ -306,7 +306,7 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     are not rounded, and more than 2^25 of them are not kept: the backward computes them
     again, a piece of the vocabulary at a time, in workspaces of half a GiB each.
     Differentiable in ``hidden`` and ``weight`` (either may be without gradient, which saves
-    its product).
+    its product); forward-mode derivatives are refused.
 
     A row of ``ignore_index`` has loss 0 and no gradient; any other target outside the
     vocabulary makes its loss NaN, and its gradients where the loss takes part.  A row that
@@ -321,6 +321,7 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     if targets.device != hidden.device:
         raise ValueError('Targets and hidden states must share a device')
     _check_options(temperature, reduction)
+    _refuse_tangents("linear_cross_entropy", hidden, weight)
     _require_gpu(hidden, "linear_cross_entropy")
     args = (hidden, weight, targets.contiguous(), None, None, 1.0 / temperature, int(ignore_index), False,
             _REDUCTIONS[reduction])
@@ -340,7 +341,7 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, temperature=1.0, r
     all other tokens taken as one, q_r = max(0, 1 - sum_k q_k); where no other token can be
     (all are known, or their logits -inf) it takes no part.  float32, the mean over the rows
     that have a teacher's token (0 if none has), their sum, or each row's with
-    ``reduction="none"``.  Differentiable in ``logits``.
+    ``reduction="none"``.  Differentiable in ``logits``; forward-mode derivatives are refused.
 
     An id below 0 is no token (rows of fewer, down to none: loss 0 and no gradient); one
     given twice counts twice; one outside the vocabulary makes the row's loss NaN, and its
@@ -354,6 +355,7 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, temperature=1.0, r
     _lib.dtype_code(logits.dtype)
     _check_teacher(logits, teacher_ids, teacher_log_probs)
     _check_options(temperature, reduction)
+    _refuse_tangents("distillation_loss", logits, teacher_log_probs)
     _require_gpu(logits, "distillation_loss")
     args = (logits, teacher_ids.contiguous(), teacher_log_probs.contiguous(), 1.0 / temperature, bool(rest),
             _REDUCTIONS[reduction])
@@ -370,6 +372,7 @@ def linear_distillation_loss(hidden, weight, teacher_ids, teacher_log_probs, tem
     _check_factors(hidden, weight)
     _check_teacher(hidden, teacher_ids, teacher_log_probs)
     _check_options(temperature, reduction)
+    _refuse_tangents("linear_distillation_loss", hidden, weight, teacher_log_probs)
     _require_gpu(hidden, "linear_distillation_loss")
     args = (hidden, weight, None, teacher_ids.contiguous(), teacher_log_probs.contiguous(), 1.0 / temperature,
             0, bool(rest), _REDUCTIONS[reduction])
