@@ -182,7 +182,8 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
     vocab] over ``temperature``, with each row's entropy and its ``top`` most likely
     tokens (up to 64, in order, the lower id first among equal logits) and their log
     probabilities: a ``TokenLogProbs``, all float32 but the ids.  Differentiable in
-    ``logits``, through the entropies and the alternatives' log probabilities too.
+    ``logits``, through the entropies and the alternatives' log probabilities too;
+    forward-mode derivatives are refused.
 
     A target of ``ignore_index`` has log probability 0 and no gradient; any other
     target outside the vocabulary gives NaN, in the gradient too unless the log
@@ -204,6 +205,7 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
         raise ValueError(f'top must be between 0 and {MAX_TOP} and at most the vocabulary')
     if not 0 < temperature < float("inf"):
         raise ValueError('temperature must be positive and finite')
+    _refuse_tangents("token_log_probs", logits)
     _require_gpu(logits, "token_log_probs")
     args = logits, targets.contiguous(), int(top), 1.0 / temperature, int(ignore_index)
     if logits.requires_grad and torch.is_grad_enabled():
