@@ -12,6 +12,6 @@ int64_t few_f32_planes(int64_t tokens, int64_t width);
 // planes [few_f32_planes][rows][width] whose sum is D^T weight.
 void few_f32_hidden(const float* D, const float* weight, int64_t ldw, int64_t rows, int64_t tokens,
                     int64_t width, float* planes, hipStream_t st);
-// out [tokens][width] = D hidden.
+// out [tokens][width] = D hidden, rows of hidden 16-byte aligned.
 void few_f32_weight(const float* D, const float* hidden, int64_t ldh, int64_t rows, int64_t tokens,
                     int64_t width, float* out, hipStream_t st);

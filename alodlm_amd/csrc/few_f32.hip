@@ -79,9 +79,7 @@ few_weight_kernel(const float* __restrict__ D, const float* __restrict__ hidden,
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     h[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < rows)  // element by element: rows need no alignment
-      h[r] = make_float4(hidden[r * ldh + at], hidden[r * ldh + at + 1], hidden[r * ldh + at + 2],
-                         hidden[r * ldh + at + 3]);
+    if (r < rows) h[r] = *reinterpret_cast<const float4*>(hidden + r * ldh + at);
   }
 #pragma unroll 4
   for (int64_t v = first; v < last; ++v) {

@@ -308,16 +308,13 @@ int64_t gemm_mid_launch(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t
   return nsplit;
 }
 
-int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t* B, int64_t ldb,
-                        int b_kmajor, int64_t M, int64_t N, int64_t K, int64_t splits,
-                        float* planes, hipStream_t st) {
+int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t* B, int64_t ldb, int64_t M,
+                        int64_t N, int64_t K, int64_t splits, float* planes, hipStream_t st) {
   const int epi = ALODLM_EPI_STORE;  // with planes given, the kernel leaves its sums there
   const int64_t kps = ((K + splits - 1) / splits + KD - 1) / KD * KD;
   const int64_t nsplit = (K + kps - 1) / kps;
   const int rows = gemm_mid_rows(a_kmajor, M, epi);
-  if (a_kmajor && b_kmajor) launch_rows<true, true>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
-  else if (a_kmajor) launch_rows<true, false>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
-  else if (b_kmajor) launch_rows<false, true>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
+  if (a_kmajor) launch_rows<true, false>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
   else launch_rows<false, false>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
   return nsplit;
 }

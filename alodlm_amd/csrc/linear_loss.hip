@@ -712,7 +712,7 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
             planes += count;
             done = true;
           } else if (take * a.ldw < (1ll << 30)) {
-            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, 0, d_rows, H, take, s.planes, to, a.st);
+            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, d_rows, H, take, s.planes, to, a.st);
             done = true;
           }
         }
@@ -742,7 +742,7 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
                                                            KSegs{}, ScaleHooks{up});
         } else {
           if (p.parts > 1 || R * a.deep_ldh < (1ll << 30))
-            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, 0, padded, H, d_rows, s.planes, rows, a.st);
+            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, padded, H, d_rows, s.planes, rows, a.st);
           else
             LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, rows, H, nullptr, 0, padded, H, R, 1.f, f32_out,
                                 a.dtype, nullptr, a.st));
