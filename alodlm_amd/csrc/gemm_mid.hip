@@ -310,11 +310,40 @@ int64_t gemm_mid_launch(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t
 
 int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t* B, int64_t ldb, int64_t M,
                         int64_t N, int64_t K, int64_t splits, float* planes, hipStream_t st) {
-  const int epi = ALODLM_EPI_STORE;  // with planes given, the kernel leaves its sums there
   const int64_t kps = ((K + splits - 1) / splits + KD - 1) / KD * KD;
   const int64_t nsplit = (K + kps - 1) / kps;
-  const int rows = gemm_mid_rows(a_kmajor, M, epi);
-  if (a_kmajor) launch_rows<true, false>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
-  else launch_rows<false, false>(A, lda, B, ldb, nullptr, 0, nullptr, 0, M, N, K, 1.f, epi, kps, nsplit, planes, rows, st);
+  // What one launch takes of the operands ends below 2 GiB, its 32-bit buffer offsets' reach:
+  // rows of a k-contiguous A, k rows of the others (with those that are filled up with zeros)
+  constexpr int64_t MOST = (1ll << 30) - 1;  // elements
+  const int64_t rows_most = a_kmajor && M * lda > MOST ? MOST / lda / 128 * 128 : M;
+  const int64_t k_most = MOST / (a_kmajor || ldb > lda ? ldb : lda) / KD * KD;
+  auto at = [&](int64_t m, int64_t k) { return A + (a_kmajor ? m * lda + k : k * lda); };
+  if (rows_most == M && kps <= k_most) {
+    const int epi = ALODLM_EPI_STORE;  // with planes given, the kernel leaves its sums there
+    const int rows = gemm_mid_rows(a_kmajor, M, epi);
+    const int64_t per = (K + KD - 1) / KD * KD <= k_most ? nsplit : k_most / kps;  // splits of a launch
+    for (int64_t s = 0; s < nsplit; s += per) {
+      const int64_t n = nsplit - s < per ? nsplit - s : per, k = s * kps;
+      const int64_t depth = K - k < n * kps ? K - k : n * kps;
+      float* to = planes + s * M * N;
+      if (a_kmajor) launch_rows<true, false>(at(0, k), lda, B + k * ldb, ldb, nullptr, 0, nullptr, 0, M, N, depth, 1.f, epi, kps, n, to, rows, st);
+      else launch_rows<false, false>(at(0, k), lda, B + k * ldb, ldb, nullptr, 0, nullptr, 0, M, N, depth, 1.f, epi, kps, n, to, rows, st);
+    }
+    return nsplit;
+  }
+  // a split of more: part by part, a plane's parts of k into it one after the other
+  for (int64_t s = 0; s < nsplit; ++s) {
+    const int64_t first = s * kps, last = first + kps < K ? first + kps : K;
+    for (int64_t k = first; k < last; k += k_most) {
+      const int64_t depth = last - k < k_most ? last - k : k_most, kpd = (depth + KD - 1) / KD * KD;
+      const int epi = k == first ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_ACCUM;
+      for (int64_t m = 0; m < M; m += rows_most) {
+        const int64_t n = M - m < rows_most ? M - m : rows_most;
+        float* C = planes + (s * M + m) * N;
+        if (a_kmajor) launch_rows<true, false>(at(m, k), lda, B + k * ldb, ldb, C, N, nullptr, 0, n, N, depth, 1.f, epi, kpd, 1, nullptr, 128, st);
+        else launch_rows<false, false>(at(m, k), lda, B + k * ldb, ldb, C, N, nullptr, 0, n, N, depth, 1.f, epi, kpd, 1, nullptr, 128, st);
+      }
+    }
+  }
   return nsplit;
 }

@@ -656,7 +656,6 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
   const Plan& p = a.p;
   constexpr bool half = sizeof(T) == 2;
   const int64_t R = a.R, V = a.V, H = a.H, d_rows = p.parts * R;
-  const int f32_out = half ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_STORE;
   T* D = reinterpret_cast<T*>(a.ws + p.D);
   float* sums = a.ws + p.sums;
   int64_t planes = 0, rest = 0;
@@ -703,22 +702,18 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
       if (take) {
         const Split s = last ? p.last_split : p.hidden_split;
         float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * d_rows * H;
-        bool done = false;
         if constexpr (half) {
           if (s.large) {
             int64_t count = 1;
             gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
                            s.planes, &count, 0, a.st);
             planes += count;
-            done = true;
-          } else if (take * a.ldw < (1ll << 30)) {
+          } else {
             planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, d_rows, H, take, s.planes, to, a.st);
-            done = true;
           }
-        }
-        if (!done) {
-          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, f32_out, a.dtype,
-                              half ? nullptr : a.gemm(), a.st));
+        } else {
+          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE,
+                              a.dtype, a.gemm(), a.st));
           ++planes;
         }
         ALODLM_CHECK_LAUNCH("linear_loss_bwd");
@@ -733,7 +728,6 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
       if constexpr (half) {
         float* rows = a.ws + p.rows;
         const Split s = split_product(padded, H, d_rows, true, true, false);
-        int64_t count = 1;
         if (s.large) {
           const int64_t tiles = ceil_div(padded, TB) * ceil_div(H, TB);
           gemm_dl_kernel<false, false, ALODLM_EPI_STORE, 4, true, false, ScaleHooks>
@@ -741,16 +735,13 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
                                                            padded, H, p.deep_rows, 1.f, p.deep_rows, nullptr, 0,
                                                            KSegs{}, ScaleHooks{up});
         } else {
-          if (p.parts > 1 || R * a.deep_ldh < (1ll << 30))
-            count = gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, padded, H, d_rows, s.planes, rows, a.st);
-          else
-            LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, rows, H, nullptr, 0, padded, H, R, 1.f, f32_out,
-                                a.dtype, nullptr, a.st));
+          const int64_t count =
+              gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, padded, H, d_rows, s.planes, rows, a.st);
           finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, 1, to, a.st);
         }
       } else {
-        LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, to, H, nullptr, 0, up_to(n, 8), H, R, 1.f, f32_out, a.dtype,
-                            a.gemm(), a.st));
+        LL_CALL(alodlm_gemm(D, ldd, 0, a.hidden, a.ldh, 0, to, H, nullptr, 0, up_to(n, 8), H, R, 1.f, ALODLM_EPI_STORE,
+                            a.dtype, a.gemm(), a.st));
       }
       ALODLM_CHECK_LAUNCH("linear_loss_bwd");
     }

@@ -1,0 +1,69 @@
+"""The vocabulary losses at their edges: operands past 2 GiB.  Against 64 bits, with the
+tolerances of test_vocab_losses_gpu.py."""
+
+import pytest
+import torch
+
+from alodlm_amd.loss import linear_cross_entropy
+from tests.helpers import log
+from tests.test_vocab_losses_gpu import B, BF16, DEV, EPS, check_linear, factors, sizes
+from tests.vocab_loss_oracle import divergence, targets_as_known
+
+pytestmark = pytest.mark.gpu
+
+
+def check_repeated(R, V, H, dtype, n=1000, seed=0):
+    """R rows of which only n differ: row i is row i % n.  What 64 bits say of n rows holds for all."""
+    hidden, weight, targets = factors(n, V, H, dtype, seed)
+    at = torch.arange(R, device=DEV) % n
+    h, w = hidden[at].requires_grad_(), weight.clone().requires_grad_()
+    loss = linear_cross_entropy(h, w, targets[at], reduction="sum")
+    gh, gw = torch.autograd.grad(loss, (h, w))
+    del h
+    loss = float(loss.detach())
+    ids, log_q = targets_as_known(targets)
+    h64, w64 = hidden.double(), weight.double()
+    logits = h64 @ w64.T
+    want, D, mass, p = divergence(logits, ids, log_q, 1.0, False)
+    count = torch.bincount(at, minlength=n).double()
+    # as in check_linear: a log probability's error, D's rounding, the products' sums
+    noise = (H / 32 + 8) * EPS * (h64.abs().amax(-1) * w64.abs().sum(-1).amax())
+    tol = sizes(logits, V, 1.0, noise)
+    assert abs(loss - float((want * count).sum())) <= float(((tol + 8 * EPS * want) * count).sum()) + EPS * loss
+    own = torch.zeros(n, V + 1, dtype=torch.float64, device=DEV).scatter_(1, torch.where(ids >= 0, ids, V), 1.0)[:, :V]
+    size = p * mass[:, None] + own + mass[:, None] * torch.where(own > 0, 0.0, p)
+    step = B if dtype == BF16 else 0.0
+    one = B if dtype == BF16 else EPS
+    far = 8 * (tol[:, None] + 2 * EPS) * size + step * D.abs()
+    each, wide = D @ w64, (far + V / 32 * EPS * D.abs()) @ w64.abs()
+    assert bool((gh == gh[:n][at]).all())
+    assert bool(((gh[:n].double() - each).abs() <= wide + 2 * one * each.abs()).all())
+    D, far = D * count[:, None], (far + R / 32 * EPS * D.abs()) * count[:, None]
+    ref, wide = D.T @ h64, far.T @ h64.abs()
+    off = (gw.double() - ref).abs()
+    assert bool((off <= wide + 2 * one * ref.abs()).all())
+    if dtype == BF16:
+        rms = ((D * D).T @ (h64 * h64)).sqrt()
+        assert float(off.norm()) <= B * (float(ref.norm()) + float(rms.norm()))
+
+
+def test_gradients_past_4_gib():
+    """2^23 rows: the logits' gradient of 256 tokens takes 4 GiB, and both its products must
+    not wrap their 32-bit offsets (the last 8 tokens and 40 rows fill no tile)."""
+    log("linear cross entropy 2^23 + 40 rows")
+    check_repeated(2 ** 23 + 40, 200, 64, BF16)
+
+
+@pytest.mark.parametrize("stride", [2 ** 19, 2 ** 22 - 8])
+def test_rows_far_apart(stride):
+    """Weight rows, and hidden rows, of more than 2 GiB from the first to the last: several
+    launches a product, or several a part of one."""
+    for R, V, which in ((90, 3000, 1), (3000, 40, 0)):
+        log(f"linear cross entropy, rows {stride} apart, {R} x {V}")
+        data = list(factors(R, V, 64, BF16))
+        rows = data[which].shape[0]
+        buf = torch.empty(rows * stride, dtype=BF16, device=DEV)
+        data[which] = buf.as_strided((rows, 64), (stride, 1)).copy_(data[which])
+        check_linear(*data, reduction="mean")
+        check_linear(*data, reduction="none")
+        del data, buf
