@@ -309,7 +309,8 @@ int64_t gemm_mid_launch(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t
 }
 
 int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t* B, int64_t ldb, int64_t M,
-                        int64_t N, int64_t K, int64_t splits, float* planes, hipStream_t st) {
+                        int64_t N, int64_t K, int64_t splits, float* planes, bool add, hipStream_t st) {
+  if (add) splits = 1;
   const int64_t kps = ((K + splits - 1) / splits + KD - 1) / KD * KD;
   const int64_t nsplit = (K + kps - 1) / kps;
   // What one launch takes of the operands ends below 2 GiB, its 32-bit buffer offsets' reach:
@@ -318,7 +319,7 @@ int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t
   const int64_t rows_most = a_kmajor && M * lda > MOST ? MOST / lda / 128 * 128 : M;
   const int64_t k_most = MOST / (a_kmajor || ldb > lda ? ldb : lda) / KD * KD;
   auto at = [&](int64_t m, int64_t k) { return A + (a_kmajor ? m * lda + k : k * lda); };
-  if (rows_most == M && kps <= k_most) {
+  if (!add && rows_most == M && kps <= k_most) {
     const int epi = ALODLM_EPI_STORE;  // with planes given, the kernel leaves its sums there
     const int rows = gemm_mid_rows(a_kmajor, M, epi);
     const int64_t per = (K + KD - 1) / KD * KD <= k_most ? nsplit : k_most / kps;  // splits of a launch
@@ -331,12 +332,12 @@ int64_t gemm_mid_planes(const bf16_t* A, int64_t lda, int a_kmajor, const bf16_t
     }
     return nsplit;
   }
-  // a split of more: part by part, a plane's parts of k into it one after the other
+  // added up, or a split of more: part by part, a plane's parts of k into it one after the other
   for (int64_t s = 0; s < nsplit; ++s) {
     const int64_t first = s * kps, last = first + kps < K ? first + kps : K;
     for (int64_t k = first; k < last; k += k_most) {
       const int64_t depth = last - k < k_most ? last - k : k_most, kpd = (depth + KD - 1) / KD * KD;
-      const int epi = k == first ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_ACCUM;
+      const int epi = k == first && !add ? ALODLM_EPI_STORE_F32 : ALODLM_EPI_ACCUM;
       for (int64_t m = 0; m < M; m += rows_most) {
         const int64_t n = M - m < rows_most ? M - m : rows_most;
         float* C = planes + (s * M + m) * N;

@@ -4,11 +4,11 @@
 //
 // Forward: the logits leave the matrix cores tile by tile (256 rows x 256 tokens, the
 // two-stage kernel of gemm_dl_tile.h) and are summed where they are, in the epilogue: a
-// tile leaves one part (largest logit, sum) a row.  Nothing of the size of the logits is
-// written.  Backward: a piece of the vocabulary at a time, the tiles are computed once more
+// tile leaves one part (largest logit, sum) a row, 8 bytes for 256 logits.  Backward: a piece of the vocabulary at a time, the tiles are computed once more
 // and leave the piece's gradient D = dloss / dlogits in bf16, from which two products give
-// its share of d_hidden (D W, in float32 planes that one pass adds up) and its rows of
-// d_weight (D^T hidden, written once).  Four products of 2 rows vocab width operations in
+// its share of d_hidden (D W, in float32 planes that one pass adds up; where the planes would
+// pass 1 GiB the pieces add to one in their epilogues, at the same speed: 16384 rows of width
+// 4096 59.5 -> 59.1 ms, 2.97 -> 0.72 GiB) and its rows of d_weight (D^T hidden, written once).  Four products of 2 rows vocab width operations in
 // all, of which the second computation of the logits is what not keeping them costs.
 //
 // Logits of at most 2^25 values are cheaper to keep, in float32, than to compute again (and
@@ -372,12 +372,13 @@ void finish_product(const float* planes, int64_t count, int64_t rows, int64_t wi
 // Which bf16 tiles a product [M, N] over K runs on and how its K is split: the least of
 // the times that gemm.hip's rule is made of (a 32-deep step of a round of 256 workgroups:
 // 0.58 to 0.78 us on 256x256 tiles, 0.28 us on 128x128 ones and 0.3 on 32 or 64 rows), and
-// the float planes, written and read at 5.5 TB/s; `direct`: 256x256 tiles need none.
+// the float planes, written and read at 5.5 TB/s; `direct`: 256x256 tiles need none; `whole`: K is
+// not split.
 struct Split {
   bool large;
   int64_t planes;
 };
-Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct, bool few) {
+Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct, bool few, bool whole = false) {
   const int64_t steps = ceil_div(K, 32);
   Split best = {true, 1};
   double least = 1e30;
@@ -391,19 +392,22 @@ Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct,
   };
   if (large_ok) {
     const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
-    for (int64_t s = 1; s <= (direct ? 1 : 32) && (s == 1 || steps / s >= 16); ++s) {
+    for (int64_t s = 1; s <= (direct || whole ? 1 : 32) && (s == 1 || steps / s >= 16); ++s) {
       const double fill = tiles * s < 256 ? (double)(tiles * s) / 256.0 : 1.0;
       offer(true, s, tiles, 0.58 + 0.2 * fill);
     }
   }
   const int64_t rows = !few ? 128 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const int64_t tiles = ceil_div(M, rows) * ceil_div(N, 128);
-  for (int64_t s = 1; s <= 64 && (s == 1 || steps / s >= 8); ++s) offer(false, s, tiles, rows == 128 ? 0.28 : 0.3);
+  for (int64_t s = 1; s <= (whole ? 1 : 64) && (s == 1 || steps / s >= 8); ++s) offer(false, s, tiles, rows == 128 ? 0.28 : 0.3);
   return best;
 }
 
 constexpr int64_t KEPT = 1 << 25;                // logits that a forward keeps for its backward
 constexpr int64_t PIECE_BYTES = 512ll << 20;     // of what is held of the vocabulary at a time
+// of d_hidden's planes; where they would be more, all pieces add to one (the pieces get smaller
+// with the rows, so that their number times a plane's size grows with the square of the rows)
+constexpr int64_t PLANE_BYTES = 1ll << 30;
 constexpr int64_t FEW = ALODLM_FEW_ROWS;
 
 // How a call runs, from its sizes alone.
@@ -417,6 +421,7 @@ struct Plan {
   bool copy_hidden, copy_weight;
   int64_t chunks, sum_parts;  // of a piece's rows, of all
   int64_t planes;           // of d_hidden, most
+  bool add;                 // one, which the pieces add to
   bool direct;              // d_hidden needs no planes
   Split hidden_split, last_split;
   // workspace, in floats
@@ -500,9 +505,18 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
       if (d_hidden) p.sums = room(p.planes * R * H);
     } else if (d_hidden) {
       const bool large = H >= 256;
-      p.hidden_split = p.half ? split_product(d_rows, H, p.piece, large, false, true) : Split{true, 1};
-      p.last_split = p.half && whole ? split_product(d_rows, H, whole, large, false, true) : Split{true, 1};
+      auto split = [&](int64_t K) {
+        return p.half && K ? split_product(d_rows, H, K, large, false, true, p.add) : Split{true, 1};
+      };
+      p.hidden_split = split(p.piece);
+      p.last_split = split(whole);
       p.planes = (p.pieces - 1) * p.hidden_split.planes + (whole ? p.last_split.planes : 0);
+      if (p.planes > 1 && p.planes * d_rows * H * 4 > PLANE_BYTES) {
+        p.add = true;
+        p.hidden_split = split(p.piece);
+        p.last_split = split(whole);
+        p.planes = 1;
+      }
       p.direct = !p.half && p.planes == 1 && rest == 0;
       if (!p.direct) p.sums = room(p.planes * d_rows * H);
       if (!p.half) {
@@ -701,21 +715,20 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
       rest_weight = w + take * a.ldw;
       if (take) {
         const Split s = last ? p.last_split : p.hidden_split;
-        float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + planes * d_rows * H;
+        const bool more = p.add && planes > 0;
+        float* to = p.direct ? reinterpret_cast<float*>(d_hidden) : sums + (more ? 0 : planes) * d_rows * H;
+        int64_t count = 1;
         if constexpr (half) {
-          if (s.large) {
-            int64_t count = 1;
-            gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE_F32, to,
-                           s.planes, &count, 0, a.st);
-            planes += count;
-          } else {
-            planes += gemm_mid_planes(D, ldd, 1, w, a.ldw, d_rows, H, take, s.planes, to, a.st);
-          }
+          if (s.large)
+            gemm_dl_launch(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f,
+                           more ? ALODLM_EPI_ACCUM : ALODLM_EPI_STORE_F32, to, s.planes, &count, more, a.st);
+          else
+            count = gemm_mid_planes(D, ldd, 1, w, a.ldw, d_rows, H, take, s.planes, to, more, a.st);
         } else {
-          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f, ALODLM_EPI_STORE,
-                              a.dtype, a.gemm(), a.st));
-          ++planes;
+          LL_CALL(alodlm_gemm(D, ldd, 1, w, a.ldw, 0, to, H, nullptr, 0, d_rows, H, take, 1.f,
+                              more ? ALODLM_EPI_ACCUM : ALODLM_EPI_STORE, a.dtype, a.gemm(), a.st));
         }
+        if (!more) planes += count;
         ALODLM_CHECK_LAUNCH("linear_loss_bwd");
       }
       if (last && !p.direct)
@@ -736,7 +749,7 @@ int backward(Call<T>& a, const KnownRows& k, float c, const Upstream& up, const 
                                                            KSegs{}, ScaleHooks{up});
         } else {
           const int64_t count =
-              gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, padded, H, d_rows, s.planes, rows, a.st);
+              gemm_mid_planes(D, ldd, 0, a.deep_hidden, a.deep_ldh, padded, H, d_rows, s.planes, rows, false, a.st);
           finish_product<T>(rows, count, padded, H, up, nullptr, 0, nullptr, 0, 0, 1, to, a.st);
         }
       } else {

@@ -304,7 +304,9 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     ``temperature``: float32, the mean over the rows whose target is not ``ignore_index``
     (0 if there is none), their sum, or with ``reduction="none"`` the rows' own.  The logits
     are not rounded, and more than 2^25 of them are not kept: the backward computes them
-    again, a piece of the vocabulary at a time, in workspaces of half a GiB each.
+    again, a piece of the vocabulary at a time, in a workspace of half a GiB for the piece
+    and, with a gradient in ``hidden``, up to 1 GiB (or once its size in float32, if that is
+    more) for its sums.
     Differentiable in ``hidden`` and ``weight`` (either may be without gradient, which saves
     its product); forward-mode derivatives are refused.
 

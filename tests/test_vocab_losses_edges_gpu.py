@@ -1,4 +1,5 @@
-"""The vocabulary losses at their edges: operands past 2 GiB.  Against 64 bits, with the
+"""The vocabulary losses at their edges: operands past 2 GiB, pieces of the vocabulary that
+add to one plane.  Against 64 bits, with the
 tolerances of test_vocab_losses_gpu.py."""
 
 import pytest
@@ -6,7 +7,7 @@ import torch
 
 from alodlm_amd.loss import linear_cross_entropy
 from tests.helpers import log
-from tests.test_vocab_losses_gpu import B, BF16, DEV, EPS, check_linear, factors, sizes
+from tests.test_vocab_losses_gpu import B, BF16, DEV, EPS, F32, check_linear, factors, sizes
 from tests.vocab_loss_oracle import divergence, targets_as_known
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,12 @@ def test_rows_far_apart(stride):
         check_linear(*data, reduction="mean")
         check_linear(*data, reduction="none")
         del data, buf
+
+
+# bf16 tiles of 128 and of 256 rows, float32 with and without tokens left over (the latter adds
+# to the gradient itself); the planes of all pieces would be 1 to 2.3 GiB
+@pytest.mark.parametrize("R,V,H,dtype", [(2 ** 20 + 100, 1000, 64, BF16), (300000, 2001, 512, BF16),
+                                         (300000, 901, 512, F32), (300040, 896, 512, F32)])
+def test_pieces_add_to_one_plane(R, V, H, dtype):
+    log(f"linear cross entropy {R} x {V} x {H} {dtype}, one plane")
+    check_repeated(R, V, H, dtype)
