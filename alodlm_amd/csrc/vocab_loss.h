@@ -77,7 +77,8 @@ enum { VL_EACH = 0, VL_SUM = 1, VL_MEAN = 2 };
 // The upstream gradient over the temperature.  `apart`: a reduced loss's, which all rows
 // share, is left to the end (all()), so that a row's gradient is Q p - q itself and loses
 // nothing to another factor's mantissa when it is rounded; a row's is then 1, or 0 where
-// the whole is.
+// the whole is.  (One that is NaN or infinite stays with the rows: at the end it would meet
+// the zeros of rows that have no gradient.)
 struct Upstream {
   const float* call;
   const float* d_loss;
@@ -86,10 +87,21 @@ struct Upstream {
   __device__ __forceinline__ float shared() const { return d_loss[0] * call[0] * inv_t; }
   __device__ __forceinline__ float row(int64_t r) const {
     if (reduction == VL_EACH) return d_loss[r] * inv_t;
-    return apart ? (shared() != 0.f ? 1.f : 0.f) : shared();
+    const float s = shared();
+    return apart && s - s == 0.f ? (s != 0.f ? 1.f : 0.f) : s;
   }
-  __device__ __forceinline__ float all() const { return apart && reduction != VL_EACH ? shared() : 1.f; }
+  __device__ __forceinline__ float all() const {
+    if (!apart || reduction == VL_EACH) return 1.f;
+    const float s = shared();
+    return s - s == 0.f ? s : 1.f;
+  }
 };
+
+// What a row's share of the others is times: nothing where the row takes no part, which may
+// hold NaN, or where it has no gradient, whose upstream gradient may be NaN or infinite.
+__device__ __forceinline__ float row_factor(float up, float factor) {
+  return up == 0.f || factor == 0.f ? 0.f : up * factor;
+}
 
 // Launches (vocab_loss.hip).
 //

@@ -450,7 +450,7 @@ row_grads_kernel(const TI* logits, int64_t ld, int64_t rows, int width, int64_t 
     g = up.row(row);
     m = info[RI_M];
     log_rest = info[RI_LOG];
-    factor = g == 0.f ? 0.f : g * info[RI_FACTOR];  // (a row that takes no part may hold NaN)
+    factor = row_factor(g, info[RI_FACTOR]);
   }
   const bool flat = factor == 0.f;  // nothing but the known tokens has a gradient
   auto gradient = [&](float v) { return factor * __builtin_amdgcn_exp2f((v - m) * c - log_rest); };
@@ -514,7 +514,7 @@ few_grads_kernel(const float* __restrict__ logits, int64_t ld, int rows, int wid
     const float g = up.row(threadIdx.x);
     s_m[threadIdx.x] = info[RI_M];
     s_log[threadIdx.x] = info[RI_LOG];
-    s_factor[threadIdx.x] = g == 0.f ? 0.f : g * info[RI_FACTOR];
+    s_factor[threadIdx.x] = row_factor(g, info[RI_FACTOR]);
     s_up[threadIdx.x] = g;
   }
   __syncthreads();

@@ -1,14 +1,16 @@
 """The vocabulary losses at their edges: operands past 2 GiB, pieces of the vocabulary that
-add to one plane.  Against 64 bits, with the
+add to one plane, upstream gradients that are NaN or inf.  Against 64 bits, with the
 tolerances of test_vocab_losses_gpu.py."""
+
+import math
 
 import pytest
 import torch
 
-from alodlm_amd.loss import linear_cross_entropy
+from alodlm_amd.loss import distillation_loss, linear_cross_entropy, linear_distillation_loss
 from tests.helpers import log
-from tests.test_vocab_losses_gpu import B, BF16, DEV, EPS, F32, check_linear, factors, sizes
-from tests.vocab_loss_oracle import divergence, targets_as_known
+from tests.test_vocab_losses_gpu import B, BF16, DEV, EPS, F32, check_linear, factors, generator, sizes
+from tests.vocab_loss_oracle import divergence, targets_as_known, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +79,39 @@ def test_rows_far_apart(stride):
 def test_pieces_add_to_one_plane(R, V, H, dtype):
     log(f"linear cross entropy {R} x {V} x {H} {dtype}, one plane")
     check_repeated(R, V, H, dtype)
+
+
+def check_wild_upstream(call, leaves, ignored):
+    """call(leaves, reduction) -> loss; row i of leaves[0] is ignored where ignored[i]."""
+    R = ignored.numel()
+    grads = lambda reduction, up: torch.autograd.grad(call(leaves, reduction), leaves, up)
+    up = torch.randn(R, generator=generator(R), device=DEV)
+    clean = grads("none", torch.where(ignored, 0.0, up))
+    for value in (math.nan, math.inf, -math.inf):
+        for a, b in zip(grads("none", torch.where(ignored, value, up)), clean):
+            assert torch.equal(a, b)
+        for reduction in ("mean", "sum"):
+            g = grads(reduction, torch.tensor(value, device=DEV))[0]
+            assert not bool(g[ignored].any())
+            assert not bool(g[~ignored].isfinite().all(1).any())
+
+
+@pytest.mark.parametrize("R,V,H,dtype", [(300, 1500, 64, BF16), (300, 120001, 64, BF16), (40, 1500, 64, BF16),
+                                         (40, 40000, 72, BF16), (20, 20000, 64, F32), (70, 900, 64, F32)])
+def test_upstream_of_rows_that_are_ignored(R, V, H, dtype):
+    """An ignored row has no gradient whatever its upstream gradient is: one a row (0 / 0 of a
+    row's weight, say), or a reduced loss's."""
+    log(f"wild upstream {R} x {V} x {H} {dtype}")
+    hidden, weight, targets = factors(R, V, H, dtype)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    check_wild_upstream(lambda x, reduction: linear_cross_entropy(*x, targets, reduction=reduction), (h, w),
+                        targets == -100)
+    ids, log_q = tokens(R, V, 3, generator(R), DEV)
+    ids[::5] = -1
+    ignored = (ids < 0).all(1)
+    for rest in (True, False):
+        check_wild_upstream(lambda x, reduction: linear_distillation_loss(*x, ids, log_q, rest=rest, reduction=reduction),
+                            (h, w), ignored)
+        z = (h @ w.T).detach().requires_grad_()
+        check_wild_upstream(lambda x, reduction: distillation_loss(*x, ids, log_q, rest=rest, reduction=reduction), (z,),
+                            ignored)
