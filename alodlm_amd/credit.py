@@ -35,6 +35,14 @@ def _refuse_tangents(what, *tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
+def _ignored_id(ignore_index):
+    """As the library takes it: ctypes would drop what passes 64 bits."""
+    i = int(ignore_index)
+    if not -2 ** 63 <= i < 2 ** 63:
+        raise ValueError('ignore_index must fit 64 bits')
+    return i
+
+
 def check_sequence_boundaries(masked_indices, cum_seqlens):
     """The argument checks of alodlm/credit.py:8-19."""
     if masked_indices.ndim != 1 or masked_indices.dtype != torch.bool:
@@ -205,9 +213,10 @@ def token_log_probs(logits, targets, top=0, temperature=1.0, ignore_index=-100):
         raise ValueError(f'top must be between 0 and {MAX_TOP} and at most the vocabulary')
     if not 0 < temperature < float("inf"):
         raise ValueError('temperature must be positive and finite')
+    ignored = _ignored_id(ignore_index)
     _refuse_tangents("token_log_probs", logits)
     _require_gpu(logits, "token_log_probs")
-    args = logits, targets.contiguous(), int(top), 1.0 / temperature, int(ignore_index)
+    args = logits, targets.contiguous(), int(top), 1.0 / temperature, ignored
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogProbs(*_TokenLogProbs.apply(*args))
     return TokenLogProbs(*_log_probs(*args)[:4])

@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, call_on, ptr, query
-from .credit import _refuse_tangents, _require_gpu, _vocabulary_rows, check_sequence_boundaries
+from .credit import _ignored_id, _refuse_tangents, _require_gpu, _vocabulary_rows, check_sequence_boundaries
 
 METRIC_KEYS = ("denoising", "actor", "sampled_mean_depth", "prediction_cost",
                "regularization_cost", "profile_mean_depth", "first_pass_halt_probability")
@@ -323,9 +323,10 @@ def linear_cross_entropy(hidden, weight, targets, temperature=1.0, ignore_index=
     if targets.device != hidden.device:
         raise ValueError('Targets and hidden states must share a device')
     _check_options(temperature, reduction)
+    ignored = _ignored_id(ignore_index)
     _refuse_tangents("linear_cross_entropy", hidden, weight)
     _require_gpu(hidden, "linear_cross_entropy")
-    args = (hidden, weight, targets.contiguous(), None, None, 1.0 / temperature, int(ignore_index), False,
+    args = (hidden, weight, targets.contiguous(), None, None, 1.0 / temperature, ignored, False,
             _REDUCTIONS[reduction])
     if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _Linear.apply(*args)

@@ -1,4 +1,5 @@
-"""token_log_probs without a GPU: forward-mode derivatives are refused."""
+"""token_log_probs without a GPU: forward-mode derivatives and ignored ids that do not fit
+the library's integers are refused."""
 
 import pytest
 import torch
@@ -19,3 +20,10 @@ def test_tangents_are_refused(grad):
         # where they are not in force, the call goes on to ask for a GPU
         with torch.inference_mode(), pytest.raises(ValueError, match="GPU|device"):
             token_log_probs(dual, targets, top=2)
+
+
+@pytest.mark.parametrize("ignore", [2 ** 63, 2 ** 64, 2 ** 64 + 5, -2 ** 63 - 1])
+def test_ignored_ids_past_64_bits(ignore):
+    """2^64 + 5 would be 5 to the library, a token."""
+    with pytest.raises(ValueError, match="ignore_index"):
+        token_log_probs(torch.zeros(4, 9), torch.zeros(4, dtype=torch.int64), ignore_index=ignore)

@@ -1,5 +1,6 @@
-"""The vocabulary losses' edges without a GPU: forward-mode derivatives are refused, the
-backward's workspace is bounded whatever the rows are."""
+"""The vocabulary losses' edges without a GPU: forward-mode derivatives and ignored ids
+that do not fit the library's integers are refused, the backward's workspace is bounded
+whatever the rows are."""
 
 import pytest
 import torch
@@ -36,6 +37,16 @@ def test_tangents_are_refused(call, dual, grad):
         args[dual] = forward_ad.unpack_dual(args[dual]).primal.detach()
         with pytest.raises(ValueError, match="GPU|device"):
             calls(*args)[call]()
+
+
+@pytest.mark.parametrize("ignore", [2 ** 63, 2 ** 64, 2 ** 64 + 5, -2 ** 63 - 1])
+def test_ignored_ids_past_64_bits(ignore):
+    """2^64 + 5 would be 5 to the library, a token."""
+    with pytest.raises(ValueError, match="ignore_index"):
+        linear_cross_entropy(torch.zeros(4, 8), torch.zeros(9, 8), torch.zeros(4, dtype=I64), ignore_index=ignore)
+    for largest in (2 ** 63 - 1, -2 ** 63):
+        with pytest.raises(ValueError, match="GPU|device"):
+            linear_cross_entropy(torch.zeros(4, 8), torch.zeros(9, 8), torch.zeros(4, dtype=I64), ignore_index=largest)
 
 
 @pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2)])
