@@ -4,12 +4,14 @@
 //
 // Forward: the logits leave the matrix cores tile by tile (256 rows x 256 tokens, the
 // two-stage kernel of gemm_dl_tile.h) and are summed where they are, in the epilogue: a
-// tile leaves one part (largest logit, sum) a row, 8 bytes for 256 logits.  Backward: a piece of the vocabulary at a time, the tiles are computed once more
-// and leave the piece's gradient D = dloss / dlogits in bf16, from which two products give
-// its share of d_hidden (D W, in float32 planes that one pass adds up; where the planes would
-// pass 1 GiB the pieces add to one in their epilogues, at the same speed: 16384 rows of width
-// 4096 59.5 -> 59.1 ms, 2.97 -> 0.72 GiB) and its rows of d_weight (D^T hidden, written once).  Four products of 2 rows vocab width operations in
-// all, of which the second computation of the logits is what not keeping them costs.
+// tile leaves one part (largest logit, sum) a row, 8 bytes for 256 logits.  Backward: a piece
+// of the vocabulary at a time, the tiles are computed once more and leave the piece's gradient
+// D = dloss / dlogits in bf16, from which two products give its share of d_hidden (D W, in
+// float32 planes that one pass adds up; where the planes would pass 1 GiB the pieces add to one
+// in their epilogues, at the same speed: 16384 rows of width 4096 59.5 -> 59.1 ms, 2.97 -> 0.72
+// GiB) and its rows of d_weight (D^T hidden, written once).  Four products of 2 rows vocab width
+// operations in all, of which the second computation of the logits is what not keeping them
+// costs.
 //
 // Logits of at most 2^25 values are cheaper to keep, in float32, than to compute again (and
 // the products of few rows read the weight, which a tile of 256 rows would wait for): they
@@ -399,11 +401,12 @@ Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct,
   }
   const int64_t rows = !few ? 128 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const int64_t tiles = ceil_div(M, rows) * ceil_div(N, 128);
-  for (int64_t s = 1; s <= (whole ? 1 : 64) && (s == 1 || steps / s >= 8); ++s) offer(false, s, tiles, rows == 128 ? 0.28 : 0.3);
+  for (int64_t s = 1; s <= (whole ? 1 : 64) && (s == 1 || steps / s >= 8); ++s)
+    offer(false, s, tiles, rows == 128 ? 0.28 : 0.3);
   return best;
 }
 
-constexpr int64_t KEPT = 1 << 25;                // logits that a forward keeps for its backward
+constexpr int64_t KEPT = 1 << 25;                // logits that a forward keeps for its backward (128 MiB)
 constexpr int64_t PIECE_BYTES = 512ll << 20;     // of what is held of the vocabulary at a time
 // of d_hidden's planes; where they would be more, all pieces add to one (the pieces get smaller
 // with the rows, so that their number times a plane's size grows with the square of the rows)
@@ -459,7 +462,7 @@ Plan make_plan(int64_t R, int64_t V, int64_t H, int dtype, bool keep, bool backw
   if (computes && !p.tiles && !p.small) limit(4 * R);
   if (backward && p.few) limit(4 * few_f32_pad(R));
   if (p.copy_weight) limit(2 * p.deep);
-  if (p.half) {  // the 128x128 tiles' operands stay below 2 GiB
+  if (p.half) {  // a piece of a weight without gaps stays in one launch of 128x128 tiles
     const int64_t n = (1ll << 30) / up_to(H, 64) / 256 * 256;
     most = n < most ? n : most;
   }

@@ -3,7 +3,9 @@
 // A row knows tokens id_k with probabilities q_k: one of probability 1 (cross entropy) or
 // a teacher's most likely ones.  With z the row's logits over T, p = softmax(z),
 //   loss = sum_k q_k (ln q_k - ln p[id_k])  [+ q_r (ln q_r - ln p_r)],
-// q_r = max(0, 1 - sum_k q_k) and p_r the probability of all tokens that are not known.
+// q_r = max(0, 1 - sum_k q_k) and p_r the probability of all tokens that are not known.  Where
+// none of these can be, q_r counts as 0: of a vocabulary that teacher and student mask alike it is
+// what rounding leaves of 1, and would make the loss infinite.
 // The known tokens are kept out of the sum over the vocabulary and joined to it at the
 // end, so p_r is a sum of its own and never a difference from 1.  With Q = sum_k q_k [+ q_r]
 // and s_r the softmax over the other tokens,

@@ -342,7 +342,8 @@ def distillation_loss(logits, teacher_ids, teacher_log_probs, temperature=1.0, r
         sum_k q_k (log q_k - log p[id_k])  and with ``rest``  + q_r (log q_r - log p_r),
 
     all other tokens taken as one, q_r = max(0, 1 - sum_k q_k); where no other token can be
-    (all are known, or their logits -inf) it takes no part.  float32, the mean over the rows
+    (all are known, or their logits -inf) it takes no part: of a vocabulary that teacher and
+    student mask alike, q_r is what rounding leaves of 1.  float32, the mean over the rows
     that have a teacher's token (0 if none has), their sum, or each row's with
     ``reduction="none"``.  Differentiable in ``logits``; forward-mode derivatives are refused.
 
