@@ -407,7 +407,9 @@ Split split_product(int64_t M, int64_t N, int64_t K, bool large_ok, bool direct,
 }
 
 constexpr int64_t KEPT = 1 << 25;                // logits that a forward keeps for its backward (128 MiB)
-constexpr int64_t PIECE_BYTES = 512ll << 20;     // of what is held of the vocabulary at a time
+// of what is held of the vocabulary at a time: the logits, their gradient and copied rows of the
+// weight, each
+constexpr int64_t PIECE_BYTES = 512ll << 20;
 // of d_hidden's planes; where they would be more, all pieces add to one (the pieces get smaller
 // with the rows, so that their number times a plane's size grows with the square of the rows)
 constexpr int64_t PLANE_BYTES = 1ll << 30;
